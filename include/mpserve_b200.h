@@ -333,6 +333,67 @@ MPS_API int mps_build_shared_emit(mps_build_state* state, const uint16_t* bf16_b
                                   int32_t* out_idx_i32, int64_t* stream_chunk_ofs_i64, int32_t* stream_chunk_ids_i32,
                                   void* stream);
 
+/* 4-bit serving --------------------------------------------------------------------------------
+ * No counterpart in the reference, whose products are BF16: what a layer needs to be served from weights in MXFP4 (E2M1 codes,
+ * one E8M0 scale per 32 columns) once they are decoded.  A matrix of `rows` x `cols` in MXFP4 is an array of tiles of 128 x 256,
+ * row-major, mps_mx4_bytes() device bytes, 16-byte aligned; csrc/mx4.cuh says what is in them, mps_mx4_pack and
+ * mps_mx4_unpack convert from and to checkpoint parts: codes [rows, ceil(cols / 2)], two a byte with the even column low, and scale
+ * bytes [rows, ceil(cols / 32)].  All other matrices have unit column stride and a row stride in elements. */
+enum { MPS_BF16 = 0, MPS_F16 = 1, MPS_F32 = 2, MPS_MX4 = 3 };
+enum { MPS_SILU = 0, MPS_GELU_TANH = 1 };
+
+/* Bytes of the tiles, or -1 for sizes that are not served (rows up to 2^31, cols in [1, 2^24]). */
+MPS_API int64_t mps_mx4_bytes(int64_t rows, int64_t cols);
+/* Nearest codes (halfway to the even one) under the scale 2^(floor(log2 max) - 2) of every block; a block with an infinity or a
+ * NaN becomes NaN. */
+MPS_API int mps_mx4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, void* tiles, void* stream);
+MPS_API int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dtype, void* out, void* stream);
+MPS_API int mps_mx4_pack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* tiles, void* stream);
+MPS_API int mps_mx4_unpack(const void* tiles, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales, void* stream);
+
+/* Norms, gate and residual of a block, row by row, in FP32:
+ *   t = y * rsqrt(mean(y^2) + eps) * post_weight    (t = y where post_weight is null)
+ *   h_out = residual_scale * h + gate * t           (nothing of the kind where y is null)
+ *   n_out = h_out * rsqrt(mean(h_out^2) + eps) * next_weight, in n_dtype, MPS_MX4 included   (where next_weight is given)
+ * gate: null, or a value per column (row stride 0), per row (column stride 0) or per element.  h_out has h's type and may be h.
+ * cols up to 32768. */
+typedef struct mps_mx4_norm {
+    const void* y;
+    const void* h;
+    const void* post_weight;
+    const void* gate;
+    const void* next_weight;
+    void* h_out;
+    void* n_out;
+    int64_t rows, cols;
+    int64_t y_stride, h_stride, h_out_stride, n_stride, gate_row_stride;
+    int32_t gate_col_stride;            /* 0 or 1 */
+    int32_t y_dtype, h_dtype, n_dtype, gate_dtype, weight_dtype;
+    float eps, residual_scale;
+} mps_mx4_norm;
+MPS_API int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream);
+
+/* out[t, r] = sum_k x[t, k] w[r, k], or with w_up act(sum_k x w) * (sum_k x w_up): tokens x rows, summed in FP32.  x: MXFP4 tiles
+ * (x_dtype MPS_MX4), or a matrix that the call quantises into x_tiles (mps_mx4_bytes(tokens, cols) bytes) first.
+ * out_dtype: MPS_BF16, MPS_F16, or with w_up also MPS_MX4 (tiles of tokens x rows). */
+typedef struct mps_mx4_linear {
+    const void* x;
+    void* x_tiles;
+    const void* w;
+    const void* w_up;
+    void* out;
+    int64_t tokens, cols, rows;
+    int64_t x_stride, out_stride;
+    int32_t x_dtype, out_dtype, activation, reserved;
+} mps_mx4_linear;
+/* Scratch of the products on the current device: zero-filled once, one per stream that may run them concurrently, 256-byte
+ * aligned; handed back with its counters zeroed.  Negative: an error code. */
+MPS_API int64_t mps_mx4_workspace_bytes(void);
+MPS_API int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
+/* Every wait inside the products is bounded: waits for the stream, tells whether any since the last query gave up (its outputs are
+ * then incomplete), and clears the workspace. */
+MPS_API int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out);
+
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of
  * (pattern * (index+1)) -- what ranks all-reduce after a sharded decode.  result_dev: device
  * uint64[2], accumulated into (zero it first). */

@@ -18,10 +18,12 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "lib" / "libmpserve_b200.so"
 OBJ = PKG / "lib" / "obj"
-SOURCES = ["decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu"]
+SOURCES = ["decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu", "mx4_convert.cu", "mx4_norm.cu", "mx4_linear.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CFLAGS = ["-O3", "-std=c++17", "-lineinfo", *ARCH_FLAGS, "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-          "--use_fast_math"]
+CFLAGS = ["-O3", "-std=c++17", "-lineinfo", *ARCH_FLAGS, "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
+# The codec has no arithmetic but on integers and bit patterns.  The 4-bit operators keep subnormals (a scale goes down to 2^-127) and
+# CUDA's accurate functions.
+FAST_MATH = {"decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu"}
 
 
 def nvcc_path() -> str:
@@ -59,7 +61,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     def compile_one(src: str) -> Path:
         obj = OBJ / (Path(src).stem + ".o")
         if force or _stale(obj, [CSRC / src] + _headers()):
-            subprocess.run([nvcc, *CFLAGS, *extra, "-c", str(CSRC / src), "-o", str(obj)], check=True, env=env)
+            flags = [*CFLAGS, *(["--use_fast_math"] if src in FAST_MATH else []), *extra]
+            subprocess.run([nvcc, *flags, "-c", str(CSRC / src), "-o", str(obj)], check=True, env=env)
         return obj
 
     with ThreadPoolExecutor(max_workers=len(SOURCES)) as pool:

@@ -1,0 +1,423 @@
+// Products of MXFP4 matrices: out[t, r] = sum_k x[t, k] w[r, k], and the gated pair act(x Wg) * (x Wu).
+#include "mx4.cuh"
+#include "mx4_tensor.cuh"
+#include "stream_common.cuh"
+
+namespace mps {
+
+int launched(const char* what);
+
+// ---- what the kernels share -------------------------------------------------------------------------
+
+constexpr int kMx4MostSms = 192;               // CTAs of a launch are at most the SMs
+constexpr uint32_t kMx4SpinLimit = 1u << 20;
+constexpr int kMx4SmemMost = 232448;           // 227 KB
+
+// Workspace: word 0 records a wait that ran out; from byte 4096 on, counters; then partial sums.
+constexpr int64_t kMx4CounterBytes = 4096, kMx4PartialOffset = 4096 + kMx4CounterBytes;
+constexpr int64_t kMx4PartialFloats = 128 * 256;   // most of one CTA's accumulator, features x tokens
+constexpr int64_t kMx4WorkspaceBytes = kMx4PartialOffset + 2 * kMx4MostSms * kMx4PartialFloats * 4;
+
+struct ProductArgs {
+    const uint8_t* x;        // tiles
+    const uint8_t* w;
+    const uint8_t* w_up;
+    void* out;
+    uint32_t* workspace;
+    int64_t out_stride;
+    int64_t tokens;
+    int32_t rows;            // of the weight: features
+    int32_t chunks;          // tiles of a row
+    int32_t row_tiles, token_tiles;
+    int32_t out_dtype, activation;
+    bool x_follows;          // x is written by the kernel before, which this one may overlap
+};
+
+__device__ __forceinline__ float act(float g, int which) {
+    // exp and tanh as CUDA's accurate functions: the epilogue is a small part of a product
+    if (which == MPS_SILU) return g / (1.f + expf(-g));
+    return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
+}
+
+// A wait that gives up when another one has.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kMx4SpinLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u && *failed) return false;
+    }
+    *failed = 1u;
+    return false;
+}
+
+// ---- few tokens: weights on the accumulator's lanes -------------------------------------------------
+//
+// One CTA per SM streams weight tiles through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
+// product's narrow side.  The work is cut evenly into runs of (tile of the output, tile of K) pairs, a run per CTA, so that
+// every SM reads the same number of bytes whatever the sizes; a tile of the output that several CTAs have parts of is summed by
+// whichever of them ends last, always in the same order.  Nothing waits for another CTA.
+//
+// Warps: 0 copies, 1 multiplies, 2 to 5 take the accumulator over, two of which take turns.
+template <int TOKENS, bool GATED>
+struct StreamShape {
+    static constexpr int kWeights = GATED ? 2 : 1;
+    static constexpr int kXBytes = kMx4ScaleBytes + TOKENS * kMx4RowBytes;
+    static constexpr int kStageBytes = kWeights * kMx4TileBytes + kXBytes;
+    static constexpr int kStages = (kMx4SmemMost - 2048) / kStageBytes < 12 ? (kMx4SmemMost - 2048) / kStageBytes : 12;
+    static constexpr int kSmem = kStages * kStageBytes + 2048;
+    static constexpr int kAcc = TOKENS * kWeights;              // columns of one accumulator
+    static constexpr int kScaleColumns = 8 * kWeights + 8;      // of one stage
+    static constexpr int kBuffers = kAcc <= 128 ? 2 : 1;        // accumulators that take turns
+    static constexpr int kScaleBase = kBuffers * kAcc;
+    static constexpr int kColumns = 512;
+    static_assert(kScaleBase + kStages * kScaleColumns <= kColumns, "tensor memory");
+    static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
+    static_assert(kAcc * 128 <= kMx4PartialFloats, "partial sums");
+};
+constexpr int kStreamThreads = 192;
+
+struct StreamRun { int64_t first, last; };   // units [first, last) of a CTA
+__device__ __forceinline__ StreamRun run_of(int64_t units, int cta, int ctas) {
+    return {units * cta / ctas, units * (cta + 1) / ctas};
+}
+// The CTA that has unit u: the largest c with units * c / ctas <= u.
+__device__ __forceinline__ int cta_of(int64_t units, int64_t u, int ctas) { return (int)(((u + 1) * ctas - 1) / units); }
+
+// Sixteen tokens of one feature, `up` too where the pair is gated: into the output.
+template <bool GATED>
+__device__ __forceinline__ void finish16(const ProductArgs& p, int row_tile, int quarter, int lane, int64_t token0, float (&v)[16], float (&up)[16]) {
+    const int feature = row_tile * kMx4Rows + quarter * 32 + lane;
+    if (GATED) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = act(v[i], p.activation) * up[i];
+    }
+    if (GATED && p.out_dtype == MPS_MX4) {
+        // the warp's 32 features are one block of every token
+        const int first = row_tile * kMx4Rows + quarter * 32, chunks = (int)mx4_chunks(p.rows);
+        const int chunk = first / kMx4Cols, block = (first % kMx4Cols) / kMx4Block;
+        // the last tile's second half may lie beyond the last feature and is filled up with zeros
+        const bool fill = row_tile == p.row_tiles - 1 && (row_tile & 1) == 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t t = token0 + i;
+            if (t >= p.tokens) break;
+            const float f = feature < p.rows ? v[i] : 0.f;
+            const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f) & 0x7FFFFFFFu));
+            const float q[8] = {byte == 255u ? 0.f : f * mx4_inverse_scale(byte), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            uint32_t code = mx4_codes8(q) & 15u;
+            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1) << 4;    // right in the even lanes, then in every fourth, then in every eighth
+            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2) << 8;
+            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 4) << 16;
+            uint8_t* tile = static_cast<uint8_t*>(p.out) + mx4_tile_offset(t / kMx4Rows, chunk, chunks);
+            const int row = (int)(t % kMx4Rows);
+            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block) + (lane >> 3) * 4) = code;
+            if (lane == 0) tile[mx4_scale_offset(row, block >> 2) + (block & 3)] = (uint8_t)byte;
+            if (fill) {
+                if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block + 4) + (lane >> 3) * 4) = 0u;
+                if (lane == 0) tile[mx4_scale_offset(row, 1) + (block & 3)] = 0u;
+            }
+        }
+        return;
+    }
+    if (feature >= p.rows) return;
+    uint16_t* out = static_cast<uint16_t*>(p.out) + feature;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (token0 + i < p.tokens) out[(token0 + i) * p.out_stride] = (uint16_t)pack2(v[i], 0.f, p.out_dtype);
+}
+
+template <int TOKENS, bool GATED>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+mx4_stream_kernel(const ProductArgs p) {
+    using S = StreamShape<TOKENS, GATED>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * S::kStages + 5];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(bars);
+    const auto full = [&](int s) { return bar0 + 8u * s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (2 * S::kStages + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * S::kStages + 2 + b); };
+    const uint32_t drained = bar0 + 8u * (2 * S::kStages + 4);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 4); }
+        mbar_init(drained, 1);
+        failed = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    const int chunks = p.chunks;
+    const int64_t units = (int64_t)p.row_tiles * p.token_tiles * chunks;
+    const StreamRun run = run_of(units, blockIdx.x, gridDim.x);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int64_t count = run.last - run.first;
+            const auto weights = [&](int64_t i) {      // of the run's i-th unit, into its stage
+                const int64_t u = run.first + i, tile = u / chunks;
+                const int s = (int)(i % S::kStages), k = (int)(u - tile * chunks);
+                const int64_t at = mx4_tile_offset(tile / p.token_tiles, k, chunks);
+                const uint32_t to = ring + s * S::kStageBytes;
+                mbar_expect_tx(full(s), S::kStageBytes);
+                bulk_g2s(to, p.w + at, kMx4TileBytes, full(s));
+                if (GATED) bulk_g2s(to + kMx4TileBytes, p.w_up + at, kMx4TileBytes, full(s));
+            };
+            const auto activations = [&](int64_t i) {
+                const int64_t u = run.first + i, tile = u / chunks;
+                const int s = (int)(i % S::kStages), k = (int)(u - tile * chunks);
+                bulk_g2s(ring + s * S::kStageBytes + S::kWeights * kMx4TileBytes, p.x + mx4_tile_offset(tile % p.token_tiles, k, chunks),
+                         S::kXBytes, full(s));
+            };
+            // weights do not depend on the kernel before: the first of them are on their way while it still runs
+            const int64_t ahead = p.x_follows ? (count < S::kStages ? count : S::kStages) : 0;
+            for (int64_t i = 0; i < ahead; ++i) weights(i);
+            if (p.x_follows) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int64_t i = 0; i < ahead; ++i) activations(i);
+            int64_t i = ahead;
+            for (; i < count; ++i) {
+                if (i >= S::kStages && !bar_wait(empty(i % S::kStages), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
+                weights(i);
+                activations(i);
+            }
+            // no copy and no arrival may come after this CTA is gone
+            for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
+                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
+                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int64_t i = 0;
+            int segment = 0;
+            for (int64_t u = run.first; u < run.last; ++segment) {
+                const int64_t tile = u / chunks;
+                const int64_t end = (tile + 1) * chunks < run.last ? (tile + 1) * chunks : run.last;
+                const int b = segment % S::kBuffers;
+                if (segment >= S::kBuffers && !bar_wait(acc_empty(b), (uint32_t)(segment / S::kBuffers - 1) & 1u, &failed)) break;
+                tensor_fence_after();
+                bool first = true;
+                for (; u < end; ++u, ++i) {
+                    const int s = (int)(i % S::kStages);
+                    if (!bar_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+                    tensor_fence_after();
+                    const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
+                    const uint32_t sf = tmem + S::kScaleBase + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes + h * 512));
+                        copy_scales<1>(sfx + h * 4, scale_desc(x + h * 512));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t ins = mx4_instruction(128, TOKENS, (j & 1) * 2);
+#pragma unroll
+                        for (int w = 0; w < S::kWeights; ++w)
+                            mx4_multiply<1>(tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes + j * 32),
+                                            operand_desc(x + kMx4ScaleBytes + j * 32), ins, sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4,
+                                            first && j == 0 ? 0u : 1u);
+                    }
+                    first = false;
+                    tensor_commit(empty(s));
+                }
+                if (u < end) break;
+                tensor_commit(acc_full(b));
+            }
+            tensor_commit(drained);
+            bar_wait(drained, 0, &failed);
+        }
+    } else {
+        const int quarter = warp & 3;
+        uint32_t* counters = p.workspace + 4096 / 4;
+        float* partials = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.workspace) + kMx4PartialOffset);
+        int segment = 0;
+        for (int64_t u = run.first; u < run.last; ++segment) {
+            const int64_t tile = u / chunks, from = tile * chunks, to = from + chunks;
+            const int64_t end = to < run.last ? to : run.last;
+            const int b = segment % S::kBuffers;
+            const bool ok = bar_wait(acc_full(b), (uint32_t)(segment / S::kBuffers) & 1u, &failed);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            tensor_fence_after();
+            const int row_tile = (int)(tile / p.token_tiles);
+            const int64_t token0 = (tile % p.token_tiles) * TOKENS;
+            const uint32_t acc = tmem + b * S::kAcc + ((uint32_t)quarter << 21);
+            const bool whole = u == from && end == to;
+            constexpr int64_t kSlot = (int64_t)S::kAcc * 128;
+            float* mine = partials + (2 * (int64_t)blockIdx.x + (segment ? 1 : 0)) * kSlot + quarter * 32 + lane;
+            float v[16], up[16];
+#pragma unroll 1
+            for (int c = 0; c < TOKENS; c += 16) {
+                if (token0 + c >= p.tokens) break;
+                tmem_load16(acc + c, v);
+                if (GATED) tmem_load16(acc + TOKENS + c, up);
+                if (whole) {
+                    finish16<GATED>(p, row_tile, quarter, lane, token0 + c, v, up);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        __stcg(mine + (c + i) * 128, v[i]);
+                        if (GATED) __stcg(mine + (TOKENS + c + i) * 128, up[i]);
+                    }
+                }
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty(b));
+            if (!whole) {
+                // every warp's 32 features are counted by themselves, so that no barrier is needed
+                const int c0 = cta_of(units, from, gridDim.x), c1 = cta_of(units, to - 1, gridDim.x);
+                uint32_t before = 0u;
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) before = atomicAdd(&counters[c0 * 4 + quarter], 1u);
+                before = __shfl_sync(0xFFFFFFFFu, before, 0);
+                if (before == (uint32_t)(c1 - c0)) {
+                    __threadfence();
+                    if (lane == 0) counters[c0 * 4 + quarter] = 0u;
+                    // c0's part is its last segment, the others' their first; c0 has only one segment where its run begins inside the tile
+                    const int64_t at0 = 2 * (int64_t)c0 + (run_of(units, c0, gridDim.x).first / chunks == tile ? 0 : 1);
+#pragma unroll 1
+                    for (int c = 0; c < TOKENS; c += 16) {
+                        if (token0 + c >= p.tokens) break;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = up[i] = 0.f;
+                        for (int g = c0; g <= c1; ++g) {
+                            const float* from_g = partials + (g == c0 ? at0 : 2 * (int64_t)g) * kSlot + quarter * 32 + lane;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                v[i] += __ldcg(from_g + (c + i) * 128);
+                                if (GATED) up[i] += __ldcg(from_g + (TOKENS + c + i) * 128);
+                            }
+                        }
+                        finish16<GATED>(p, row_tile, quarter, lane, token0 + c, v, up);
+                    }
+                }
+            }
+            u = end;
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
+    if (warp == 1) tmem_free<1>(tmem, S::kColumns);
+}
+
+template <typename Kernel>
+static int launch_product(Kernel kernel, int smem, int threads, int ctas, const ProductArgs& p, cudaStream_t st) {
+    MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)ctas);
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = st;
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = p.x_follows ? 1 : 0;
+    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    return MPS_OK;
+}
+
+template <int TOKENS, bool GATED>
+static int launch_stream(ProductArgs p, int sms, cudaStream_t st) {
+    using S = StreamShape<TOKENS, GATED>;
+    p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
+    const int64_t units = (int64_t)p.row_tiles * p.token_tiles * p.chunks;
+    return launch_product(mx4_stream_kernel<TOKENS, GATED>, S::kSmem, kStreamThreads, (int)(units < sms ? units : sms), p, st);
+}
+
+static int sm_count(int* sms) {
+    int dev = 0;
+    MPS_CUDA_TRY(cudaGetDevice(&dev));
+    MPS_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+    if (*sms > kMx4MostSms) *sms = kMx4MostSms;
+    return MPS_OK;
+}
+
+}  // namespace mps
+
+using namespace mps;
+
+extern "C" {
+
+int64_t mps_mx4_workspace_bytes(void) { return kMx4WorkspaceBytes; }
+
+int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!args) { set_error("mps_mx4_product: null arguments"); return MPS_ERR_INVALID; }
+    const mps_mx4_linear& a = *args;
+    if (a.tokens < 0 || a.tokens > kMx4MostRows || a.rows <= 0 || a.rows > kMx4MostCols || a.cols <= 0 || a.cols > kMx4MostCols) {
+        set_error("mps_mx4_product: tokens must be in [0, %lld], rows and cols in [1, %lld]", (long long)kMx4MostRows, (long long)kMx4MostCols);
+        return MPS_ERR_INVALID;
+    }
+    if (a.out_dtype != MPS_BF16 && a.out_dtype != MPS_F16 && !(a.out_dtype == MPS_MX4 && a.w_up)) {
+        set_error("mps_mx4_product: the output is BF16 or F16, or MXFP4 where the product is gated");
+        return MPS_ERR_INVALID;
+    }
+    if (a.x_dtype != MPS_MX4 && !mx4_dtype_ok(a.x_dtype)) { set_error("mps_mx4_product: unknown dtype %d", (int)a.x_dtype); return MPS_ERR_INVALID; }
+    if (a.w_up && a.activation != MPS_SILU && a.activation != MPS_GELU_TANH) { set_error("mps_mx4_product: unknown activation %d", (int)a.activation); return MPS_ERR_INVALID; }
+    if (a.tokens == 0) return MPS_OK;
+    if (!workspace || workspace_bytes < kMx4WorkspaceBytes) { set_error("workspace missing or too small"); return MPS_ERR_WORKSPACE; }
+    const void* tiles = a.x_dtype == MPS_MX4 ? a.x : a.x_tiles;
+    if (!a.x || !tiles || !a.w || !a.out) { set_error("mps_mx4_product: null pointer"); return MPS_ERR_INVALID; }
+    if (((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.w_up) |
+          (a.out_dtype == MPS_MX4 ? reinterpret_cast<uintptr_t>(a.out) : 0)) & 15u) || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
+        set_error("mps_mx4_product: tiles must be 16-byte aligned, the workspace 256");
+        return MPS_ERR_INVALID;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int sms = 0, rc = sm_count(&sms);
+    if (rc) return rc;
+    if (a.x_dtype != MPS_MX4) {
+        rc = mps_mx4_quantize(a.x, a.x_dtype, a.tokens, a.cols, a.x_stride, a.x_tiles, stream);
+        if (rc) return rc;
+    }
+    ProductArgs p = {};
+    p.x = static_cast<const uint8_t*>(tiles);
+    p.w = static_cast<const uint8_t*>(a.w);
+    p.w_up = static_cast<const uint8_t*>(a.w_up);
+    p.out = a.out;
+    p.workspace = static_cast<uint32_t*>(workspace);
+    p.out_stride = a.out_stride;
+    p.tokens = a.tokens;
+    p.rows = (int32_t)a.rows;
+    p.chunks = (int32_t)mx4_chunks(a.cols);
+    p.row_tiles = (int32_t)mx4_row_tiles(a.rows);
+    p.out_dtype = a.out_dtype;
+    p.activation = a.activation;
+    p.x_follows = a.x_dtype != MPS_MX4;
+    if (a.w_up) {
+        if (a.tokens <= 16) return launch_stream<16, true>(p, sms, st);
+        if (a.tokens <= 32) return launch_stream<32, true>(p, sms, st);
+        if (a.tokens <= 64) return launch_stream<64, true>(p, sms, st);
+        return launch_stream<128, true>(p, sms, st);
+    }
+    if (a.tokens <= 16) return launch_stream<16, false>(p, sms, st);
+    if (a.tokens <= 32) return launch_stream<32, false>(p, sms, st);
+    if (a.tokens <= 64) return launch_stream<64, false>(p, sms, st);
+    return launch_stream<128, false>(p, sms, st);
+}
+
+int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out) {
+    if (!timed_out || !workspace || workspace_bytes < kMx4WorkspaceBytes) { set_error("mps_mx4_status: bad argument"); return MPS_ERR_INVALID; }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    uint32_t flag = 0;
+    MPS_CUDA_TRY(cudaMemcpyAsync(&flag, workspace, sizeof(flag), cudaMemcpyDeviceToHost, st));
+    MPS_CUDA_TRY(cudaStreamSynchronize(st));
+    if (flag) MPS_CUDA_TRY(cudaMemsetAsync(workspace, 0, (size_t)kMx4PartialOffset, st));
+    *timed_out = flag ? 1 : 0;
+    return MPS_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,77 @@
+// The tensor-core side of the MXFP4 products: descriptors, scale copies, block-scaled multiplications and accumulator reads.
+#pragma once
+
+#include <stdint.h>
+
+namespace mps {
+
+// Shared-memory operand: rows of 128 bytes, 8-row groups of 1024 bytes one after the other, 16-byte pieces XORed with the row
+// (the 128-byte swizzle), columns innermost.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t smem) {
+    return (uint64_t)((smem >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 512 bytes of scales, 32 rows of 16 bytes, not swizzled.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem) {
+    return (uint64_t)((smem >> 4) & 0x3FFFu) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// E2M1 x E2M1, E8M0 scales, FP32 accumulator of m x n; `sf` says which two of a scale word's four blocks a step of 64 columns uses.
+__device__ __forceinline__ uint32_t mx4_instruction(uint32_t m, uint32_t n, uint32_t sf) {
+    return sf << 4 | 1u << 7 | 1u << 10 | (n >> 3) << 17 | 1u << 23 | (m >> 7) << 27 | sf << 29;
+}
+
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, uint32_t columns) {
+    if (CTAS == 1) asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(columns) : "memory");
+    else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(columns) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+    if (CTAS == 1) {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    } else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+    }
+}
+// 128 rows' scales of 128 columns into four columns of tensor memory, the same in each of its four lane quarters.
+template <int CTAS>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+    if (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void mx4_multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t sfa, uint32_t sfb, uint32_t add) {
+    if (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add) : "memory");
+}
+// The barrier gets an arrival when everything this thread has issued to the tensor core is done.
+__device__ __forceinline__ void tensor_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Sixteen columns of the accumulator, a lane of tensor memory per thread; the whole warp takes part.  Load and wait are one
+// statement: the compiler knows nothing of the wait and might use a register before it.
+__device__ __forceinline__ void tmem_load16(uint32_t tmem, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem) : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+}  // namespace mps
