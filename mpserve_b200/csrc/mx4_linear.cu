@@ -247,6 +247,7 @@ mx4_stream_kernel(const ProductArgs p) {
             const int b = segment % S::kBuffers;
             const bool ok = bar_wait(acc_full(b), (uint32_t)(segment / S::kBuffers) & 1u, &failed);
             if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            __syncwarp();
             tensor_fence_after();
             const int row_tile = (int)(tile / p.token_tiles);
             const int64_t token0 = (tile % p.token_tiles) * TOKENS;
@@ -258,6 +259,7 @@ mx4_stream_kernel(const ProductArgs p) {
 #pragma unroll 1
             for (int c = 0; c < TOKENS; c += 16) {
                 if (token0 + c >= p.tokens) break;
+                __syncwarp();
                 tmem_load16(acc + c, v);
                 if (GATED) tmem_load16(acc + TOKENS + c, up);
                 if (whole) {
@@ -306,6 +308,7 @@ mx4_stream_kernel(const ProductArgs p) {
             u = end;
         }
     }
+    __syncwarp();
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
@@ -313,8 +316,244 @@ mx4_stream_kernel(const ProductArgs p) {
     if (warp == 1) tmem_free<1>(tmem, S::kColumns);
 }
 
-template <typename Kernel>
-static int launch_product(Kernel kernel, int smem, int threads, int ctas, const ProductArgs& p, cudaStream_t st) {
+// ---- many tokens: tokens on the accumulator's lanes ------------------------------------------------
+//
+// A pair of CTAs on neighbouring SMs works on 256 tokens x 256 features (with a gate: 128 features of both weights): each holds
+// 128 tokens and half of the features in shared memory, and one instruction multiplies what both hold, so that a byte of shared memory
+// feeds twice the work that it would feed one CTA.  A thread of the epilogue has one token and neighbouring features in its
+// registers: an MXFP4 block needs no exchange with other threads, and rows go out in whole sectors.  The accumulator takes all
+// but the scales' columns of the tensor memory, so it is read into registers as a whole (some 300 cycles) and multiplied into again
+// while it is converted and stored.
+//
+// Warps: 0 copies, 1 multiplies (first CTA) or hands on the arrival of the copies (second), 2 to 9 take the accumulator over, two
+// on each quarter of the lanes, one on each half of the columns.
+struct WideShape {
+    static constexpr int kCodes = kMx4Rows * kMx4RowBytes;
+    static constexpr int kWeightScales = kMx4TileBytes;                     // of a stage: tokens, weights' scales, weights' codes
+    static constexpr int kWeightCodes = kWeightScales + 2 * kMx4ScaleBytes;
+    static constexpr int kStageBytes = kWeightCodes + kCodes;
+    static constexpr int kStages = 6;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;
+    static_assert(kScaleBase + kStages * kScaleColumns <= kColumns, "tensor memory");
+    static_assert(kStageBytes % 1024 == 0 && kWeightCodes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
+    static_assert(kSmem + 1024 <= kMx4SmemMost, "shared memory");
+};
+constexpr int kWideThreads = 320;
+
+struct WideTile { int token, feature; };      // in units of a pair's tile
+__device__ __forceinline__ WideTile wide_tile(int64_t tile, int token_tiles) {
+    return {(int)(tile % token_tiles), (int)(tile / token_tiles)};
+}
+
+// 32 neighbouring values of one token, as a block.
+__device__ __forceinline__ uint4 block_codes(const float* v, uint32_t& byte) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    byte = mx4_scale_byte(m);
+    const float inverse = mx4_inverse_scale(byte);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = byte == 255u ? 0.f : v[j * 8 + i] * inverse;
+        w[j] = mx4_codes8(q);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// `count` (a multiple of 8) neighbouring 16-bit values of a row, packed in pairs; only the first `valid` belong to it.
+template <int COUNT>
+__device__ __forceinline__ void store_row(uint16_t* out, const uint32_t (&w)[COUNT / 2], int valid, int align) {
+    if (valid >= COUNT && align >= 16) {
+#pragma unroll
+        for (int i = 0; i < COUNT / 8; ++i) *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) if (i < valid) out[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+}
+
+template <bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
+mx4_wide_kernel(const ProductArgs p, const int align) {
+    using S = WideShape;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[3 * S::kStages + 3];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(bars);
+    const auto full = [&](int s) { return bar0 + 8u * s; };                       // this CTA's copies have come
+    const auto both = [&](int s) { return bar0 + 8u * (S::kStages + s); };       // (first CTA) the second's too
+    const auto empty = [&](int s) { return bar0 + 8u * (2 * S::kStages + s); };
+    const uint32_t acc_full = bar0 + 8u * (3 * S::kStages), acc_empty = acc_full + 8u, drained = acc_full + 16u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(both(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 16);
+        mbar_init(drained, 1);
+        failed = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<2>(smem_u32(&tmem_slot), S::kColumns);
+    tensor_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tensor_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    const int chunks = p.chunks, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int feature_tiles = GATED ? p.row_tiles : (p.row_tiles + 1) / 2;
+    const int64_t tiles = (int64_t)p.token_tiles * feature_tiles;
+    const int last_token_tile = (int)((p.tokens - 1) / kMx4Rows);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int64_t i = 0;
+            bool ok = true;
+            if (p.x_follows) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
+                const WideTile t = wide_tile(tile, p.token_tiles);
+                // what lies beyond the last tile of 128 is multiplied as the last and not stored
+                const uint8_t* x = p.x + mx4_tile_offset(min(2 * t.token + rank, last_token_tile), 0, chunks);
+                const uint8_t* w0 = GATED ? p.w + mx4_tile_offset(t.feature, 0, chunks) : p.w + mx4_tile_offset(2 * t.feature, 0, chunks);
+                const uint8_t* w1 = GATED ? p.w_up + mx4_tile_offset(t.feature, 0, chunks)
+                                          : p.w + mx4_tile_offset(min(2 * t.feature + 1, p.row_tiles - 1), 0, chunks);
+                for (int k = 0; k < chunks; ++k, ++i) {
+                    const int s = (int)(i % S::kStages);
+                    if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) { ok = false; break; }
+                    const uint32_t to = ring + s * S::kStageBytes;
+                    const int64_t at = (int64_t)k * kMx4TileBytes;
+                    mbar_expect_tx(full(s), S::kStageBytes);
+                    bulk_g2s(to, x + at, kMx4TileBytes, full(s));
+                    bulk_g2s(to + S::kWeightScales, w0 + at, kMx4ScaleBytes, full(s));
+                    bulk_g2s(to + S::kWeightScales + kMx4ScaleBytes, w1 + at, kMx4ScaleBytes, full(s));
+                    bulk_g2s(to + S::kWeightCodes, (rank ? w1 : w0) + at + kMx4ScaleBytes, S::kCodes, full(s));
+                }
+            }
+            for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
+                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
+                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 1) {
+            int64_t units = 0;
+            for (int64_t tile = pair; tile < tiles; tile += pairs) units += chunks;
+            for (int64_t i = 0; i < units; ++i) {
+                if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+                arrive_at_first(both(i % S::kStages));
+            }
+            bar_wait(drained, 0, &failed);
+        } else if (lane == 0) {
+            int64_t i = 0;
+            uint32_t round = 0;
+            bool ok = true;
+            for (int64_t tile = pair; tile < tiles && ok; tile += pairs, ++round) {
+                if (round && !bar_wait(acc_empty, (round - 1) & 1u, &failed)) break;
+                tensor_fence_after();
+                for (int k = 0; k < chunks; ++k, ++i) {
+                    const int s = (int)(i % S::kStages);
+                    const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
+                    if (!bar_wait(full(s), parity, &failed) || !bar_wait(both(s), parity, &failed)) { ok = false; break; }
+                    tensor_fence_after();
+                    const uint32_t stage = ring + s * S::kStageBytes;
+                    const uint32_t sfx = tmem + S::kScaleBase + s * S::kScaleColumns, sfw = sfx + 8;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        copy_scales<2>(sfx + h * 4, scale_desc(stage + h * 512));
+                        copy_scales<2>(sfw + h * 8, scale_desc(stage + S::kWeightScales + h * 512));
+                        copy_scales<2>(sfw + h * 8 + 4, scale_desc(stage + S::kWeightScales + kMx4ScaleBytes + h * 512));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mx4_multiply<2>(tmem, operand_desc(stage + kMx4ScaleBytes + j * 32), operand_desc(stage + S::kWeightCodes + j * 32),
+                                        mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4, sfw + (j >> 1) * 8, k || j ? 1u : 0u);
+                    tensor_commit_pair(empty(s));
+                }
+                if (ok) tensor_commit_pair(acc_full);
+            }
+            tensor_commit_pair(drained);
+            bar_wait(drained, 0, &failed);
+        }
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        uint32_t round = 0;
+        for (int64_t tile = pair; tile < tiles; tile += pairs, ++round) {
+            const bool ok = bar_wait(acc_full, round & 1u, &failed);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            __syncwarp();
+            tensor_fence_after();
+            const WideTile t = wide_tile(tile, p.token_tiles);
+            const int64_t token = ((int64_t)2 * t.token + rank) * kMx4Rows + quarter * 32 + lane;
+            const uint32_t acc = tmem + ((uint32_t)quarter << 21);
+            const auto release = [&] {
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_at_first(acc_empty);
+            };
+            if (GATED) {
+                float g[64], u[64];
+#pragma unroll
+                for (int c = 0; c < 64; c += 32) {
+                    tmem_load32(acc + half * 64 + c, g + c);
+                    tmem_load32(acc + 128 + half * 64 + c, u + c);
+                }
+                release();
+                const int first = t.feature * kMx4Rows + half * 64, valid = p.rows - first;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) g[i] = i < valid ? act(g[i], p.activation) * u[i] : 0.f;
+                if (token >= p.tokens) continue;
+                if (p.out_dtype == MPS_MX4) {
+                    const int out_chunks = (int)mx4_chunks(p.rows), row = (int)(token % kMx4Rows), part = t.feature & 1;
+                    uint8_t* to = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, t.feature >> 1, out_chunks);
+                    uint32_t b0, b1;
+                    *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2)) = block_codes(g, b0);
+                    *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2 + 1)) = block_codes(g + 32, b1);
+                    *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, part) + half * 2) = (uint16_t)(b0 | b1 << 8);
+                    if (t.feature == p.row_tiles - 1 && part == 0) {      // fill up the last tile
+                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 4 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 5 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, 1) + half * 2) = 0;
+                    }
+                } else {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] = pack2(g[2 * i], g[2 * i + 1], p.out_dtype);
+                    store_row<64>(static_cast<uint16_t*>(p.out) + token * p.out_stride + first, w, valid, align);
+                }
+            } else {
+                uint32_t w[64];
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    float v[32];
+                    tmem_load32(acc + half * 128 + c, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[c / 2 + i] = pack2(v[2 * i], v[2 * i + 1], p.out_dtype);
+                }
+                release();
+                const int first = t.feature * 256 + half * 128;
+                if (token < p.tokens) store_row<128>(static_cast<uint16_t*>(p.out) + token * p.out_stride + first, w, p.rows - first, align);
+            }
+        }
+    }
+    __syncwarp();
+    tensor_fence_before();
+    __syncthreads();
+    cluster_sync();      // what the pair's instructions read and write is there until both are done
+    tensor_fence_after();
+    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
+    if (warp == 1) tmem_free<2>(tmem, S::kColumns);
+}
+
+template <typename Kernel, typename... More>
+static int launch_product(Kernel kernel, int smem, int threads, int ctas, cudaStream_t st, const ProductArgs& p, More... more) {
     MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)ctas);
@@ -326,7 +565,7 @@ static int launch_product(Kernel kernel, int smem, int threads, int ctas, const 
     overlap.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &overlap;
     config.numAttrs = p.x_follows ? 1 : 0;
-    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p, more...));
     return MPS_OK;
 }
 
@@ -335,8 +574,18 @@ static int launch_stream(ProductArgs p, int sms, cudaStream_t st) {
     using S = StreamShape<TOKENS, GATED>;
     p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
     const int64_t units = (int64_t)p.row_tiles * p.token_tiles * p.chunks;
-    return launch_product(mx4_stream_kernel<TOKENS, GATED>, S::kSmem, kStreamThreads, (int)(units < sms ? units : sms), p, st);
+    return launch_product(mx4_stream_kernel<TOKENS, GATED>, S::kSmem, kStreamThreads, (int)(units < sms ? units : sms), st, p);
 }
+
+template <bool GATED>
+static int launch_wide(ProductArgs p, int sms, cudaStream_t st) {
+    p.token_tiles = (int)((p.tokens + 255) / 256);
+    const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
+    const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+    const bool even = p.out_dtype != MPS_MX4 && p.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    return launch_product(mx4_wide_kernel<GATED>, WideShape::kSmem, kWideThreads, 2 * pairs, st, p, even ? 16 : 2);
+}
+
 
 static int sm_count(int* sms) {
     int dev = 0;
@@ -397,6 +646,7 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     p.out_dtype = a.out_dtype;
     p.activation = a.activation;
     p.x_follows = a.x_dtype != MPS_MX4;
+    if (a.tokens > 128) return a.w_up ? launch_wide<true>(p, sms, st) : launch_wide<false>(p, sms, st);
     if (a.w_up) {
         if (a.tokens <= 16) return launch_stream<16, true>(p, sms, st);
         if (a.tokens <= 32) return launch_stream<32, true>(p, sms, st);
