@@ -50,6 +50,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     return false;
 }
 
+// The same for a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, failed));
+}
+
 // ---- few tokens: weights on the accumulator's lanes -------------------------------------------------
 //
 // One CTA per SM streams weight tiles through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
@@ -154,7 +159,7 @@ mx4_stream_kernel(const ProductArgs p) {
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
     const int chunks = p.chunks;
     const int64_t units = (int64_t)p.row_tiles * p.token_tiles * chunks;
@@ -196,46 +201,48 @@ mx4_stream_kernel(const ProductArgs p) {
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            int64_t i = 0;
-            int segment = 0;
-            for (int64_t u = run.first; u < run.last; ++segment) {
-                const int64_t tile = u / chunks;
-                const int64_t end = (tile + 1) * chunks < run.last ? (tile + 1) * chunks : run.last;
-                const int b = segment % S::kBuffers;
-                if (segment >= S::kBuffers && !bar_wait(acc_empty(b), (uint32_t)(segment / S::kBuffers - 1) & 1u, &failed)) break;
+        int s = 0, segment = 0;
+        uint32_t parity = 0;
+        for (int64_t u = run.first; u < run.last; ++segment) {
+            const int64_t tile = u / chunks;
+            const int64_t end = (tile + 1) * chunks < run.last ? (tile + 1) * chunks : run.last;
+            const int b = segment % S::kBuffers;
+            if (segment >= S::kBuffers && !warp_wait(acc_empty(b), (uint32_t)(segment / S::kBuffers - 1) & 1u, &failed)) break;
+            tensor_fence_after();
+            uint32_t add = 0u;
+            for (; u < end; ++u) {
+                if (!warp_wait(full(s), parity, &failed)) break;
                 tensor_fence_after();
-                bool first = true;
-                for (; u < end; ++u, ++i) {
-                    const int s = (int)(i % S::kStages);
-                    if (!bar_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
-                    tensor_fence_after();
-                    const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
-                    const uint32_t sf = tmem + S::kScaleBase + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
+                const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
+                const uint32_t sf = tmem + S::kScaleBase + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
+                if (elect_one()) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes + h * 512));
-                        copy_scales<1>(sfx + h * 4, scale_desc(x + h * 512));
+                        for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes) + 32 * h);
+                        copy_scales<1>(sfx + h * 4, scale_desc(x) + 32 * h);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t ins = mx4_instruction(128, TOKENS, (j & 1) * 2);
 #pragma unroll
                         for (int w = 0; w < S::kWeights; ++w)
-                            mx4_multiply<1>(tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes + j * 32),
-                                            operand_desc(x + kMx4ScaleBytes + j * 32), ins, sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4,
-                                            first && j == 0 ? 0u : 1u);
+                            mx4_multiply<1>(tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes) + 2 * j,
+                                            operand_desc(x + kMx4ScaleBytes) + 2 * j, mx4_instruction(128, TOKENS, (j & 1) * 2),
+                                            sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4, j ? 1u : add);
                     }
-                    first = false;
                     tensor_commit(empty(s));
                 }
-                if (u < end) break;
-                tensor_commit(acc_full(b));
+                __syncwarp();
+                add = 1u;
+                if (++s == S::kStages) { s = 0; parity ^= 1u; }
             }
-            tensor_commit(drained);
-            bar_wait(drained, 0, &failed);
+            if (u < end) break;
+            if (elect_one()) tensor_commit(acc_full(b));
+            __syncwarp();
         }
+        if (elect_one()) tensor_commit(drained);
+        __syncwarp();
+        warp_wait(drained, 0, &failed);
     } else {
         const int quarter = warp & 3;
         uint32_t* counters = p.workspace + 4096 / 4;
@@ -245,8 +252,7 @@ mx4_stream_kernel(const ProductArgs p) {
             const int64_t tile = u / chunks, from = tile * chunks, to = from + chunks;
             const int64_t end = to < run.last ? to : run.last;
             const int b = segment % S::kBuffers;
-            const bool ok = bar_wait(acc_full(b), (uint32_t)(segment / S::kBuffers) & 1u, &failed);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (!warp_wait(acc_full(b), (uint32_t)(segment / S::kBuffers) & 1u, &failed)) break;
             __syncwarp();
             tensor_fence_after();
             const int row_tile = (int)(tile / p.token_tiles);
@@ -329,13 +335,15 @@ mx4_stream_kernel(const ProductArgs p) {
 // on each quarter of the lanes, one on each half of the columns.
 struct WideShape {
     static constexpr int kCodes = kMx4Rows * kMx4RowBytes;
-    static constexpr int kWeightScales = kMx4TileBytes;                     // of a stage: tokens, weights' scales, weights' codes
-    static constexpr int kWeightCodes = kWeightScales + 2 * kMx4ScaleBytes;
-    static constexpr int kStageBytes = kWeightCodes + kCodes;
-    static constexpr int kStages = 6;
+    static constexpr int kTiles = 2;                                        // tiles along the columns that a stage holds at most
+    // of a stage: token tiles, scales of the weights' two halves, codes of this CTA's half
+    static constexpr int kWeightScales = kTiles * kMx4TileBytes;
+    static constexpr int kWeightCodes = kWeightScales + kTiles * 2 * kMx4ScaleBytes;
+    static constexpr int kStageBytes = kWeightCodes + kTiles * kCodes;
+    static constexpr int kStages = 3;
     static constexpr int kSmem = kStages * kStageBytes + 1024;
-    static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;
-    static_assert(kScaleBase + kStages * kScaleColumns <= kColumns, "tensor memory");
+    static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;   // scale columns of a tile
+    static_assert(kScaleBase + kStages * kTiles * kScaleColumns <= kColumns, "tensor memory");
     static_assert(kStageBytes % 1024 == 0 && kWeightCodes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
     static_assert(kSmem + 1024 <= kMx4SmemMost, "shared memory");
 };
@@ -406,7 +414,7 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
     __syncthreads();
     cluster_sync();
     tensor_fence_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
     const int chunks = p.chunks, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int feature_tiles = GATED ? p.row_tiles : (p.row_tiles + 1) / 2;
@@ -425,16 +433,19 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
                 const uint8_t* w0 = GATED ? p.w + mx4_tile_offset(t.feature, 0, chunks) : p.w + mx4_tile_offset(2 * t.feature, 0, chunks);
                 const uint8_t* w1 = GATED ? p.w_up + mx4_tile_offset(t.feature, 0, chunks)
                                           : p.w + mx4_tile_offset(min(2 * t.feature + 1, p.row_tiles - 1), 0, chunks);
-                for (int k = 0; k < chunks; ++k, ++i) {
-                    const int s = (int)(i % S::kStages);
+                for (int k = 0; k < chunks; k += S::kTiles, ++i) {
+                    const int s = (int)(i % S::kStages), n = min(S::kTiles, chunks - k);
                     if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) { ok = false; break; }
                     const uint32_t to = ring + s * S::kStageBytes;
                     const int64_t at = (int64_t)k * kMx4TileBytes;
-                    mbar_expect_tx(full(s), S::kStageBytes);
-                    bulk_g2s(to, x + at, kMx4TileBytes, full(s));
-                    bulk_g2s(to + S::kWeightScales, w0 + at, kMx4ScaleBytes, full(s));
-                    bulk_g2s(to + S::kWeightScales + kMx4ScaleBytes, w1 + at, kMx4ScaleBytes, full(s));
-                    bulk_g2s(to + S::kWeightCodes, (rank ? w1 : w0) + at + kMx4ScaleBytes, S::kCodes, full(s));
+                    mbar_expect_tx(full(s), n * (S::kStageBytes / S::kTiles));
+                    bulk_g2s(to, x + at, n * kMx4TileBytes, full(s));
+                    for (int q = 0; q < n; ++q) {
+                        const int64_t from = at + q * kMx4TileBytes;
+                        bulk_g2s(to + S::kWeightScales + 2 * q * kMx4ScaleBytes, w0 + from, kMx4ScaleBytes, full(s));
+                        bulk_g2s(to + S::kWeightScales + (2 * q + 1) * kMx4ScaleBytes, w1 + from, kMx4ScaleBytes, full(s));
+                        bulk_g2s(to + S::kWeightCodes + q * S::kCodes, (rank ? w1 : w0) + from + kMx4ScaleBytes, S::kCodes, full(s));
+                    }
                 }
             }
             for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
@@ -443,51 +454,85 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 1) {
+        if (rank == 1) {
             int64_t units = 0;
-            for (int64_t tile = pair; tile < tiles; tile += pairs) units += chunks;
-            for (int64_t i = 0; i < units; ++i) {
-                if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
-                arrive_at_first(both(i % S::kStages));
+            for (int64_t tile = pair; tile < tiles; tile += pairs) units += (chunks + S::kTiles - 1) / S::kTiles;
+            if (lane == 0) {
+                for (int64_t i = 0; i < units; ++i) {
+                    if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+                    arrive_at_first(both(i % S::kStages));
+                }
+                bar_wait(drained, 0, &failed);
             }
-            bar_wait(drained, 0, &failed);
-        } else if (lane == 0) {
-            int64_t i = 0;
-            uint32_t round = 0;
+        } else {
+            // The scales of a stage are copied before the multiplications of the stage before are issued: the tensor core runs in
+            // order, and a multiplication would wait for scales that were copied just before it.
+            int s = 0;
+            uint32_t parity = 0, round = 0;
             bool ok = true;
-            for (int64_t tile = pair; tile < tiles && ok; tile += pairs, ++round) {
-                if (round && !bar_wait(acc_empty, (round - 1) & 1u, &failed)) break;
+            int behind = -1, behind_tiles = 0;       // the stage whose multiplications are still to be issued
+            bool behind_first = false, behind_last = false;
+            const auto multiply = [&]() -> bool {
+                if (behind_first && round && !warp_wait(acc_empty, (round - 1) & 1u, &failed)) return false;
                 tensor_fence_after();
-                for (int k = 0; k < chunks; ++k, ++i) {
-                    const int s = (int)(i % S::kStages);
-                    const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
-                    if (!bar_wait(full(s), parity, &failed) || !bar_wait(both(s), parity, &failed)) { ok = false; break; }
+                const uint32_t stage = ring + behind * S::kStageBytes;
+                for (int q = 0; q < behind_tiles; ++q) {
+                    const uint32_t sfx = tmem + S::kScaleBase + (behind * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
+                    const uint64_t a = operand_desc(stage + q * kMx4TileBytes + kMx4ScaleBytes), b = operand_desc(stage + S::kWeightCodes + q * S::kCodes);
+                    const uint32_t add = behind_first && !q ? 0u : 1u;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)      // 32 bytes on: two in the descriptors' unit
+                            mx4_multiply<2>(tmem, a + 2 * j, b + 2 * j, mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4,
+                                            sfw + (j >> 1) * 8, j ? 1u : add);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) {
+                    tensor_commit_pair(empty(behind));
+                    if (behind_last) tensor_commit_pair(acc_full);
+                }
+                __syncwarp();
+                if (behind_last) ++round;
+                return true;
+            };
+            for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
+                for (int k = 0; k < chunks; k += S::kTiles) {
+                    const int n = min(S::kTiles, chunks - k);
+                    if (!warp_wait(full(s), parity, &failed) || !warp_wait(both(s), parity, &failed)) { ok = false; break; }
                     tensor_fence_after();
                     const uint32_t stage = ring + s * S::kStageBytes;
-                    const uint32_t sfx = tmem + S::kScaleBase + s * S::kScaleColumns, sfw = sfx + 8;
+                    for (int q = 0; q < n; ++q) {
+                        const uint32_t sfx = tmem + S::kScaleBase + (s * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
+                        const uint64_t x = scale_desc(stage + q * kMx4TileBytes), w = scale_desc(stage + S::kWeightScales + 2 * q * kMx4ScaleBytes);
+                        if (elect_one()) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        copy_scales<2>(sfx + h * 4, scale_desc(stage + h * 512));
-                        copy_scales<2>(sfw + h * 8, scale_desc(stage + S::kWeightScales + h * 512));
-                        copy_scales<2>(sfw + h * 8 + 4, scale_desc(stage + S::kWeightScales + kMx4ScaleBytes + h * 512));
+                            for (int h = 0; h < 2; ++h) {      // 512 bytes on: 32 in the descriptors' unit
+                                copy_scales<2>(sfx + h * 4, x + 32 * h);
+                                copy_scales<2>(sfw + h * 8, w + 32 * h);
+                                copy_scales<2>(sfw + h * 8 + 4, w + 64 + 32 * h);
+                            }
+                        }
+                        __syncwarp();
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mx4_multiply<2>(tmem, operand_desc(stage + kMx4ScaleBytes + j * 32), operand_desc(stage + S::kWeightCodes + j * 32),
-                                        mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4, sfw + (j >> 1) * 8, k || j ? 1u : 0u);
-                    tensor_commit_pair(empty(s));
+                    if (behind >= 0 && !multiply()) { ok = false; break; }
+                    behind = s;
+                    behind_tiles = n;
+                    behind_first = k == 0;
+                    behind_last = k + n == chunks;
+                    if (++s == S::kStages) { s = 0; parity ^= 1u; }
                 }
-                if (ok) tensor_commit_pair(acc_full);
             }
-            tensor_commit_pair(drained);
-            bar_wait(drained, 0, &failed);
+            if (ok && behind >= 0) multiply();
+            if (elect_one()) tensor_commit_pair(drained);
+            __syncwarp();
+            warp_wait(drained, 0, &failed);
         }
     } else {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         uint32_t round = 0;
         for (int64_t tile = pair; tile < tiles; tile += pairs, ++round) {
-            const bool ok = bar_wait(acc_full, round & 1u, &failed);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (!warp_wait(acc_full, round & 1u, &failed)) break;
             __syncwarp();
             tensor_fence_after();
             const WideTile t = wide_tile(tile, p.token_tiles);

@@ -74,10 +74,18 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
+        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// One lane of a converged warp.  What issues to the tensor core runs as a whole warp with this around each instruction: addresses
+// and descriptors are then the same in all lanes and stay in uniform registers, where the instructions take them from.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 // Sixteen columns of the accumulator, a lane of tensor memory per thread; the whole warp takes part.  Load and wait are one
