@@ -33,10 +33,11 @@ struct ProductArgs {
     bool x_follows;          // x is written by the kernel before, which this one may overlap
 };
 
+// Both activations are g / (1 + exp(-t)): SiLU with t = g, and GELU's tanh form since (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)).  The
+// exponential is CUDA's accurate one; the quotient's two units in the last place are far below what the result is rounded to.
 __device__ __forceinline__ float act(float g, int which) {
-    // exp and tanh as CUDA's accurate functions: the epilogue is a small part of a product
-    if (which == MPS_SILU) return g / (1.f + expf(-g));
-    return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
+    const float t = which == MPS_SILU ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.f);
+    return __fdividef(g, 1.f + expf(-t));
 }
 
 // A wait that gives up when another one has.
@@ -159,7 +160,7 @@ mx4_stream_kernel(const ProductArgs p) {
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    constexpr uint32_t tmem = 0;       // all columns were asked for: the allocation begins at the first
 
     const int chunks = p.chunks;
     const int64_t units = (int64_t)p.row_tiles * p.token_tiles * chunks;
@@ -201,6 +202,7 @@ mx4_stream_kernel(const ProductArgs p) {
             }
         }
     } else if (warp == 1) {
+        const uint32_t lead = elect_one();
         int s = 0, segment = 0;
         uint32_t parity = 0;
         for (int64_t u = run.first; u < run.last; ++segment) {
@@ -215,33 +217,28 @@ mx4_stream_kernel(const ProductArgs p) {
                 tensor_fence_after();
                 const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
                 const uint32_t sf = tmem + S::kScaleBase + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
-                if (elect_one()) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes) + 32 * h);
-                        copy_scales<1>(sfx + h * 4, scale_desc(x) + 32 * h);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                        for (int w = 0; w < S::kWeights; ++w)
-                            mx4_multiply<1>(tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes) + 2 * j,
-                                            operand_desc(x + kMx4ScaleBytes) + 2 * j, mx4_instruction(128, TOKENS, (j & 1) * 2),
-                                            sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4, j ? 1u : add);
-                    }
-                    tensor_commit(empty(s));
+                    for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(lead, sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes) + 32 * h);
+                    copy_scales<1>(lead, sfx + h * 4, scale_desc(x) + 32 * h);
                 }
-                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {      // 32 bytes on: two in the descriptors' unit
+#pragma unroll
+                    for (int w = 0; w < S::kWeights; ++w)
+                        mx4_multiply<1>(lead, tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes) + 2 * j,
+                                        operand_desc(x + kMx4ScaleBytes) + 2 * j, mx4_instruction(128, TOKENS, (j & 1) * 2),
+                                        sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4, j ? 1u : add);
+                }
+                tensor_commit(lead, empty(s));
                 add = 1u;
                 if (++s == S::kStages) { s = 0; parity ^= 1u; }
             }
             if (u < end) break;
-            if (elect_one()) tensor_commit(acc_full(b));
-            __syncwarp();
+            tensor_commit(lead, acc_full(b));
         }
-        if (elect_one()) tensor_commit(drained);
-        __syncwarp();
+        tensor_commit(lead, drained);
         warp_wait(drained, 0, &failed);
     } else {
         const int quarter = warp & 3;
@@ -319,7 +316,7 @@ mx4_stream_kernel(const ProductArgs p) {
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
-    if (warp == 1) tmem_free<1>(tmem, S::kColumns);
+    if (warp == 1) tmem_free<1>(tmem_slot, S::kColumns);
 }
 
 // ---- many tokens: tokens on the accumulator's lanes ------------------------------------------------
@@ -335,13 +332,14 @@ mx4_stream_kernel(const ProductArgs p) {
 // on each quarter of the lanes, one on each half of the columns.
 struct WideShape {
     static constexpr int kCodes = kMx4Rows * kMx4RowBytes;
-    static constexpr int kTiles = 2;                                        // tiles along the columns that a stage holds at most
+    static constexpr int kTiles = 1;                                        // tiles along the columns that a stage holds at most
     // of a stage: token tiles, scales of the weights' two halves, codes of this CTA's half
     static constexpr int kWeightScales = kTiles * kMx4TileBytes;
     static constexpr int kWeightCodes = kWeightScales + kTiles * 2 * kMx4ScaleBytes;
     static constexpr int kStageBytes = kWeightCodes + kTiles * kCodes;
-    static constexpr int kStages = 3;
-    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr int kStages = 5 / kTiles;
+    static constexpr int kStageRows = kStages * kStageBytes;                // eight warps' rows on their way out
+    static constexpr int kSmem = kStageRows + 8 * 4096 + 1024;
     static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;   // scale columns of a tile
     static_assert(kScaleBase + kStages * kTiles * kScaleColumns <= kColumns, "tensor memory");
     static_assert(kStageBytes % 1024 == 0 && kWeightCodes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
@@ -372,37 +370,53 @@ __device__ __forceinline__ uint4 block_codes(const float* v, uint32_t& byte) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// `count` (a multiple of 8) neighbouring 16-bit values of a row, packed in pairs; only the first `valid` belong to it.
-template <int COUNT>
-__device__ __forceinline__ void store_row(uint16_t* out, const uint32_t (&w)[COUNT / 2], int valid, int align) {
-    if (valid >= COUNT && align >= 16) {
+// A warp's 32 tokens x 64 features, a token per lane, go out by way of 4 KB of shared memory: written straight from the registers every
+// instruction would touch 32 rows with 16 bytes each.  `w`: 64 values in pairs; rows below `tokens`, columns below `valid` are stored.
+__device__ __forceinline__ void store_rows(uint32_t buffer, int lane, const uint32_t* w, uint16_t* out, int64_t stride, int64_t tokens, int valid,
+                                           bool even) {
+    __syncwarp();
 #pragma unroll
-        for (int i = 0; i < COUNT / 8; ++i) *reinterpret_cast<uint4*>(out + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        return;
+    for (int c = 0; c < 8; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]), "r"(w[4 * c + 1]),
+                     "r"(w[4 * c + 2]), "r"(w[4 * c + 3]) : "memory");
+    __syncwarp();
+    if (even && valid >= 64) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3), c = lane & 7;
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(buffer + row * 128 + ((c ^ (row & 7)) << 4)));
+            if (row < tokens) *reinterpret_cast<uint4*>(out + row * stride + c * 8) = v;
+        }
+    } else {
+        const int rows = tokens < 32 ? (int)tokens : 32;
+        for (int row = 0; row < rows; ++row) {
+            uint32_t v;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buffer + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4));
+            if (2 * lane < valid) out[row * stride + 2 * lane] = (uint16_t)v;
+            if (2 * lane + 1 < valid) out[row * stride + 2 * lane + 1] = (uint16_t)(v >> 16);
+        }
     }
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) if (i < valid) out[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
 }
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
-mx4_wide_kernel(const ProductArgs p, const int align) {
+mx4_wide_kernel(const ProductArgs p, const bool even) {
     using S = WideShape;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[3 * S::kStages + 3];
+    __shared__ __align__(8) uint64_t bars[2 * S::kStages + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bar0 = smem_u32(bars);
-    const auto full = [&](int s) { return bar0 + 8u * s; };                       // this CTA's copies have come
-    const auto both = [&](int s) { return bar0 + 8u * (S::kStages + s); };       // (first CTA) the second's too
-    const auto empty = [&](int s) { return bar0 + 8u * (2 * S::kStages + s); };
-    const uint32_t acc_full = bar0 + 8u * (3 * S::kStages), acc_empty = acc_full + 8u, drained = acc_full + 16u;
+    const auto full = [&](int s) { return bar0 + 8u * s; };                       // this CTA's copies have come; in the first CTA, the second's too
+    const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), acc_empty = acc_full + 8u, drained = acc_full + 16u;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(both(s), 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), rank == 0 ? 2 : 1); mbar_init(empty(s), 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 16);
         mbar_init(drained, 1);
@@ -414,7 +428,7 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
     __syncthreads();
     cluster_sync();
     tensor_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    constexpr uint32_t tmem = 0;       // all columns were asked for: the allocation begins at the first
 
     const int chunks = p.chunks, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int feature_tiles = GATED ? p.row_tiles : (p.row_tiles + 1) / 2;
@@ -460,13 +474,14 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
             if (lane == 0) {
                 for (int64_t i = 0; i < units; ++i) {
                     if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
-                    arrive_at_first(both(i % S::kStages));
+                    arrive_at_first(full(i % S::kStages));
                 }
                 bar_wait(drained, 0, &failed);
             }
         } else {
             // The scales of a stage are copied before the multiplications of the stage before are issued: the tensor core runs in
             // order, and a multiplication would wait for scales that were copied just before it.
+            const uint32_t lead = elect_one();
             int s = 0;
             uint32_t parity = 0, round = 0;
             bool ok = true;
@@ -480,40 +495,31 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
                     const uint32_t sfx = tmem + S::kScaleBase + (behind * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
                     const uint64_t a = operand_desc(stage + q * kMx4TileBytes + kMx4ScaleBytes), b = operand_desc(stage + S::kWeightCodes + q * S::kCodes);
                     const uint32_t add = behind_first && !q ? 0u : 1u;
-                    if (elect_one()) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)      // 32 bytes on: two in the descriptors' unit
-                            mx4_multiply<2>(tmem, a + 2 * j, b + 2 * j, mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4,
-                                            sfw + (j >> 1) * 8, j ? 1u : add);
-                    }
-                    __syncwarp();
+                    for (int j = 0; j < 4; ++j)      // 32 bytes on: two in the descriptors' unit
+                        mx4_multiply<2>(lead, tmem, a + 2 * j, b + 2 * j, mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4,
+                                        sfw + (j >> 1) * 8, j ? 1u : add);
                 }
-                if (elect_one()) {
-                    tensor_commit_pair(empty(behind));
-                    if (behind_last) tensor_commit_pair(acc_full);
-                }
-                __syncwarp();
+                tensor_commit_pair(lead, empty(behind));
+                if (behind_last) tensor_commit_pair(lead, acc_full);
                 if (behind_last) ++round;
                 return true;
             };
             for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
                 for (int k = 0; k < chunks; k += S::kTiles) {
                     const int n = min(S::kTiles, chunks - k);
-                    if (!warp_wait(full(s), parity, &failed) || !warp_wait(both(s), parity, &failed)) { ok = false; break; }
+                    if (!warp_wait(full(s), parity, &failed)) { ok = false; break; }
                     tensor_fence_after();
                     const uint32_t stage = ring + s * S::kStageBytes;
                     for (int q = 0; q < n; ++q) {
                         const uint32_t sfx = tmem + S::kScaleBase + (s * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
                         const uint64_t x = scale_desc(stage + q * kMx4TileBytes), w = scale_desc(stage + S::kWeightScales + 2 * q * kMx4ScaleBytes);
-                        if (elect_one()) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {      // 512 bytes on: 32 in the descriptors' unit
-                                copy_scales<2>(sfx + h * 4, x + 32 * h);
-                                copy_scales<2>(sfw + h * 8, w + 32 * h);
-                                copy_scales<2>(sfw + h * 8 + 4, w + 64 + 32 * h);
-                            }
+                        for (int h = 0; h < 2; ++h) {      // 512 bytes on: 32 in the descriptors' unit
+                            copy_scales<2>(lead, sfx + h * 4, x + 32 * h);
+                            copy_scales<2>(lead, sfw + h * 8, w + 32 * h);
+                            copy_scales<2>(lead, sfw + h * 8 + 4, w + 64 + 32 * h);
                         }
-                        __syncwarp();
                     }
                     if (behind >= 0 && !multiply()) { ok = false; break; }
                     behind = s;
@@ -524,8 +530,7 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
                 }
             }
             if (ok && behind >= 0) multiply();
-            if (elect_one()) tensor_commit_pair(drained);
-            __syncwarp();
+            tensor_commit_pair(lead, drained);
             warp_wait(drained, 0, &failed);
         }
     } else {
@@ -536,8 +541,9 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
             __syncwarp();
             tensor_fence_after();
             const WideTile t = wide_tile(tile, p.token_tiles);
-            const int64_t token = ((int64_t)2 * t.token + rank) * kMx4Rows + quarter * 32 + lane;
-            const uint32_t acc = tmem + ((uint32_t)quarter << 21);
+            const int64_t token0 = ((int64_t)2 * t.token + rank) * kMx4Rows + quarter * 32, tokens = p.tokens - token0;   // this warp's
+            const uint32_t acc = tmem + ((uint32_t)quarter << 21), buffer = ring + S::kStageRows + (warp - 2) * 4096;
+            uint16_t* rows = static_cast<uint16_t*>(p.out) + token0 * p.out_stride;
             const auto release = [&] {
                 tensor_fence_before();
                 __syncwarp();
@@ -554,24 +560,26 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
                 const int first = t.feature * kMx4Rows + half * 64, valid = p.rows - first;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) g[i] = i < valid ? act(g[i], p.activation) * u[i] : 0.f;
-                if (token >= p.tokens) continue;
                 if (p.out_dtype == MPS_MX4) {
-                    const int out_chunks = (int)mx4_chunks(p.rows), row = (int)(token % kMx4Rows), part = t.feature & 1;
-                    uint8_t* to = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, t.feature >> 1, out_chunks);
-                    uint32_t b0, b1;
-                    *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2)) = block_codes(g, b0);
-                    *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2 + 1)) = block_codes(g + 32, b1);
-                    *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, part) + half * 2) = (uint16_t)(b0 | b1 << 8);
-                    if (t.feature == p.row_tiles - 1 && part == 0) {      // fill up the last tile
-                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 4 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
-                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 5 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
-                        *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, 1) + half * 2) = 0;
+                    const int64_t token = token0 + lane;
+                    if (token < p.tokens) {
+                        const int out_chunks = (int)mx4_chunks(p.rows), row = (int)(token % kMx4Rows), part = t.feature & 1;
+                        uint8_t* to = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, t.feature >> 1, out_chunks);
+                        uint32_t b0, b1;
+                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2)) = block_codes(g, b0);
+                        *reinterpret_cast<uint4*>(to + mx4_code_offset(row, part * 4 + half * 2 + 1)) = block_codes(g + 32, b1);
+                        *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, part) + half * 2) = (uint16_t)(b0 | b1 << 8);
+                        if (t.feature == p.row_tiles - 1 && part == 0) {      // fill up the last tile
+                            *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 4 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(to + mx4_code_offset(row, 5 + half * 2)) = make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint16_t*>(to + mx4_scale_offset(row, 1) + half * 2) = 0;
+                        }
                     }
                 } else {
                     uint32_t w[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) w[i] = pack2(g[2 * i], g[2 * i + 1], p.out_dtype);
-                    store_row<64>(static_cast<uint16_t*>(p.out) + token * p.out_stride + first, w, valid, align);
+                    store_rows(buffer, lane, w, rows + first, p.out_stride, tokens, valid, even);
                 }
             } else {
                 uint32_t w[64];
@@ -583,8 +591,11 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
                     for (int i = 0; i < 16; ++i) w[c / 2 + i] = pack2(v[2 * i], v[2 * i + 1], p.out_dtype);
                 }
                 release();
-                const int first = t.feature * 256 + half * 128;
-                if (token < p.tokens) store_row<128>(static_cast<uint16_t*>(p.out) + token * p.out_stride + first, w, p.rows - first, align);
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    const int first = t.feature * 256 + half * 128 + c;
+                    store_rows(buffer, lane, w + c / 2, rows + first, p.out_stride, tokens, p.rows - first, even);
+                }
             }
         }
     }
@@ -594,7 +605,7 @@ mx4_wide_kernel(const ProductArgs p, const int align) {
     cluster_sync();      // what the pair's instructions read and write is there until both are done
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
-    if (warp == 1) tmem_free<2>(tmem, S::kColumns);
+    if (warp == 1) tmem_free<2>(tmem_slot, S::kColumns);
 }
 
 template <typename Kernel, typename... More>
@@ -628,7 +639,7 @@ static int launch_wide(ProductArgs p, int sms, cudaStream_t st) {
     const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
     const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
     const bool even = p.out_dtype != MPS_MX4 && p.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
-    return launch_product(mx4_wide_kernel<GATED>, WideShape::kSmem, kWideThreads, 2 * pairs, st, p, even ? 16 : 2);
+    return launch_product(mx4_wide_kernel<GATED>, WideShape::kSmem, kWideThreads, 2 * pairs, st, p, even);
 }
 
 

@@ -34,36 +34,52 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
     }
 }
+// What issues to the tensor core runs as a whole warp, and the lane that `lead` (elect_one, taken once) names issues: without a branch around the
+// instructions their addresses and descriptors, the same in all lanes, stay in uniform registers, where they are taken from.  Measured with a branch
+// around them: some 80 cycles an instruction, twice what a stage's multiplications take.
+
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
 // 128 rows' scales of 128 columns into four columns of tensor memory, the same in each of its four lane quarters.
 template <int CTAS>
-__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
-    if (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t lead, uint32_t tmem, uint64_t desc) {
+    if (CTAS == 1)
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %2, 0;\n\t@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
+                     ::"r"(tmem), "l"(desc), "r"(lead) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %2, 0;\n\t@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}"
+                     ::"r"(tmem), "l"(desc), "r"(lead) : "memory");
 }
 template <int CTAS>
-__device__ __forceinline__ void mx4_multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t sfa, uint32_t sfb, uint32_t add) {
+__device__ __forceinline__ void mx4_multiply(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t sfa, uint32_t sfb, uint32_t add) {
     if (CTAS == 1)
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add) : "memory");
+            "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %6, 0;\n\tsetp.ne.u32 e, %7, 0;\n\t"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add), "r"(lead) : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add) : "memory");
+            "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %6, 0;\n\tsetp.ne.u32 e, %7, 0;\n\t"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add), "r"(lead) : "memory");
 }
-// The barrier gets an arrival when everything this thread has issued to the tensor core is done.
-__device__ __forceinline__ void tensor_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The barrier gets an arrival when everything that lane has issued to the tensor core is done.
+__device__ __forceinline__ void tensor_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(bar), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // The same for a pair of CTAs: at this place in the shared memory of both.
-__device__ __forceinline__ void tensor_commit_pair(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+__device__ __forceinline__ void tensor_commit_pair(uint32_t lead, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %2, 0;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                 ::"r"(bar), "h"((uint16_t)3), "r"(lead) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -78,14 +94,6 @@ __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// One lane of a converged warp.  What issues to the tensor core runs as a whole warp with this around each instruction: addresses
-// and descriptors are then the same in all lanes and stay in uniform registers, where the instructions take them from.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
 }
 
 // Sixteen columns of the accumulator, a lane of tensor memory per thread; the whole warp takes part.  Load and wait are one
