@@ -332,18 +332,17 @@ mx4_stream_kernel(const ProductArgs p) {
 // on each quarter of the lanes, one on each half of the columns.
 struct WideShape {
     static constexpr int kCodes = kMx4Rows * kMx4RowBytes;
-    static constexpr int kTiles = 1;                                        // tiles along the columns that a stage holds at most
-    // of a stage: token tiles, scales of the weights' two halves, codes of this CTA's half
-    static constexpr int kWeightScales = kTiles * kMx4TileBytes;
-    static constexpr int kWeightCodes = kWeightScales + kTiles * 2 * kMx4ScaleBytes;
-    static constexpr int kStageBytes = kWeightCodes + kTiles * kCodes;
-    static constexpr int kStages = 5 / kTiles;
-    static constexpr int kStageRows = kStages * kStageBytes;                // eight warps' rows on their way out
-    static constexpr int kSmem = kStageRows + 8 * 4096 + 1024;
-    static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;   // scale columns of a tile
-    static_assert(kScaleBase + kStages * kTiles * kScaleColumns <= kColumns, "tensor memory");
+    static constexpr int kWeightScales = kMx4TileBytes;                     // of a stage: tokens, the weights' scales, their codes
+    static constexpr int kWeightCodes = kWeightScales + 2 * kMx4ScaleBytes;
+    static constexpr int kStageBytes = kWeightCodes + kCodes;
+    static constexpr int kStages = 6;
+    static constexpr int kStageRows = kStages * kStageBytes;                // eight warps' rows on their way out, 2 KB each
+    static constexpr int kBars = kStageRows + 8 * 2048;
+    static constexpr int kSmem = kBars + (2 * kStages + 3) * 8 + 16;
+    static constexpr int kScaleBase = 256, kScaleColumns = 24, kColumns = 512;
+    static_assert(kScaleBase + kStages * kScaleColumns <= kColumns, "tensor memory");
     static_assert(kStageBytes % 1024 == 0 && kWeightCodes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
-    static_assert(kSmem + 1024 <= kMx4SmemMost, "shared memory");
+    static_assert(kSmem <= kMx4SmemMost, "shared memory");
 };
 constexpr int kWideThreads = 320;
 
@@ -370,31 +369,32 @@ __device__ __forceinline__ uint4 block_codes(const float* v, uint32_t& byte) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A warp's 32 tokens x 64 features, a token per lane, go out by way of 4 KB of shared memory: written straight from the registers every
-// instruction would touch 32 rows with 16 bytes each.  `w`: 64 values in pairs; rows below `tokens`, columns below `valid` are stored.
+// A warp's 32 tokens x 32 features, a token per lane, go out by way of 2 KB of shared memory: written straight from the registers every
+// instruction would touch 32 rows with 16 bytes each.  `w`: 32 values in pairs; rows below `tokens`, columns below `valid` are stored.
 __device__ __forceinline__ void store_rows(uint32_t buffer, int lane, const uint32_t* w, uint16_t* out, int64_t stride, int64_t tokens, int valid,
                                            bool even) {
+    // a row is four pieces of 16 bytes; two rows share the banks, so the pieces change places with every second row
+    const auto place = [&](int row, int piece) { return buffer + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); };
     __syncwarp();
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buffer + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(w[4 * c]), "r"(w[4 * c + 1]),
-                     "r"(w[4 * c + 2]), "r"(w[4 * c + 3]) : "memory");
+    for (int c = 0; c < 4; ++c)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, c)), "r"(w[4 * c]), "r"(w[4 * c + 1]), "r"(w[4 * c + 2]),
+                     "r"(w[4 * c + 3]) : "memory");
     __syncwarp();
-    if (even && valid >= 64) {
+    if (even && valid >= 32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = i * 4 + (lane >> 3), c = lane & 7;
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2), c = lane & 3;
             uint4 v;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(buffer + row * 128 + ((c ^ (row & 7)) << 4)));
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(place(row, c)));
             if (row < tokens) *reinterpret_cast<uint4*>(out + row * stride + c * 8) = v;
         }
     } else {
         const int rows = tokens < 32 ? (int)tokens : 32;
         for (int row = 0; row < rows; ++row) {
-            uint32_t v;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(buffer + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4));
-            if (2 * lane < valid) out[row * stride + 2 * lane] = (uint16_t)v;
-            if (2 * lane + 1 < valid) out[row * stride + 2 * lane + 1] = (uint16_t)(v >> 16);
+            uint16_t v;
+            asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(place(row, lane >> 3) + (lane & 7) * 2));
+            if (lane < valid) out[row * stride + lane] = v;
         }
     }
 }
@@ -403,14 +403,12 @@ template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
 mx4_wide_kernel(const ProductArgs p, const bool even) {
     using S = WideShape;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * S::kStages + 3];
-    __shared__ uint32_t tmem_slot;
-    __shared__ volatile uint32_t failed;
+    extern __shared__ __align__(1024) uint8_t ring_bytes[];      // all of the shared memory: rings begin at multiples of 1024
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t ring = smem_u32(ring_bytes), bar0 = ring + S::kBars;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(ring_bytes + S::kSmem - 16);
+    volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(ring_bytes + S::kSmem - 12);
     const auto full = [&](int s) { return bar0 + 8u * s; };                       // this CTA's copies have come; in the first CTA, the second's too
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
     const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), acc_empty = acc_full + 8u, drained = acc_full + 16u;
@@ -447,19 +445,16 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
                 const uint8_t* w0 = GATED ? p.w + mx4_tile_offset(t.feature, 0, chunks) : p.w + mx4_tile_offset(2 * t.feature, 0, chunks);
                 const uint8_t* w1 = GATED ? p.w_up + mx4_tile_offset(t.feature, 0, chunks)
                                           : p.w + mx4_tile_offset(min(2 * t.feature + 1, p.row_tiles - 1), 0, chunks);
-                for (int k = 0; k < chunks; k += S::kTiles, ++i) {
-                    const int s = (int)(i % S::kStages), n = min(S::kTiles, chunks - k);
+                for (int k = 0; k < chunks; ++k, ++i) {
+                    const int s = (int)(i % S::kStages);
                     if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) { ok = false; break; }
                     const uint32_t to = ring + s * S::kStageBytes;
                     const int64_t at = (int64_t)k * kMx4TileBytes;
-                    mbar_expect_tx(full(s), n * (S::kStageBytes / S::kTiles));
-                    bulk_g2s(to, x + at, n * kMx4TileBytes, full(s));
-                    for (int q = 0; q < n; ++q) {
-                        const int64_t from = at + q * kMx4TileBytes;
-                        bulk_g2s(to + S::kWeightScales + 2 * q * kMx4ScaleBytes, w0 + from, kMx4ScaleBytes, full(s));
-                        bulk_g2s(to + S::kWeightScales + (2 * q + 1) * kMx4ScaleBytes, w1 + from, kMx4ScaleBytes, full(s));
-                        bulk_g2s(to + S::kWeightCodes + q * S::kCodes, (rank ? w1 : w0) + from + kMx4ScaleBytes, S::kCodes, full(s));
-                    }
+                    mbar_expect_tx(full(s), S::kStageBytes);
+                    bulk_g2s(to, x + at, kMx4TileBytes, full(s));
+                    bulk_g2s(to + S::kWeightScales, w0 + at, kMx4ScaleBytes, full(s));
+                    bulk_g2s(to + S::kWeightScales + kMx4ScaleBytes, w1 + at, kMx4ScaleBytes, full(s));
+                    bulk_g2s(to + S::kWeightCodes, (rank ? w1 : w0) + at + kMx4ScaleBytes, S::kCodes, full(s));
                 }
             }
             for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
@@ -469,8 +464,7 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
         }
     } else if (warp == 1) {
         if (rank == 1) {
-            int64_t units = 0;
-            for (int64_t tile = pair; tile < tiles; tile += pairs) units += (chunks + S::kTiles - 1) / S::kTiles;
+            const int64_t units = (tiles - pair + pairs - 1) / pairs * chunks;
             if (lane == 0) {
                 for (int64_t i = 0; i < units; ++i) {
                     if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
@@ -479,57 +473,34 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
                 bar_wait(drained, 0, &failed);
             }
         } else {
-            // The scales of a stage are copied before the multiplications of the stage before are issued: the tensor core runs in
-            // order, and a multiplication would wait for scales that were copied just before it.
             const uint32_t lead = elect_one();
             int s = 0;
             uint32_t parity = 0, round = 0;
             bool ok = true;
-            int behind = -1, behind_tiles = 0;       // the stage whose multiplications are still to be issued
-            bool behind_first = false, behind_last = false;
-            const auto multiply = [&]() -> bool {
-                if (behind_first && round && !warp_wait(acc_empty, (round - 1) & 1u, &failed)) return false;
-                tensor_fence_after();
-                const uint32_t stage = ring + behind * S::kStageBytes;
-                for (int q = 0; q < behind_tiles; ++q) {
-                    const uint32_t sfx = tmem + S::kScaleBase + (behind * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
-                    const uint64_t a = operand_desc(stage + q * kMx4TileBytes + kMx4ScaleBytes), b = operand_desc(stage + S::kWeightCodes + q * S::kCodes);
-                    const uint32_t add = behind_first && !q ? 0u : 1u;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)      // 32 bytes on: two in the descriptors' unit
-                        mx4_multiply<2>(lead, tmem, a + 2 * j, b + 2 * j, mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4,
-                                        sfw + (j >> 1) * 8, j ? 1u : add);
-                }
-                tensor_commit_pair(lead, empty(behind));
-                if (behind_last) tensor_commit_pair(lead, acc_full);
-                if (behind_last) ++round;
-                return true;
-            };
-            for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
-                for (int k = 0; k < chunks; k += S::kTiles) {
-                    const int n = min(S::kTiles, chunks - k);
+            for (int64_t tile = pair; tile < tiles && ok; tile += pairs, ++round) {
+                if (round && !warp_wait(acc_empty, (round - 1) & 1u, &failed)) break;
+                for (int k = 0; k < chunks; ++k) {
                     if (!warp_wait(full(s), parity, &failed)) { ok = false; break; }
                     tensor_fence_after();
                     const uint32_t stage = ring + s * S::kStageBytes;
-                    for (int q = 0; q < n; ++q) {
-                        const uint32_t sfx = tmem + S::kScaleBase + (s * S::kTiles + q) * S::kScaleColumns, sfw = sfx + 8;
-                        const uint64_t x = scale_desc(stage + q * kMx4TileBytes), w = scale_desc(stage + S::kWeightScales + 2 * q * kMx4ScaleBytes);
+                    const uint32_t sfx = tmem + S::kScaleBase + s * S::kScaleColumns, sfw = sfx + 8;
+                    const uint64_t x = scale_desc(stage), w = scale_desc(stage + S::kWeightScales);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {      // 512 bytes on: 32 in the descriptors' unit
-                            copy_scales<2>(lead, sfx + h * 4, x + 32 * h);
-                            copy_scales<2>(lead, sfw + h * 8, w + 32 * h);
-                            copy_scales<2>(lead, sfw + h * 8 + 4, w + 64 + 32 * h);
-                        }
+                    for (int h = 0; h < 2; ++h) {      // 512 bytes on: 32 in the descriptors' unit
+                        copy_scales<2>(lead, sfx + h * 4, x + 32 * h);
+                        copy_scales<2>(lead, sfw + h * 8, w + 32 * h);
+                        copy_scales<2>(lead, sfw + h * 8 + 4, w + 64 + 32 * h);
                     }
-                    if (behind >= 0 && !multiply()) { ok = false; break; }
-                    behind = s;
-                    behind_tiles = n;
-                    behind_first = k == 0;
-                    behind_last = k + n == chunks;
+                    const uint64_t a = operand_desc(stage + kMx4ScaleBytes), b = operand_desc(stage + S::kWeightCodes);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)      // 32 bytes on: two in the descriptors' unit
+                        mx4_multiply<2>(lead, tmem, a + 2 * j, b + 2 * j, mx4_instruction(256, 256, (j & 1) * 2), sfx + (j >> 1) * 4,
+                                        sfw + (j >> 1) * 8, k || j ? 1u : 0u);
+                    tensor_commit_pair(lead, empty(s));
                     if (++s == S::kStages) { s = 0; parity ^= 1u; }
                 }
+                if (ok) tensor_commit_pair(lead, acc_full);
             }
-            if (ok && behind >= 0) multiply();
             tensor_commit_pair(lead, drained);
             warp_wait(drained, 0, &failed);
         }
@@ -542,7 +513,7 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
             tensor_fence_after();
             const WideTile t = wide_tile(tile, p.token_tiles);
             const int64_t token0 = ((int64_t)2 * t.token + rank) * kMx4Rows + quarter * 32, tokens = p.tokens - token0;   // this warp's
-            const uint32_t acc = tmem + ((uint32_t)quarter << 21), buffer = ring + S::kStageRows + (warp - 2) * 4096;
+            const uint32_t acc = tmem + ((uint32_t)quarter << 21), buffer = ring + S::kStageRows + (warp - 2) * 2048;
             uint16_t* rows = static_cast<uint16_t*>(p.out) + token0 * p.out_stride;
             const auto release = [&] {
                 tensor_fence_before();
@@ -579,7 +550,8 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
                     uint32_t w[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) w[i] = pack2(g[2 * i], g[2 * i + 1], p.out_dtype);
-                    store_rows(buffer, lane, w, rows + first, p.out_stride, tokens, valid, even);
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) store_rows(buffer, lane, w + c / 2, rows + first + c, p.out_stride, tokens, valid - c, even);
                 }
             } else {
                 uint32_t w[64];
@@ -592,7 +564,7 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
                 }
                 release();
 #pragma unroll
-                for (int c = 0; c < 128; c += 64) {
+                for (int c = 0; c < 128; c += 32) {
                     const int first = t.feature * 256 + half * 128 + c;
                     store_rows(buffer, lane, w + c / 2, rows + first, p.out_stride, tokens, p.rows - first, even);
                 }
