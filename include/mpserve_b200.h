@@ -384,14 +384,15 @@ typedef struct mps_mx4_linear {
     void* out;
     int64_t tokens, cols, rows;
     int64_t x_stride, out_stride;
-    int32_t x_dtype, out_dtype, activation, reserved;
+    int32_t x_dtype, out_dtype, activation;
+    int32_t weights_ready;              /* the kernel before in the stream writes no weight: they may be read before it is done */
 } mps_mx4_linear;
-/* Scratch of the products on the current device: zero-filled once, one per stream that may run them concurrently, 256-byte
- * aligned; handed back with its counters zeroed.  Negative: an error code. */
+/* Scratch of the products: zero-filled once, one per stream that may run them concurrently, 256-byte aligned.  x_tiles may be null
+ * where mps_mx4_bytes(tokens, cols) fits into it (8 MB). */
 MPS_API int64_t mps_mx4_workspace_bytes(void);
 MPS_API int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
 /* Every wait inside the products is bounded: waits for the stream, tells whether any since the last query gave up (its outputs are
- * then incomplete), and clears the workspace. */
+ * then incomplete), and clears the record. */
 MPS_API int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out);
 
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of

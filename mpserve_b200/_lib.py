@@ -51,7 +51,7 @@ class Mx4Linear(C.Structure):
         ("x", _p), ("x_tiles", _p), ("w", _p), ("w_up", _p), ("out", _p),
         ("tokens", _i64), ("cols", _i64), ("rows", _i64),
         ("x_stride", _i64), ("out_stride", _i64),
-        ("x_dtype", _i32), ("out_dtype", _i32), ("activation", _i32), ("reserved", _i32),
+        ("x_dtype", _i32), ("out_dtype", _i32), ("activation", _i32), ("weights_ready", _i32),
     ]
 
 

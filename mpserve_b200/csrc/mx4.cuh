@@ -199,6 +199,12 @@ __device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int ro
     if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_scale_offset(row, lane >> 4)) = w;
 }
 
+// The kernels of these operators may be launched while the kernel before them in the stream ends.  A kernel waits for that one before it reads what
+// others write and before it writes anything, and only then lets the next begin: so whatever begins early can rely on all but
+// the kernel right before it being done.
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 inline bool mx4_dtype_ok(int dtype) { return dtype == MPS_BF16 || dtype == MPS_F16 || dtype == MPS_F32; }
 inline int64_t mx4_dtype_bytes(int dtype) { return dtype == MPS_F32 ? 4 : 2; }
 inline bool mx4_vec_ok(const void* p, int64_t row_stride, int dtype) {
@@ -206,5 +212,25 @@ inline bool mx4_vec_ok(const void* p, int64_t row_stride, int dtype) {
 }
 // Row and column counts that every entry point accepts: tile counts and launch grids stay within 31 bits.
 constexpr int64_t kMx4MostRows = int64_t(1) << 31, kMx4MostCols = int64_t(1) << 24;
+
+
+struct Device { int ordinal, sms; };
+int current_device(Device& d);
+
+// A launch that may overlap the end of the kernel before it.
+template <typename... Params, typename... Args>
+inline int launch_overlapping(const char* what, void (*kernel)(Params...), unsigned int ctas, int threads, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3((unsigned)threads);
+    config.stream = st;
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
+}
 
 }  // namespace mps

@@ -4,6 +4,8 @@
 // tiles, so that a lane has four 16-byte loads under way, and each tile row leaves as one 128-byte line.
 #include "mx4.cuh"
 
+#include <atomic>
+
 namespace mps {
 
 constexpr int kConvertThreads = 256;
@@ -21,6 +23,8 @@ static __device__ __forceinline__ bool convert_place(int64_t rows, int segments,
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_quantize_kernel(const void* __restrict__ x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, bool vec, int chunks,
                     int segments, uint8_t* __restrict__ out) {
+    griddep_wait();
+    griddep_launch();
     ConvertPlace p;
     if (!convert_place(rows, segments, p)) return;
     const int lane = threadIdx.x & 31;
@@ -42,6 +46,8 @@ mx4_quantize_kernel(const void* __restrict__ x, int dtype, int64_t rows, int64_t
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int chunks, int segments, int dtype, bool vec,
                       void* __restrict__ out) {
+    griddep_wait();
+    griddep_launch();
     ConvertPlace p;
     if (!convert_place(rows, segments, p)) return;
     const int lane = threadIdx.x & 31, row = (int)(p.row % kMx4Rows);
@@ -73,6 +79,8 @@ mx4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols,
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_pack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int64_t cols, int chunks,
                 int segments, uint8_t* __restrict__ out) {
+    griddep_wait();
+    griddep_launch();
     ConvertPlace p;
     if (!convert_place(rows, segments, p)) return;
     const int lane = threadIdx.x & 31, row = (int)(p.row % kMx4Rows);
@@ -102,6 +110,8 @@ mx4_pack_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ s
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_unpack_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int chunks, int segments, uint8_t* __restrict__ codes,
                   uint8_t* __restrict__ scales) {
+    griddep_wait();
+    griddep_launch();
     ConvertPlace p;
     if (!convert_place(rows, segments, p)) return;
     const int lane = threadIdx.x & 31, row = (int)(p.row % kMx4Rows);
@@ -136,9 +146,17 @@ static int convert_grid(const char* who, int64_t rows, int64_t cols, ConvertGrid
     return MPS_OK;
 }
 
-int launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
+// The current device, its SMs counted once.
+int current_device(Device& d) {
+    static std::atomic<int> sms[64];
+    MPS_CUDA_TRY(cudaGetDevice(&d.ordinal));
+    if (d.ordinal < 0 || d.ordinal >= 64) { set_error("device ordinal %d out of range", d.ordinal); return MPS_ERR_UNSUPPORTED; }
+    d.sms = sms[d.ordinal].load(std::memory_order_relaxed);
+    if (d.sms == 0) {
+        MPS_CUDA_TRY(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, d.ordinal));
+        sms[d.ordinal].store(d.sms, std::memory_order_relaxed);
+    }
+    return MPS_OK;
 }
 
 }  // namespace mps
@@ -159,9 +177,8 @@ int mps_mx4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, i
     if (!mx4_dtype_ok(dtype)) { set_error("mps_mx4_quantize: unknown dtype %d", (int)dtype); return MPS_ERR_INVALID; }
     if (rows == 0) return MPS_OK;
     if (!x || !tiles || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_quantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    mx4_quantize_kernel<<<g.ctas, kConvertThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        x, dtype, rows, cols, row_stride, mx4_vec_ok(x, row_stride, dtype), g.chunks, g.segments, static_cast<uint8_t*>(tiles));
-    return launched("mx4_quantize_kernel");
+    return launch_overlapping("mx4_quantize_kernel", mx4_quantize_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream), x, (int)dtype, rows,
+                              cols, row_stride, mx4_vec_ok(x, row_stride, dtype), g.chunks, g.segments, static_cast<uint8_t*>(tiles));
 }
 
 int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dtype, void* out, void* stream) {
@@ -171,9 +188,8 @@ int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dt
     if (!mx4_dtype_ok(dtype)) { set_error("mps_mx4_dequantize: unknown dtype %d", (int)dtype); return MPS_ERR_INVALID; }
     if (rows == 0) return MPS_OK;
     if (!tiles || !out || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_dequantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    mx4_dequantize_kernel<<<g.ctas, kConvertThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const uint8_t*>(tiles), rows, cols, g.chunks, g.segments, dtype, mx4_vec_ok(out, cols, dtype), out);
-    return launched("mx4_dequantize_kernel");
+    return launch_overlapping("mx4_dequantize_kernel", mx4_dequantize_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream),
+                              static_cast<const uint8_t*>(tiles), rows, cols, g.chunks, g.segments, (int)dtype, mx4_vec_ok(out, cols, dtype), out);
 }
 
 int mps_mx4_pack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* tiles, void* stream) {
@@ -181,9 +197,8 @@ int mps_mx4_pack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int6
     int rc = convert_grid("mps_mx4_pack", rows, cols, g);
     if (rc || rows == 0) return rc;
     if (!codes || !scales || !tiles || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_pack: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    mx4_pack_kernel<<<g.ctas, kConvertThreads, 0, static_cast<cudaStream_t>(stream)>>>(codes, scales, rows, cols, g.chunks, g.segments,
-                                                                                     static_cast<uint8_t*>(tiles));
-    return launched("mx4_pack_kernel");
+    return launch_overlapping("mx4_pack_kernel", mx4_pack_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream), codes, scales, rows, cols,
+                              g.chunks, g.segments, static_cast<uint8_t*>(tiles));
 }
 
 int mps_mx4_unpack(const void* tiles, int64_t rows, int64_t cols, uint8_t* codes, uint8_t* scales, void* stream) {
@@ -191,9 +206,8 @@ int mps_mx4_unpack(const void* tiles, int64_t rows, int64_t cols, uint8_t* codes
     int rc = convert_grid("mps_mx4_unpack", rows, cols, g);
     if (rc || rows == 0) return rc;
     if (!tiles || !codes || !scales || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_unpack: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    mx4_unpack_kernel<<<g.ctas, kConvertThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(tiles), rows, cols,
-                                                                                       g.chunks, g.segments, codes, scales);
-    return launched("mx4_unpack_kernel");
+    return launch_overlapping("mx4_unpack_kernel", mx4_unpack_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream),
+                              static_cast<const uint8_t*>(tiles), rows, cols, g.chunks, g.segments, codes, scales);
 }
 
 }  // extern "C"

@@ -3,34 +3,32 @@
 #include "mx4_tensor.cuh"
 #include "stream_common.cuh"
 
-namespace mps {
+#include <atomic>
 
-int launched(const char* what);
+namespace mps {
 
 // ---- what the kernels share -------------------------------------------------------------------------
 
-constexpr int kMx4MostSms = 192;               // CTAs of a launch are at most the SMs
 constexpr uint32_t kMx4SpinLimit = 1u << 20;
 constexpr int kMx4SmemMost = 232448;           // 227 KB
 
-// Workspace: word 0 records a wait that ran out; from byte 4096 on, counters; then partial sums.
-constexpr int64_t kMx4CounterBytes = 4096, kMx4PartialOffset = 4096 + kMx4CounterBytes;
-constexpr int64_t kMx4PartialFloats = 128 * 256;   // most of one CTA's accumulator, features x tokens
-constexpr int64_t kMx4WorkspaceBytes = kMx4PartialOffset + 2 * kMx4MostSms * kMx4PartialFloats * 4;
+// Workspace: word 0 records a wait that ran out; from byte 1024 on, the tokens of a call that quantises them in a kernel of its own.
+constexpr int64_t kMx4ScratchOffset = 1024, kMx4WorkspaceBytes = kMx4ScratchOffset + (int64_t)480 * kMx4TileBytes;
 
 struct ProductArgs {
-    const uint8_t* x;        // tiles
+    const uint8_t* x;        // tiles, or (stream kernel with QUANTIZE) the tokens as they came
     const uint8_t* w;
     const uint8_t* w_up;
     void* out;
     uint32_t* workspace;
-    int64_t out_stride;
+    int64_t out_stride, x_stride;
     int64_t tokens;
-    int32_t rows;            // of the weight: features
+    int32_t rows, cols;      // of the weight
     int32_t chunks;          // tiles of a row
-    int32_t row_tiles, token_tiles;
-    int32_t out_dtype, activation;
-    bool x_follows;          // x is written by the kernel before, which this one may overlap
+    int32_t row_tiles, token_tiles, parts;
+    int32_t x_dtype, out_dtype, activation;
+    bool x_vec;
+    bool early;              // the kernel before writes no weight: weights may be read before it is done
 };
 
 // Both activations are g / (1 + exp(-t)): SiLU with t = g, and GELU's tanh form since (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)).  The
@@ -58,100 +56,78 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 // ---- few tokens: weights on the accumulator's lanes -------------------------------------------------
 //
-// One CTA per SM streams weight tiles through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
-// product's narrow side.  The work is cut evenly into runs of (tile of the output, tile of K) pairs, a run per CTA, so that
-// every SM reads the same number of bytes whatever the sizes; a tile of the output that several CTAs have parts of is summed by
-// whichever of them ends last, always in the same order.  Nothing waits for another CTA.
+// A CTA streams the weight tiles of 128 features through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
+// product's narrow side.  Two CTAs share an SM, and a cluster of up to eight shares the columns of one tile of the output, as many as
+// fill the GPU: then every SM has some 200 KB under way, and all end together.  The parts of a tile meet in the cluster's shared memory,
+// where every CTA adds up a share of them, always in the same order.
 //
-// Warps: 0 copies, 1 multiplies, 2 to 5 take the accumulator over, two of which take turns.
+// Warps: 0 copies, 1 multiplies, 2 to 5 take the accumulator over; with QUANTIZE, one more for every stage of the ring quantises the tokens'
+// columns on their way into it, instead of a kernel before this one.
 template <int TOKENS, bool GATED>
 struct StreamShape {
     static constexpr int kWeights = GATED ? 2 : 1;
     static constexpr int kXBytes = kMx4ScaleBytes + TOKENS * kMx4RowBytes;
     static constexpr int kStageBytes = kWeights * kMx4TileBytes + kXBytes;
-    static constexpr int kStages = (kMx4SmemMost - 2048) / kStageBytes < 12 ? (kMx4SmemMost - 2048) / kStageBytes : 12;
-    static constexpr int kSmem = kStages * kStageBytes + 2048;
-    static constexpr int kAcc = TOKENS * kWeights;              // columns of one accumulator
+    static constexpr int kMost = 115712 - 1024;                 // of an SM's 228 KB, for two CTAs and the KB that each costs
+    static constexpr int kStages = kMost / kStageBytes;
+    static constexpr int kBars = kStages * kStageBytes;
+    static constexpr int kSmem = kBars + (2 * kStages + 2) * 8 + 16;
+    static constexpr int kAcc = TOKENS * kWeights;              // columns of the accumulator
     static constexpr int kScaleColumns = 8 * kWeights + 8;      // of one stage
-    static constexpr int kBuffers = kAcc <= 128 ? 2 : 1;        // accumulators that take turns
-    static constexpr int kScaleBase = kBuffers * kAcc;
-    static constexpr int kColumns = 512;
-    static_assert(kScaleBase + kStages * kScaleColumns <= kColumns, "tensor memory");
+    static constexpr int kUsed = kAcc + kStages * kScaleColumns;
+    static constexpr int kColumns = kUsed <= 128 ? 128 : 256;   // an allocation is a power of two
+    static_assert(kUsed <= kColumns, "tensor memory");
     static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
-    static_assert(kAcc * 128 <= kMx4PartialFloats, "partial sums");
+    static_assert(kAcc * 128 * 4 <= kBars, "a part of the accumulator takes the ring's place");
 };
-constexpr int kStreamThreads = 192;
+constexpr int kStreamWarps = 6;
+constexpr int kMostQuantizedInside = 16;       // tokens that the kernel quantises itself
+constexpr int kMostParts = 8;                  // CTAs of a cluster, on any device
 
-struct StreamRun { int64_t first, last; };   // units [first, last) of a CTA
-__device__ __forceinline__ StreamRun run_of(int64_t units, int cta, int ctas) {
-    return {units * cta / ctas, units * (cta + 1) / ctas};
-}
-// The CTA that has unit u: the largest c with units * c / ctas <= u.
-__device__ __forceinline__ int cta_of(int64_t units, int64_t u, int ctas) { return (int)(((u + 1) * ctas - 1) / units); }
-
-// Sixteen tokens of one feature, `up` too where the pair is gated: into the output.
+// One token of a warp's 32 features, `up` too where the pair is gated, into the output.
 template <bool GATED>
-__device__ __forceinline__ void finish16(const ProductArgs& p, int row_tile, int quarter, int lane, int64_t token0, float (&v)[16], float (&up)[16]) {
-    const int feature = row_tile * kMx4Rows + quarter * 32 + lane;
-    if (GATED) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = act(v[i], p.activation) * up[i];
-    }
+__device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int quarter, int lane, int64_t token, float v, float up) {
+    const int first = row_tile * kMx4Rows + quarter * 32, feature = first + lane;
+    if (GATED) v = act(v, p.activation) * up;
     if (GATED && p.out_dtype == MPS_MX4) {
-        // the warp's 32 features are one block of every token
-        const int first = row_tile * kMx4Rows + quarter * 32, chunks = (int)mx4_chunks(p.rows);
-        const int chunk = first / kMx4Cols, block = (first % kMx4Cols) / kMx4Block;
-        // the last tile's second half may lie beyond the last feature and is filled up with zeros
-        const bool fill = row_tile == p.row_tiles - 1 && (row_tile & 1) == 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int64_t t = token0 + i;
-            if (t >= p.tokens) break;
-            const float f = feature < p.rows ? v[i] : 0.f;
-            const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f) & 0x7FFFFFFFu));
-            const float q[8] = {byte == 255u ? 0.f : f * mx4_inverse_scale(byte), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            uint32_t code = mx4_codes8(q) & 15u;
-            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1) << 4;    // right in the even lanes, then in every fourth, then in every eighth
-            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2) << 8;
-            code |= __shfl_xor_sync(0xFFFFFFFFu, code, 4) << 16;
-            uint8_t* tile = static_cast<uint8_t*>(p.out) + mx4_tile_offset(t / kMx4Rows, chunk, chunks);
-            const int row = (int)(t % kMx4Rows);
-            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block) + (lane >> 3) * 4) = code;
-            if (lane == 0) tile[mx4_scale_offset(row, block >> 2) + (block & 3)] = (uint8_t)byte;
-            if (fill) {
-                if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block + 4) + (lane >> 3) * 4) = 0u;
-                if (lane == 0) tile[mx4_scale_offset(row, 1) + (block & 3)] = 0u;
-            }
+        // the 32 features are one block
+        const int chunks = (int)mx4_chunks(p.rows), block = (first % kMx4Cols) / kMx4Block, row = (int)(token % kMx4Rows);
+        const float f = feature < p.rows ? v : 0.f;
+        const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f) & 0x7FFFFFFFu));
+        const float q[8] = {byte == 255u ? 0.f : f * mx4_inverse_scale(byte), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        uint32_t code = mx4_codes8(q) & 15u;
+        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1) << 4;    // right in the even lanes, then in every fourth, then in every eighth
+        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2) << 8;
+        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 4) << 16;
+        uint8_t* tile = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, first / kMx4Cols, chunks);
+        if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block) + (lane >> 3) * 4) = code;
+        if (lane == 0) tile[mx4_scale_offset(row, block >> 2) + (block & 3)] = (uint8_t)byte;
+        if (row_tile == p.row_tiles - 1 && (row_tile & 1) == 0) {
+            // the second half of the last tile lies beyond the last feature and is filled up with zeros
+            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block + 4) + (lane >> 3) * 4) = 0u;
+            if (lane == 0) tile[mx4_scale_offset(row, 1) + (block & 3)] = 0u;
         }
-        return;
+    } else if (feature < p.rows) {
+        static_cast<uint16_t*>(p.out)[token * p.out_stride + feature] = (uint16_t)pack2(v, 0.f, p.out_dtype);
     }
-    if (feature >= p.rows) return;
-    uint16_t* out = static_cast<uint16_t*>(p.out) + feature;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (token0 + i < p.tokens) out[(token0 + i) * p.out_stride] = (uint16_t)pack2(v[i], 0.f, p.out_dtype);
 }
 
-template <int TOKENS, bool GATED>
-__global__ void __launch_bounds__(kStreamThreads, 1)
+template <int TOKENS, bool GATED, bool QUANTIZE>
+__global__ void __launch_bounds__((kStreamWarps + (QUANTIZE ? StreamShape<TOKENS, GATED>::kStages : 0)) * 32, 2)
 mx4_stream_kernel(const ProductArgs p) {
     using S = StreamShape<TOKENS, GATED>;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * S::kStages + 5];
-    __shared__ uint32_t tmem_slot;
-    __shared__ volatile uint32_t failed;
+    extern __shared__ __align__(1024) uint8_t ring_bytes[];      // all of the shared memory: rings begin at multiples of 1024
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t ring = smem_u32(ring_bytes), bar0 = ring + S::kBars;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(ring_bytes + S::kSmem - 16);
+    volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(ring_bytes + S::kSmem - 12);
     const auto full = [&](int s) { return bar0 + 8u * s; };
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
-    const auto acc_full = [&](int b) { return bar0 + 8u * (2 * S::kStages + b); };
-    const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * S::kStages + 2 + b); };
-    const uint32_t drained = bar0 + 8u * (2 * S::kStages + 4);
+    const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), drained = acc_full + 8u;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(acc_full(b), 1); mbar_init(acc_empty(b), 4); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), QUANTIZE ? 2 : 1); mbar_init(empty(s), 1); }
+        mbar_init(acc_full, 1);
         mbar_init(drained, 1);
         failed = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -160,163 +136,175 @@ mx4_stream_kernel(const ProductArgs p) {
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    constexpr uint32_t tmem = 0;       // all columns were asked for: the allocation begins at the first
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
-    const int chunks = p.chunks;
-    const int64_t units = (int64_t)p.row_tiles * p.token_tiles * chunks;
-    const StreamRun run = run_of(units, blockIdx.x, gridDim.x);
+    // this CTA's tile of the output, and its share of the columns
+    const int part = blockIdx.x % p.parts, chunks = p.chunks;
+    const int64_t tile = blockIdx.x / p.parts;
+    const int row_tile = (int)(tile / p.token_tiles);
+    const int64_t token0 = (tile % p.token_tiles) * TOKENS;
+    const int k0 = (int)((int64_t)chunks * part / p.parts), k1 = (int)((int64_t)chunks * (part + 1) / p.parts);
 
     if (warp == 0) {
         if (lane == 0) {
-            const int64_t count = run.last - run.first;
-            const auto weights = [&](int64_t i) {      // of the run's i-th unit, into its stage
-                const int64_t u = run.first + i, tile = u / chunks;
-                const int s = (int)(i % S::kStages), k = (int)(u - tile * chunks);
-                const int64_t at = mx4_tile_offset(tile / p.token_tiles, k, chunks);
+            const uint8_t* w = p.w + mx4_tile_offset(row_tile, 0, chunks);
+            const uint8_t* w_up = GATED ? p.w_up + mx4_tile_offset(row_tile, 0, chunks) : nullptr;
+            const uint8_t* x = QUANTIZE ? nullptr : p.x + mx4_tile_offset(tile % p.token_tiles, 0, chunks);
+            const auto weights = [&](int k, int s) {
                 const uint32_t to = ring + s * S::kStageBytes;
-                mbar_expect_tx(full(s), S::kStageBytes);
-                bulk_g2s(to, p.w + at, kMx4TileBytes, full(s));
-                if (GATED) bulk_g2s(to + kMx4TileBytes, p.w_up + at, kMx4TileBytes, full(s));
+                mbar_expect_tx(full(s), S::kStageBytes - (QUANTIZE ? S::kXBytes : 0));
+                bulk_g2s(to, w + (int64_t)k * kMx4TileBytes, kMx4TileBytes, full(s));
+                if (GATED) bulk_g2s(to + kMx4TileBytes, w_up + (int64_t)k * kMx4TileBytes, kMx4TileBytes, full(s));
             };
-            const auto activations = [&](int64_t i) {
-                const int64_t u = run.first + i, tile = u / chunks;
-                const int s = (int)(i % S::kStages), k = (int)(u - tile * chunks);
-                bulk_g2s(ring + s * S::kStageBytes + S::kWeights * kMx4TileBytes, p.x + mx4_tile_offset(tile % p.token_tiles, k, chunks),
-                         S::kXBytes, full(s));
+            const auto activations = [&](int k, int s) {
+                if (!QUANTIZE) bulk_g2s(ring + s * S::kStageBytes + S::kWeights * kMx4TileBytes, x + (int64_t)k * kMx4TileBytes, S::kXBytes, full(s));
             };
-            // weights do not depend on the kernel before: the first of them are on their way while it still runs
-            const int64_t ahead = p.x_follows ? (count < S::kStages ? count : S::kStages) : 0;
-            for (int64_t i = 0; i < ahead; ++i) weights(i);
-            if (p.x_follows) asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (int64_t i = 0; i < ahead; ++i) activations(i);
-            int64_t i = ahead;
-            for (; i < count; ++i) {
-                if (i >= S::kStages && !bar_wait(empty(i % S::kStages), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
-                weights(i);
-                activations(i);
+            // weights that the kernel before does not write are on their way while it still runs
+            const int ahead = p.early ? min(k1 - k0, S::kStages) : 0;
+            for (int i = 0; i < ahead; ++i) weights(k0 + i, i);
+            griddep_wait();
+            for (int i = 0; i < ahead; ++i) activations(k0 + i, i);
+            griddep_launch();
+            int k = k0 + ahead;
+            for (; k < k1; ++k) {
+                const int i = k - k0, s = i % S::kStages;
+                if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
+                weights(k, s);
+                activations(k, s);
             }
             // no copy and no arrival may come after this CTA is gone
-            for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
-                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
-                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
+            for (int i = max(0, k - k0 - S::kStages); i < k - k0; ++i) {
+                const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
+                if (!bar_wait(empty(i % S::kStages), parity, &failed)) mbar_wait(full(i % S::kStages), parity, kMx4SpinLimit);
             }
         }
     } else if (warp == 1) {
         const uint32_t lead = elect_one();
-        int s = 0, segment = 0;
-        uint32_t parity = 0;
-        for (int64_t u = run.first; u < run.last; ++segment) {
-            const int64_t tile = u / chunks;
-            const int64_t end = (tile + 1) * chunks < run.last ? (tile + 1) * chunks : run.last;
-            const int b = segment % S::kBuffers;
-            if (segment >= S::kBuffers && !warp_wait(acc_empty(b), (uint32_t)(segment / S::kBuffers - 1) & 1u, &failed)) break;
+        int s = 0;
+        uint32_t parity = 0, add = 0;
+        bool ok = true;
+        for (int k = k0; k < k1; ++k) {
+            ok = warp_wait(full(s), parity, &failed);
+            if (!ok) break;
             tensor_fence_after();
-            uint32_t add = 0u;
-            for (; u < end; ++u) {
-                if (!warp_wait(full(s), parity, &failed)) break;
-                tensor_fence_after();
-                const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
-                const uint32_t sf = tmem + S::kScaleBase + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
+            const uint32_t stage = ring + s * S::kStageBytes, x = stage + S::kWeights * kMx4TileBytes;
+            const uint32_t sf = tmem + S::kAcc + s * S::kScaleColumns, sfx = sf + 8 * S::kWeights;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(lead, sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes) + 32 * h);
-                    copy_scales<1>(lead, sfx + h * 4, scale_desc(x) + 32 * h);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {      // 32 bytes on: two in the descriptors' unit
-#pragma unroll
-                    for (int w = 0; w < S::kWeights; ++w)
-                        mx4_multiply<1>(lead, tmem + b * S::kAcc + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes) + 2 * j,
-                                        operand_desc(x + kMx4ScaleBytes) + 2 * j, mx4_instruction(128, TOKENS, (j & 1) * 2),
-                                        sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4, j ? 1u : add);
-                }
-                tensor_commit(lead, empty(s));
-                add = 1u;
-                if (++s == S::kStages) { s = 0; parity ^= 1u; }
+                for (int w = 0; w < S::kWeights; ++w) copy_scales<1>(lead, sf + w * 8 + h * 4, scale_desc(stage + w * kMx4TileBytes) + 32 * h);
+                copy_scales<1>(lead, sfx + h * 4, scale_desc(x) + 32 * h);
             }
-            if (u < end) break;
-            tensor_commit(lead, acc_full(b));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {      // 32 bytes on: two in the descriptors' unit
+#pragma unroll
+                for (int w = 0; w < S::kWeights; ++w)
+                    mx4_multiply<1>(lead, tmem + w * TOKENS, operand_desc(stage + w * kMx4TileBytes + kMx4ScaleBytes) + 2 * j,
+                                    operand_desc(x + kMx4ScaleBytes) + 2 * j, mx4_instruction(128, TOKENS, (j & 1) * 2),
+                                    sf + w * 8 + (j >> 1) * 4, sfx + (j >> 1) * 4, j ? 1u : add);
+            }
+            tensor_commit(lead, empty(s));
+            add = 1u;
+            if (++s == S::kStages) { s = 0; parity ^= 1u; }
         }
+        if (ok) tensor_commit(lead, acc_full);
         tensor_commit(lead, drained);
         warp_wait(drained, 0, &failed);
-    } else {
+    } else if (warp < kStreamWarps) {
         const int quarter = warp & 3;
-        uint32_t* counters = p.workspace + 4096 / 4;
-        float* partials = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.workspace) + kMx4PartialOffset);
-        int segment = 0;
-        for (int64_t u = run.first; u < run.last; ++segment) {
-            const int64_t tile = u / chunks, from = tile * chunks, to = from + chunks;
-            const int64_t end = to < run.last ? to : run.last;
-            const int b = segment % S::kBuffers;
-            if (!warp_wait(acc_full(b), (uint32_t)(segment / S::kBuffers) & 1u, &failed)) break;
-            __syncwarp();
-            tensor_fence_after();
-            const int row_tile = (int)(tile / p.token_tiles);
-            const int64_t token0 = (tile % p.token_tiles) * TOKENS;
-            const uint32_t acc = tmem + b * S::kAcc + ((uint32_t)quarter << 21);
-            const bool whole = u == from && end == to;
-            constexpr int64_t kSlot = (int64_t)S::kAcc * 128;
-            float* mine = partials + (2 * (int64_t)blockIdx.x + (segment ? 1 : 0)) * kSlot + quarter * 32 + lane;
-            float v[16], up[16];
+        if (warp_wait(acc_full, 0, &failed)) {
+            const uint32_t acc = tmem + ((uint32_t)quarter << 21);
+            float* mine = reinterpret_cast<float*>(ring_bytes) + quarter * 32 + lane;      // what it held has been multiplied
 #pragma unroll 1
-            for (int c = 0; c < TOKENS; c += 16) {
-                if (token0 + c >= p.tokens) break;
+            for (int c = 0; c < TOKENS && token0 + c < p.tokens; c += 16) {
+                float v[16], up[16];
                 __syncwarp();
+                tensor_fence_after();
                 tmem_load16(acc + c, v);
                 if (GATED) tmem_load16(acc + TOKENS + c, up);
-                if (whole) {
-                    finish16<GATED>(p, row_tile, quarter, lane, token0 + c, v, up);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (p.parts > 1) {
+                        mine[(c + i) * 128] = v[i];
+                        if (GATED) mine[(TOKENS + c + i) * 128] = up[i];
+                    } else if (token0 + c + i < p.tokens) {
+                        finish<GATED>(p, row_tile, quarter, lane, token0 + c + i, v[i], GATED ? up[i] : 0.f);
+                    }
+                }
+            }
+        }
+    } else {
+        // Each has one stage, and so sees every phase of its barriers: a wait for a parity is right only for who has seen the phase before.
+        const int rows = (int)min((int64_t)TOKENS, p.tokens - token0), s = warp - kStreamWarps;
+        uint8_t* to = ring_bytes + s * S::kStageBytes + S::kWeights * kMx4TileBytes;
+        griddep_wait();
+        for (int i = s; i < k1 - k0; i += S::kStages) {
+            const int64_t c = (int64_t)(k0 + i) * kMx4Cols + lane * 8, left = p.cols - c;
+            const bool simple = p.x_vec && p.x_dtype != MPS_F32 && (int64_t)(k0 + i + 1) * kMx4Cols <= p.cols;
+            bool ok = true;
+            for (int r = 0; r < rows; r += 4) {
+                Raw8 raw[4];
+                if (simple) {       // no branch between the loads, so that they are under way together
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        raw[j].a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + (token0 + min(r + j, rows - 1)) * p.x_stride + c);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        __stcg(mine + (c + i) * 128, v[i]);
-                        if (GATED) __stcg(mine + (TOKENS + c + i) * 128, up[i]);
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        raw[j] = load_raw8(p.x, p.x_dtype, (token0 + r + j) * p.x_stride + c, r + j >= rows ? 0 : left > 8 ? 8 : (int)left, p.x_vec);
+                }
+                if (r == 0 && i >= S::kStages) ok = warp_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed);
+                if (!ok) break;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (r + j >= rows) break;
+                    float v[8];
+                    unpack8(raw[j], p.x_dtype, v);
+                    mx4_store_row(to, r + j, lane, v);
                 }
             }
-            tensor_fence_before();
+            if (!ok) break;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written here
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(b));
-            if (!whole) {
-                // every warp's 32 features are counted by themselves, so that no barrier is needed
-                const int c0 = cta_of(units, from, gridDim.x), c1 = cta_of(units, to - 1, gridDim.x);
-                uint32_t before = 0u;
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) before = atomicAdd(&counters[c0 * 4 + quarter], 1u);
-                before = __shfl_sync(0xFFFFFFFFu, before, 0);
-                if (before == (uint32_t)(c1 - c0)) {
-                    __threadfence();
-                    if (lane == 0) counters[c0 * 4 + quarter] = 0u;
-                    // c0's part is its last segment, the others' their first; c0 has only one segment where its run begins inside the tile
-                    const int64_t at0 = 2 * (int64_t)c0 + (run_of(units, c0, gridDim.x).first / chunks == tile ? 0 : 1);
-#pragma unroll 1
-                    for (int c = 0; c < TOKENS; c += 16) {
-                        if (token0 + c >= p.tokens) break;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = up[i] = 0.f;
-                        for (int g = c0; g <= c1; ++g) {
-                            const float* from_g = partials + (g == c0 ? at0 : 2 * (int64_t)g) * kSlot + quarter * 32 + lane;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                v[i] += __ldcg(from_g + (c + i) * 128);
-                                if (GATED) up[i] += __ldcg(from_g + (TOKENS + c + i) * 128);
-                            }
-                        }
-                        finish16<GATED>(p, row_tile, quarter, lane, token0 + c, v, up);
-                    }
-                }
-            }
-            u = end;
+            if (lane == 0) mbar_arrive(full(s));
         }
     }
     __syncwarp();
     tensor_fence_before();
+    if (p.parts > 1) {
+        cluster_sync();
+        if (warp >= 2 && warp < kStreamWarps && !failed) {
+            // every CTA adds up a share: some tokens of 32 features a step, all parts of them under way together
+            constexpr int kStep = TOKENS < 32 ? 4 : 8;
+            const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
+            for (int i = part * 4 + warp - 2; i < 4 * ((tokens + kStep - 1) / kStep); i += 4 * p.parts) {
+                const int c = (i >> 2) * kStep, quarter = i & 3;
+                float v[kStep], up[kStep];
+#pragma unroll
+                for (int j = 0; j < kStep; ++j) v[j] = up[j] = 0.f;
+#pragma unroll
+                for (int g = 0; g < kMostParts; ++g) {
+                    if (g < p.parts) {
+                        const uint32_t from = peer_address(ring + (c * 128 + quarter * 32 + lane) * 4, g);
+#pragma unroll
+                        for (int j = 0; j < kStep; ++j) {
+                            v[j] += load_peer(from + j * 512);
+                            if (GATED) up[j] += load_peer(from + (TOKENS + j) * 512);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kStep; ++j)
+                    if (c + j < tokens) finish<GATED>(p, row_tile, quarter, lane, token0 + c + j, v[j], up[j]);
+            }
+        }
+        __syncwarp();
+        cluster_sync();      // nobody leaves while his part is read
+    }
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
-    if (warp == 1) tmem_free<1>(tmem_slot, S::kColumns);
+    if (warp == 1) tmem_free<1>(tmem, S::kColumns);
 }
 
 // ---- many tokens: tokens on the accumulator's lanes ------------------------------------------------
@@ -437,7 +425,8 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
         if (lane == 0) {
             int64_t i = 0;
             bool ok = true;
-            if (p.x_follows) asm volatile("griddepcontrol.wait;" ::: "memory");
+            griddep_wait();
+            griddep_launch();
             for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
                 const WideTile t = wide_tile(tile, p.token_tiles);
                 // what lies beyond the last tile of 128 is multiplied as the last and not stored
@@ -580,47 +569,54 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
     if (warp == 1) tmem_free<2>(tmem_slot, S::kColumns);
 }
 
+// Every launch may begin while the kernel before it in its stream ends: what it reads of it, and all it writes, comes after griddep_wait.
+// What is set once per kernel and device is remembered in `ready`, a bit a device.
 template <typename Kernel, typename... More>
-static int launch_product(Kernel kernel, int smem, int threads, int ctas, cudaStream_t st, const ProductArgs& p, More... more) {
-    MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+static int launch_product(Kernel kernel, std::atomic<uint64_t>& ready, const Device& d, int smem, int threads, int ctas, int cluster, cudaStream_t st,
+                          const ProductArgs& p, More... more) {
+    if (!(ready.load(std::memory_order_relaxed) >> d.ordinal & 1)) {
+        MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        ready.fetch_or(uint64_t(1) << d.ordinal, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)ctas);
     config.blockDim = dim3((unsigned)threads);
     config.dynamicSmemBytes = (size_t)smem;
     config.stream = st;
-    cudaLaunchAttribute overlap;
-    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &overlap;
-    config.numAttrs = p.x_follows ? 1 : 0;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = (unsigned)cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p, more...));
     return MPS_OK;
 }
 
-template <int TOKENS, bool GATED>
-static int launch_stream(ProductArgs p, int sms, cudaStream_t st) {
+template <int TOKENS, bool GATED, bool QUANTIZE = false>
+static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
     using S = StreamShape<TOKENS, GATED>;
+    static std::atomic<uint64_t> ready{0};
     p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
-    const int64_t units = (int64_t)p.row_tiles * p.token_tiles * p.chunks;
-    return launch_product(mx4_stream_kernel<TOKENS, GATED>, S::kSmem, kStreamThreads, (int)(units < sms ? units : sms), st, p);
+    const int64_t tiles = (int64_t)p.row_tiles * p.token_tiles;
+    if (tiles * kMostParts > 0x7FFFFFFF) { set_error("mps_mx4_product: output too large"); return MPS_ERR_INVALID; }
+    p.parts = (int)(2 * d.sms / tiles);
+    p.parts = p.parts < 1 ? 1 : p.parts > kMostParts ? kMostParts : p.parts;
+    if (p.parts > p.chunks) p.parts = p.chunks;
+    return launch_product(mx4_stream_kernel<TOKENS, GATED, QUANTIZE>, ready, d, S::kSmem, (kStreamWarps + (QUANTIZE ? S::kStages : 0)) * 32,
+                          (int)tiles * p.parts, p.parts, st, p);
 }
 
 template <bool GATED>
-static int launch_wide(ProductArgs p, int sms, cudaStream_t st) {
+static int launch_wide(ProductArgs p, const Device& d, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
     p.token_tiles = (int)((p.tokens + 255) / 256);
     const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
-    const int pairs = (int)(tiles < sms / 2 ? tiles : sms / 2);
+    const int pairs = (int)(tiles < d.sms / 2 ? tiles : d.sms / 2);
     const bool even = p.out_dtype != MPS_MX4 && p.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
-    return launch_product(mx4_wide_kernel<GATED>, WideShape::kSmem, kWideThreads, 2 * pairs, st, p, even);
-}
-
-
-static int sm_count(int* sms) {
-    int dev = 0;
-    MPS_CUDA_TRY(cudaGetDevice(&dev));
-    MPS_CUDA_TRY(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
-    if (*sms > kMx4MostSms) *sms = kMx4MostSms;
-    return MPS_OK;
+    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p, even);
 }
 
 }  // namespace mps
@@ -646,18 +642,30 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     if (a.w_up && a.activation != MPS_SILU && a.activation != MPS_GELU_TANH) { set_error("mps_mx4_product: unknown activation %d", (int)a.activation); return MPS_ERR_INVALID; }
     if (a.tokens == 0) return MPS_OK;
     if (!workspace || workspace_bytes < kMx4WorkspaceBytes) { set_error("workspace missing or too small"); return MPS_ERR_WORKSPACE; }
-    const void* tiles = a.x_dtype == MPS_MX4 ? a.x : a.x_tiles;
-    if (!a.x || !tiles || !a.w || !a.out) { set_error("mps_mx4_product: null pointer"); return MPS_ERR_INVALID; }
-    if (((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.w_up) |
+    if (!a.x || !a.w || !a.out) { set_error("mps_mx4_product: null pointer"); return MPS_ERR_INVALID; }
+    const bool quantized = a.x_dtype == MPS_MX4, inside = !quantized && a.tokens <= kMostQuantizedInside;
+    const void* tiles = a.x;
+    if (!quantized && !inside) {
+        tiles = a.x_tiles;
+        if (!tiles) {
+            if (mps_mx4_bytes(a.tokens, a.cols) > kMx4WorkspaceBytes - kMx4ScratchOffset) {
+                set_error("mps_mx4_product: x_tiles missing");
+                return MPS_ERR_WORKSPACE;
+            }
+            tiles = static_cast<uint8_t*>(workspace) + kMx4ScratchOffset;
+        }
+    }
+    if (((reinterpret_cast<uintptr_t>(inside ? nullptr : tiles) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.w_up) |
           (a.out_dtype == MPS_MX4 ? reinterpret_cast<uintptr_t>(a.out) : 0)) & 15u) || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {
         set_error("mps_mx4_product: tiles must be 16-byte aligned, the workspace 256");
         return MPS_ERR_INVALID;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    int sms = 0, rc = sm_count(&sms);
+    Device d;
+    int rc = current_device(d);
     if (rc) return rc;
-    if (a.x_dtype != MPS_MX4) {
-        rc = mps_mx4_quantize(a.x, a.x_dtype, a.tokens, a.cols, a.x_stride, a.x_tiles, stream);
+    if (!quantized && !inside) {
+        rc = mps_mx4_quantize(a.x, a.x_dtype, a.tokens, a.cols, a.x_stride, const_cast<void*>(tiles), stream);
         if (rc) return rc;
     }
     ProductArgs p = {};
@@ -667,24 +675,30 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     p.out = a.out;
     p.workspace = static_cast<uint32_t*>(workspace);
     p.out_stride = a.out_stride;
+    p.x_stride = a.x_stride;
     p.tokens = a.tokens;
     p.rows = (int32_t)a.rows;
+    p.cols = (int32_t)a.cols;
     p.chunks = (int32_t)mx4_chunks(a.cols);
     p.row_tiles = (int32_t)mx4_row_tiles(a.rows);
+    p.x_dtype = a.x_dtype;
     p.out_dtype = a.out_dtype;
     p.activation = a.activation;
-    p.x_follows = a.x_dtype != MPS_MX4;
-    if (a.tokens > 128) return a.w_up ? launch_wide<true>(p, sms, st) : launch_wide<false>(p, sms, st);
+    p.x_vec = inside && mx4_vec_ok(a.x, a.x_stride, a.x_dtype);
+    p.early = (!quantized && !inside) || a.weights_ready;
     if (a.w_up) {
-        if (a.tokens <= 16) return launch_stream<16, true>(p, sms, st);
-        if (a.tokens <= 32) return launch_stream<32, true>(p, sms, st);
-        if (a.tokens <= 64) return launch_stream<64, true>(p, sms, st);
-        return launch_stream<128, true>(p, sms, st);
+        if (inside) return launch_stream<16, true, true>(p, d, st);
+        if (a.tokens <= 16) return launch_stream<16, true>(p, d, st);
+        if (a.tokens <= 32) return launch_stream<32, true>(p, d, st);
+        if (a.tokens <= 64) return launch_stream<64, true>(p, d, st);
+        return launch_wide<true>(p, d, st);
     }
-    if (a.tokens <= 16) return launch_stream<16, false>(p, sms, st);
-    if (a.tokens <= 32) return launch_stream<32, false>(p, sms, st);
-    if (a.tokens <= 64) return launch_stream<64, false>(p, sms, st);
-    return launch_stream<128, false>(p, sms, st);
+    if (inside) return launch_stream<16, false, true>(p, d, st);
+    if (a.tokens <= 16) return launch_stream<16, false>(p, d, st);
+    if (a.tokens <= 32) return launch_stream<32, false>(p, d, st);
+    if (a.tokens <= 64) return launch_stream<64, false>(p, d, st);
+    if (a.tokens <= 128) return launch_stream<128, false>(p, d, st);
+    return launch_wide<false>(p, d, st);
 }
 
 int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out) {
@@ -693,7 +707,7 @@ int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32
     uint32_t flag = 0;
     MPS_CUDA_TRY(cudaMemcpyAsync(&flag, workspace, sizeof(flag), cudaMemcpyDeviceToHost, st));
     MPS_CUDA_TRY(cudaStreamSynchronize(st));
-    if (flag) MPS_CUDA_TRY(cudaMemsetAsync(workspace, 0, (size_t)kMx4PartialOffset, st));
+    if (flag) MPS_CUDA_TRY(cudaMemsetAsync(workspace, 0, sizeof(flag), st));
     *timed_out = flag ? 1 : 0;
     return MPS_OK;
 }

@@ -40,6 +40,8 @@ template <int STEPS>
 __global__ void __launch_bounds__(kNormMostThreads)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
+    griddep_wait();
+    griddep_launch();
     const mps_mx4_norm& a = p.a;
     const int64_t row = blockIdx.x;
     const int cols = (int)a.cols;
@@ -122,8 +124,6 @@ mx4_norm_kernel(const NormArgs p) {
     }
 }
 
-int launched(const char* what);
-
 }  // namespace mps
 
 using namespace mps;
@@ -163,10 +163,9 @@ extern "C" int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned int rows = (unsigned int)a.rows;
     switch (steps) {
-        case 1: mx4_norm_kernel<1><<<rows, threads, 0, st>>>(p); break;
-        case 2: mx4_norm_kernel<2><<<rows, threads, 0, st>>>(p); break;
-        case 4: mx4_norm_kernel<4><<<rows, threads, 0, st>>>(p); break;
-        default: mx4_norm_kernel<8><<<rows, threads, 0, st>>>(p); break;
+        case 1: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<1>, rows, threads, st, p);
+        case 2: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<2>, rows, threads, st, p);
+        case 4: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<4>, rows, threads, st, p);
+        default: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<8>, rows, threads, st, p);
     }
-    return launched("mx4_norm_kernel");
 }

@@ -92,6 +92,17 @@ __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
         "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
 }
+// Another CTA's shared memory, at the place that has this address in one's own.
+__device__ __forceinline__ uint32_t peer_address(uint32_t smem, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float load_peer(uint32_t address) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -26,65 +26,67 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 _MOST_NORM_COLS = 32768
 
+# Of the products' workspace, what x_tiles may take (include/mpserve_b200.h).
+_SCRATCH = 480 * 17408
+
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_stream_of = torch._C._cuda_getCurrentRawStream      # the current stream's handle by device index, without an object around it
+_current_device = torch._C._cuda_getDevice
 
 
-def _workspace(device: torch.device, stream: int) -> torch.Tensor:
-    """Zeroed counters and partial sums, one per (device, stream); the products hand the counters back zeroed."""
-    key = (device.index, stream)
-    ws = _workspaces.get(key)
+def _workspace(index: int, stream: int) -> torch.Tensor:
+    """Scratch of the products, one per (device, stream), as they hand it back."""
+    ws = _workspaces.get((index, stream))
     if ws is None:
-        ws = torch.zeros(int(_lib.load().mps_mx4_workspace_bytes()), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
+        ws = torch.zeros(int(_lib.load().mps_mx4_workspace_bytes()), dtype=torch.uint8, device=torch.device("cuda", index))
+        _workspaces[index, stream] = ws
     return ws
 
 
-class _on:
-    """The device of the inputs, and its current stream's handle."""
-
-    def __init__(self, device: torch.device):
-        self.device = device
-        self.other = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self) -> int:
-        if self.other is not None:
-            self.other.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
+def _launch(index: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device ``index``."""
+    if _current_device() == index:
+        rc = fn(*args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream_of(index))
+    if rc:
+        _lib.check(rc)
 
 
-def _matrix(t, name: str) -> tuple[torch.Tensor, int, int, int]:
-    """``t`` as rows x columns of unit column stride: (tensor, rows, cols, row stride)."""
+def _matrix(t, name: str) -> tuple[int, int, int]:
+    """``t`` as rows x columns of unit column stride: (rows, cols, row stride)."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be bfloat16, float16 or float32")
-    if t.dim() == 2:
-        rows, cols = t.shape
-        if cols > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
+        stride, unit = t.stride()
+        if cols > 1 and unit != 1:
             raise ValueError(f"{name} must have unit stride along its last dimension")
-        stride = t.stride(0) if rows > 1 else cols
-        if stride < 0 or cols == 0:
+        if cols == 0:
             raise ValueError(f"{name} must have at least one column")
-        return t, rows, cols, stride
-    if t.dim() == 0 or t.shape[-1] == 0:
+        return rows, cols, stride if rows > 1 else cols
+    if len(shape) == 0 or shape[-1] == 0:
         raise ValueError(f"{name} must have at least one dimension and one column")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous where it is not a matrix")
-    cols = t.shape[-1]
-    return t, t.numel() // cols, cols, cols
+    cols = shape[-1]
+    return t.numel() // cols, cols, cols
+
+
+def _tile_bytes(rows: int, cols: int) -> int:
+    if rows > 1 << 31 or cols > 1 << 24:
+        raise ValueError("an MXFP4 matrix has at most 2^31 rows and 2^24 columns")
+    return (rows + 127) // 128 * ((cols + 255) // 256) * 17408
 
 
 def _tiles(rows: int, cols: int, device: torch.device) -> torch.Tensor:
-    nbytes = int(_lib.load().mps_mx4_bytes(rows, cols))
-    if nbytes < 0:
-        raise ValueError("an MXFP4 matrix has at most 2^31 rows and 2^24 columns")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return torch.empty(_tile_bytes(rows, cols), dtype=torch.uint8, device=device)
 
 
 class Mx4Tensor:
@@ -113,8 +115,7 @@ class Mx4Tensor:
         dev = self.device
         codes = torch.empty((self.rows, (self.cols + 1) // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty((self.rows, -(-self.cols // BLOCK)), dtype=torch.uint8, device=dev)
-        with _on(dev) as stream:
-            _lib.check(_lib.load().mps_mx4_unpack(self.data.data_ptr(), self.rows, self.cols, codes.data_ptr(), scales.data_ptr(), stream))
+        _launch(dev.index, _lib.load().mps_mx4_unpack, self.data.data_ptr(), self.rows, self.cols, codes.data_ptr(), scales.data_ptr())
         return codes, scales
 
 
@@ -128,11 +129,10 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
 
     A block's scale is 2^(floor(log2 max) - 2); codes are rounded to nearest, halfway to the even code, and saturate at 6.  A
     block with an infinity or a NaN becomes NaN."""
-    x, rows, cols, stride = _matrix(x, "x")
+    rows, cols, stride = _matrix(x, "x")
     dev = x.device
     data = _tiles(rows, cols, dev)
-    with _on(dev) as s:
-        _lib.check(_lib.load().mps_mx4_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr(), s))
+    _launch(dev.index, _lib.load().mps_mx4_quantize, x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr())
     return Mx4Tensor(data, rows, cols, x.shape)
 
 
@@ -141,10 +141,9 @@ def dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
     _check_mx4(q, "q")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
-    dev = q.device
+    dev = q.data.device
     out = torch.empty(q.shape, dtype=dtype, device=dev)
-    with _on(dev) as s:
-        _lib.check(_lib.load().mps_mx4_dequantize(q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr(), s))
+    _launch(dev.index, _lib.load().mps_mx4_dequantize, q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -167,55 +166,67 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
         raise ValueError("codes and scales must have the same rows and device")
     rows, dev = codes.shape[0], codes.device
     data = _tiles(rows, cols, dev)
-    with _on(dev) as s:
-        _lib.check(_lib.load().mps_mx4_pack(codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr(), s))
+    _launch(dev.index, _lib.load().mps_mx4_pack, codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr())
     return Mx4Tensor(data, rows, cols)
 
 
 # ---- products --------------------------------------------------------------------------------------------
 
-def _product(x, w, w_up, activation: int, dtype, quantized: bool):
+def _run_product(args, index: int) -> None:
+    stream = _stream_of(index)
+    ws = _workspace(index, stream)
+    rc = _lib.load().mps_mx4_product(C.byref(args), ws.data_ptr(), ws.numel(), stream)
+    if rc:
+        _lib.check(rc)
+
+
+def _product(x, w, w_up, activation: int, dtype, quantized: bool, weights_ready: bool = False):
+    """``weights_ready``: what was launched last on the stream wrote no weight (a block's own norm or product)."""
     _check_mx4(w, "w" if w_up is None else "w_gate")
+    out_cols, w_cols, dev = w.rows, w.cols, w.data.device
+    up = None
     if w_up is not None:
         _check_mx4(w_up, "w_up")
-        if (w_up.rows, w_up.cols) != (w.rows, w.cols):
+        if w_up.rows != out_cols or w_up.cols != w_cols:
             raise ValueError("w_gate and w_up must have the same shape")
-    if w.rows == 0:
+        if w_up.data.device != dev:
+            raise ValueError("all tensors must be on the same CUDA device")
+        up = w_up.data.data_ptr()
+    if out_cols == 0:
         raise ValueError("a weight must have at least one row")
-    dev = w.device
-    a = _lib.Mx4Linear()
+    tiles, stride = None, 0
     if isinstance(x, Mx4Tensor):
-        rows, cols, tiles = x.rows, x.cols, None
-        a.x, a.x_dtype = x.data.data_ptr(), _MX4
+        rows, cols, x_dtype, data = x.rows, x.cols, _MX4, x.data
         if dtype is None:
             dtype = torch.bfloat16
     else:
-        x, rows, cols, a.x_stride = _matrix(x, "x")
+        rows, cols, stride = _matrix(x, "x")
+        data, x_dtype = x, _DTYPES[x.dtype]
         if dtype is None:
-            dtype = torch.bfloat16 if x.dtype == torch.float32 else x.dtype
-        tiles = _tiles(rows, cols, dev)
-        a.x, a.x_dtype, a.x_tiles = x.data_ptr(), _DTYPES[x.dtype], tiles.data_ptr()
-    if cols != w.cols:
-        raise ValueError(f"x has {cols} columns, the weight {w.cols}")
-    if x.device != dev or (w_up is not None and w_up.device != dev):
+            dtype = torch.bfloat16 if x_dtype == 2 else x.dtype
+        if _tile_bytes(rows, cols) > _SCRATCH:
+            tiles = _tiles(rows, cols, dev)
+    if cols != w_cols:
+        raise ValueError(f"x has {cols} columns, the weight {w_cols}")
+    if data.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    shape = (*x.shape[:-1], w.rows)
+    shape = (*x.shape[:-1], out_cols)
     if quantized:
-        out = _tiles(rows, w.rows, dev)
-        a.out, a.out_dtype = out.data_ptr(), _MX4
-        result = Mx4Tensor(out, rows, w.rows, shape)
+        out = _tiles(rows, out_cols, dev)
+        out_dtype, result = _MX4, Mx4Tensor(out, rows, out_cols, shape)
     else:
-        if dtype not in (torch.bfloat16, torch.float16):
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError("a product's dtype must be bfloat16 or float16")
-        result = torch.empty(shape, dtype=dtype, device=dev)
-        a.out, a.out_dtype, a.out_stride = result.data_ptr(), _DTYPES[dtype], w.rows
-    a.w = w.data.data_ptr()
-    if w_up is not None:
-        a.w_up = w_up.data.data_ptr()
-    a.tokens, a.cols, a.rows, a.activation = rows, cols, w.rows, activation
-    with _on(dev) as s:
-        ws = _workspace(dev, s)
-        _lib.check(_lib.load().mps_mx4_product(C.byref(a), ws.data_ptr(), ws.numel(), s))
+        out = result = torch.empty(shape, dtype=dtype, device=dev)
+        out_dtype = _DTYPES[dtype]
+    args = _lib.Mx4Linear(data.data_ptr(), None if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
+                          stride, out_cols, x_dtype, out_dtype, activation, weights_ready)
+    index = dev.index
+    if _current_device() == index:
+        _run_product(args, index)
+    else:
+        with torch.cuda.device(index):
+            _run_product(args, index)
     return result
 
 
@@ -241,24 +252,24 @@ def gated_linear(x, w_gate: Mx4Tensor, w_up: Mx4Tensor, *, activation: str = "si
 def product_timed_out(device: torch.device | None = None) -> bool:
     """Waits for the current stream and tells whether a product launched on it since the last call gave up on one of its bounded
     waits (its outputs are then incomplete).  Always False in normal operation."""
-    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    with _on(dev) as s:
-        ws = _workspace(dev, s)
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    with torch.cuda.device(index):
+        stream = _stream_of(index)
+        ws = _workspace(index, stream)
         flag = C.c_int32(0)
-        _lib.check(_lib.load().mps_mx4_status(ws.data_ptr(), ws.numel(), s, C.byref(flag)))
+        _lib.check(_lib.load().mps_mx4_status(ws.data_ptr(), ws.numel(), stream, C.byref(flag)))
     return bool(flag.value)
 
 
 # ---- norms, gate and residual ------------------------------------------------------------------------------
 
-def _gain(t, name: str, cols: int, dev, a) -> int:
+def _gain(t, name: str, cols: int, dev) -> int:
     if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.shape[0] != cols:
         raise ValueError(f"{name} must be a bfloat16, float16 or float32 vector of {cols} values")
     if t.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    if cols > 1 and t.stride(0) != 1:
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
@@ -268,36 +279,29 @@ def _check_norm_cols(cols: int) -> None:
         raise ValueError(f"a norm has at most {_MOST_NORM_COLS} columns")
 
 
-def _normed(a, shape, rows, cols, dtype, dev, quantized: bool):
+def _normed(shape, rows, cols, dtype, dev, quantized: bool):
+    """Where a norm's result goes: (what the caller gets, pointer, dtype)."""
     if quantized:
         data = _tiles(rows, cols, dev)
-        a.n_out, a.n_dtype = data.data_ptr(), _MX4
-        return Mx4Tensor(data, rows, cols, shape)
+        return Mx4Tensor(data, rows, cols, shape), data.data_ptr(), _MX4
     n = torch.empty(shape, dtype=dtype, device=dev)
-    a.n_out, a.n_dtype, a.n_stride = n.data_ptr(), _DTYPES[dtype], cols
-    return n
-
-
-def _launch_norm(a, dev) -> None:
-    with _on(dev) as s:
-        _lib.check(_lib.load().mps_mx4_norm_rows(C.byref(a), s))
+    return n, n.data_ptr(), _DTYPES[dtype]
 
 
 def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype: torch.dtype | None = None, quantized: bool = False):
     """``h * rsqrt(mean(h^2) + eps) * weight`` along the last dimension, in ``dtype`` (by default ``h``'s) or, ``quantized``, as an
     ``Mx4Tensor`` that never was anything but FP32 before."""
-    h, rows, cols, stride = _matrix(h, "h")
+    rows, cols, stride = _matrix(h, "h")
     _check_norm_cols(cols)
     dtype = h.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
     dev = h.device
-    a = _lib.Mx4Norm()
-    a.next_weight, a.weight_dtype = _gain(weight, "weight", cols, dev, a), _DTYPES[weight.dtype]
-    a.h, a.h_stride, a.h_dtype = h.data_ptr(), stride, _DTYPES[h.dtype]
-    a.rows, a.cols, a.eps, a.residual_scale = rows, cols, eps, 1.0
-    n = _normed(a, h.shape, rows, cols, dtype, dev, quantized)
-    _launch_norm(a, dev)
+    w = _gain(weight, "weight", cols, dev)
+    n, n_ptr, n_dtype = _normed(h.shape, rows, cols, dtype, dev, quantized)
+    args = _lib.Mx4Norm(None, h.data_ptr(), None, None, w, None, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
+                        _DTYPES[weight.dtype], eps, 1.0)
+    _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
     return n
 
 
@@ -312,37 +316,36 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
     Returns ``(h', n)``; ``n`` is None without ``next_weight``, in ``y``'s dtype otherwise or, ``quantized``, an ``Mx4Tensor``.
     ``gate``: None, or any shape that broadcasts to ``y``'s with one value per column, per row or per element.  ``h`` may be
     FP32 beside a 16-bit ``y``; ``h'`` has its type, and is ``h`` itself where ``inplace``.  The two weights share a dtype."""
-    y, rows, cols, y_stride = _matrix(y, "y")
-    h, h_rows, h_cols, h_stride = _matrix(h, "h")
-    if y.shape != h.shape:
+    rows, cols, y_stride = _matrix(y, "y")
+    _, _, h_stride = _matrix(h, "h")
+    shape, dev = y.shape, y.device
+    if shape != h.shape:
         raise ValueError("y and h must have the same shape")
     _check_norm_cols(cols)
-    dev = y.device
     if h.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    a = _lib.Mx4Norm()
+    post = nxt = g = n = n_ptr = None
+    weight_dtype = n_dtype = g_dtype = g_row = g_col = 0
     if post_weight is not None:
-        a.post_weight, a.weight_dtype = _gain(post_weight, "post_weight", cols, dev, a), _DTYPES[post_weight.dtype]
+        post, weight_dtype = _gain(post_weight, "post_weight", cols, dev), _DTYPES[post_weight.dtype]
     if next_weight is not None:
-        a.next_weight = _gain(next_weight, "next_weight", cols, dev, a)
+        nxt = _gain(next_weight, "next_weight", cols, dev)
         if post_weight is not None and post_weight.dtype != next_weight.dtype:
             raise ValueError("post_weight and next_weight must have the same dtype")
-        a.weight_dtype = _DTYPES[next_weight.dtype]
+        weight_dtype = _DTYPES[next_weight.dtype]
     if gate is not None:
-        a.gate, a.gate_dtype, a.gate_row_stride, a.gate_col_stride = _gate(gate, y, rows, cols)
-    a.y, a.y_stride, a.y_dtype = y.data_ptr(), y_stride, _DTYPES[y.dtype]
-    a.h, a.h_stride, a.h_dtype = h.data_ptr(), h_stride, _DTYPES[h.dtype]
+        g, g_dtype, g_row, g_col = _gate(gate, y, rows, cols)
     if inplace:
-        joined = h
+        joined, out_stride = h, h_stride
         if rows > 1 and h_stride < cols:
             raise ValueError("h has rows that share memory and cannot be updated in place")
-        a.h_out, a.h_out_stride = h.data_ptr(), h_stride
     else:
-        joined = torch.empty(h.shape, dtype=h.dtype, device=dev)
-        a.h_out, a.h_out_stride = joined.data_ptr(), cols
-    a.rows, a.cols, a.eps, a.residual_scale = rows, cols, eps, residual_scale
-    n = None if next_weight is None else _normed(a, y.shape, rows, cols, y.dtype, dev, quantized)
-    _launch_norm(a, dev)
+        joined, out_stride = torch.empty(shape, dtype=h.dtype, device=dev), cols
+    if nxt is not None:
+        n, n_ptr, n_dtype = _normed(shape, rows, cols, y.dtype, dev, quantized)
+    args = _lib.Mx4Norm(y.data_ptr(), h.data_ptr(), post, g, nxt, joined.data_ptr(), n_ptr, rows, cols, y_stride, h_stride, out_stride, cols, g_row,
+                        g_col, _DTYPES[y.dtype], _DTYPES[h.dtype], n_dtype, g_dtype, weight_dtype, eps, residual_scale)
+    _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
     return joined, n
 
 
@@ -352,14 +355,15 @@ def _gate(gate, y, rows: int, cols: int):
         raise ValueError("gate must be a bfloat16, float16 or float32 tensor")
     if gate.device != y.device:
         raise ValueError("all tensors must be on the same CUDA device")
-    shape = (1,) * (y.dim() - gate.dim()) + tuple(gate.shape)
-    if len(shape) == y.dim() and gate.is_contiguous() and shape[-1] in (1, cols):
-        lead = gate.numel() // shape[-1]
-        per_column = shape[-1] == cols and cols > 1
-        if lead == 1:
-            return gate.data_ptr(), _DTYPES[gate.dtype], 0, int(per_column)
-        if shape[:-1] == tuple(y.shape[:-1]):
-            return gate.data_ptr(), _DTYPES[gate.dtype], shape[-1], int(per_column)
+    if gate.dim() <= y.dim() and gate.is_contiguous():
+        shape = (1,) * (y.dim() - gate.dim()) + tuple(gate.shape)
+        last = shape[-1]
+        if last == 1 or last == cols:
+            per_column = int(last == cols and cols > 1)
+            if gate.numel() == last:
+                return gate.data_ptr(), _DTYPES[gate.dtype], 0, per_column
+            if shape[:-1] == tuple(y.shape[:-1]):
+                return gate.data_ptr(), _DTYPES[gate.dtype], last, per_column
     raise ValueError("gate must be contiguous and have one value per column, per row or per element of y")
 
 
@@ -384,8 +388,9 @@ class GatedMlp:
 
     def forward(self, h: torch.Tensor, *, inplace: bool = False):
         x = rms_norm(h, self.pre_weight, eps=self.eps, quantized=True)
-        a = gated_linear(x, self.gate_proj, self.up_proj, activation=self.activation, quantized=True)
-        y = linear(a, self.down_proj, dtype=torch.bfloat16 if h.dtype == torch.float32 else h.dtype)
+        # the kernel before each product is this block's own: no weight comes out of it
+        a = _product(x, self.gate_proj, self.up_proj, _ACTIVATIONS[self.activation], None, True, True)
+        y = _product(a, self.down_proj, None, 0, torch.bfloat16 if h.dtype == torch.float32 else h.dtype, False, True)
         return block_join(y, h, post_weight=self.post_weight, gate=self.gate, residual_scale=self.residual_scale,
                           next_weight=self.next_weight, eps=self.eps, inplace=inplace)
 

@@ -54,6 +54,31 @@ def test_linear(tokens, cols, rows):
     assert mx4.product_timed_out() is False
 
 
+# so many rows that a tile of the output is one CTA's, whose ring goes round several times over the columns
+@pytest.mark.parametrize("tokens,cols,rows", [(1, 5000, 38000), (9, 8192, 20000), (16, 4097, 37900), (40, 3000, 38000), (64, 6144, 20000), (128, 4096, 19999)])
+def test_linear_with_long_rows_in_one_cta(tokens, cols, rows):
+    x, w = _inputs(tokens, cols, rows, 11)
+    ref.poison()
+    y = mx4.linear(x, w)
+    q = mx4.quantize(x)
+    pick = torch.randint(0, rows, (1500,), device="cuda")
+    want = _values(q) @ _sampled(w, pick).t()
+    off = _values(q).abs() @ _sampled(w, pick).abs().t() * ((cols / 32 + 256) * 2.0 ** -23) + want.abs() * ref.ROUND[torch.bfloat16] * (1 + 2.0 ** -8)
+    assert ((y[:, pick].double() - want).abs() <= off).all()
+    assert torch.equal(y, mx4.linear(q, w)) and torch.equal(y, mx4.linear(x, w))
+    gated = mx4.gated_linear(x, w, w)
+    assert torch.equal(gated, mx4.gated_linear(q, w, w))
+    want, off = _gated_off(_values(q), _sampled(w, pick), _sampled(w, pick), "silu")
+    assert ((gated[:, pick].double() - want).abs() <= off + want.abs() * ref.ROUND[torch.bfloat16] * (1 + 2.0 ** -8)).all()
+    assert mx4.product_timed_out() is False
+
+
+def _sampled(w, rows):
+    """Some of a weight's rows, as values in 64 bits."""
+    codes, scales = w.parts()
+    return torch.from_numpy(ref.decode(ref.unpack(codes[rows].cpu().numpy(), w.cols), scales[rows].cpu().numpy())).cuda()
+
+
 @pytest.mark.parametrize("tokens,cols,rows", [(1, 512, 300), (40, 1000, 129), (300, 640, 517)])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_linear_types(tokens, cols, rows, dtype):
