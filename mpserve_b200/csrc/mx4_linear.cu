@@ -28,6 +28,7 @@ struct ProductArgs {
     int32_t row_tiles, token_tiles, parts;
     int32_t x_dtype, out_dtype, activation;
     bool x_vec;
+    bool even;               // rows of a 16-bit output begin at multiples of 16 bytes
     bool early;              // the kernel before writes no weight: weights may be read before it is done
 };
 
@@ -57,7 +58,7 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // ---- few tokens: weights on the accumulator's lanes -------------------------------------------------
 //
 // A CTA streams the weight tiles of 128 features through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
-// product's narrow side.  Two CTAs share an SM, and a cluster of up to eight shares the columns of one tile of the output, as many as
+// product's narrow side.  Two CTAs share an SM, and a cluster of up to four shares the columns of one tile of the output, as many as
 // fill the GPU: then every SM has some 200 KB under way, and all end together.  The parts of a tile meet in the cluster's shared memory,
 // where every CTA adds up a share of them, always in the same order.
 //
@@ -82,33 +83,50 @@ struct StreamShape {
 };
 constexpr int kStreamWarps = 6;
 constexpr int kMostQuantizedInside = 16;       // tokens that the kernel quantises itself
-constexpr int kMostParts = 8;                  // CTAs of a cluster, on any device
+constexpr int kMostParts = 4;                  // CTAs of a cluster
 
-// One token of a warp's 32 features, `up` too where the pair is gated, into the output.
+// One token of a tile's 128 features, four neighbouring ones a lane (`up` too where the pair is gated), into the output.
 template <bool GATED>
-__device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int quarter, int lane, int64_t token, float v, float up) {
-    const int first = row_tile * kMx4Rows + quarter * 32, feature = first + lane;
-    if (GATED) v = act(v, p.activation) * up;
+__device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int lane, int64_t token, float4 v, float4 up) {
+    const int first = row_tile * kMx4Rows + lane * 4, valid = p.rows - first;
+    float f[4] = {v.x, v.y, v.z, v.w};
+    if (GATED) {
+        const float u[4] = {up.x, up.y, up.z, up.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = i < valid ? act(f[i], p.activation) * u[i] : 0.f;
+    }
     if (GATED && p.out_dtype == MPS_MX4) {
-        // the 32 features are one block
-        const int chunks = (int)mx4_chunks(p.rows), block = (first % kMx4Cols) / kMx4Block, row = (int)(token % kMx4Rows);
-        const float f = feature < p.rows ? v : 0.f;
-        const uint32_t byte = mx4_scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f) & 0x7FFFFFFFu));
-        const float q[8] = {byte == 255u ? 0.f : f * mx4_inverse_scale(byte), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t code = mx4_codes8(q) & 15u;
-        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 1) << 4;    // right in the even lanes, then in every fourth, then in every eighth
-        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 2) << 8;
-        code |= __shfl_xor_sync(0xFFFFFFFFu, code, 4) << 16;
-        uint8_t* tile = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, first / kMx4Cols, chunks);
-        if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block) + (lane >> 3) * 4) = code;
-        if (lane == 0) tile[mx4_scale_offset(row, block >> 2) + (block & 3)] = (uint8_t)byte;
-        if (row_tile == p.row_tiles - 1 && (row_tile & 1) == 0) {
+        // eight lanes hold a block
+        uint32_t m = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 1; o < 8; o *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        const uint32_t byte = mx4_scale_byte(m);
+        const float inverse = mx4_inverse_scale(byte);
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = i < 4 && byte != 255u ? f[i & 3] * inverse : 0.f;
+        const int part = row_tile & 1, block = part * 4 + (lane >> 3), row = (int)(token % kMx4Rows);
+        uint8_t* tile = static_cast<uint8_t*>(p.out) + mx4_tile_offset(token / kMx4Rows, row_tile >> 1, mx4_chunks(p.rows));
+        *reinterpret_cast<uint16_t*>(tile + mx4_code_offset(row, block) + (lane & 7) * 2) = (uint16_t)mx4_codes8(q);
+        if ((lane & 7) == 0) tile[mx4_scale_offset(row, part) + (lane >> 3)] = (uint8_t)byte;
+        if (row_tile == p.row_tiles - 1 && part == 0) {
             // the second half of the last tile lies beyond the last feature and is filled up with zeros
-            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, block + 4) + (lane >> 3) * 4) = 0u;
-            if (lane == 0) tile[mx4_scale_offset(row, 1) + (block & 3)] = 0u;
+            *reinterpret_cast<uint16_t*>(tile + mx4_code_offset(row, block + 4) + (lane & 7) * 2) = 0;
+            if (lane == 0) *reinterpret_cast<uint32_t*>(tile + mx4_scale_offset(row, 1)) = 0u;
         }
-    } else if (feature < p.rows) {
-        static_cast<uint16_t*>(p.out)[token * p.out_stride + feature] = (uint16_t)pack2(v, 0.f, p.out_dtype);
+        return;
+    }
+    uint16_t* out = static_cast<uint16_t*>(p.out) + token * p.out_stride + first;
+    const uint2 w = make_uint2(pack2(f[0], f[1], p.out_dtype), pack2(f[2], f[3], p.out_dtype));
+    if (valid >= 4 && p.even) {
+        *reinterpret_cast<uint2*>(out) = w;
+    } else {
+        if (valid > 0) out[0] = (uint16_t)w.x;
+        if (valid > 1) out[1] = (uint16_t)(w.x >> 16);
+        if (valid > 2) out[2] = (uint16_t)w.y;
+        if (valid > 3) out[3] = (uint16_t)(w.y >> 16);
     }
 }
 
@@ -211,26 +229,18 @@ mx4_stream_kernel(const ProductArgs p) {
         tensor_commit(lead, drained);
         warp_wait(drained, 0, &failed);
     } else if (warp < kStreamWarps) {
-        const int quarter = warp & 3;
+        // the accumulator, token by token, to where the ring was: what that held has been multiplied
+        const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21), to = ring + ((warp & 3) * 32 + lane) * 4;
         if (warp_wait(acc_full, 0, &failed)) {
-            const uint32_t acc = tmem + ((uint32_t)quarter << 21);
-            float* mine = reinterpret_cast<float*>(ring_bytes) + quarter * 32 + lane;      // what it held has been multiplied
+            tensor_fence_after();
+            const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
 #pragma unroll 1
-            for (int c = 0; c < TOKENS && token0 + c < p.tokens; c += 16) {
-                float v[16], up[16];
-                __syncwarp();
-                tensor_fence_after();
+            for (int c = 0; c < S::kAcc; c += 16) {
+                if (c % TOKENS >= tokens) continue;
+                float v[16];
                 tmem_load16(acc + c, v);
-                if (GATED) tmem_load16(acc + TOKENS + c, up);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (p.parts > 1) {
-                        mine[(c + i) * 128] = v[i];
-                        if (GATED) mine[(TOKENS + c + i) * 128] = up[i];
-                    } else if (token0 + c + i < p.tokens) {
-                        finish<GATED>(p, row_tile, quarter, lane, token0 + c + i, v[i], GATED ? up[i] : 0.f);
-                    }
-                }
+                for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (c + i) * 512), "f"(v[i]) : "memory");
             }
         }
     } else {
@@ -271,36 +281,27 @@ mx4_stream_kernel(const ProductArgs p) {
     }
     __syncwarp();
     tensor_fence_before();
-    if (p.parts > 1) {
-        cluster_sync();
-        if (warp >= 2 && warp < kStreamWarps && !failed) {
-            // every CTA adds up a share: some tokens of 32 features a step, all parts of them under way together
-            constexpr int kStep = TOKENS < 32 ? 4 : 8;
-            const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
-            for (int i = part * 4 + warp - 2; i < 4 * ((tokens + kStep - 1) / kStep); i += 4 * p.parts) {
-                const int c = (i >> 2) * kStep, quarter = i & 3;
-                float v[kStep], up[kStep];
+    if (p.parts > 1) cluster_sync(); else __syncthreads();
+    if (!failed) {
+        // the parts meet: every warp of the cluster takes a token in turn (the code is short on purpose: it runs once, and what it costs is
+        // to fetch it)
+        const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0), warps = blockDim.x >> 5;
+#pragma unroll 1
+        for (int c = warp * p.parts + part; c < tokens; c += warps * p.parts) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), up = v;
 #pragma unroll
-                for (int j = 0; j < kStep; ++j) v[j] = up[j] = 0.f;
-#pragma unroll
-                for (int g = 0; g < kMostParts; ++g) {
-                    if (g < p.parts) {
-                        const uint32_t from = peer_address(ring + (c * 128 + quarter * 32 + lane) * 4, g);
-#pragma unroll
-                        for (int j = 0; j < kStep; ++j) {
-                            v[j] += load_peer(from + j * 512);
-                            if (GATED) up[j] += load_peer(from + (TOKENS + j) * 512);
-                        }
-                    }
+            for (int g = 0; g < kMostParts; ++g) {
+                if (g < p.parts) {
+                    const uint32_t from = p.parts > 1 ? peer_address(ring + c * 512 + lane * 16, g) : ring + c * 512 + lane * 16;
+                    add4(v, load_peer(from));
+                    if (GATED) add4(up, load_peer(from + TOKENS * 512));
                 }
-#pragma unroll
-                for (int j = 0; j < kStep; ++j)
-                    if (c + j < tokens) finish<GATED>(p, row_tile, quarter, lane, token0 + c + j, v[j], up[j]);
             }
+            finish<GATED>(p, row_tile, lane, token0 + c, v, up);
         }
-        __syncwarp();
-        cluster_sync();      // nobody leaves while his part is read
     }
+    __syncwarp();
+    if (p.parts > 1) cluster_sync();      // nobody leaves while his part is read
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
@@ -389,7 +390,7 @@ __device__ __forceinline__ void store_rows(uint32_t buffer, int lane, const uint
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
-mx4_wide_kernel(const ProductArgs p, const bool even) {
+mx4_wide_kernel(const ProductArgs p) {
     using S = WideShape;
     extern __shared__ __align__(1024) uint8_t ring_bytes[];      // all of the shared memory: rings begin at multiples of 1024
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -540,7 +541,7 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) w[i] = pack2(g[2 * i], g[2 * i + 1], p.out_dtype);
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) store_rows(buffer, lane, w + c / 2, rows + first + c, p.out_stride, tokens, valid - c, even);
+                    for (int c = 0; c < 64; c += 32) store_rows(buffer, lane, w + c / 2, rows + first + c, p.out_stride, tokens, valid - c, p.even);
                 }
             } else {
                 uint32_t w[64];
@@ -555,7 +556,7 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
 #pragma unroll
                 for (int c = 0; c < 128; c += 32) {
                     const int first = t.feature * 256 + half * 128 + c;
-                    store_rows(buffer, lane, w + c / 2, rows + first, p.out_stride, tokens, p.rows - first, even);
+                    store_rows(buffer, lane, w + c / 2, rows + first, p.out_stride, tokens, p.rows - first, p.even);
                 }
             }
         }
@@ -571,11 +572,11 @@ mx4_wide_kernel(const ProductArgs p, const bool even) {
 
 // Every launch may begin while the kernel before it in its stream ends: what it reads of it, and all it writes, comes after griddep_wait.
 // What is set once per kernel and device is remembered in `ready`, a bit a device.
-template <typename Kernel, typename... More>
-static int launch_product(Kernel kernel, std::atomic<uint64_t>& ready, const Device& d, int smem, int threads, int ctas, int cluster, cudaStream_t st,
-                          const ProductArgs& p, More... more) {
+static int launch_product(void (*kernel)(ProductArgs), std::atomic<uint64_t>& ready, const Device& d, int smem, int threads, int ctas, int cluster,
+                          cudaStream_t st, const ProductArgs& p) {
     if (!(ready.load(std::memory_order_relaxed) >> d.ordinal & 1)) {
         MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
         ready.fetch_or(uint64_t(1) << d.ordinal, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t config = {};
@@ -591,7 +592,7 @@ static int launch_product(Kernel kernel, std::atomic<uint64_t>& ready, const Dev
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = cluster > 1 ? 2 : 1;
-    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p, more...));
+    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
     return MPS_OK;
 }
 
@@ -615,8 +616,7 @@ static int launch_wide(ProductArgs p, const Device& d, cudaStream_t st) {
     p.token_tiles = (int)((p.tokens + 255) / 256);
     const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
     const int pairs = (int)(tiles < d.sms / 2 ? tiles : d.sms / 2);
-    const bool even = p.out_dtype != MPS_MX4 && p.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
-    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p, even);
+    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p);
 }
 
 }  // namespace mps
@@ -685,6 +685,7 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     p.out_dtype = a.out_dtype;
     p.activation = a.activation;
     p.x_vec = inside && mx4_vec_ok(a.x, a.x_stride, a.x_dtype);
+    p.even = a.out_dtype != MPS_MX4 && a.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
     p.early = (!quantized && !inside) || a.weights_ready;
     if (a.w_up) {
         if (inside) return launch_stream<16, true, true>(p, d, st);
