@@ -129,6 +129,23 @@ __device__ __forceinline__ void store8(void* __restrict__ base, int dtype, int64
     }
 }
 
+// A warp's 256 neighbouring values, eight a lane, into a row that begins anywhere: by way of 1 KB of shared memory, so that neighbouring
+// lanes store neighbouring elements.  (Stored by the lanes that hold them, every instruction would touch 32 pieces: 2047 x 1337 FP32 took 14 us
+// that way.)  All 32 lanes take part; elements from `valid` on, counted from the warp's first, are not stored.
+__device__ __forceinline__ void store_span(void* __restrict__ base, int dtype, int64_t at, int valid, float* __restrict__ buffer, int lane, const float (&v)[8]) {
+    __syncwarp();
+    reinterpret_cast<float4*>(buffer)[2 * lane] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(buffer)[2 * lane + 1] = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int e = i * 32 + lane;
+        if (e >= valid) break;
+        if (dtype == MPS_F32) static_cast<float*>(base)[at + e] = buffer[e];
+        else static_cast<uint16_t*>(base)[at + e] = (uint16_t)pack2(buffer[e], 0.f, dtype);
+    }
+}
+
 // ---- codes ------------------------------------------------------------------------------------------
 
 // Scale byte of a block whose largest magnitude has these bits.  An exponent field of e stands for 2^(e - 127), so the byte of
@@ -181,22 +198,21 @@ __device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
     return m;
 }
 
-// A warp quantises and stores one row of a tile: lane l holds columns 8 l to 8 l + 7 (zeros beyond the matrix).  Four lanes share a
-// block; 128 bytes of codes go out in one piece, the scales as two words.  All 32 lanes take part.
-__device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int row, int lane, const float (&v)[8]) {
-    uint32_t m = max_bits8(v);
+// A warp quantises and stores one row of a tile: lane l holds columns 8 l to 8 l + 7 (zeros beyond the matrix), `m` the bits of the largest of
+// its magnitudes.  Four lanes share a block; 128 bytes of codes go out in one piece.  All 32 lanes take part.
+__device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int row, int lane, const float (&v)[8], uint32_t m) {
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
     const uint32_t byte = mx4_scale_byte(m);
     const float inverse = mx4_inverse_scale(byte);
     float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = byte == 255u ? 0.f : v[i] * inverse;
+    for (int i = 0; i < 8; ++i) q[i] = v[i] * inverse;      // of a NaN block, whatever it gives: its codes say nothing
     *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, lane >> 2) + (lane & 3) * 4) = mx4_codes8(q);
-    uint32_t w = byte << (8 * ((lane >> 2) & 3));
-    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
-    if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx4_scale_offset(row, lane >> 4)) = w;
+    if ((lane & 3) == 0) tile[mx4_scale_offset(row, lane >> 4) + ((lane >> 2) & 3)] = (uint8_t)byte;
+}
+__device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int row, int lane, const float (&v)[8]) {
+    mx4_store_row(tile, row, lane, v, max_bits8(v));
 }
 
 // The kernels of these operators may be launched while the kernel before them in the stream ends.  A kernel waits for that one before it reads what

@@ -20,57 +20,69 @@ static __device__ __forceinline__ bool convert_place(int64_t rows, int segments,
     return p.row < rows;
 }
 
-__global__ void __launch_bounds__(kConvertThreads)
-mx4_quantize_kernel(const void* __restrict__ x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, bool vec, int chunks,
-                    int segments, uint8_t* __restrict__ out) {
-    griddep_wait();
-    griddep_launch();
-    ConvertPlace p;
-    if (!convert_place(rows, segments, p)) return;
-    const int lane = threadIdx.x & 31;
-    Raw8 raw[kConvertChunks];
-#pragma unroll
-    for (int i = 0; i < kConvertChunks; ++i) {
-        const int64_t c = (p.chunk0 + i) * kMx4Cols + lane * 8, left = cols - c;
-        raw[i] = load_raw8(x, dtype, p.row * row_stride + c, left > 8 ? 8 : (int)left, vec);
-    }
-#pragma unroll
-    for (int i = 0; i < kConvertChunks; ++i) {
-        if (p.chunk0 + i >= chunks) break;
-        float v[8];
-        unpack8(raw[i], dtype, v);
-        mx4_store_row(out + mx4_tile_offset(p.row / kMx4Rows, p.chunk0 + i, chunks), (int)(p.row % kMx4Rows), lane, v);
-    }
+// The largest magnitude's bits, as FP32, of eight values as they were loaded: BF16 compares as it is, two at a time.
+template <int DTYPE>
+__device__ __forceinline__ uint32_t raw_max_bits(const Raw8& r, const float (&v)[8]) {
+    if (DTYPE != MPS_BF16) return max_bits8(v);
+    const uint32_t a = __vmaxu2(__vmaxu2(r.a.x & 0x7FFF7FFFu, r.a.y & 0x7FFF7FFFu), __vmaxu2(r.a.z & 0x7FFF7FFFu, r.a.w & 0x7FFF7FFFu));
+    return max(a & 0xFFFF0000u, a << 16);
 }
 
+template <int DTYPE>
 __global__ void __launch_bounds__(kConvertThreads)
-mx4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int chunks, int segments, int dtype, bool vec,
-                      void* __restrict__ out) {
+mx4_quantize_kernel(const void* __restrict__ x, int64_t rows, int64_t cols, int64_t row_stride, bool vec, int chunks, int segments,
+                    uint8_t* __restrict__ out) {
     griddep_wait();
     griddep_launch();
     ConvertPlace p;
     if (!convert_place(rows, segments, p)) return;
     const int lane = threadIdx.x & 31, row = (int)(p.row % kMx4Rows);
+    Raw8 raw[kConvertChunks];
+#pragma unroll
+    for (int i = 0; i < kConvertChunks; ++i) {
+        const int64_t c = (p.chunk0 + i) * kMx4Cols + lane * 8, left = cols - c;
+        raw[i] = load_raw8(x, DTYPE, p.row * row_stride + c, left > 8 ? 8 : (int)left, vec);
+    }
+    uint8_t* tile = out + mx4_tile_offset(p.row / kMx4Rows, p.chunk0, chunks);
+#pragma unroll
+    for (int i = 0; i < kConvertChunks; ++i, tile += kMx4TileBytes) {
+        if (p.chunk0 + i >= chunks) break;
+        float v[8];
+        unpack8(raw[i], DTYPE, v);
+        mx4_store_row(tile, row, lane, v, raw_max_bits<DTYPE>(raw[i], v));
+    }
+}
+
+template <int DTYPE>
+__global__ void __launch_bounds__(kConvertThreads)
+mx4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols, int chunks, int segments, bool vec, void* __restrict__ out) {
+    __shared__ __align__(16) float buffers[kConvertThreads / 32][256];
+    griddep_wait();
+    griddep_launch();
+    ConvertPlace p;
+    if (!convert_place(rows, segments, p)) return;
+    const int lane = threadIdx.x & 31, row = (int)(p.row % kMx4Rows);
+    const uint8_t* tile = q + mx4_tile_offset(p.row / kMx4Rows, p.chunk0, chunks);
     uint32_t codes[kConvertChunks], scale[kConvertChunks];
 #pragma unroll
     for (int i = 0; i < kConvertChunks; ++i) {
         codes[i] = scale[i] = 0u;
         if (p.chunk0 + i < chunks) {
-            const uint8_t* tile = q + mx4_tile_offset(p.row / kMx4Rows, p.chunk0 + i, chunks);
-            codes[i] = *reinterpret_cast<const uint32_t*>(tile + mx4_code_offset(row, lane >> 2) + (lane & 3) * 4);
-            scale[i] = tile[mx4_scale_offset(row, lane >> 4) + ((lane >> 2) & 3)];
+            codes[i] = *reinterpret_cast<const uint32_t*>(tile + i * kMx4TileBytes + mx4_code_offset(row, lane >> 2) + (lane & 3) * 4);
+            scale[i] = tile[i * kMx4TileBytes + mx4_scale_offset(row, lane >> 4) + ((lane >> 2) & 3)];
         }
     }
 #pragma unroll
     for (int i = 0; i < kConvertChunks; ++i) {
         if (p.chunk0 + i >= chunks) break;
-        const int64_t c = (p.chunk0 + i) * kMx4Cols + lane * 8, left = cols - c;
+        const int64_t c = (p.chunk0 + i) * kMx4Cols, left = cols - c;
         const float s = mx4_scale(scale[i]);
         float v[8];
         mx4_values8(codes[i], v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= s;
-        store8(out, dtype, p.row * cols + c, left > 8 ? 8 : (int)left, vec, v);
+        if (vec && left >= kMx4Cols) store8(out, DTYPE, p.row * cols + c + lane * 8, 8, true, v);
+        else store_span(out, DTYPE, p.row * cols + c, left > kMx4Cols ? kMx4Cols : (int)left, buffers[threadIdx.x >> 5], lane, v);
     }
 }
 
@@ -177,8 +189,9 @@ int mps_mx4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, i
     if (!mx4_dtype_ok(dtype)) { set_error("mps_mx4_quantize: unknown dtype %d", (int)dtype); return MPS_ERR_INVALID; }
     if (rows == 0) return MPS_OK;
     if (!x || !tiles || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_quantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    return launch_overlapping("mx4_quantize_kernel", mx4_quantize_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream), x, (int)dtype, rows,
-                              cols, row_stride, mx4_vec_ok(x, row_stride, dtype), g.chunks, g.segments, static_cast<uint8_t*>(tiles));
+    const auto kernel = dtype == MPS_BF16 ? mx4_quantize_kernel<MPS_BF16> : dtype == MPS_F16 ? mx4_quantize_kernel<MPS_F16> : mx4_quantize_kernel<MPS_F32>;
+    return launch_overlapping("mx4_quantize_kernel", kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream), x, rows, cols, row_stride,
+                              mx4_vec_ok(x, row_stride, dtype), g.chunks, g.segments, static_cast<uint8_t*>(tiles));
 }
 
 int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dtype, void* out, void* stream) {
@@ -188,8 +201,9 @@ int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dt
     if (!mx4_dtype_ok(dtype)) { set_error("mps_mx4_dequantize: unknown dtype %d", (int)dtype); return MPS_ERR_INVALID; }
     if (rows == 0) return MPS_OK;
     if (!tiles || !out || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_dequantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    return launch_overlapping("mx4_dequantize_kernel", mx4_dequantize_kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream),
-                              static_cast<const uint8_t*>(tiles), rows, cols, g.chunks, g.segments, (int)dtype, mx4_vec_ok(out, cols, dtype), out);
+    const auto kernel = dtype == MPS_BF16 ? mx4_dequantize_kernel<MPS_BF16> : dtype == MPS_F16 ? mx4_dequantize_kernel<MPS_F16> : mx4_dequantize_kernel<MPS_F32>;
+    return launch_overlapping("mx4_dequantize_kernel", kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream),
+                              static_cast<const uint8_t*>(tiles), rows, cols, g.chunks, g.segments, mx4_vec_ok(out, cols, dtype), out);
 }
 
 int mps_mx4_pack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* tiles, void* stream) {

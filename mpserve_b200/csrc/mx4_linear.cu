@@ -82,7 +82,7 @@ struct StreamShape {
     static_assert(kAcc * 128 * 4 <= kBars, "a part of the accumulator takes the ring's place");
 };
 constexpr int kStreamWarps = 6;
-constexpr int kMostQuantizedInside = 16;       // tokens that the kernel quantises itself
+constexpr int kMostQuantizedInside = 8;        // tokens that the kernel quantises itself
 constexpr int kMostParts = 4;                  // CTAs of a cluster
 
 // One token of a tile's 128 features, four neighbouring ones a lane (`up` too where the pair is gated), into the output.

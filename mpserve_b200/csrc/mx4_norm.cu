@@ -40,6 +40,9 @@ template <int STEPS>
 __global__ void __launch_bounds__(kNormMostThreads)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
+    __shared__ __align__(16) float buffers[kNormMostThreads / 32][256];
+    float* buffer = buffers[threadIdx.x >> 5];
+    const int lane = threadIdx.x & 31;
     griddep_wait();
     griddep_launch();
     const mps_mx4_norm& a = p.a;
@@ -69,7 +72,7 @@ mx4_norm_kernel(const NormArgs p) {
         sum = 0.f;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const int c = (s * blockDim.x + threadIdx.x) * 8, valid = min(cols - c, 8);
+            const int c = (s * blockDim.x + threadIdx.x) * 8, valid = min(cols - c, 8), span = c - lane * 8;    // the warp's first
             float y[8], h[8], w[8];
             unpack8(ry[s], a.y_dtype, y);
             unpack8(rh[s], a.h_dtype, h);
@@ -94,7 +97,8 @@ mx4_norm_kernel(const NormArgs p) {
                 v[s][i] = i < valid ? fmaf(a.residual_scale, h[i], y[i]) : 0.f;
                 sum = fmaf(v[s][i], v[s][i], sum);
             }
-            store8(a.h_out, a.h_dtype, row * a.h_out_stride + c, valid, p.vec_h_out, v[s]);
+            if (p.vec_h_out) store8(a.h_out, a.h_dtype, row * a.h_out_stride + c, valid, true, v[s]);
+            else store_span(a.h_out, a.h_dtype, row * a.h_out_stride + span, cols - span, buffer, lane, v[s]);
         }
         if (!a.n_out) return;
     } else {
@@ -108,7 +112,7 @@ mx4_norm_kernel(const NormArgs p) {
     const float r = 1.f / sqrtf(fmaf(row_sum(sum, slots[1]), p.inv_cols, a.eps));
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const int g = s * blockDim.x + threadIdx.x, c = g * 8, valid = min(cols - c, 8);
+        const int g = s * blockDim.x + threadIdx.x, c = g * 8, valid = min(cols - c, 8), span = c - lane * 8;
         if ((g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
         float w[8];
         unpack8(load_raw8(a.next_weight, a.weight_dtype, c, valid, p.vec_next), a.weight_dtype, w);
@@ -117,9 +121,10 @@ mx4_norm_kernel(const NormArgs p) {
         if (a.n_dtype == MPS_MX4) {
             const int chunks = (int)mx4_chunks(cols);
             mx4_store_row(static_cast<uint8_t*>(a.n_out) + mx4_tile_offset(row / kMx4Rows, c / kMx4Cols, chunks),
-                          (int)(row % kMx4Rows), threadIdx.x & 31, w);
+                          (int)(row % kMx4Rows), lane, w);
         } else {
-            store8(a.n_out, a.n_dtype, row * a.n_stride + c, valid, p.vec_n, w);
+            if (p.vec_n) store8(a.n_out, a.n_dtype, row * a.n_stride + c, valid, true, w);
+            else store_span(a.n_out, a.n_dtype, row * a.n_stride + span, cols - span, buffer, lane, w);
         }
     }
 }
