@@ -391,6 +391,25 @@ typedef struct mps_mx4_linear {
  * where mps_mx4_bytes(tokens, cols) fits into it (8 MB). */
 MPS_API int64_t mps_mx4_workspace_bytes(void);
 MPS_API int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
+/* A gated MLP block, everything but the tokens: h_out, n_out = block_join(product(gated(rms_norm(h, pre_weight)))), what passes between in MXFP4
+ * but the block's result, which has h's type (BF16 where that is FP32).  Fields as above; scratch: 256-byte aligned, contents
+ * irrelevant before and after. */
+typedef struct mps_mx4_mlp {
+    const void* gate_proj;              /* MXFP4 tiles of inter x hidden, as up_proj; down_proj of hidden x inter */
+    const void* up_proj;
+    const void* down_proj;
+    const void* pre_weight;
+    const void* post_weight;            /* or null */
+    const void* gate;                   /* or null */
+    const void* next_weight;            /* or null */
+    int64_t hidden, inter, gate_row_stride;
+    int32_t gate_col_stride, gate_dtype, pre_dtype, weight_dtype, activation;
+    float eps, residual_scale;
+} mps_mx4_mlp;
+MPS_API int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_t inter);
+MPS_API int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out,
+                              int64_t h_out_stride, void* n_out, int32_t n_dtype, void* scratch, int64_t scratch_bytes, void* workspace,
+                              int64_t workspace_bytes, void* stream);
 /* Every wait inside the products is bounded: waits for the stream, tells whether any since the last query gave up (its outputs are
  * then incomplete), and clears the record. */
 MPS_API int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out);

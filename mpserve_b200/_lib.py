@@ -55,6 +55,17 @@ class Mx4Linear(C.Structure):
     ]
 
 
+class Mx4Mlp(C.Structure):
+    """struct mps_mx4_mlp"""
+
+    _fields_ = [
+        ("gate_proj", _p), ("up_proj", _p), ("down_proj", _p), ("pre_weight", _p), ("post_weight", _p), ("gate", _p), ("next_weight", _p),
+        ("hidden", _i64), ("inter", _i64), ("gate_row_stride", _i64),
+        ("gate_col_stride", _i32), ("gate_dtype", _i32), ("pre_dtype", _i32), ("weight_dtype", _i32), ("activation", _i32),
+        ("eps", C.c_float), ("residual_scale", C.c_float),
+    ]
+
+
 _PROTOS = {
     "mps_abi_version": (C.c_int, []),
     "mps_last_error": (C.c_char_p, []),
@@ -93,6 +104,8 @@ _PROTOS = {
     "mps_mx4_norm_rows": (C.c_int, [C.POINTER(Mx4Norm), _p]),
     "mps_mx4_workspace_bytes": (_i64, []),
     "mps_mx4_product": (C.c_int, [C.POINTER(Mx4Linear), _p, _i64, _p]),
+    "mps_mx4_mlp_scratch_bytes": (_i64, [_i64, _i64, _i64]),
+    "mps_mx4_gated_mlp": (C.c_int, [C.POINTER(Mx4Mlp), _p, _i32, _i64, _i64, _p, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mps_mx4_status": (C.c_int, [_p, _i64, _p, C.POINTER(_i32)]),
     "mps_checksum_u16": (C.c_int, [_p, _i64, _p, _p]),
     "mps_build_workspace_bytes": (C.c_size_t, [_i64, _i64]),

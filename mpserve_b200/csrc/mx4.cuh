@@ -146,6 +146,28 @@ __device__ __forceinline__ void store_span(void* __restrict__ base, int dtype, i
     }
 }
 
+// And the other way: a warp's 256 neighbouring values of a row that begins anywhere, every 32nd a lane as they are loaded; then, as values, eight
+// neighbouring ones a lane.
+__device__ __forceinline__ void load_spread(const void* __restrict__ base, int dtype, int64_t at, int valid, int lane, uint32_t (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int e = i * 32 + lane;
+        w[i] = 0u;
+        if (e < valid) w[i] = dtype == MPS_F32 ? static_cast<const uint32_t*>(base)[at + e] : (uint32_t)static_cast<const uint16_t*>(base)[at + e];
+    }
+}
+__device__ __forceinline__ void gather_spread(const uint32_t (&w)[8], int dtype, float* __restrict__ buffer, int lane, float (&v)[8]) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        buffer[i * 32 + lane] = dtype == MPS_F32 ? __uint_as_float(w[i]) : dtype == MPS_BF16 ? __uint_as_float(w[i] << 16)
+                                                                                            : __half2float(__ushort_as_half((uint16_t)w[i]));
+    __syncwarp();
+    const float4 a = reinterpret_cast<const float4*>(buffer)[2 * lane], b = reinterpret_cast<const float4*>(buffer)[2 * lane + 1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
 // ---- codes ------------------------------------------------------------------------------------------
 
 // Scale byte of a block whose largest magnitude has these bits.  An exponent field of e stands for 2^(e - 127), so the byte of
@@ -235,10 +257,10 @@ int current_device(Device& d);
 
 // A launch that may overlap the end of the kernel before it.
 template <typename... Params, typename... Args>
-inline int launch_overlapping(const char* what, void (*kernel)(Params...), unsigned int ctas, int threads, cudaStream_t st, Args... args) {
+inline int launch_overlapping(const char* what, void (*kernel)(Params...), unsigned int ctas, dim3 threads, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(ctas);
-    config.blockDim = dim3((unsigned)threads);
+    config.blockDim = threads;
     config.stream = st;
     cudaLaunchAttribute overlap;
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -702,6 +702,80 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     return launch_wide<false>(p, d, st);
 }
 
+int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_t inter) {
+    const int64_t x = mps_mx4_bytes(tokens, hidden), a = mps_mx4_bytes(tokens, inter);
+    return x < 0 || a < 0 ? -1 : x + a + tokens * hidden * 2;      // both are multiples of 256
+}
+
+int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out, int64_t h_out_stride,
+                      void* n_out, int32_t n_dtype, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!block || !block->gate_proj || !block->up_proj || !block->down_proj || !block->pre_weight) { set_error("mps_mx4_gated_mlp: null argument"); return MPS_ERR_INVALID; }
+    const int64_t need = mps_mx4_mlp_scratch_bytes(tokens, block->hidden, block->inter);
+    if (need < 0) { set_error("mps_mx4_gated_mlp: sizes out of range"); return MPS_ERR_INVALID; }
+    if (tokens == 0) return MPS_OK;
+    if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 255u)) { set_error("mps_mx4_gated_mlp: scratch missing, too small or unaligned"); return MPS_ERR_WORKSPACE; }
+    uint8_t* x = static_cast<uint8_t*>(scratch);
+    uint8_t* a = x + mps_mx4_bytes(tokens, block->hidden);
+    uint8_t* y = a + mps_mx4_bytes(tokens, block->inter);
+    const int32_t y_dtype = h_dtype == MPS_F32 ? MPS_BF16 : h_dtype;
+
+    mps_mx4_norm norm = {};
+    norm.h = h;
+    norm.next_weight = block->pre_weight;
+    norm.n_out = x;
+    norm.rows = tokens;
+    norm.cols = block->hidden;
+    norm.h_stride = h_stride;
+    norm.h_dtype = h_dtype;
+    norm.n_dtype = MPS_MX4;
+    norm.weight_dtype = block->pre_dtype;
+    norm.eps = block->eps;
+    norm.residual_scale = 1.f;
+    int rc = mps_mx4_norm_rows(&norm, stream);
+    if (rc) return rc;
+
+    mps_mx4_linear product = {};
+    product.x = x;
+    product.w = block->gate_proj;
+    product.w_up = block->up_proj;
+    product.out = a;
+    product.tokens = tokens;
+    product.cols = block->hidden;
+    product.rows = block->inter;
+    product.x_dtype = product.out_dtype = MPS_MX4;
+    product.activation = block->activation;
+    product.weights_ready = 1;          // the kernel before each of the two is this block's own
+    rc = mps_mx4_product(&product, workspace, workspace_bytes, stream);
+    if (rc) return rc;
+
+    product.x = a;
+    product.w = block->down_proj;
+    product.w_up = nullptr;
+    product.out = y;
+    product.cols = block->inter;
+    product.rows = product.out_stride = block->hidden;
+    product.out_dtype = y_dtype;
+    rc = mps_mx4_product(&product, workspace, workspace_bytes, stream);
+    if (rc) return rc;
+
+    norm.y = y;
+    norm.post_weight = block->post_weight;
+    norm.gate = block->gate;
+    norm.next_weight = block->next_weight;
+    norm.h_out = h_out;
+    norm.n_out = block->next_weight ? n_out : nullptr;
+    norm.y_stride = norm.n_stride = block->hidden;
+    norm.h_out_stride = h_out_stride;
+    norm.gate_row_stride = block->gate_row_stride;
+    norm.gate_col_stride = block->gate_col_stride;
+    norm.y_dtype = y_dtype;
+    norm.n_dtype = n_dtype;
+    norm.gate_dtype = block->gate_dtype;
+    norm.weight_dtype = block->weight_dtype;
+    norm.residual_scale = block->residual_scale;
+    return mps_mx4_norm_rows(&norm, stream);
+}
+
 int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out) {
     if (!timed_out || !workspace || workspace_bytes < kMx4WorkspaceBytes) { set_error("mps_mx4_status: bad argument"); return MPS_ERR_INVALID; }
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -4,15 +4,17 @@
 //   h' = residual_scale * h + gate * t                 (h' = h without y)
 //   n  = h' * rsqrt(mean(h'^2) + eps) * next_weight    (in a 16-bit type, FP32, or quantised to MXFP4)
 //
-// One CTA has one row in registers, eight neighbouring columns per lane and step, so that y and h are read once and the two means
-// cost two barriers.  All arithmetic is in FP32; h' is normalised as it was before it is rounded to the stream's type.  Four lanes
+// A CTA has one row in registers (several short ones), eight neighbouring columns per lane and step, so that y and h are read once and the two
+// means cost two barriers.  All arithmetic is in FP32; h' is normalised as it was before it is rounded to the stream's type.  Four lanes
 // hold an MXFP4 block and a warp a whole row of a tile, so the quantised form needs nothing but shuffles.
-// Bounds: memory, and for a few rows the two barriers and the launch.
+// Bounds: memory, and for a few rows the two barriers and the launch.  Weights and gate are under way with y and h: asked for after the
+// barrier that they wait behind, each would add a trip to the L2 to every row.
 #include "mx4.cuh"
 
 namespace mps {
 
-constexpr int kNormMostThreads = 512;
+constexpr int kNormThreads = 256, kNormMostThreads = 512;
+constexpr int64_t kNormManyRows = 512;
 constexpr int kNormMostCols = 32768;    // 512 threads x 8 steps x 8 columns
 
 struct NormArgs {
@@ -22,48 +24,107 @@ struct NormArgs {
     bool vec_y, vec_h, vec_post, vec_gate, vec_next, vec_h_out, vec_n;
 };
 
-// Sum over the CTA, the same in every thread.  `slot` is not used by another sum without a barrier in between.
+// Eight neighbouring elements of a 16-bit type at a multiple of 16 bytes, or zeros.
+static __device__ __forceinline__ Raw8 load_half8(const void* __restrict__ base, int64_t at, int valid) {
+    Raw8 r;
+    r.a = valid > 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at) : make_uint4(0u, 0u, 0u, 0u);
+    r.b = r.a;
+    return r;
+}
+
+// Eight columns of an operand.  VEC: columns are a multiple of 8 and every row begins at a multiple of 16 bytes; else any row, `vec` telling whether
+// this operand's do.  WIDE: FP32 (or, without VEC, whatever its dtype says).
+template <bool VEC, bool WIDE>
+struct Eight {
+    uint32_t w[8];
+    __device__ __forceinline__ void load(const void* __restrict__ base, int dtype, int64_t row, int column, int cols, bool vec, int lane) {
+        const int valid = min(cols - column, 8);
+        if (VEC || vec) {
+            const Raw8 r = VEC && !WIDE ? load_half8(base, row + column, valid) : load_raw8(base, VEC ? MPS_F32 : dtype, row + column, VEC && valid > 0 ? 8 : valid, true);
+            w[0] = r.a.x; w[1] = r.a.y; w[2] = r.a.z; w[3] = r.a.w;
+            if (WIDE) { w[4] = r.b.x; w[5] = r.b.y; w[6] = r.b.z; w[7] = r.b.w; }
+        } else {
+            load_spread(base, dtype, row + column - lane * 8, cols - column + lane * 8, lane, w);
+        }
+    }
+    __device__ __forceinline__ void values(int dtype, bool vec, float* buffer, int lane, float (&v)[8]) const {
+        if (VEC || vec) {
+            Raw8 r;
+            r.a = make_uint4(w[0], w[1], w[2], w[3]);
+            r.b = WIDE ? make_uint4(w[4], w[5], w[6], w[7]) : r.a;
+            unpack8(r, VEC ? (WIDE ? MPS_F32 : dtype == MPS_BF16 ? MPS_BF16 : MPS_F16) : dtype, v);
+        } else {
+            gather_spread(w, dtype, buffer, lane, v);
+        }
+    }
+};
+
+// Sum over a row's threads (whole warps), the same in each of them.  `slot`, a word a warp, is not used by another sum without a barrier in between.
 static __device__ __forceinline__ float row_sum(float v, float* slot) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31, first = threadIdx.y * warps;
     if (warps == 1) return v;
-    if (lane == 0) slot[threadIdx.x >> 5] = v;
+    if (lane == 0) slot[first + (threadIdx.x >> 5)] = v;
     __syncthreads();
-    v = lane < warps ? slot[lane] : 0.f;
+    v = lane < warps ? slot[first + lane] : 0.f;
 #pragma unroll
     for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return __shfl_sync(0xFFFFFFFFu, v, 0);
 }
 
-template <int STEPS>
-__global__ void __launch_bounds__(kNormMostThreads)
+template <int STEPS, bool VEC, bool WIDE_Y, bool WIDE_H, bool WIDE_W>
+__global__ void __launch_bounds__(kNormMostThreads, STEPS == 1 ? 2 : 1)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
-    __shared__ __align__(16) float buffers[kNormMostThreads / 32][256];
-    float* buffer = buffers[threadIdx.x >> 5];
-    const int lane = threadIdx.x & 31;
+    __shared__ __align__(16) float buffers[VEC ? 1 : kNormMostThreads / 32][256];
+    constexpr bool kAhead = STEPS <= 2;      // with more, the registers are for y and h
     griddep_wait();
     griddep_launch();
     const mps_mx4_norm& a = p.a;
-    const int64_t row = blockIdx.x;
-    const int cols = (int)a.cols;
-    Raw8 ry[STEPS], rh[STEPS];
+    const int per_row = blockDim.x, place = threadIdx.x, warp = (threadIdx.y * blockDim.x + threadIdx.x) >> 5;
+    float* buffer = buffers[VEC ? 0 : warp];
+    const int lane = threadIdx.x & 31, cols = (int)a.cols;
+    const int64_t own_row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const bool live = own_row < a.rows;                    // whole warps; the last CTA may have rows too many, which repeat the last and store nothing
+    const int64_t row = live ? own_row : a.rows - 1;
+    const auto column = [&](int s) { return (s * per_row + place) * 8; };
+    Eight<VEC, WIDE_Y> ry[STEPS];
+    Eight<VEC, WIDE_H> rh[STEPS];
+    Eight<VEC, WIDE_W> post[STEPS], gate[STEPS], next[STEPS];
+    const auto load_post = [&](int s) { if (a.y && a.post_weight) post[s].load(a.post_weight, a.weight_dtype, 0, column(s), cols, p.vec_post, lane); };
+    const auto load_gate = [&](int s) {
+        if (a.y && a.gate && a.gate_col_stride) gate[s].load(a.gate, a.gate_dtype, row * a.gate_row_stride, column(s), cols, p.vec_gate, lane);
+    };
+    const auto load_next = [&](int s) { if (a.next_weight) next[s].load(a.next_weight, a.weight_dtype, 0, column(s), cols, p.vec_next, lane); };
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const int c = (s * blockDim.x + threadIdx.x) * 8, valid = min(cols - c, 8);
-        if (a.y) ry[s] = load_raw8(a.y, a.y_dtype, row * a.y_stride + c, valid, p.vec_y);
-        rh[s] = load_raw8(a.h, a.h_dtype, row * a.h_stride + c, valid, p.vec_h);
+        if (a.y) ry[s].load(a.y, a.y_dtype, row * a.y_stride, column(s), cols, p.vec_y, lane);
+        rh[s].load(a.h, a.h_dtype, row * a.h_stride, column(s), cols, p.vec_h, lane);
+    }
+    if (kAhead) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            load_post(s);
+            load_gate(s);
+            load_next(s);
+        }
     }
     float v[STEPS][8];
     float sum = 0.f;
     if (a.y) {
+        float row_gate = 1.f;      // one gate for the row
+        if (a.gate && !a.gate_col_stride) {
+            float w[8];
+            unpack8(load_raw8(a.gate, a.gate_dtype, row * a.gate_row_stride, 1, false), a.gate_dtype, w);
+            row_gate = w[0];
+        }
         float r = 1.f;
         if (a.post_weight) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 float y[8];
-                unpack8(ry[s], a.y_dtype, y);
+                ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) sum = fmaf(y[i], y[i], sum);
             }
@@ -72,39 +133,43 @@ mx4_norm_kernel(const NormArgs p) {
         sum = 0.f;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            const int c = (s * blockDim.x + threadIdx.x) * 8, valid = min(cols - c, 8), span = c - lane * 8;    // the warp's first
             float y[8], h[8], w[8];
-            unpack8(ry[s], a.y_dtype, y);
-            unpack8(rh[s], a.h_dtype, h);
+            ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y);
+            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, h);
             if (a.post_weight) {
-                unpack8(load_raw8(a.post_weight, a.weight_dtype, c, valid, p.vec_post), a.weight_dtype, w);
+                if (!kAhead) load_post(s);
+                post[s].values(a.weight_dtype, p.vec_post, buffer, lane, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] *= r * w[i];
             }
-            if (a.gate) {
-                if (a.gate_col_stride) {
-                    unpack8(load_raw8(a.gate, a.gate_dtype, row * a.gate_row_stride + c, valid, p.vec_gate), a.gate_dtype, w);
-                } else {
-                    unpack8(load_raw8(a.gate, a.gate_dtype, row * a.gate_row_stride, 1, false), a.gate_dtype, w);
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) w[i] = w[0];
-                }
+            if (a.gate && a.gate_col_stride) {
+                if (!kAhead) load_gate(s);
+                gate[s].values(a.gate_dtype, p.vec_gate, buffer, lane, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] *= w[i];
+            } else if (a.gate) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] *= row_gate;
             }
+            const int left = cols - column(s);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                v[s][i] = i < valid ? fmaf(a.residual_scale, h[i], y[i]) : 0.f;
+                v[s][i] = i < left ? fmaf(a.residual_scale, h[i], y[i]) : 0.f;
                 sum = fmaf(v[s][i], v[s][i], sum);
             }
-            if (p.vec_h_out) store8(a.h_out, a.h_dtype, row * a.h_out_stride + c, valid, true, v[s]);
-            else store_span(a.h_out, a.h_dtype, row * a.h_out_stride + span, cols - span, buffer, lane, v[s]);
+            if (!live) continue;
+            if (VEC || p.vec_h_out) {
+                store8(a.h_out, a.h_dtype, row * a.h_out_stride + column(s), left, true, v[s]);
+            } else {
+                const int first = column(s) - lane * 8;      // the warp's
+                store_span(a.h_out, a.h_dtype, row * a.h_out_stride + first, cols - first, buffer, lane, v[s]);
+            }
         }
         if (!a.n_out) return;
     } else {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            unpack8(rh[s], a.h_dtype, v[s]);
+            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, v[s]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fmaf(v[s][i], v[s][i], sum);
         }
@@ -112,21 +177,41 @@ mx4_norm_kernel(const NormArgs p) {
     const float r = 1.f / sqrtf(fmaf(row_sum(sum, slots[1]), p.inv_cols, a.eps));
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const int g = s * blockDim.x + threadIdx.x, c = g * 8, valid = min(cols - c, 8), span = c - lane * 8;
-        if ((g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
+        const int g = s * per_row + place, left = cols - g * 8;
+        if (!live || (g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
         float w[8];
-        unpack8(load_raw8(a.next_weight, a.weight_dtype, c, valid, p.vec_next), a.weight_dtype, w);
+        if (!kAhead) load_next(s);
+        next[s].values(a.weight_dtype, p.vec_next, buffer, lane, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = i < valid ? v[s][i] * r * w[i] : 0.f;
+        for (int i = 0; i < 8; ++i) w[i] = i < left ? v[s][i] * r * w[i] : 0.f;
         if (a.n_dtype == MPS_MX4) {
             const int chunks = (int)mx4_chunks(cols);
-            mx4_store_row(static_cast<uint8_t*>(a.n_out) + mx4_tile_offset(row / kMx4Rows, c / kMx4Cols, chunks),
-                          (int)(row % kMx4Rows), lane, w);
+            mx4_store_row(static_cast<uint8_t*>(a.n_out) + mx4_tile_offset(row / kMx4Rows, g >> 5, chunks), (int)(row % kMx4Rows), lane, w);
+        } else if (VEC || p.vec_n) {
+            store8(a.n_out, a.n_dtype, row * a.n_stride + g * 8, left, true, w);
         } else {
-            if (p.vec_n) store8(a.n_out, a.n_dtype, row * a.n_stride + c, valid, true, w);
-            else store_span(a.n_out, a.n_dtype, row * a.n_stride + span, cols - span, buffer, lane, w);
+            const int first = (g - lane) * 8;
+            store_span(a.n_out, a.n_dtype, row * a.n_stride + first, cols - first, buffer, lane, w);
         }
     }
+}
+
+template <int STEPS>
+static int launch_norm(const NormArgs& p, bool vec, bool wide_w, int per_row, cudaStream_t st) {
+    const mps_mx4_norm& a = p.a;
+    // short rows share a CTA: 20000 of 512 columns 22 us with a CTA each
+    const int rows_per_cta = per_row >= kNormThreads ? 1 : kNormThreads / per_row;
+    const bool wide_y = a.y && a.y_dtype == MPS_F32, wide_h = a.h_dtype == MPS_F32;
+    void (*kernel)(NormArgs) = mx4_norm_kernel<STEPS, false, true, true, true>;
+    if (vec) {
+        static void (*const fast[8])(NormArgs) = {
+            mx4_norm_kernel<STEPS, true, false, false, false>, mx4_norm_kernel<STEPS, true, false, false, true>,
+            mx4_norm_kernel<STEPS, true, false, true, false>,  mx4_norm_kernel<STEPS, true, false, true, true>,
+            mx4_norm_kernel<STEPS, true, true, false, false>,  mx4_norm_kernel<STEPS, true, true, false, true>,
+            mx4_norm_kernel<STEPS, true, true, true, false>,   mx4_norm_kernel<STEPS, true, true, true, true>};
+        kernel = fast[wide_y * 4 + wide_h * 2 + wide_w];
+    }
+    return launch_overlapping("mx4_norm_kernel", kernel, (unsigned int)((a.rows + rows_per_cta - 1) / rows_per_cta), dim3(per_row, rows_per_cta), st, p);
 }
 
 }  // namespace mps
@@ -162,15 +247,23 @@ extern "C" int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream) {
     p.vec_gate = a.gate && mx4_vec_ok(a.gate, a.gate_row_stride, a.gate_dtype);
     p.vec_h_out = a.h_out && mx4_vec_ok(a.h_out, a.h_out_stride, a.h_dtype);
     p.vec_n = a.n_out && a.n_dtype != MPS_MX4 && mx4_vec_ok(a.n_out, a.n_stride, a.n_dtype);
+    // the weights, and a gate that has columns, share a width in the kernels for aligned rows
+    const bool column_gate = a.y && a.gate && a.gate_col_stride, weights = a.next_weight || (a.y && a.post_weight);
+    const bool wide_w = weights ? a.weight_dtype == MPS_F32 : column_gate && a.gate_dtype == MPS_F32;
+    const bool vec = a.cols % 8 == 0 && p.vec_h && (!a.y || (p.vec_y && p.vec_h_out)) && (!a.n_out || a.n_dtype == MPS_MX4 || p.vec_n) &&
+                     (!a.y || !a.post_weight || p.vec_post) && (!a.next_weight || p.vec_next) &&
+                     (!column_gate || (p.vec_gate && (a.gate_dtype == MPS_F32) == wide_w));
+    // 256 threads for a row where there are many rows (8191 x 4096: 68 us, with 512 78 us), 512 where a few wait for their own length (64 x 4096: 2.7 us,
+    // with 256 3.0 us) or where 256 would hold 32 columns each and more (2048 x 14336: 55 us, with 256 79 us)
+    const int most = a.rows < kNormManyRows ? kNormMostThreads : p.groups <= 64 ? 32 : p.groups <= 4 * kNormThreads ? kNormThreads : kNormMostThreads;
     int steps = 1;
-    while ((p.groups + steps - 1) / steps > kNormMostThreads) steps *= 2;
-    const int threads = ((p.groups + steps - 1) / steps + 31) / 32 * 32;
+    while ((p.groups + steps - 1) / steps > most) steps *= 2;
+    const int per_row = ((p.groups + steps - 1) / steps + 31) / 32 * 32;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned int rows = (unsigned int)a.rows;
     switch (steps) {
-        case 1: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<1>, rows, threads, st, p);
-        case 2: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<2>, rows, threads, st, p);
-        case 4: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<4>, rows, threads, st, p);
-        default: return launch_overlapping("mx4_norm_kernel", mx4_norm_kernel<8>, rows, threads, st, p);
+        case 1: return launch_norm<1>(p, vec, wide_w, per_row, st);
+        case 2: return launch_norm<2>(p, vec, wide_w, per_row, st);
+        case 4: return launch_norm<4>(p, vec, wide_w, per_row, st);
+        default: return launch_norm<8>(p, vec, wide_w, per_row, st);
     }
 }

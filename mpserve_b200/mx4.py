@@ -141,9 +141,8 @@ def dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
     _check_mx4(q, "q")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
-    dev = q.data.device
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
-    _launch(dev.index, _lib.load().mps_mx4_dequantize, q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
+    out = q.data.new_empty(q.shape, dtype=dtype)
+    _launch(out.device.index, _lib.load().mps_mx4_dequantize, q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -180,8 +179,7 @@ def _run_product(args, index: int) -> None:
         _lib.check(rc)
 
 
-def _product(x, w, w_up, activation: int, dtype, quantized: bool, weights_ready: bool = False):
-    """``weights_ready``: what was launched last on the stream wrote no weight (a block's own norm or product)."""
+def _product(x, w, w_up, activation: int, dtype, quantized: bool):
     _check_mx4(w, "w" if w_up is None else "w_gate")
     out_cols, w_cols, dev = w.rows, w.cols, w.data.device
     up = None
@@ -205,22 +203,22 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool, weights_ready:
         if dtype is None:
             dtype = torch.bfloat16 if x_dtype == 2 else x.dtype
         if _tile_bytes(rows, cols) > _SCRATCH:
-            tiles = _tiles(rows, cols, dev)
+            tiles = w.data.new_empty(_tile_bytes(rows, cols))
     if cols != w_cols:
         raise ValueError(f"x has {cols} columns, the weight {w_cols}")
     if data.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
     shape = (*x.shape[:-1], out_cols)
     if quantized:
-        out = _tiles(rows, out_cols, dev)
+        out = w.data.new_empty(_tile_bytes(rows, out_cols))
         out_dtype, result = _MX4, Mx4Tensor(out, rows, out_cols, shape)
     else:
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError("a product's dtype must be bfloat16 or float16")
-        out = result = torch.empty(shape, dtype=dtype, device=dev)
+        out = result = data.new_empty(shape) if data.dtype is dtype else data.new_empty(shape, dtype=dtype)
         out_dtype = _DTYPES[dtype]
     args = _lib.Mx4Linear(data.data_ptr(), None if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
-                          stride, out_cols, x_dtype, out_dtype, activation, weights_ready)
+                          stride, out_cols, x_dtype, out_dtype, activation, 0)
     index = dev.index
     if _current_device() == index:
         _run_product(args, index)
@@ -265,7 +263,7 @@ def product_timed_out(device: torch.device | None = None) -> bool:
 # ---- norms, gate and residual ------------------------------------------------------------------------------
 
 def _gain(t, name: str, cols: int, dev) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.shape[0] != cols:
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.numel() != cols:
         raise ValueError(f"{name} must be a bfloat16, float16 or float32 vector of {cols} values")
     if t.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
@@ -274,17 +272,30 @@ def _gain(t, name: str, cols: int, dev) -> int:
     return t.data_ptr()
 
 
+def _gains(post_weight, next_weight, cols: int, dev):
+    """(pointers or None, the dtype that the two share)."""
+    post = nxt = None
+    dtype = 0
+    if post_weight is not None:
+        post, dtype = _gain(post_weight, "post_weight", cols, dev), _DTYPES[post_weight.dtype]
+    if next_weight is not None:
+        nxt, dtype = _gain(next_weight, "next_weight", cols, dev), _DTYPES[next_weight.dtype]
+        if post_weight is not None and post_weight.dtype != next_weight.dtype:
+            raise ValueError("post_weight and next_weight must have the same dtype")
+    return post, nxt, dtype
+
+
 def _check_norm_cols(cols: int) -> None:
     if cols > _MOST_NORM_COLS:
         raise ValueError(f"a norm has at most {_MOST_NORM_COLS} columns")
 
 
-def _normed(shape, rows, cols, dtype, dev, quantized: bool):
-    """Where a norm's result goes: (what the caller gets, pointer, dtype)."""
+def _normed(like, rows, cols, dtype, quantized: bool):
+    """Where a norm's result goes, in ``like``'s shape: (what the caller gets, pointer, dtype)."""
     if quantized:
-        data = _tiles(rows, cols, dev)
-        return Mx4Tensor(data, rows, cols, shape), data.data_ptr(), _MX4
-    n = torch.empty(shape, dtype=dtype, device=dev)
+        data = like.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
+        return Mx4Tensor(data, rows, cols, like.shape), data.data_ptr(), _MX4
+    n = like.new_empty(like.shape) if like.dtype is dtype else like.new_empty(like.shape, dtype=dtype)
     return n, n.data_ptr(), _DTYPES[dtype]
 
 
@@ -298,7 +309,7 @@ def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype:
         raise ValueError("dtype must be bfloat16, float16 or float32")
     dev = h.device
     w = _gain(weight, "weight", cols, dev)
-    n, n_ptr, n_dtype = _normed(h.shape, rows, cols, dtype, dev, quantized)
+    n, n_ptr, n_dtype = _normed(h, rows, cols, dtype, quantized)
     args = _lib.Mx4Norm(None, h.data_ptr(), None, None, w, None, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
                         _DTYPES[weight.dtype], eps, 1.0)
     _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
@@ -324,15 +335,9 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
     _check_norm_cols(cols)
     if h.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    post = nxt = g = n = n_ptr = None
-    weight_dtype = n_dtype = g_dtype = g_row = g_col = 0
-    if post_weight is not None:
-        post, weight_dtype = _gain(post_weight, "post_weight", cols, dev), _DTYPES[post_weight.dtype]
-    if next_weight is not None:
-        nxt = _gain(next_weight, "next_weight", cols, dev)
-        if post_weight is not None and post_weight.dtype != next_weight.dtype:
-            raise ValueError("post_weight and next_weight must have the same dtype")
-        weight_dtype = _DTYPES[next_weight.dtype]
+    g = n = n_ptr = None
+    n_dtype = g_dtype = g_row = g_col = 0
+    post, nxt, weight_dtype = _gains(post_weight, next_weight, cols, dev)
     if gate is not None:
         g, g_dtype, g_row, g_col = _gate(gate, y, rows, cols)
     if inplace:
@@ -340,9 +345,9 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
         if rows > 1 and h_stride < cols:
             raise ValueError("h has rows that share memory and cannot be updated in place")
     else:
-        joined, out_stride = torch.empty(shape, dtype=h.dtype, device=dev), cols
+        joined, out_stride = h.new_empty(shape), cols
     if nxt is not None:
-        n, n_ptr, n_dtype = _normed(shape, rows, cols, y.dtype, dev, quantized)
+        n, n_ptr, n_dtype = _normed(y, rows, cols, y.dtype, quantized)
     args = _lib.Mx4Norm(y.data_ptr(), h.data_ptr(), post, g, nxt, joined.data_ptr(), n_ptr, rows, cols, y_stride, h_stride, out_stride, cols, g_row,
                         g_col, _DTYPES[y.dtype], _DTYPES[h.dtype], n_dtype, g_dtype, weight_dtype, eps, residual_scale)
     _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
@@ -356,6 +361,8 @@ def _gate(gate, y, rows: int, cols: int):
     if gate.device != y.device:
         raise ValueError("all tensors must be on the same CUDA device")
     if gate.dim() <= y.dim() and gate.is_contiguous():
+        if gate.dim() == 1 and gate.numel() == cols:
+            return gate.data_ptr(), _DTYPES[gate.dtype], 0, int(cols > 1)
         shape = (1,) * (y.dim() - gate.dim()) + tuple(gate.shape)
         last = shape[-1]
         if last == 1 or last == cols:
@@ -378,20 +385,66 @@ class GatedMlp:
                  next_weight: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "silu"):
         for q, name in ((gate_proj, "gate_proj"), (up_proj, "up_proj"), (down_proj, "down_proj")):
             _check_mx4(q, name)
-        if (up_proj.rows, up_proj.cols) != (gate_proj.rows, gate_proj.cols) or (down_proj.rows, down_proj.cols) != (gate_proj.cols, gate_proj.rows):
+            if q.device != gate_proj.device:
+                raise ValueError("all tensors must be on the same CUDA device")
+        inter, hidden = gate_proj.rows, gate_proj.cols
+        if inter == 0 or (up_proj.rows, up_proj.cols) != (inter, hidden) or (down_proj.rows, down_proj.cols) != (hidden, inter):
             raise ValueError("gate_proj and up_proj must be [inter, hidden], down_proj [hidden, inter]")
         if activation not in _ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
+        _check_norm_cols(hidden)
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self.pre_weight, self.post_weight, self.gate, self.next_weight = pre_weight, post_weight, gate, next_weight
-        self.residual_scale, self.eps, self.activation = float(residual_scale), float(eps), activation
+        self.hidden, self.inter = hidden, inter
+        dev = self.device = gate_proj.device
+        b = self._block = _lib.Mx4Mlp()
+        b.gate_proj, b.up_proj, b.down_proj = (q.data.data_ptr() for q in (gate_proj, up_proj, down_proj))
+        b.pre_weight, b.pre_dtype = _gain(pre_weight, "pre_weight", hidden, dev), _DTYPES[pre_weight.dtype]
+        b.post_weight, b.next_weight, b.weight_dtype = _gains(post_weight, next_weight, hidden, dev)
+        b.hidden, b.inter, b.activation, b.eps, b.residual_scale = hidden, inter, _ACTIVATIONS[activation], eps, residual_scale
+        self._gate_per_call = gate is not None and (not isinstance(gate, torch.Tensor) or gate.dim() != 1 or gate.numel() != hidden)
+        if gate is not None and not self._gate_per_call:
+            b.gate, b.gate_dtype, b.gate_row_stride, b.gate_col_stride = _gate(gate, pre_weight, 1, hidden)
 
     def forward(self, h: torch.Tensor, *, inplace: bool = False):
-        x = rms_norm(h, self.pre_weight, eps=self.eps, quantized=True)
-        # the kernel before each product is this block's own: no weight comes out of it
-        a = _product(x, self.gate_proj, self.up_proj, _ACTIVATIONS[self.activation], None, True, True)
-        y = _product(a, self.down_proj, None, 0, torch.bfloat16 if h.dtype == torch.float32 else h.dtype, False, True)
-        return block_join(y, h, post_weight=self.post_weight, gate=self.gate, residual_scale=self.residual_scale,
-                          next_weight=self.next_weight, eps=self.eps, inplace=inplace)
+        rows, cols, stride = _matrix(h, "h")
+        if cols != self.hidden:
+            raise ValueError(f"h has {cols} columns, the block {self.hidden}")
+        dev = h.device
+        if dev != self.device:
+            raise ValueError("all tensors must be on the same CUDA device")
+        block = self._block
+        if self._gate_per_call:      # a value per row or per element: it has to fit this h
+            block = _lib.Mx4Mlp.from_buffer_copy(block)
+            block.gate, block.gate_dtype, block.gate_row_stride, block.gate_col_stride = _gate(self.gate, h, rows, cols)
+        h_dtype = _DTYPES[h.dtype]
+        if inplace:
+            joined, out_stride = h, stride
+            if rows > 1 and stride < cols:
+                raise ValueError("h has rows that share memory and cannot be updated in place")
+        else:
+            joined, out_stride = h.new_empty(h.shape), cols
+        n = None
+        if block.next_weight:
+            n = h.new_empty(h.shape, dtype=torch.bfloat16) if h_dtype == 2 else h.new_empty(h.shape)
+        scratch_bytes = _tile_bytes(rows, cols) + _tile_bytes(rows, self.inter) + rows * cols * 2
+        scratch = self.gate_proj.data.new_empty(scratch_bytes)      # of this call: freed on return, and not handed to another stream before it is done
+        index = dev.index
+        args = (C.byref(block), h.data_ptr(), h_dtype, stride, rows, joined.data_ptr(), out_stride, None if n is None else n.data_ptr(),
+                0 if h_dtype == 2 else h_dtype, scratch.data_ptr(), scratch_bytes)
+        if _current_device() == index:
+            self._run(args, index)
+        else:
+            with torch.cuda.device(index):
+                self._run(args, index)
+        return joined, n
 
     __call__ = forward
+
+    @staticmethod
+    def _run(args, index: int) -> None:
+        stream = _stream_of(index)
+        ws = _workspace(index, stream)
+        rc = _lib.load().mps_mx4_gated_mlp(*args, ws.data_ptr(), ws.numel(), stream)
+        if rc:
+            _lib.check(rc)

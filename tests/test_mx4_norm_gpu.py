@@ -89,6 +89,27 @@ def test_block_join(rows, cols, dtype, stream, gate, post, nxt, alpha, quantized
             assert (np.abs(ref.to64(n) - want) <= n_off + np.abs(want) * ref.ROUND[y.dtype] * (1 + 2.0 ** -8) + least).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(1000, 40), (515, 256), (700, 300), (600, 500), (513, 2000), (600, 2056), (520, 9000), (530, 1337)])
+def test_many_rows_are_each_themselves(rows, cols):
+    """Rows that share a CTA, and the last CTA's missing ones: what a row gives does not depend on its neighbours."""
+    y, h = _make((rows, cols), "bf16", 6), _make((rows, cols), "f32", 7)
+    w = _make((cols,), "f32", 8) + 1
+    g = _make((rows, 1), "f32", 9)
+    guard = torch.full((rows + 8, cols), 7.0, device="cuda")
+    guard[:rows] = h
+    joined, n = mx4.block_join(y, guard[:rows], post_weight=w, gate=g, next_weight=w, inplace=True)
+    assert (guard[rows:] == 7).all()
+    q = mx4.rms_norm(h, w, quantized=True).dequantize()
+    for first in (0, 17, rows - 3):
+        some = slice(first, first + 3)
+        few = mx4.block_join(y[some], h[some], post_weight=w, gate=g[some], next_weight=w)
+        torch.testing.assert_close(joined[some], few[0], rtol=2.0 ** -20, atol=2.0 ** -18)
+        torch.testing.assert_close(n[some], few[1], rtol=2.0 ** -7, atol=2.0 ** -18)
+        assert torch.isfinite(q[some]).all()
+    want = _norm(ref.to64(h), ref.to64(w), float(np.float32(1e-5)))
+    ref.check_rounded(mx4.rms_norm(h, w, quantized=True), want, np.abs(want) * 80 * U)
+
+
 def test_rows_of_zeros_and_of_nan_keep_to_themselves():
     h = torch.randn((4, 512), device="cuda").to(torch.bfloat16)
     h[1], h[2, 7] = 0, float("nan")
