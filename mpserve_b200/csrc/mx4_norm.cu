@@ -74,7 +74,7 @@ static __device__ __forceinline__ float row_sum(float v, float* slot) {
 }
 
 template <int STEPS, bool VEC, bool WIDE_Y, bool WIDE_H, bool WIDE_W>
-__global__ void __launch_bounds__(kNormMostThreads, STEPS == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kNormMostThreads)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
     __shared__ __align__(16) float buffers[VEC ? 1 : kNormMostThreads / 32][256];
