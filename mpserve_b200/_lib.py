@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -31,28 +32,10 @@ class BucketTensor(C.Structure):
     ]
 
 
-class Mx4Norm(C.Structure):
-    """struct mps_mx4_norm"""
-
-    _fields_ = [
-        ("y", _p), ("h", _p), ("post_weight", _p), ("gate", _p), ("next_weight", _p), ("h_out", _p), ("n_out", _p),
-        ("rows", _i64), ("cols", _i64),
-        ("y_stride", _i64), ("h_stride", _i64), ("h_out_stride", _i64), ("n_stride", _i64), ("gate_row_stride", _i64),
-        ("gate_col_stride", _i32),
-        ("y_dtype", _i32), ("h_dtype", _i32), ("n_dtype", _i32), ("gate_dtype", _i32), ("weight_dtype", _i32),
-        ("eps", C.c_float), ("residual_scale", C.c_float),
-    ]
-
-
-class Mx4Linear(C.Structure):
-    """struct mps_mx4_linear"""
-
-    _fields_ = [
-        ("x", _p), ("x_tiles", _p), ("w", _p), ("w_up", _p), ("out", _p),
-        ("tokens", _i64), ("cols", _i64), ("rows", _i64),
-        ("x_stride", _i64), ("out_stride", _i64),
-        ("x_dtype", _i32), ("out_dtype", _i32), ("activation", _i32), ("weights_ready", _i32),
-    ]
+# struct mps_mx4_norm and struct mps_mx4_linear, packed in the order of their fields: their calls take a few microseconds, of which filling a
+# C.Structure would be one.
+MX4_NORM = struct.Struct("@7P7q6i2f")
+MX4_LINEAR = struct.Struct("@5P5q4i")
 
 
 class Mx4Mlp(C.Structure):
@@ -101,9 +84,9 @@ _PROTOS = {
     "mps_mx4_dequantize": (C.c_int, [_p, _i64, _i64, _i32, _p, _p]),
     "mps_mx4_pack": (C.c_int, [_p, _p, _i64, _i64, _p, _p]),
     "mps_mx4_unpack": (C.c_int, [_p, _i64, _i64, _p, _p, _p]),
-    "mps_mx4_norm_rows": (C.c_int, [C.POINTER(Mx4Norm), _p]),
+    "mps_mx4_norm_rows": (C.c_int, [C.c_char_p, _p]),
     "mps_mx4_workspace_bytes": (_i64, []),
-    "mps_mx4_product": (C.c_int, [C.POINTER(Mx4Linear), _p, _i64, _p]),
+    "mps_mx4_product": (C.c_int, [C.c_char_p, _p, _i64, _p]),
     "mps_mx4_mlp_scratch_bytes": (_i64, [_i64, _i64, _i64]),
     "mps_mx4_gated_mlp": (C.c_int, [C.POINTER(Mx4Mlp), _p, _i32, _i64, _i64, _p, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mps_mx4_status": (C.c_int, [_p, _i64, _p, C.POINTER(_i32)]),

@@ -7,8 +7,8 @@
 // A CTA has one row in registers (several short ones), eight neighbouring columns per lane and step, so that y and h are read once and the two
 // means cost two barriers.  All arithmetic is in FP32; h' is normalised as it was before it is rounded to the stream's type.  Four lanes
 // hold an MXFP4 block and a warp a whole row of a tile, so the quantised form needs nothing but shuffles.
-// Bounds: memory, and for a few rows the two barriers and the launch.  Weights and gate are under way with y and h: asked for after the
-// barrier that they wait behind, each would add a trip to the L2 to every row.
+// Bounds: memory, and for a few rows the two barriers and the launch.  Weights and gate are asked for before the barrier that they wait behind,
+// not after it: each would add a trip to the L2 to every row.
 #include "mx4.cuh"
 
 namespace mps {
@@ -73,7 +73,8 @@ static __device__ __forceinline__ float row_sum(float v, float* slot) {
     return __shfl_sync(0xFFFFFFFFu, v, 0);
 }
 
-template <int STEPS, bool VEC, bool WIDE_Y, bool WIDE_H, bool WIDE_W>
+// JOIN: there is a y.
+template <int STEPS, bool VEC, bool JOIN, bool WIDE_Y, bool WIDE_H, bool WIDE_W>
 __global__ void __launch_bounds__(kNormMostThreads)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
@@ -92,14 +93,14 @@ mx4_norm_kernel(const NormArgs p) {
     Eight<VEC, WIDE_Y> ry[STEPS];
     Eight<VEC, WIDE_H> rh[STEPS];
     Eight<VEC, WIDE_W> post[STEPS], gate[STEPS], next[STEPS];
-    const auto load_post = [&](int s) { if (a.y && a.post_weight) post[s].load(a.post_weight, a.weight_dtype, 0, column(s), cols, p.vec_post, lane); };
+    const auto load_post = [&](int s) { if (JOIN && a.post_weight) post[s].load(a.post_weight, a.weight_dtype, 0, column(s), cols, p.vec_post, lane); };
     const auto load_gate = [&](int s) {
-        if (a.y && a.gate && a.gate_col_stride) gate[s].load(a.gate, a.gate_dtype, row * a.gate_row_stride, column(s), cols, p.vec_gate, lane);
+        if (JOIN && a.gate && a.gate_col_stride) gate[s].load(a.gate, a.gate_dtype, row * a.gate_row_stride, column(s), cols, p.vec_gate, lane);
     };
     const auto load_next = [&](int s) { if (a.next_weight) next[s].load(a.next_weight, a.weight_dtype, 0, column(s), cols, p.vec_next, lane); };
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        if (a.y) ry[s].load(a.y, a.y_dtype, row * a.y_stride, column(s), cols, p.vec_y, lane);
+        if (JOIN) ry[s].load(a.y, a.y_dtype, row * a.y_stride, column(s), cols, p.vec_y, lane);
         rh[s].load(a.h, a.h_dtype, row * a.h_stride, column(s), cols, p.vec_h, lane);
     }
     if (kAhead) {
@@ -107,12 +108,12 @@ mx4_norm_kernel(const NormArgs p) {
         for (int s = 0; s < STEPS; ++s) {
             load_post(s);
             load_gate(s);
-            load_next(s);
+            if (!JOIN) load_next(s);
         }
     }
     float v[STEPS][8];
     float sum = 0.f;
-    if (a.y) {
+    if (JOIN) {
         float row_gate = 1.f;      // one gate for the row
         if (a.gate && !a.gate_col_stride) {
             float w[8];
@@ -166,6 +167,10 @@ mx4_norm_kernel(const NormArgs p) {
             }
         }
         if (!a.n_out) return;
+        if (kAhead) {      // on their way during the second sum
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) load_next(s);
+        }
     } else {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -202,14 +207,19 @@ static int launch_norm(const NormArgs& p, bool vec, bool wide_w, int per_row, cu
     // short rows share a CTA: 20000 of 512 columns 22 us with a CTA each
     const int rows_per_cta = per_row >= kNormThreads ? 1 : kNormThreads / per_row;
     const bool wide_y = a.y && a.y_dtype == MPS_F32, wide_h = a.h_dtype == MPS_F32;
-    void (*kernel)(NormArgs) = mx4_norm_kernel<STEPS, false, true, true, true>;
-    if (vec) {
+    void (*kernel)(NormArgs) = a.y ? mx4_norm_kernel<STEPS, false, true, true, true, true> : mx4_norm_kernel<STEPS, false, false, true, true, true>;
+    if (vec && a.y) {
         static void (*const fast[8])(NormArgs) = {
-            mx4_norm_kernel<STEPS, true, false, false, false>, mx4_norm_kernel<STEPS, true, false, false, true>,
-            mx4_norm_kernel<STEPS, true, false, true, false>,  mx4_norm_kernel<STEPS, true, false, true, true>,
-            mx4_norm_kernel<STEPS, true, true, false, false>,  mx4_norm_kernel<STEPS, true, true, false, true>,
-            mx4_norm_kernel<STEPS, true, true, true, false>,   mx4_norm_kernel<STEPS, true, true, true, true>};
+            mx4_norm_kernel<STEPS, true, true, false, false, false>, mx4_norm_kernel<STEPS, true, true, false, false, true>,
+            mx4_norm_kernel<STEPS, true, true, false, true, false>,  mx4_norm_kernel<STEPS, true, true, false, true, true>,
+            mx4_norm_kernel<STEPS, true, true, true, false, false>,  mx4_norm_kernel<STEPS, true, true, true, false, true>,
+            mx4_norm_kernel<STEPS, true, true, true, true, false>,   mx4_norm_kernel<STEPS, true, true, true, true, true>};
         kernel = fast[wide_y * 4 + wide_h * 2 + wide_w];
+    } else if (vec) {
+        static void (*const fast[4])(NormArgs) = {
+            mx4_norm_kernel<STEPS, true, false, false, false, false>, mx4_norm_kernel<STEPS, true, false, false, false, true>,
+            mx4_norm_kernel<STEPS, true, false, false, true, false>,  mx4_norm_kernel<STEPS, true, false, false, true, true>};
+        kernel = fast[wide_h * 2 + wide_w];
     }
     return launch_overlapping("mx4_norm_kernel", kernel, (unsigned int)((a.rows + rows_per_cta - 1) / rows_per_cta), dim3(per_row, rows_per_cta), st, p);
 }

@@ -174,7 +174,7 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
 def _run_product(args, index: int) -> None:
     stream = _stream_of(index)
     ws = _workspace(index, stream)
-    rc = _lib.load().mps_mx4_product(C.byref(args), ws.data_ptr(), ws.numel(), stream)
+    rc = _lib.load().mps_mx4_product(args, ws.data_ptr(), ws.numel(), stream)
     if rc:
         _lib.check(rc)
 
@@ -182,7 +182,7 @@ def _run_product(args, index: int) -> None:
 def _product(x, w, w_up, activation: int, dtype, quantized: bool):
     _check_mx4(w, "w" if w_up is None else "w_gate")
     out_cols, w_cols, dev = w.rows, w.cols, w.data.device
-    up = None
+    up = 0
     if w_up is not None:
         _check_mx4(w_up, "w_up")
         if w_up.rows != out_cols or w_up.cols != w_cols:
@@ -217,8 +217,8 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool):
             raise ValueError("a product's dtype must be bfloat16 or float16")
         out = result = data.new_empty(shape) if data.dtype is dtype else data.new_empty(shape, dtype=dtype)
         out_dtype = _DTYPES[dtype]
-    args = _lib.Mx4Linear(data.data_ptr(), None if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
-                          stride, out_cols, x_dtype, out_dtype, activation, 0)
+    args = _lib.MX4_LINEAR.pack(data.data_ptr(), 0 if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
+                                stride, out_cols, x_dtype, out_dtype, activation, 0)
     index = dev.index
     if _current_device() == index:
         _run_product(args, index)
@@ -273,9 +273,8 @@ def _gain(t, name: str, cols: int, dev) -> int:
 
 
 def _gains(post_weight, next_weight, cols: int, dev):
-    """(pointers or None, the dtype that the two share)."""
-    post = nxt = None
-    dtype = 0
+    """(pointers or 0, the dtype that the two share)."""
+    post = nxt = dtype = 0
     if post_weight is not None:
         post, dtype = _gain(post_weight, "post_weight", cols, dev), _DTYPES[post_weight.dtype]
     if next_weight is not None:
@@ -310,9 +309,9 @@ def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype:
     dev = h.device
     w = _gain(weight, "weight", cols, dev)
     n, n_ptr, n_dtype = _normed(h, rows, cols, dtype, quantized)
-    args = _lib.Mx4Norm(None, h.data_ptr(), None, None, w, None, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
-                        _DTYPES[weight.dtype], eps, 1.0)
-    _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
+    args = _lib.MX4_NORM.pack(0, h.data_ptr(), 0, 0, w, 0, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
+                              _DTYPES[weight.dtype], eps, 1.0)
+    _launch(dev.index, _lib.load().mps_mx4_norm_rows, args)
     return n
 
 
@@ -335,8 +334,8 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
     _check_norm_cols(cols)
     if h.device != dev:
         raise ValueError("all tensors must be on the same CUDA device")
-    g = n = n_ptr = None
-    n_dtype = g_dtype = g_row = g_col = 0
+    n = None
+    n_ptr = n_dtype = g = g_dtype = g_row = g_col = 0
     post, nxt, weight_dtype = _gains(post_weight, next_weight, cols, dev)
     if gate is not None:
         g, g_dtype, g_row, g_col = _gate(gate, y, rows, cols)
@@ -346,11 +345,11 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
             raise ValueError("h has rows that share memory and cannot be updated in place")
     else:
         joined, out_stride = h.new_empty(shape), cols
-    if nxt is not None:
+    if nxt:
         n, n_ptr, n_dtype = _normed(y, rows, cols, y.dtype, quantized)
-    args = _lib.Mx4Norm(y.data_ptr(), h.data_ptr(), post, g, nxt, joined.data_ptr(), n_ptr, rows, cols, y_stride, h_stride, out_stride, cols, g_row,
-                        g_col, _DTYPES[y.dtype], _DTYPES[h.dtype], n_dtype, g_dtype, weight_dtype, eps, residual_scale)
-    _launch(dev.index, _lib.load().mps_mx4_norm_rows, C.byref(args))
+    args = _lib.MX4_NORM.pack(y.data_ptr(), h.data_ptr(), post, g, nxt, joined.data_ptr(), n_ptr, rows, cols, y_stride, h_stride, out_stride, cols,
+                              g_row, g_col, _DTYPES[y.dtype], _DTYPES[h.dtype], n_dtype, g_dtype, weight_dtype, eps, residual_scale)
+    _launch(dev.index, _lib.load().mps_mx4_norm_rows, args)
     return joined, n
 
 
