@@ -596,6 +596,14 @@ static int launch_product(void (*kernel)(ProductArgs), std::atomic<uint64_t>& re
     return MPS_OK;
 }
 
+// CTAs that share a tile's columns: a power of two (three took longer than two: 384 tokens, 14336 x 4096, 26 us against 19 for 512), at most what fills
+// every SM with two.
+static int parts_of(int64_t tiles, int chunks, int sms) {
+    int parts = 1;
+    while (parts < kMostParts && 2 * parts * tiles <= 2 * sms && 2 * parts <= chunks) parts *= 2;
+    return parts;
+}
+
 template <int TOKENS, bool GATED, bool QUANTIZE = false>
 static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
     using S = StreamShape<TOKENS, GATED>;
@@ -603,11 +611,19 @@ static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
     p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
     const int64_t tiles = (int64_t)p.row_tiles * p.token_tiles;
     if (tiles * kMostParts > 0x7FFFFFFF) { set_error("mps_mx4_product: output too large"); return MPS_ERR_INVALID; }
-    p.parts = (int)(2 * d.sms / tiles);
-    p.parts = p.parts < 1 ? 1 : p.parts > kMostParts ? kMostParts : p.parts;
-    if (p.parts > p.chunks) p.parts = p.chunks;
+    p.parts = parts_of(tiles, p.chunks, d.sms);
     return launch_product(mx4_stream_kernel<TOKENS, GATED, QUANTIZE>, ready, d, S::kSmem, (kStreamWarps + (QUANTIZE ? S::kStages : 0)) * 32,
                           (int)tiles * p.parts, p.parts, st, p);
+}
+
+// Whether 128 tokens a tile with the weights on the lanes take less time than 256 with the tokens on the lanes, by what a tile of K, a round of CTAs
+// and a launch cost in each, us.  Measured, stream | wide: 14336 x 4096, 64 tokens 10.2 | 11.1, 128: 12.5 | 11.9, 512: 26.5 | 18.0; 4096 x 14336,
+// 128: 12.1 | 26.4, 512: 19.1 | 26.4, 1024: 29.9 | 27.1; 4096 x 4096, 256: 9.5 | 10.6, 1024: 13.4 | 11.3; 517 x 1000, 1024: 7.3 | 8.9.
+static bool stream_pays(const ProductArgs& p, int sms) {
+    const int64_t tiles = (int64_t)p.row_tiles * ((p.tokens + 127) / 128), wide = (int64_t)((p.row_tiles + 1) / 2) * ((p.tokens + 255) / 256);
+    const int parts = parts_of(tiles, p.chunks, sms);
+    const int64_t waves = (tiles * parts + 2 * sms - 1) / (2 * sms), rounds = (wide + sms / 2 - 1) / (sms / 2);
+    return 4.2 + (double)waves * 0.54 * ((p.chunks + parts - 1) / parts) + 2.5 * (double)(waves - 1) < 5.5 + (double)rounds * 0.39 * p.chunks;
 }
 
 template <bool GATED>
@@ -698,7 +714,7 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     if (a.tokens <= 16) return launch_stream<16, false>(p, d, st);
     if (a.tokens <= 32) return launch_stream<32, false>(p, d, st);
     if (a.tokens <= 64) return launch_stream<64, false>(p, d, st);
-    if (a.tokens <= 128) return launch_stream<128, false>(p, d, st);
+    if (stream_pays(p, d.sms)) return launch_stream<128, false>(p, d, st);
     return launch_wide<false>(p, d, st);
 }
 
