@@ -62,11 +62,13 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // fill the GPU: then every SM has some 200 KB under way, and all end together.  The parts of a tile meet in the cluster's shared memory,
 // where every CTA adds up a share of them, always in the same order.
 //
-// Warps: 0 copies, 1 multiplies, 2 to 5 take the accumulator over; with QUANTIZE, one more for every stage of the ring quantises the tokens'
-// columns on their way into it, instead of a kernel before this one.
+// Warps: 0 copies, 1 multiplies, the next four or eight take the accumulator over, one or two on each quarter of its lanes (four launch a little
+// sooner, 1 token 7.9 us and 8.0 with eight; eight are done sooner where there are more tokens, the gated pair for 64 18.5 us and 17.7); all of them add the
+// parts up.  With QUANTIZE, one more for every stage of the ring quantises the tokens' columns on their way into it, instead of a kernel before this one.
 template <int TOKENS, bool GATED>
 struct StreamShape {
     static constexpr int kWeights = GATED ? 2 : 1;
+    static constexpr int kTakeOver = TOKENS <= 16 ? 4 : 8, kWarps = 2 + kTakeOver;
     static constexpr int kXBytes = kMx4ScaleBytes + TOKENS * kMx4RowBytes;
     static constexpr int kStageBytes = kWeights * kMx4TileBytes + kXBytes;
     static constexpr int kMost = 115712 - 1024;                 // of an SM's 228 KB, for two CTAs and the KB that each costs
@@ -81,7 +83,6 @@ struct StreamShape {
     static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
     static_assert(kAcc * 128 * 4 <= kBars, "a part of the accumulator takes the ring's place");
 };
-constexpr int kStreamWarps = 6;
 constexpr int kMostQuantizedInside = 8;        // tokens that the kernel quantises itself
 constexpr int kMostParts = 4;                  // CTAs of a cluster
 
@@ -131,7 +132,7 @@ __device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int l
 }
 
 template <int TOKENS, bool GATED, bool QUANTIZE>
-__global__ void __launch_bounds__((kStreamWarps + (QUANTIZE ? StreamShape<TOKENS, GATED>::kStages : 0)) * 32, 2)
+__global__ void __launch_bounds__((StreamShape<TOKENS, GATED>::kWarps + (QUANTIZE ? StreamShape<TOKENS, GATED>::kStages : 0)) * 32, 2)
 mx4_stream_kernel(const ProductArgs p) {
     using S = StreamShape<TOKENS, GATED>;
     extern __shared__ __align__(1024) uint8_t ring_bytes[];      // all of the shared memory: rings begin at multiples of 1024
@@ -228,14 +229,14 @@ mx4_stream_kernel(const ProductArgs p) {
         if (ok) tensor_commit(lead, acc_full);
         tensor_commit(lead, drained);
         warp_wait(drained, 0, &failed);
-    } else if (warp < kStreamWarps) {
+    } else if (warp < S::kWarps) {
         // the accumulator, token by token, to where the ring was: what that held has been multiplied
         const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21), to = ring + ((warp & 3) * 32 + lane) * 4;
         if (warp_wait(acc_full, 0, &failed)) {
             tensor_fence_after();
             const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
 #pragma unroll 1
-            for (int c = 0; c < S::kAcc; c += 16) {
+            for (int c = ((warp - 2) >> 2) * 16; c < S::kAcc; c += S::kTakeOver * 4) {
                 if (c % TOKENS >= tokens) continue;
                 float v[16];
                 tmem_load16(acc + c, v);
@@ -245,7 +246,7 @@ mx4_stream_kernel(const ProductArgs p) {
         }
     } else {
         // Each has one stage, and so sees every phase of its barriers: a wait for a parity is right only for who has seen the phase before.
-        const int rows = (int)min((int64_t)TOKENS, p.tokens - token0), s = warp - kStreamWarps;
+        const int rows = (int)min((int64_t)TOKENS, p.tokens - token0), s = warp - S::kWarps;
         uint8_t* to = ring_bytes + s * S::kStageBytes + S::kWeights * kMx4TileBytes;
         griddep_wait();
         for (int i = s; i < k1 - k0; i += S::kStages) {
@@ -612,7 +613,7 @@ static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
     const int64_t tiles = (int64_t)p.row_tiles * p.token_tiles;
     if (tiles * kMostParts > 0x7FFFFFFF) { set_error("mps_mx4_product: output too large"); return MPS_ERR_INVALID; }
     p.parts = parts_of(tiles, p.chunks, d.sms);
-    return launch_product(mx4_stream_kernel<TOKENS, GATED, QUANTIZE>, ready, d, S::kSmem, (kStreamWarps + (QUANTIZE ? S::kStages : 0)) * 32,
+    return launch_product(mx4_stream_kernel<TOKENS, GATED, QUANTIZE>, ready, d, S::kSmem, (S::kWarps + (QUANTIZE ? S::kStages : 0)) * 32,
                           (int)tiles * p.parts, p.parts, st, p);
 }
 
