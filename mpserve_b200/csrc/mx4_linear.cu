@@ -60,7 +60,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // A CTA streams the weight tiles of 128 features through a ring in shared memory, 17 KB a bulk copy; TOKENS tokens (16 to 128) are the
 // product's narrow side.  Two CTAs share an SM, and a cluster of up to four shares the columns of one tile of the output, as many as
 // fill the GPU: then every SM has some 200 KB under way, and all end together.  The parts of a tile meet in the cluster's shared memory,
-// where every CTA adds up a share of them, always in the same order.
+// where every CTA adds up a share of the tokens, always in the same order.  Up to 32 tokens (16 with a gate) each sends its parts to where they are
+// added, as they come out of the accumulator, and a barrier there counts them: nothing but that barrier is waited for (1 token through 14336 x 4096
+// 7.4 us).  More would take stages from the ring; they take its place, and the adding CTA fetches them between two barriers of the whole cluster
+// (1 token 7.9 us that way; 64 tokens through 4096 x 14336 9.8 us, sent 10.1).
 //
 // Warps: 0 copies, 1 multiplies, the next four or eight take the accumulator over, one or two on each quarter of its lanes (four launch a little
 // sooner, 1 token 7.9 us and 8.0 with eight; eight are done sooner where there are more tokens, the gated pair for 64 18.5 us and 17.7); all of them add the
@@ -72,16 +75,18 @@ struct StreamShape {
     static constexpr int kXBytes = kMx4ScaleBytes + TOKENS * kMx4RowBytes;
     static constexpr int kStageBytes = kWeights * kMx4TileBytes + kXBytes;
     static constexpr int kMost = 115712 - 1024;                 // of an SM's 228 KB, for two CTAs and the KB that each costs
-    static constexpr int kStages = kMost / kStageBytes;
-    static constexpr int kBars = kStages * kStageBytes;
-    static constexpr int kSmem = kBars + (2 * kStages + 2) * 8 + 16;
     static constexpr int kAcc = TOKENS * kWeights;              // columns of the accumulator
+    static constexpr bool kSend = kAcc <= 32;
+    static constexpr int kStages = (kMost - (kSend ? kAcc * 512 : 0)) / kStageBytes;
+    static constexpr int kReceived = kStages * kStageBytes;     // where the parts of this CTA's tokens come in
+    static constexpr int kBars = kReceived + (kSend ? kAcc * 512 : 0);
+    static constexpr int kSmem = kBars + (2 * kStages + 3) * 8 + 16;
     static constexpr int kScaleColumns = 8 * kWeights + 8;      // of one stage
     static constexpr int kUsed = kAcc + kStages * kScaleColumns;
     static constexpr int kColumns = kUsed <= 128 ? 128 : 256;   // an allocation is a power of two
     static_assert(kUsed <= kColumns, "tensor memory");
     static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
-    static_assert(kAcc * 128 * 4 <= kBars, "a part of the accumulator takes the ring's place");
+    static_assert(kAcc * 128 * 4 <= kReceived, "a part of the accumulator takes the ring's place");
 };
 constexpr int kMostQuantizedInside = 8;        // tokens that the kernel quantises itself
 constexpr int kMostParts = 4;                  // CTAs of a cluster
@@ -142,27 +147,33 @@ mx4_stream_kernel(const ProductArgs p) {
     volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(ring_bytes + S::kSmem - 12);
     const auto full = [&](int s) { return bar0 + 8u * s; };
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
-    const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), drained = acc_full + 8u;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), QUANTIZE ? 2 : 1); mbar_init(empty(s), 1); }
-        mbar_init(acc_full, 1);
-        mbar_init(drained, 1);
-        failed = 0u;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
-    tensor_fence_before();
-    __syncthreads();
-    tensor_fence_after();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), drained = acc_full + 8u, received = acc_full + 16u;
 
     // this CTA's tile of the output, and its share of the columns
     const int part = blockIdx.x % p.parts, chunks = p.chunks;
     const int64_t tile = blockIdx.x / p.parts;
     const int row_tile = (int)(tile / p.token_tiles);
     const int64_t token0 = (tile % p.token_tiles) * TOKENS;
+    const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
     const int k0 = (int)((int64_t)chunks * part / p.parts), k1 = (int)((int64_t)chunks * (part + 1) / p.parts);
+    const bool send = S::kSend && p.parts > 1;
+    const int shares = (tokens + p.parts - 1) / p.parts;        // tokens of a part: every parts-th, from its own number on
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), QUANTIZE ? 2 : 1); mbar_init(empty(s), 1); }
+        mbar_init(acc_full, 1);
+        mbar_init(drained, 1);
+        mbar_init(received, 1);
+        failed = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (send) mbar_expect_tx(received, (uint32_t)((tokens - part + p.parts - 1) / p.parts * p.parts * S::kWeights * 512));
+    }
+    if (warp == 1) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (send) cluster_arrive();      // `received` can be sent to
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
     if (warp == 0) {
         if (lane == 0) {
@@ -230,23 +241,36 @@ mx4_stream_kernel(const ProductArgs p) {
         tensor_commit(lead, drained);
         warp_wait(drained, 0, &failed);
     } else if (warp < S::kWarps) {
-        // the accumulator, token by token, to where the ring was: what that held has been multiplied
-        const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21), to = ring + ((warp & 3) * 32 + lane) * 4;
-        if (warp_wait(acc_full, 0, &failed)) {
-            tensor_fence_after();
-            const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
+        // the accumulator, token by token, to where the parts meet, or to where the ring was: what that held has been multiplied
+        const int feature = (warp & 3) * 32 + lane;
+        const uint32_t acc = tmem + ((uint32_t)(warp & 3) << 21);
+        const bool ok = warp_wait(acc_full, 0, &failed);
+        tensor_fence_after();
+        if (send) cluster_wait();
+        if (ok) {
 #pragma unroll 1
             for (int c = ((warp - 2) >> 2) * 16; c < S::kAcc; c += S::kTakeOver * 4) {
-                if (c % TOKENS >= tokens) continue;
+                const int w = c / TOKENS, t0 = c % TOKENS;
+                if (t0 >= tokens) continue;
                 float v[16];
                 tmem_load16(acc + c, v);
+                if (send) {
+                    const uint32_t to = ring + S::kReceived + ((w * p.parts + part) * shares * 128 + feature) * 4;
+                    const int shift = __ffs(p.parts) - 1;      // parts are a power of two
 #pragma unroll
-                for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (c + i) * 512), "f"(v[i]) : "memory");
+                    for (int i = 0; i < 16; ++i) {
+                        const int t = t0 + i, owner = t & (p.parts - 1);
+                        if (t < tokens) send_to(peer_address(to + (t >> shift) * 512, owner), peer_address(received, owner), v[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + ((c + i) * 128 + feature) * 4), "f"(v[i]) : "memory");
+                }
             }
         }
     } else {
         // Each has one stage, and so sees every phase of its barriers: a wait for a parity is right only for who has seen the phase before.
-        const int rows = (int)min((int64_t)TOKENS, p.tokens - token0), s = warp - S::kWarps;
+        const int rows = tokens, s = warp - S::kWarps;
         uint8_t* to = ring_bytes + s * S::kStageBytes + S::kWeights * kMx4TileBytes;
         griddep_wait();
         for (int i = s; i < k1 - k0; i += S::kStages) {
@@ -282,27 +306,48 @@ mx4_stream_kernel(const ProductArgs p) {
     }
     __syncwarp();
     tensor_fence_before();
-    if (p.parts > 1) cluster_sync(); else __syncthreads();
-    if (!failed) {
-        // the parts meet: every warp of the cluster takes a token in turn (the code is short on purpose: it runs once, and what it costs is
-        // to fetch it)
-        const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0), warps = blockDim.x >> 5;
+    // The parts meet: every warp of the cluster takes a token in turn.  (The code is short on purpose: it runs once, and what it costs is to fetch it.)
+    const int warps = blockDim.x >> 5;
+    if (send) {
+        if (warp < 2 || warp >= S::kWarps) cluster_wait();      // the other warps have
+        cluster_arrive();
+        if (warp_wait(received, 0, &failed)) {
 #pragma unroll 1
-        for (int c = warp * p.parts + part; c < tokens; c += warps * p.parts) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f), up = v;
+            for (int i = warp; i * p.parts + part < tokens; i += warps) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f), up = v;
 #pragma unroll
-            for (int g = 0; g < kMostParts; ++g) {
-                if (g < p.parts) {
-                    const uint32_t from = p.parts > 1 ? peer_address(ring + c * 512 + lane * 16, g) : ring + c * 512 + lane * 16;
-                    add4(v, load_peer(from));
-                    if (GATED) add4(up, load_peer(from + TOKENS * 512));
+                for (int g = 0; g < kMostParts; ++g) {
+                    if (g < p.parts) {
+                        const uint8_t* from = ring_bytes + S::kReceived + ((g * shares + i) * 128 + lane * 4) * 4;
+                        add4(v, *reinterpret_cast<const float4*>(from));
+                        if (GATED) add4(up, *reinterpret_cast<const float4*>(from + p.parts * shares * 512));
+                    }
                 }
+                finish<GATED>(p, row_tile, lane, token0 + i * p.parts + part, v, up);
             }
-            finish<GATED>(p, row_tile, lane, token0 + c, v, up);
         }
+        __syncwarp();
+        cluster_wait();      // nobody leaves before all have sent: they long have
+    } else {
+        if (p.parts > 1) cluster_sync(); else __syncthreads();
+        if (!failed) {
+#pragma unroll 1
+            for (int c = warp * p.parts + part; c < tokens; c += warps * p.parts) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f), up = v;
+#pragma unroll
+                for (int g = 0; g < kMostParts; ++g) {
+                    if (g < p.parts) {
+                        const uint32_t from = p.parts > 1 ? peer_address(ring + c * 512 + lane * 16, g) : ring + c * 512 + lane * 16;
+                        add4(v, load_peer(from));
+                        if (GATED) add4(up, load_peer(from + TOKENS * 512));
+                    }
+                }
+                finish<GATED>(p, row_tile, lane, token0 + c, v, up);
+            }
+        }
+        __syncwarp();
+        if (p.parts > 1) cluster_sync();      // nobody leaves while his part is read
     }
-    __syncwarp();
-    if (p.parts > 1) cluster_sync();      // nobody leaves while his part is read
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);

@@ -105,6 +105,13 @@ __device__ __forceinline__ float4 load_peer(uint32_t address) {
     return v;
 }
 __device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+// One value into another CTA's shared memory; the barrier there counts its four bytes once they are there.
+__device__ __forceinline__ void send_to(uint32_t address, uint32_t bar, float v) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(address), "r"(__float_as_uint(v)), "r"(bar) : "memory");
+}
+// The cluster's barrier in two halves.  An arrival orders nothing; who has waited knows that all have arrived.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
