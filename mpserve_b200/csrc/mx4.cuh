@@ -213,11 +213,43 @@ __device__ __forceinline__ void mx4_values8(uint32_t codes, float (&v)[8]) {
     }
 }
 
+// The largest of eight magnitudes, as bits; NaN where there is one.
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
-    uint32_t m = 0u;
+    return __float_as_uint(max_abs3(max_abs3(max_abs3(v[0], v[1], v[2]), v[3], v[4]), max_abs3(v[5], v[6], v[7]), 0.f)) & 0x7FFFFFFFu;
+}
+
+// Two FP32 values at a time.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+    return r;
+}
+struct Pairs {       // eight values
+    float2 p[4];
+    __device__ __forceinline__ float (&each())[8] { return reinterpret_cast<float(&)[8]>(p); }
+};
+__device__ __forceinline__ Pairs times(const Pairs& a, const Pairs& b) {
+    Pairs r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return m;
+    for (int i = 0; i < 4; ++i) r.p[i] = mul2(a.p[i], b.p[i]);
+    return r;
+}
+__device__ __forceinline__ Pairs times(const Pairs& a, float b) {
+    Pairs r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.p[i] = mul2(a.p[i], make_float2(b, b));
+    return r;
 }
 
 // A warp quantises and stores one row of a tile: lane l holds columns 8 l to 8 l + 7 (zeros beyond the matrix), `m` the bits of the largest of
@@ -227,10 +259,8 @@ __device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int ro
     m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
     const uint32_t byte = mx4_scale_byte(m);
     const float inverse = mx4_inverse_scale(byte);
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = v[i] * inverse;      // of a NaN block, whatever it gives: its codes say nothing
-    *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, lane >> 2) + (lane & 3) * 4) = mx4_codes8(q);
+    Pairs q = times(reinterpret_cast<const Pairs&>(v), inverse);      // of a NaN block, whatever it gives: its codes say nothing
+    *reinterpret_cast<uint32_t*>(tile + mx4_code_offset(row, lane >> 2) + (lane & 3) * 4) = mx4_codes8(q.each());
     if ((lane & 3) == 0) tile[mx4_scale_offset(row, lane >> 4) + ((lane >> 2) & 3)] = (uint8_t)byte;
 }
 __device__ __forceinline__ void mx4_store_row(uint8_t* __restrict__ tile, int row, int lane, const float (&v)[8]) {

@@ -111,8 +111,9 @@ mx4_norm_kernel(const NormArgs p) {
             if (!JOIN) load_next(s);
         }
     }
-    float v[STEPS][8];
-    float sum = 0.f;
+    // Columns beyond the last are zeros all through.
+    Pairs v[STEPS];
+    float2 sum = make_float2(0.f, 0.f);
     if (JOIN) {
         float row_gate = 1.f;      // one gate for the row
         if (a.gate && !a.gate_col_stride) {
@@ -124,46 +125,43 @@ mx4_norm_kernel(const NormArgs p) {
         if (a.post_weight) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
-                float y[8];
-                ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y);
+                Pairs y;
+                ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y.each());
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(y[i], y[i], sum);
+                for (int i = 0; i < 4; ++i) sum = fma2(y.p[i], y.p[i], sum);
             }
-            r = 1.f / sqrtf(fmaf(row_sum(sum, slots[0]), p.inv_cols, a.eps));
+            r = rsqrtf(fmaf(row_sum(sum.x + sum.y, slots[0]), p.inv_cols, a.eps));
         }
-        sum = 0.f;
+        sum = make_float2(0.f, 0.f);
+        const float scale = r * row_gate;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            float y[8], h[8], w[8];
-            ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y);
-            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, h);
+            Pairs y, h, w;
+            ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y.each());
+            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, h.each());
             if (a.post_weight) {
                 if (!kAhead) load_post(s);
-                post[s].values(a.weight_dtype, p.vec_post, buffer, lane, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= r * w[i];
+                post[s].values(a.weight_dtype, p.vec_post, buffer, lane, w.each());
+                y = times(y, times(w, scale));
+            } else {
+                y = times(y, scale);
             }
             if (a.gate && a.gate_col_stride) {
                 if (!kAhead) load_gate(s);
-                gate[s].values(a.gate_dtype, p.vec_gate, buffer, lane, w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= w[i];
-            } else if (a.gate) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] *= row_gate;
+                gate[s].values(a.gate_dtype, p.vec_gate, buffer, lane, w.each());
+                y = times(y, w);
             }
-            const int left = cols - column(s);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[s][i] = i < left ? fmaf(a.residual_scale, h[i], y[i]) : 0.f;
-                sum = fmaf(v[s][i], v[s][i], sum);
+            for (int i = 0; i < 4; ++i) {
+                v[s].p[i] = fma2(make_float2(a.residual_scale, a.residual_scale), h.p[i], y.p[i]);
+                sum = fma2(v[s].p[i], v[s].p[i], sum);
             }
             if (!live) continue;
             if (VEC || p.vec_h_out) {
-                store8(a.h_out, a.h_dtype, row * a.h_out_stride + column(s), left, true, v[s]);
+                store8(a.h_out, a.h_dtype, row * a.h_out_stride + column(s), cols - column(s), true, v[s].each());
             } else {
                 const int first = column(s) - lane * 8;      // the warp's
-                store_span(a.h_out, a.h_dtype, row * a.h_out_stride + first, cols - first, buffer, lane, v[s]);
+                store_span(a.h_out, a.h_dtype, row * a.h_out_stride + first, cols - first, buffer, lane, v[s].each());
             }
         }
         if (!a.n_out) return;
@@ -174,29 +172,29 @@ mx4_norm_kernel(const NormArgs p) {
     } else {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, v[s]);
+            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, v[s].each());
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[s][i], v[s][i], sum);
+            for (int i = 0; i < 4; ++i) sum = fma2(v[s].p[i], v[s].p[i], sum);
         }
     }
-    const float r = 1.f / sqrtf(fmaf(row_sum(sum, slots[1]), p.inv_cols, a.eps));
+    const float r = rsqrtf(fmaf(row_sum(sum.x + sum.y, slots[1]), p.inv_cols, a.eps));
+    if (!live) return;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        const int g = s * per_row + place, left = cols - g * 8;
-        if (!live || (g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
-        float w[8];
+        const int g = s * per_row + place;
+        if ((g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
+        Pairs w;
         if (!kAhead) load_next(s);
-        next[s].values(a.weight_dtype, p.vec_next, buffer, lane, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = i < left ? v[s][i] * r * w[i] : 0.f;
+        next[s].values(a.weight_dtype, p.vec_next, buffer, lane, w.each());
+        w = times(times(v[s], r), w);
         if (a.n_dtype == MPS_MX4) {
             const int chunks = (int)mx4_chunks(cols);
-            mx4_store_row(static_cast<uint8_t*>(a.n_out) + mx4_tile_offset(row / kMx4Rows, g >> 5, chunks), (int)(row % kMx4Rows), lane, w);
+            mx4_store_row(static_cast<uint8_t*>(a.n_out) + mx4_tile_offset(row / kMx4Rows, g >> 5, chunks), (int)(row % kMx4Rows), lane, w.each());
         } else if (VEC || p.vec_n) {
-            store8(a.n_out, a.n_dtype, row * a.n_stride + g * 8, left, true, w);
+            store8(a.n_out, a.n_dtype, row * a.n_stride + g * 8, cols - g * 8, true, w.each());
         } else {
             const int first = (g - lane) * 8;
-            store_span(a.n_out, a.n_dtype, row * a.n_stride + first, cols - first, buffer, lane, w);
+            store_span(a.n_out, a.n_dtype, row * a.n_stride + first, cols - first, buffer, lane, w.each());
         }
     }
 }
