@@ -47,15 +47,26 @@ struct Eight {
             load_spread(base, dtype, row + column - lane * 8, cols - column + lane * 8, lane, w);
         }
     }
-    __device__ __forceinline__ void values(int dtype, bool vec, float* buffer, int lane, float (&v)[8]) const {
-        if (VEC || vec) {
+    // Once, before the first use: without VEC the words become the FP32 values of this lane's columns.
+    __device__ __forceinline__ void settle(int dtype, bool vec, float* buffer, int lane) {
+        if (VEC) return;
+        float v[8];
+        if (vec) {
             Raw8 r;
             r.a = make_uint4(w[0], w[1], w[2], w[3]);
-            r.b = WIDE ? make_uint4(w[4], w[5], w[6], w[7]) : r.a;
-            unpack8(r, VEC ? (WIDE ? MPS_F32 : dtype == MPS_BF16 ? MPS_BF16 : MPS_F16) : dtype, v);
+            r.b = make_uint4(w[4], w[5], w[6], w[7]);
+            unpack8(r, dtype, v);
         } else {
             gather_spread(w, dtype, buffer, lane, v);
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+    }
+    __device__ __forceinline__ void values(int dtype, Pairs& v) const {
+        Raw8 r;
+        r.a = make_uint4(w[0], w[1], w[2], w[3]);
+        r.b = WIDE ? make_uint4(w[4], w[5], w[6], w[7]) : r.a;
+        unpack8(r, WIDE ? MPS_F32 : dtype == MPS_BF16 ? MPS_BF16 : MPS_F16, v.each());
     }
 };
 
@@ -111,6 +122,13 @@ mx4_norm_kernel(const NormArgs p) {
             if (!JOIN) load_next(s);
         }
     }
+    if (!VEC) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            if (JOIN) ry[s].settle(a.y_dtype, p.vec_y, buffer, lane);
+            rh[s].settle(a.h_dtype, p.vec_h, buffer, lane);
+        }
+    }
     // Columns beyond the last are zeros all through.
     Pairs v[STEPS];
     float2 sum = make_float2(0.f, 0.f);
@@ -126,7 +144,7 @@ mx4_norm_kernel(const NormArgs p) {
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) {
                 Pairs y;
-                ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y.each());
+                ry[s].values(a.y_dtype, y);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum = fma2(y.p[i], y.p[i], sum);
             }
@@ -137,18 +155,20 @@ mx4_norm_kernel(const NormArgs p) {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
             Pairs y, h, w;
-            ry[s].values(a.y_dtype, p.vec_y, buffer, lane, y.each());
-            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, h.each());
+            ry[s].values(a.y_dtype, y);
+            rh[s].values(a.h_dtype, h);
             if (a.post_weight) {
                 if (!kAhead) load_post(s);
-                post[s].values(a.weight_dtype, p.vec_post, buffer, lane, w.each());
+                post[s].settle(a.weight_dtype, p.vec_post, buffer, lane);
+                post[s].values(a.weight_dtype, w);
                 y = times(y, times(w, scale));
             } else {
                 y = times(y, scale);
             }
             if (a.gate && a.gate_col_stride) {
                 if (!kAhead) load_gate(s);
-                gate[s].values(a.gate_dtype, p.vec_gate, buffer, lane, w.each());
+                gate[s].settle(a.gate_dtype, p.vec_gate, buffer, lane);
+                gate[s].values(a.gate_dtype, w);
                 y = times(y, w);
             }
 #pragma unroll
@@ -172,7 +192,7 @@ mx4_norm_kernel(const NormArgs p) {
     } else {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            rh[s].values(a.h_dtype, p.vec_h, buffer, lane, v[s].each());
+            rh[s].values(a.h_dtype, v[s]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum = fma2(v[s].p[i], v[s].p[i], sum);
         }
@@ -185,7 +205,8 @@ mx4_norm_kernel(const NormArgs p) {
         if ((g & ~31) >= p.groups) break;     // whole warps: a tile's row is one warp's
         Pairs w;
         if (!kAhead) load_next(s);
-        next[s].values(a.weight_dtype, p.vec_next, buffer, lane, w.each());
+        next[s].settle(a.weight_dtype, p.vec_next, buffer, lane);
+        next[s].values(a.weight_dtype, w);
         w = times(times(v[s], r), w);
         if (a.n_dtype == MPS_MX4) {
             const int chunks = (int)mx4_chunks(cols);
