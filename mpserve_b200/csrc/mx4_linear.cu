@@ -32,11 +32,12 @@ struct ProductArgs {
     bool early;              // the kernel before writes no weight: weights may be read before it is done
 };
 
-// Both activations are g / (1 + exp(-t)): SiLU with t = g, and GELU's tanh form since (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)).  The
-// exponential is CUDA's accurate one; the quotient's two units in the last place are far below what the result is rounded to.
-__device__ __forceinline__ float act(float g, int which) {
-    const float t = which == MPS_SILU ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.f);
-    return __fdividef(g, 1.f + expf(-t));
+// Both activations are g / (1 + exp(-t)): SiLU with t = g, and GELU's tanh form since (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)).  CUDA's fast exponential (off by
+// 2 + 1.17 |t| units in the last place) and quotient (by 2) are far below what the result is rounded to, 16 bits or 4; with the accurate ones the
+// gated epilogue of 256 tokens took 10000 cycles, as long as the multiplications of 4096 columns.
+__device__ __forceinline__ float act(float g, bool silu) {
+    const float t = silu ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.f);
+    return __fdividef(g, 1.f + __expf(-t));
 }
 
 // A wait that gives up when another one has.
@@ -99,7 +100,7 @@ __device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int l
     if (GATED) {
         const float u[4] = {up.x, up.y, up.z, up.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = i < valid ? act(f[i], p.activation) * u[i] : 0.f;
+        for (int i = 0; i < 4; ++i) f[i] = i < valid ? act(f[i], p.activation == MPS_SILU) * u[i] : 0.f;
     }
     if (GATED && p.out_dtype == MPS_MX4) {
         // eight lanes hold a block
@@ -346,7 +347,10 @@ mx4_stream_kernel(const ProductArgs p) {
             }
         }
         __syncwarp();
-        if (p.parts > 1) cluster_sync();      // nobody leaves while his part is read
+        if (p.parts > 1) {       // nobody leaves while his part is read
+            cluster_arrive();
+            cluster_wait();
+        }
     }
     __syncthreads();
     tensor_fence_after();
@@ -388,17 +392,17 @@ __device__ __forceinline__ WideTile wide_tile(int64_t tile, int token_tiles) {
 
 // 32 neighbouring values of one token, as a block.
 __device__ __forceinline__ uint4 block_codes(const float* v, uint32_t& byte) {
-    uint32_t m = 0u;
+    float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    byte = mx4_scale_byte(m);
+    for (int i = 0; i < 32; i += 2) m = max_abs3(m, v[i], v[i + 1]);
+    byte = mx4_scale_byte(__float_as_uint(m) & 0x7FFFFFFFu);
     const float inverse = mx4_inverse_scale(byte);
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float q[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = byte == 255u ? 0.f : v[j * 8 + i] * inverse;
+        for (int i = 0; i < 8; ++i) q[i] = v[j * 8 + i] * inverse;      // of a NaN block, whatever it gives: its codes say nothing
         w[j] = mx4_codes8(q);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
@@ -459,7 +463,8 @@ mx4_wide_kernel(const ProductArgs p) {
     if (warp == 1) tmem_alloc<2>(smem_u32(&tmem_slot), S::kColumns);
     tensor_fence_before();
     __syncthreads();
-    cluster_sync();
+    cluster_arrive();      // barriers can be arrived at from the other CTA
+    cluster_wait();
     tensor_fence_after();
     constexpr uint32_t tmem = 0;       // all columns were asked for: the allocation begins at the first
 
@@ -566,7 +571,11 @@ mx4_wide_kernel(const ProductArgs p) {
                 release();
                 const int first = t.feature * kMx4Rows + half * 64, valid = p.rows - first;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) g[i] = i < valid ? act(g[i], p.activation) * u[i] : 0.f;
+                for (int i = 0; i < 64; ++i) g[i] = act(g[i], p.activation == MPS_SILU) * u[i];
+                if (valid < 64) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) if (i >= valid) g[i] = 0.f;
+                }
                 if (p.out_dtype == MPS_MX4) {
                     const int64_t token = token0 + lane;
                     if (token < p.tokens) {
@@ -610,7 +619,8 @@ mx4_wide_kernel(const ProductArgs p) {
     __syncwarp();
     tensor_fence_before();
     __syncthreads();
-    cluster_sync();      // what the pair's instructions read and write is there until both are done
+    cluster_arrive();      // what the pair's instructions read and write is there until both are done
+    cluster_wait();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
     if (warp == 1) tmem_free<2>(tmem_slot, S::kColumns);
