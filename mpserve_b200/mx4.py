@@ -43,8 +43,9 @@ def _workspace(index: int, stream: int) -> torch.Tensor:
     return ws
 
 
-def _launch(index: int, fn, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of device ``index``."""
+def _launch(index: int, name: str, *args) -> None:
+    """The library's ``name(*args, stream)`` on the current stream of device ``index``."""
+    fn = getattr(_lib.load(), name)
     if _current_device() == index:
         rc = fn(*args, _stream_of(index))
     else:
@@ -85,10 +86,6 @@ def _tile_bytes(rows: int, cols: int) -> int:
     return (rows + 127) // 128 * ((cols + 255) // 256) * 17408
 
 
-def _tiles(rows: int, cols: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(_tile_bytes(rows, cols), dtype=torch.uint8, device=device)
-
-
 class Mx4Tensor:
     """A ``rows`` x ``cols`` matrix in MXFP4: E2M1 codes and one power-of-two scale per 32 columns, in the tiles that the tensor
     cores read (``data``).  ``shape`` is the shape of the tensor it was made of."""
@@ -97,7 +94,7 @@ class Mx4Tensor:
 
     def __init__(self, data: torch.Tensor, rows: int, cols: int, shape=None):
         self.data, self.rows, self.cols = data, rows, cols
-        self.shape = (rows, cols) if shape is None else tuple(shape)
+        self.shape = (rows, cols) if shape is None else shape
 
     @property
     def device(self) -> torch.device:
@@ -115,7 +112,7 @@ class Mx4Tensor:
         dev = self.device
         codes = torch.empty((self.rows, (self.cols + 1) // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty((self.rows, -(-self.cols // BLOCK)), dtype=torch.uint8, device=dev)
-        _launch(dev.index, _lib.load().mps_mx4_unpack, self.data.data_ptr(), self.rows, self.cols, codes.data_ptr(), scales.data_ptr())
+        _launch(dev.index, "mps_mx4_unpack", self.data.data_ptr(), self.rows, self.cols, codes.data_ptr(), scales.data_ptr())
         return codes, scales
 
 
@@ -130,9 +127,8 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
     A block's scale is 2^(floor(log2 max) - 2); codes are rounded to nearest, halfway to the even code, and saturate at 6.  A
     block with an infinity or a NaN becomes NaN."""
     rows, cols, stride = _matrix(x, "x")
-    dev = x.device
-    data = _tiles(rows, cols, dev)
-    _launch(dev.index, _lib.load().mps_mx4_quantize, x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr())
+    data = x.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
+    _launch(x.get_device(), "mps_mx4_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr())
     return Mx4Tensor(data, rows, cols, x.shape)
 
 
@@ -141,8 +137,8 @@ def dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
     _check_mx4(q, "q")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
-    out = q.data.new_empty(q.shape, dtype=dtype)
-    _launch(out.device.index, _lib.load().mps_mx4_dequantize, q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
+    out = q.data.new_empty(*q.shape, dtype=dtype)
+    _launch(out.get_device(), "mps_mx4_dequantize", q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -163,9 +159,9 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
             raise ValueError(f"{name} must have {width} columns for {cols} columns of values")
     if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
         raise ValueError("codes and scales must have the same rows and device")
-    rows, dev = codes.shape[0], codes.device
-    data = _tiles(rows, cols, dev)
-    _launch(dev.index, _lib.load().mps_mx4_pack, codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr())
+    rows = codes.shape[0]
+    data = codes.new_empty(_tile_bytes(rows, cols))
+    _launch(codes.get_device(), "mps_mx4_pack", codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr())
     return Mx4Tensor(data, rows, cols)
 
 
@@ -181,13 +177,12 @@ def _run_product(args, index: int) -> None:
 
 def _product(x, w, w_up, activation: int, dtype, quantized: bool):
     _check_mx4(w, "w" if w_up is None else "w_gate")
-    out_cols, w_cols, dev = w.rows, w.cols, w.data.device
-    up = 0
+    out_cols, w_cols, index, up = w.rows, w.cols, w.data.get_device(), 0
     if w_up is not None:
         _check_mx4(w_up, "w_up")
         if w_up.rows != out_cols or w_up.cols != w_cols:
             raise ValueError("w_gate and w_up must have the same shape")
-        if w_up.data.device != dev:
+        if w_up.data.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
         up = w_up.data.data_ptr()
     if out_cols == 0:
@@ -206,7 +201,7 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool):
             tiles = w.data.new_empty(_tile_bytes(rows, cols))
     if cols != w_cols:
         raise ValueError(f"x has {cols} columns, the weight {w_cols}")
-    if data.device != dev:
+    if data.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
     shape = (*x.shape[:-1], out_cols)
     if quantized:
@@ -215,11 +210,10 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool):
     else:
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError("a product's dtype must be bfloat16 or float16")
-        out = result = data.new_empty(shape) if data.dtype is dtype else data.new_empty(shape, dtype=dtype)
+        out = result = data.new_empty(*shape) if data.dtype is dtype else data.new_empty(*shape, dtype=dtype)
         out_dtype = _DTYPES[dtype]
     args = _lib.MX4_LINEAR.pack(data.data_ptr(), 0 if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
                                 stride, out_cols, x_dtype, out_dtype, activation, 0)
-    index = dev.index
     if _current_device() == index:
         _run_product(args, index)
     else:
@@ -262,23 +256,23 @@ def product_timed_out(device: torch.device | None = None) -> bool:
 
 # ---- norms, gate and residual ------------------------------------------------------------------------------
 
-def _gain(t, name: str, cols: int, dev) -> int:
+def _gain(t, name: str, cols: int, index: int) -> int:
     if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.numel() != cols:
         raise ValueError(f"{name} must be a bfloat16, float16 or float32 vector of {cols} values")
-    if t.device != dev:
+    if t.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
 
 
-def _gains(post_weight, next_weight, cols: int, dev):
+def _gains(post_weight, next_weight, cols: int, index: int):
     """(pointers or 0, the dtype that the two share)."""
     post = nxt = dtype = 0
     if post_weight is not None:
-        post, dtype = _gain(post_weight, "post_weight", cols, dev), _DTYPES[post_weight.dtype]
+        post, dtype = _gain(post_weight, "post_weight", cols, index), _DTYPES[post_weight.dtype]
     if next_weight is not None:
-        nxt, dtype = _gain(next_weight, "next_weight", cols, dev), _DTYPES[next_weight.dtype]
+        nxt, dtype = _gain(next_weight, "next_weight", cols, index), _DTYPES[next_weight.dtype]
         if post_weight is not None and post_weight.dtype != next_weight.dtype:
             raise ValueError("post_weight and next_weight must have the same dtype")
     return post, nxt, dtype
@@ -294,7 +288,7 @@ def _normed(like, rows, cols, dtype, quantized: bool):
     if quantized:
         data = like.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
         return Mx4Tensor(data, rows, cols, like.shape), data.data_ptr(), _MX4
-    n = like.new_empty(like.shape) if like.dtype is dtype else like.new_empty(like.shape, dtype=dtype)
+    n = like.new_empty(*like.shape) if like.dtype is dtype else like.new_empty(*like.shape, dtype=dtype)
     return n, n.data_ptr(), _DTYPES[dtype]
 
 
@@ -306,12 +300,12 @@ def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype:
     dtype = h.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
-    dev = h.device
-    w = _gain(weight, "weight", cols, dev)
+    index = h.get_device()
+    w = _gain(weight, "weight", cols, index)
     n, n_ptr, n_dtype = _normed(h, rows, cols, dtype, quantized)
     args = _lib.MX4_NORM.pack(0, h.data_ptr(), 0, 0, w, 0, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
                               _DTYPES[weight.dtype], eps, 1.0)
-    _launch(dev.index, _lib.load().mps_mx4_norm_rows, args)
+    _launch(index, "mps_mx4_norm_rows", args)
     return n
 
 
@@ -328,15 +322,15 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
     FP32 beside a 16-bit ``y``; ``h'`` has its type, and is ``h`` itself where ``inplace``.  The two weights share a dtype."""
     rows, cols, y_stride = _matrix(y, "y")
     _, _, h_stride = _matrix(h, "h")
-    shape, dev = y.shape, y.device
+    shape, index = y.shape, y.get_device()
     if shape != h.shape:
         raise ValueError("y and h must have the same shape")
     _check_norm_cols(cols)
-    if h.device != dev:
+    if h.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
     n = None
     n_ptr = n_dtype = g = g_dtype = g_row = g_col = 0
-    post, nxt, weight_dtype = _gains(post_weight, next_weight, cols, dev)
+    post, nxt, weight_dtype = _gains(post_weight, next_weight, cols, index)
     if gate is not None:
         g, g_dtype, g_row, g_col = _gate(gate, y, rows, cols)
     if inplace:
@@ -344,12 +338,12 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
         if rows > 1 and h_stride < cols:
             raise ValueError("h has rows that share memory and cannot be updated in place")
     else:
-        joined, out_stride = h.new_empty(shape), cols
+        joined, out_stride = h.new_empty(*shape), cols
     if nxt:
         n, n_ptr, n_dtype = _normed(y, rows, cols, y.dtype, quantized)
     args = _lib.MX4_NORM.pack(y.data_ptr(), h.data_ptr(), post, g, nxt, joined.data_ptr(), n_ptr, rows, cols, y_stride, h_stride, out_stride, cols,
                               g_row, g_col, _DTYPES[y.dtype], _DTYPES[h.dtype], n_dtype, g_dtype, weight_dtype, eps, residual_scale)
-    _launch(dev.index, _lib.load().mps_mx4_norm_rows, args)
+    _launch(index, "mps_mx4_norm_rows", args)
     return joined, n
 
 
@@ -357,7 +351,7 @@ def _gate(gate, y, rows: int, cols: int):
     """(pointer, dtype, row stride, column stride) of a gate that broadcasts to ``y``."""
     if not isinstance(gate, torch.Tensor) or gate.dtype not in _DTYPES:
         raise ValueError("gate must be a bfloat16, float16 or float32 tensor")
-    if gate.device != y.device:
+    if gate.get_device() != y.get_device():
         raise ValueError("all tensors must be on the same CUDA device")
     if gate.dim() <= y.dim() and gate.is_contiguous():
         if gate.dim() == 1 and gate.numel() == cols:
@@ -395,11 +389,11 @@ class GatedMlp:
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self.pre_weight, self.post_weight, self.gate, self.next_weight = pre_weight, post_weight, gate, next_weight
         self.hidden, self.inter = hidden, inter
-        dev = self.device = gate_proj.device
+        index = self._index = gate_proj.data.get_device()
         b = self._block = _lib.Mx4Mlp()
         b.gate_proj, b.up_proj, b.down_proj = (q.data.data_ptr() for q in (gate_proj, up_proj, down_proj))
-        b.pre_weight, b.pre_dtype = _gain(pre_weight, "pre_weight", hidden, dev), _DTYPES[pre_weight.dtype]
-        b.post_weight, b.next_weight, b.weight_dtype = _gains(post_weight, next_weight, hidden, dev)
+        b.pre_weight, b.pre_dtype = _gain(pre_weight, "pre_weight", hidden, index), _DTYPES[pre_weight.dtype]
+        b.post_weight, b.next_weight, b.weight_dtype = _gains(post_weight, next_weight, hidden, index)
         b.hidden, b.inter, b.activation, b.eps, b.residual_scale = hidden, inter, _ACTIVATIONS[activation], eps, residual_scale
         self._gate_per_call = gate is not None and (not isinstance(gate, torch.Tensor) or gate.dim() != 1 or gate.numel() != hidden)
         if gate is not None and not self._gate_per_call:
@@ -409,8 +403,8 @@ class GatedMlp:
         rows, cols, stride = _matrix(h, "h")
         if cols != self.hidden:
             raise ValueError(f"h has {cols} columns, the block {self.hidden}")
-        dev = h.device
-        if dev != self.device:
+        index = self._index
+        if h.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
         block = self._block
         if self._gate_per_call:      # a value per row or per element: it has to fit this h
@@ -422,13 +416,12 @@ class GatedMlp:
             if rows > 1 and stride < cols:
                 raise ValueError("h has rows that share memory and cannot be updated in place")
         else:
-            joined, out_stride = h.new_empty(h.shape), cols
+            joined, out_stride = h.new_empty(*h.shape), cols
         n = None
         if block.next_weight:
-            n = h.new_empty(h.shape, dtype=torch.bfloat16) if h_dtype == 2 else h.new_empty(h.shape)
+            n = h.new_empty(*h.shape, dtype=torch.bfloat16) if h_dtype == 2 else h.new_empty(*h.shape)
         scratch_bytes = _tile_bytes(rows, cols) + _tile_bytes(rows, self.inter) + rows * cols * 2
         scratch = self.gate_proj.data.new_empty(scratch_bytes)      # of this call: freed on return, and not handed to another stream before it is done
-        index = dev.index
         args = (C.byref(block), h.data_ptr(), h_dtype, stride, rows, joined.data_ptr(), out_stride, None if n is None else n.data_ptr(),
                 0 if h_dtype == 2 else h_dtype, scratch.data_ptr(), scratch_bytes)
         if _current_device() == index:
