@@ -38,10 +38,25 @@ def test_quantize_and_back(rows, cols, dtype):
     assert mx4.product_timed_out() is False
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_edges_of_the_number_range(dtype):
-    t = ref.TYPES[dtype]
-    rows = [
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1024), (3, 784), (130, 1040), (5, 1296), (7, 1536), (2, 1808), (33, 2064), (1, 8192), (9, 4080)])
+def test_long_rows(rows, cols, dtype):
+    """Rows of four pieces and more, a multiple of 16 columns: every number of tiles that the last step of a warp can have."""
+    x = torch.randn((rows, cols), device="cuda") * torch.exp2(torch.randint(-12, 12, (rows, cols), device="cuda").float())
+    x[0, ::37] = 0
+    x = x.to(ref.TYPES[dtype])
+    ref.poison()
+    q = mx4.quantize(x)
+    _same(q, ref.to64(x))
+    np.testing.assert_array_equal(ref.to64(q.dequantize()), ref.values(q))
+    np.testing.assert_array_equal(ref.to64(q.dequantize(torch.float32)), ref.values(q))
+    # the columns that fill up the last tile are zeros of the least scale: rows of garbage there would show in a product
+    w = mx4.quantize(torch.ones((4, cols), device="cuda"))
+    assert mx4.linear(q, w).isfinite().all()
+
+
+def _edge_rows(t):
+    return [
         [0.0] * 32, [-0.0] * 32,
         [2.0 ** e for e in range(-16, 16)],
         [2.0 ** -126 * (1 + i / 32) for i in range(32)],
@@ -58,11 +73,18 @@ def test_edges_of_the_number_range(dtype):
         # a largest value just below and at a power of two
         [(2 - 2.0 ** -7)] + [0.25] * 31, [2.0] + [0.25] * 31,
     ]
-    x = torch.tensor(rows, dtype=torch.float64).to(t).cuda()
-    q = mx4.quantize(x)
-    _same(q, ref.to64(x))
-    np.testing.assert_array_equal(ref.to64(q.dequantize(torch.float32)), ref.values(q))
-    np.testing.assert_array_equal(ref.to64(q.dequantize()), ref.values(q))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_edges_of_the_number_range(dtype):
+    t = ref.TYPES[dtype]
+    rows = _edge_rows(t)
+    for x in (torch.tensor(rows, dtype=torch.float64), torch.tensor(rows, dtype=torch.float64).repeat(1, 33)):      # short rows and long ones
+        x = x.to(t).cuda()
+        q = mx4.quantize(x)
+        _same(q, ref.to64(x))
+        np.testing.assert_array_equal(ref.to64(q.dequantize(torch.float32)), ref.values(q))
+        np.testing.assert_array_equal(ref.to64(q.dequantize()), ref.values(q))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

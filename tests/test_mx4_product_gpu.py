@@ -216,3 +216,32 @@ def test_gated_mlp(tokens, hidden, inter):
     want = mx4.block_join(y, h, post_weight=post, gate=post, residual_scale=0.5, next_weight=nxt, eps=1e-6)
     assert torch.equal(joined, want[0]) and torch.equal(n, want[1])
     assert torch.equal(block(h, inplace=True)[0], want[0]) and torch.equal(h, want[0])
+
+
+@pytest.mark.parametrize("tokens", [1, 33, 200])
+@pytest.mark.parametrize("stream,gate,activation", [("f32", "row", "gelu"), ("f16", "full", "silu"), ("bf16", None, "gelu")])
+def test_gated_mlp_forms(tokens, stream, gate, activation):
+    """Streams of every type, gates that are checked with every call, strided streams."""
+    hidden, inter = 384, 1000
+    whole, gp = _inputs(tokens, hidden + 64, inter, 12, stream)
+    h = whole[:, 32:32 + hidden]
+    gp, up, down = (mx4.quantize(torch.randn(s, device="cuda") * 0.05) for s in ((inter, hidden), (inter, hidden), (hidden, inter)))
+    pre, nxt = (torch.rand(hidden, device="cuda").to(torch.bfloat16) for _ in range(2))
+    g = None if gate is None else torch.randn((tokens, 1) if gate == "row" else (tokens, hidden), device="cuda")
+    block = mx4.GatedMlp(gp, up, down, pre_weight=pre, gate=g, next_weight=nxt, eps=1e-6, activation=activation)
+    joined, n = block(h)
+    kept = torch.bfloat16 if stream == "f32" else h.dtype
+    x = mx4.rms_norm(h, pre, eps=1e-6, quantized=True)
+    y = mx4.linear(mx4.gated_linear(x, gp, up, activation=activation, quantized=True), down, dtype=kept)
+    want = mx4.block_join(y, h, gate=g, next_weight=nxt, eps=1e-6)
+    assert torch.equal(joined, want[0]) and torch.equal(n, want[1]) and n.dtype == kept and joined.dtype == h.dtype
+    if g is not None and tokens > 1:      # (one row's gate fits any number of rows)
+        with pytest.raises(ValueError, match="gate must be contiguous"):
+            block(torch.cat([h, h]))
+
+
+def test_gated_mlp_of_no_tokens():
+    w = mx4.quantize(torch.ones((64, 64), device="cuda"))
+    one = torch.ones(64, device="cuda")
+    joined, n = mx4.GatedMlp(w, w, w, pre_weight=one, next_weight=one)(torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"))
+    assert joined.shape == n.shape == (0, 64)
