@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kNormMostThreads)
 mx4_norm_kernel(const NormArgs p) {
     __shared__ float slots[2][16];
     __shared__ __align__(16) float buffers[VEC ? 1 : kNormMostThreads / 32][256];
-    constexpr bool kAhead = STEPS <= 2;      // with more, the registers are for y and h
+    constexpr bool kAhead = STEPS <= (JOIN ? 2 : 4);      // with more, the registers are for y and h
     griddep_wait();
     griddep_launch();
     const mps_mx4_norm& a = p.a;
@@ -282,9 +282,11 @@ extern "C" int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream) {
     const bool vec = a.cols % 8 == 0 && p.vec_h && (!a.y || (p.vec_y && p.vec_h_out)) && (!a.n_out || a.n_dtype == MPS_MX4 || p.vec_n) &&
                      (!a.y || !a.post_weight || p.vec_post) && (!a.next_weight || p.vec_next) &&
                      (!column_gate || (p.vec_gate && (a.gate_dtype == MPS_F32) == wide_w));
-    // 256 threads for a row where there are many rows (8191 x 4096: 68 us, with 512 78 us), 512 where a few wait for their own length (64 x 4096: 2.7 us,
-    // with 256 3.0 us) or where 256 would hold 32 columns each and more (2048 x 14336: 55 us, with 256 79 us)
-    const int most = a.rows < kNormManyRows ? kNormMostThreads : p.groups <= 64 ? 32 : p.groups <= 4 * kNormThreads ? kNormThreads : kNormMostThreads;
+    // 256 threads for a row where there are many rows (8191 x 4096: 68 us, with 512 78 us), without a y 128 (8191 x 4096 FP32, quantised: 27 us, with 256
+    // 30 us), 512 where a few wait for their own length (64 x 4096: 2.7 us, with 256 3.0 us) or where 256 would hold 32 columns each and more (2048 x
+    // 14336: 55 us, with 256 79 us), one warp for short rows
+    const int many = a.y || p.groups > 512 ? kNormThreads : kNormThreads / 2;
+    const int most = a.rows < kNormManyRows ? kNormMostThreads : p.groups <= 64 ? 32 : p.groups <= 4 * kNormThreads ? many : kNormMostThreads;
     int steps = 1;
     while ((p.groups + steps - 1) / steps > most) steps *= 2;
     const int per_row = ((p.groups + steps - 1) / steps + 31) / 32 * 32;
