@@ -2,7 +2,7 @@
 //
 // Bounds: memory, and instructions nearly as much.  Quantising a BF16 matrix reads 2 bytes and writes 0.53 per element; a warp takes four neighbouring
 // pieces of 256 columns, of one row or of several, so that a lane has 64 bytes under way, and the codes of a piece leave as one 128-byte line.
-// Long rows that begin at multiples of 32 bytes have kernels of their own with sixteen columns a lane, half a block, which need half the instructions
+// Long 16-bit rows that begin at multiples of 32 bytes have kernels of their own with sixteen columns a lane, half a block, which need half the instructions
 // (14336 x 4096 BF16 23.3 us, 6.4 TB/s, with eight columns a lane 28; and back 24.6 us, 6.0 TB/s, with eight 27).
 #include "mx4.cuh"
 
@@ -14,7 +14,7 @@ constexpr int kConvertThreads = 256;
 constexpr int kConvertPieces = 4;   // of a warp
 
 // Where a warp's pieces are.  Of a row of at least four they are neighbours in it; SHORT rows have fewer, and a warp takes those of several rows (385667 x 128
-// BF16 59 us, one row a warp 88; 14336 x 4096 28 us, counted as short ones are 36).
+// BF16 59 us, one row a warp 96; 14336 x 4096 28 us, counted as short ones are 36).
 template <bool SHORT>
 struct Pieces {
     int64_t rows, row, tile;
@@ -109,8 +109,9 @@ mx4_dequantize_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t cols,
     }
 }
 
-// Long rows: at least four pieces, a multiple of 16 columns, every row at a multiple of 32 bytes.  A lane has sixteen columns, a warp two neighbouring tiles
-// at a time.
+// Long rows of a 16-bit type: at least four pieces, a multiple of 16 columns, every row at a multiple of 32 bytes.  A lane has sixteen columns, a warp two
+// neighbouring tiles at a time.  (FP32, 64 bytes a lane, takes longer this way than with eight columns a lane: 3000 x 5008 12.1 us against 11.7, and back
+// 25 against 18.)
 struct LongPlace {
     int64_t row;
     int chunk, column;                   // this lane's tile in the first step, and its column
@@ -134,33 +135,25 @@ static __device__ __forceinline__ LongPlace long_place(int chunks) {
 template <int DTYPE>
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_quantize_long_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t row_stride, int chunks, uint8_t* __restrict__ out) {
-    constexpr int kSteps = kConvertPieces / 2, kWords = DTYPE == MPS_F32 ? 2 : 1;
+    constexpr int kSteps = kConvertPieces / 2;
     griddep_wait();
     griddep_launch();
     const LongPlace p = long_place(chunks);
     if (p.row >= rows) return;
-    Raw8 raw[kSteps][kWords];
-    const char* from = static_cast<const char*>(x) + (p.row * row_stride + p.column) * (DTYPE == MPS_F32 ? 4 : 2);
+    Raw8 raw[kSteps];      // sixteen 16-bit values each
+    const uint16_t* from = static_cast<const uint16_t*>(x) + p.row * row_stride + p.column;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-        for (int j = 0; j < kWords; ++j) {
-            raw[i][j].a = raw[i][j].b = make_uint4(0u, 0u, 0u, 0u);
-            if (p.column + i * 2 * kMx4Cols < cols)
-                raw[i][j] = load_wide8(reinterpret_cast<const float*>(from + i * 2 * kMx4Cols * (DTYPE == MPS_F32 ? 4 : 2)) + 8 * j);
-        }
+    for (int i = 0; i < kSteps; ++i) {
+        raw[i].a = raw[i].b = make_uint4(0u, 0u, 0u, 0u);
+        if (p.column + i * 2 * kMx4Cols < cols) raw[i] = load_wide8(reinterpret_cast<const float*>(from + i * 2 * kMx4Cols));
+    }
     uint8_t* tile = out + p.tile;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i, tile += 2 * kMx4TileBytes) {
         Pairs a, b;
-        if (DTYPE == MPS_F32) {
-            unpack8(raw[i][0], DTYPE, a.each());
-            unpack8(raw[i][kWords - 1], DTYPE, b.each());
-        } else {
-            unpack8(raw[i][0], DTYPE, a.each());
-            raw[i][0].a = raw[i][0].b;
-            unpack8(raw[i][0], DTYPE, b.each());
-        }
+        unpack8(raw[i], DTYPE, a.each());
+        raw[i].a = raw[i].b;
+        unpack8(raw[i], DTYPE, b.each());
         uint32_t m = max(max_bits8(a.each()), max_bits8(b.each()));
         m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
         const uint32_t byte = mx4_scale_byte(m);
@@ -174,7 +167,6 @@ mx4_quantize_long_kernel(const void* __restrict__ x, int64_t rows, int cols, int
     }
 }
 
-// Into a 16-bit type.  (FP32, 64 bytes a lane, took longer this way than with eight columns a lane, 3000 x 5008 25 us against 18.)
 template <int DTYPE>
 __global__ void __launch_bounds__(kConvertThreads)
 mx4_dequantize_long_kernel(const uint8_t* __restrict__ q, int64_t rows, int cols, int chunks, void* __restrict__ out) {
@@ -287,7 +279,7 @@ static int convert_grid(const char* who, int64_t rows, int64_t cols, ConvertGrid
 }
 
 static bool long_ok(const void* p, int64_t row_stride, int64_t cols, int dtype) {
-    return cols % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0 && row_stride * mx4_dtype_bytes(dtype) % 32 == 0;
+    return dtype != MPS_F32 && cols % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0 && row_stride % 16 == 0;
 }
 
 // The current device, its SMs counted once.
@@ -322,7 +314,7 @@ int mps_mx4_quantize(const void* x, int32_t dtype, int64_t rows, int64_t cols, i
     if (rows == 0) return MPS_OK;
     if (!x || !tiles || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_quantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
     if (!g.few && long_ok(x, row_stride, cols, dtype)) {
-        const auto kernel = dtype == MPS_BF16 ? mx4_quantize_long_kernel<MPS_BF16> : dtype == MPS_F16 ? mx4_quantize_long_kernel<MPS_F16> : mx4_quantize_long_kernel<MPS_F32>;
+        const auto kernel = dtype == MPS_BF16 ? mx4_quantize_long_kernel<MPS_BF16> : mx4_quantize_long_kernel<MPS_F16>;
         return launch_overlapping("mx4_quantize_long_kernel", kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream), x, rows, (int)cols, row_stride,
                                   g.chunks, static_cast<uint8_t*>(tiles));
     }
@@ -339,7 +331,7 @@ int mps_mx4_dequantize(const void* tiles, int64_t rows, int64_t cols, int32_t dt
     if (!mx4_dtype_ok(dtype)) { set_error("mps_mx4_dequantize: unknown dtype %d", (int)dtype); return MPS_ERR_INVALID; }
     if (rows == 0) return MPS_OK;
     if (!tiles || !out || (reinterpret_cast<uintptr_t>(tiles) & 15u)) { set_error("mps_mx4_dequantize: null or unaligned pointer"); return MPS_ERR_INVALID; }
-    if (!g.few && dtype != MPS_F32 && long_ok(out, cols, cols, dtype)) {
+    if (!g.few && long_ok(out, cols, cols, dtype)) {
         const auto kernel = dtype == MPS_BF16 ? mx4_dequantize_long_kernel<MPS_BF16> : mx4_dequantize_long_kernel<MPS_F16>;
         return launch_overlapping("mx4_dequantize_long_kernel", kernel, g.ctas, kConvertThreads, static_cast<cudaStream_t>(stream),
                                   static_cast<const uint8_t*>(tiles), rows, (int)cols, g.chunks, out);

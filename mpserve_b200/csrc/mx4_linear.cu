@@ -64,10 +64,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // where every CTA adds up a share of the tokens, always in the same order.  Up to 32 tokens (16 with a gate) each sends its parts to where they are
 // added, as they come out of the accumulator, and a barrier there counts them: nothing but that barrier is waited for (1 token through 14336 x 4096
 // 7.4 us).  More would take stages from the ring; they take its place, and the adding CTA fetches them between two barriers of the whole cluster
-// (1 token 7.9 us that way; 64 tokens through 4096 x 14336 9.8 us, sent 10.1).
+// (1 token 7.7 us that way; 64 tokens through 4096 x 14336 9.5 us, sent 10.1).
 //
 // Warps: 0 copies, 1 multiplies, the next four or eight take the accumulator over, one or two on each quarter of its lanes (four launch a little
-// sooner, 1 token 7.9 us and 8.0 with eight; eight are done sooner where there are more tokens, the gated pair for 64 18.5 us and 17.7); all of them add the
+// sooner, 1 token 7.4 us and with eight 7.6; eight are done sooner where there are more tokens, the gated pair for 64 17.2 us and with four 18.1); all of them add the
 // parts up.  With QUANTIZE, one more for every stage of the ring quantises the tokens' columns on their way into it, instead of a kernel before this one.
 template <int TOKENS, bool GATED>
 struct StreamShape {
@@ -89,7 +89,9 @@ struct StreamShape {
     static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
     static_assert(kAcc * 128 * 4 <= kReceived, "a part of the accumulator takes the ring's place");
 };
-constexpr int kMostQuantizedInside = 8;        // tokens that the kernel quantises itself
+// Tokens that the kernel quantises itself.  us, inside | by a kernel before it: 14336 x 4096, 1 token 7.7 | 8.8, 8: 9.2 | 9.5, 9: 9.9 | 9.6, 16: 12.3 | 9.7
+// (1024 x 4096 3.1 | 4.6, 3.8 | 5.2, 4.2 | 5.2, 5.3 | 5.3); and a launch less for the host.
+constexpr int kMostQuantizedInside = 8;
 constexpr int kMostParts = 4;                  // CTAs of a cluster
 
 // One token of a tile's 128 features, four neighbouring ones a lane (`up` too where the pair is gated), into the output.
@@ -673,8 +675,8 @@ static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
 }
 
 // Whether 128 tokens a tile with the weights on the lanes take less time than 256 with the tokens on the lanes, by what a tile of K, a round of CTAs
-// and a launch cost in each, us.  Measured, stream | wide: 14336 x 4096, 64 tokens 10.2 | 11.1, 128: 12.5 | 11.9, 512: 26.5 | 18.0; 4096 x 14336,
-// 128: 12.1 | 26.4, 512: 19.1 | 26.4, 1024: 29.9 | 27.1; 4096 x 4096, 256: 9.5 | 10.6, 1024: 13.4 | 11.3; 517 x 1000, 1024: 7.3 | 8.9.
+// and a launch cost in each, us.  Measured, stream | wide: 14336 x 4096, 64 tokens 9.7 | 10.7, 128: 11.6 | 11.5, 512: 25.2 | 17.8; 4096 x 14336,
+// 128: 11.8 | 26.0, 512: 18.3 | 26.0, 1024: 29.7 | 26.5; 4096 x 4096, 256: 10.2 | 10.4, 1024: 13.1 | 10.7; 517 x 1000, 1024: 7.3 | 8.8.
 static bool stream_pays(const ProductArgs& p, int sms) {
     const int64_t tiles = (int64_t)p.row_tiles * ((p.tokens + 127) / 128), wide = (int64_t)((p.row_tiles + 1) / 2) * ((p.tokens + 255) / 256);
     const int parts = parts_of(tiles, p.chunks, sms);

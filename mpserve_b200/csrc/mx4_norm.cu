@@ -223,7 +223,7 @@ mx4_norm_kernel(const NormArgs p) {
 template <int STEPS>
 static int launch_norm(const NormArgs& p, bool vec, bool wide_w, int per_row, cudaStream_t st) {
     const mps_mx4_norm& a = p.a;
-    // short rows share a CTA: 20000 of 512 columns 22 us with a CTA each
+    // short rows share a CTA
     const int rows_per_cta = per_row >= kNormThreads ? 1 : kNormThreads / per_row;
     const bool wide_y = a.y && a.y_dtype == MPS_F32, wide_h = a.h_dtype == MPS_F32;
     void (*kernel)(NormArgs) = a.y ? mx4_norm_kernel<STEPS, false, true, true, true, true> : mx4_norm_kernel<STEPS, false, false, true, true, true>;
@@ -282,9 +282,9 @@ extern "C" int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream) {
     const bool vec = a.cols % 8 == 0 && p.vec_h && (!a.y || (p.vec_y && p.vec_h_out)) && (!a.n_out || a.n_dtype == MPS_MX4 || p.vec_n) &&
                      (!a.y || !a.post_weight || p.vec_post) && (!a.next_weight || p.vec_next) &&
                      (!column_gate || (p.vec_gate && (a.gate_dtype == MPS_F32) == wide_w));
-    // 256 threads for a row where there are many rows (8191 x 4096: 68 us, with 512 78 us), without a y 128 (8191 x 4096 FP32, quantised: 27 us, with 256
-    // 30 us), 512 where a few wait for their own length (64 x 4096: 2.7 us, with 256 3.0 us) or where 256 would hold 32 columns each and more (2048 x
-    // 14336: 55 us, with 256 79 us), one warp for short rows
+    // 256 threads for a row where there are many rows (8191 x 4096 beside FP32: 64 us, with 512 75 us), without a y 128 (8191 x 4096 FP32, quantised: 27 us,
+    // with 256 30 us), 512 where a few wait for their own length (64 x 4096: 2.4 us, with 256 2.7 us) or where 256 would hold 32 columns each and more
+    // (2048 x 14336: 50 us, with 256 73 us), one warp for short rows (20000 x 512: 17 us, with 64 threads 19 us)
     const int many = a.y || p.groups > 512 ? kNormThreads : kNormThreads / 2;
     const int most = a.rows < kNormManyRows ? kNormMostThreads : p.groups <= 64 ? 32 : p.groups <= 4 * kNormThreads ? many : kNormMostThreads;
     int steps = 1;
