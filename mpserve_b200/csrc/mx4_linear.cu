@@ -40,11 +40,12 @@ __device__ __forceinline__ float act(float g, bool silu) {
     return __fdividef(g, 1.f + __expf(-t));
 }
 
-// A wait that gives up when another one has.
+// A wait that gives up when another one has.  CLUSTER: what it waits for comes from another CTA, too.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kMx4SpinLimit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+        if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
         if ((i & 63u) == 63u && *failed) return false;
     }
     *failed = 1u;
@@ -52,8 +53,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 
 // The same for a whole warp: the same answer in every lane.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, failed));
+    return __all_sync(0xFFFFFFFFu, bar_wait<CLUSTER>(bar, parity, failed));
 }
 
 // ---- few tokens: weights on the accumulator's lanes -------------------------------------------------
@@ -314,7 +316,7 @@ mx4_stream_kernel(const ProductArgs p) {
     if (send) {
         if (warp < 2 || warp >= S::kWarps) cluster_wait();      // the other warps have
         cluster_arrive();
-        if (warp_wait(received, 0, &failed)) {
+        if (warp_wait<true>(received, 0, &failed)) {
 #pragma unroll 1
             for (int i = warp; i * p.parts + part < tokens; i += warps) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f), up = v;
@@ -349,10 +351,7 @@ mx4_stream_kernel(const ProductArgs p) {
             }
         }
         __syncwarp();
-        if (p.parts > 1) {       // nobody leaves while his part is read
-            cluster_arrive();
-            cluster_wait();
-        }
+        if (p.parts > 1) cluster_sync();       // nobody leaves while his part is read
     }
     __syncthreads();
     tensor_fence_after();
@@ -369,8 +368,15 @@ mx4_stream_kernel(const ProductArgs p) {
 // but the scales' columns of the tensor memory, so it is read into registers as a whole (some 300 cycles) and multiplied into again
 // while it is converted and stored.
 //
-// Warps: 0 copies, 1 multiplies (first CTA) or hands on the arrival of the copies (second), 2 to 9 take the accumulator over, two
+// The copies of both CTAs count at the first one's barrier, whose thread issues the multiplications, so they are tiled copies: a tile is 17 rows of 1 KB,
+// the scales the first, and box and coordinates say which are wanted.  (With untiled copies, which count at their own CTA's barriers, the second
+// CTA has to hand every stage on with a release at cluster scope: 4096 x 4096 x 14336 took 164 us that way.)
+//
+// Warps: 0 copies, 1 multiplies (first CTA) or waits for the end (second), 2 to 9 take the accumulator over, two
 // on each quarter of the lanes, one on each half of the columns.
+struct WideMaps { CUtensorMap x, w_scales, w_codes, up_scales, up_codes; };
+constexpr int kMx4MapRow = 1024, kMx4TileMapRows = kMx4TileBytes / kMx4MapRow;
+
 struct WideShape {
     static constexpr int kCodes = kMx4Rows * kMx4RowBytes;
     static constexpr int kWeightScales = kMx4TileBytes;                     // of a stage: tokens, the weights' scales, their codes
@@ -442,7 +448,7 @@ __device__ __forceinline__ void store_rows(uint32_t buffer, int lane, const uint
 
 template <bool GATED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
-mx4_wide_kernel(const ProductArgs p) {
+mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
     using S = WideShape;
     extern __shared__ __align__(1024) uint8_t ring_bytes[];      // all of the shared memory: rings begin at multiples of 1024
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -450,12 +456,12 @@ mx4_wide_kernel(const ProductArgs p) {
     const uint32_t ring = smem_u32(ring_bytes), bar0 = ring + S::kBars;
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(ring_bytes + S::kSmem - 16);
     volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(ring_bytes + S::kSmem - 12);
-    const auto full = [&](int s) { return bar0 + 8u * s; };                       // this CTA's copies have come; in the first CTA, the second's too
+    const auto full = [&](int s) { return bar0 + 8u * s; };                       // both CTAs' copies have come; the first CTA's
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
     const uint32_t acc_full = bar0 + 8u * (2 * S::kStages), acc_empty = acc_full + 8u, drained = acc_full + 16u;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), rank == 0 ? 2 : 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 16);
         mbar_init(drained, 1);
@@ -479,51 +485,51 @@ mx4_wide_kernel(const ProductArgs p) {
         if (lane == 0) {
             int64_t i = 0;
             bool ok = true;
+            prefetch_map(&maps.x);
+            prefetch_map(&maps.w_scales);
+            prefetch_map(GATED && rank ? &maps.up_codes : &maps.w_codes);
+            if (GATED) prefetch_map(&maps.up_scales);
             griddep_wait();
             griddep_launch();
             for (int64_t tile = pair; tile < tiles && ok; tile += pairs) {
                 const WideTile t = wide_tile(tile, p.token_tiles);
                 // what lies beyond the last tile of 128 is multiplied as the last and not stored
-                const uint8_t* x = p.x + mx4_tile_offset(min(2 * t.token + rank, last_token_tile), 0, chunks);
-                const uint8_t* w0 = GATED ? p.w + mx4_tile_offset(t.feature, 0, chunks) : p.w + mx4_tile_offset(2 * t.feature, 0, chunks);
-                const uint8_t* w1 = GATED ? p.w_up + mx4_tile_offset(t.feature, 0, chunks)
-                                          : p.w + mx4_tile_offset(min(2 * t.feature + 1, p.row_tiles - 1), 0, chunks);
+                const auto row_of = [&](int64_t row_tile) { return (int)(row_tile * chunks * kMx4TileMapRows); };
+                const int x = row_of(min(2 * t.token + rank, last_token_tile));
+                const int w0 = row_of(GATED ? t.feature : 2 * t.feature), w1 = row_of(GATED ? t.feature : min(2 * t.feature + 1, p.row_tiles - 1));
+                const CUtensorMap* scales1 = GATED ? &maps.up_scales : &maps.w_scales;
+                const CUtensorMap* codes = GATED && rank ? &maps.up_codes : &maps.w_codes;
                 for (int k = 0; k < chunks; ++k, ++i) {
                     const int s = (int)(i % S::kStages);
-                    if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) { ok = false; break; }
-                    const uint32_t to = ring + s * S::kStageBytes;
-                    const int64_t at = (int64_t)k * kMx4TileBytes;
-                    mbar_expect_tx(full(s), S::kStageBytes);
-                    bulk_g2s(to, x + at, kMx4TileBytes, full(s));
-                    bulk_g2s(to + S::kWeightScales, w0 + at, kMx4ScaleBytes, full(s));
-                    bulk_g2s(to + S::kWeightScales + kMx4ScaleBytes, w1 + at, kMx4ScaleBytes, full(s));
-                    bulk_g2s(to + S::kWeightCodes, (rank ? w1 : w0) + at + kMx4ScaleBytes, S::kCodes, full(s));
+                    if (i >= S::kStages && !bar_wait<true>(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) { ok = false; break; }
+                    const uint32_t to = ring + s * S::kStageBytes, bar = peer_address(full(s), 0);
+                    const int at = k * kMx4TileMapRows;
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * S::kStageBytes);
+                    tiled_g2s_pair(to, &maps.x, x + at, bar);
+                    tiled_g2s_pair(to + S::kWeightScales, &maps.w_scales, w0 + at, bar);
+                    tiled_g2s_pair(to + S::kWeightScales + kMx4ScaleBytes, scales1, w1 + at, bar);
+                    tiled_g2s_pair(to + S::kWeightCodes, codes, (rank ? w1 : w0) + at + 1, bar);
                 }
             }
+            // Copies that nobody multiplied come all the same, before this CTA is gone.  (The second CTA's count at the other's barrier: its own is never
+            // arrived at, and the wait there lasts for the limit of polls, a thousand times what a copy takes.)
             for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
                 const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
-                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
+                if (!bar_wait<true>(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), rank ? 0u : parity, kMx4SpinLimit);
             }
         }
     } else if (warp == 1) {
         if (rank == 1) {
-            const int64_t units = (tiles - pair + pairs - 1) / pairs * chunks;
-            if (lane == 0) {
-                for (int64_t i = 0; i < units; ++i) {
-                    if (!bar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
-                    arrive_at_first(full(i % S::kStages));
-                }
-                bar_wait(drained, 0, &failed);
-            }
+            warp_wait<true>(drained, 0, &failed);
         } else {
             const uint32_t lead = elect_one();
             int s = 0;
             uint32_t parity = 0, round = 0;
             bool ok = true;
             for (int64_t tile = pair; tile < tiles && ok; tile += pairs, ++round) {
-                if (round && !warp_wait(acc_empty, (round - 1) & 1u, &failed)) break;
+                if (round && !warp_wait<true>(acc_empty, (round - 1) & 1u, &failed)) break;
                 for (int k = 0; k < chunks; ++k) {
-                    if (!warp_wait(full(s), parity, &failed)) { ok = false; break; }
+                    if (!warp_wait<true>(full(s), parity, &failed)) { ok = false; break; }
                     tensor_fence_after();
                     const uint32_t stage = ring + s * S::kStageBytes;
                     const uint32_t sfx = tmem + S::kScaleBase + s * S::kScaleColumns, sfw = sfx + 8;
@@ -551,7 +557,7 @@ mx4_wide_kernel(const ProductArgs p) {
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         uint32_t round = 0;
         for (int64_t tile = pair; tile < tiles; tile += pairs, ++round) {
-            if (!warp_wait(acc_full, round & 1u, &failed)) break;
+            if (!warp_wait<true>(acc_full, round & 1u, &failed)) break;
             __syncwarp();
             tensor_fence_after();
             const WideTile t = wide_tile(tile, p.token_tiles);
@@ -621,8 +627,7 @@ mx4_wide_kernel(const ProductArgs p) {
     __syncwarp();
     tensor_fence_before();
     __syncthreads();
-    cluster_arrive();      // what the pair's instructions read and write is there until both are done
-    cluster_wait();
+    cluster_sync();      // what the pair's instructions read and write, and the barriers that one arrives at in the other, are there until both are done
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
     if (warp == 1) tmem_free<2>(tmem_slot, S::kColumns);
@@ -630,8 +635,9 @@ mx4_wide_kernel(const ProductArgs p) {
 
 // Every launch may begin while the kernel before it in its stream ends: what it reads of it, and all it writes, comes after griddep_wait.
 // What is set once per kernel and device is remembered in `ready`, a bit a device.
-static int launch_product(void (*kernel)(ProductArgs), std::atomic<uint64_t>& ready, const Device& d, int smem, int threads, int ctas, int cluster,
-                          cudaStream_t st, const ProductArgs& p) {
+template <typename... Args>
+static int launch_product(void (*kernel)(Args...), std::atomic<uint64_t>& ready, const Device& d, int smem, int threads, int ctas, int cluster,
+                          cudaStream_t st, const Args&... args) {
     if (!(ready.load(std::memory_order_relaxed) >> d.ordinal & 1)) {
         MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
@@ -650,7 +656,7 @@ static int launch_product(void (*kernel)(ProductArgs), std::atomic<uint64_t>& re
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = cluster > 1 ? 2 : 1;
-    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, p));
+    MPS_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, args...));
     return MPS_OK;
 }
 
@@ -684,13 +690,45 @@ static bool stream_pays(const ProductArgs& p, int sms) {
     return 4.2 + (double)waves * 0.54 * ((p.chunks + parts - 1) / parts) + 2.5 * (double)(waves - 1) < 5.5 + (double)rounds * 0.39 * p.chunks;
 }
 
+// Tiles as rows of 1 KB, `box` of them a copy.
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+static int tile_map(CUtensorMap& map, EncodeTiled encode, const void* tiles, int64_t row_tiles, int chunks, int box) {
+    const cuuint64_t size[2] = {kMx4MapRow / 4, (cuuint64_t)(row_tiles * chunks * kMx4TileMapRows)}, stride[1] = {kMx4MapRow};
+    const cuuint32_t boxes[2] = {kMx4MapRow / 4, (cuuint32_t)box}, steps[2] = {1, 1};
+    if (size[1] > 0x7FFFFFFFu) { set_error("mps_mx4_product: matrix too large"); return MPS_ERR_INVALID; }
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(tiles), size, stride, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
+}
+static int wide_maps(WideMaps& m, const ProductArgs& p) {
+    static std::atomic<EncodeTiled> known{nullptr};
+    EncodeTiled encode = known.load(std::memory_order_relaxed);
+    if (!encode) {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        MPS_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !entry) { set_error("the driver has no cuTensorMapEncodeTiled"); return MPS_ERR_UNSUPPORTED; }
+        encode = reinterpret_cast<EncodeTiled>(entry);
+        known.store(encode, std::memory_order_relaxed);
+    }
+    int rc = tile_map(m.x, encode, p.x, mx4_row_tiles(p.tokens), p.chunks, kMx4TileMapRows);
+    if (!rc) rc = tile_map(m.w_scales, encode, p.w, p.row_tiles, p.chunks, 1);
+    if (!rc) rc = tile_map(m.w_codes, encode, p.w, p.row_tiles, p.chunks, kMx4TileMapRows - 1);
+    if (!rc && p.w_up) rc = tile_map(m.up_scales, encode, p.w_up, p.row_tiles, p.chunks, 1);
+    if (!rc && p.w_up) rc = tile_map(m.up_codes, encode, p.w_up, p.row_tiles, p.chunks, kMx4TileMapRows - 1);
+    return rc;
+}
+
 template <bool GATED>
 static int launch_wide(ProductArgs p, const Device& d, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
+    WideMaps maps = {};
+    const int rc = wide_maps(maps, p);
+    if (rc) return rc;
     p.token_tiles = (int)((p.tokens + 255) / 256);
     const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
     const int pairs = (int)(tiles < d.sms / 2 ? tiles : d.sms / 2);
-    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p);
+    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p, maps);
 }
 
 }  // namespace mps

@@ -1,6 +1,7 @@
 // The tensor-core side of the MXFP4 products: descriptors, scale copies, block-scaled multiplications and accumulator reads.
 #pragma once
 
+#include <cuda.h>
 #include <stdint.h>
 
 namespace mps {
@@ -87,11 +88,19 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// Arrival at the first CTA's barrier of this place, from either.
+// Arrival at the first CTA's barrier of this place, from either: what this thread did or has seen done before (copies that have come, the accumulator
+// read) is done for the thread of the other CTA that waits there.  Without a scope it would be so for this CTA's threads alone.
 __device__ __forceinline__ void arrive_at_first(uint32_t bar) {
     asm volatile(
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
-        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar) : "memory");
+}
+// A poll of a barrier that is arrived at, or whose bytes are sent, from another CTA.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 // Another CTA's shared memory, at the place that has this address in one's own.
 __device__ __forceinline__ uint32_t peer_address(uint32_t smem, int rank) {
@@ -105,11 +114,19 @@ __device__ __forceinline__ float4 load_peer(uint32_t address) {
     return v;
 }
 __device__ __forceinline__ void add4(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+// A box of a tensor map, from its first column and `row` on, into this CTA's shared memory; the bytes count at a barrier of either CTA of the pair, which
+// gets them as a release at cluster scope (an untiled bulk copy counts at its own CTA's barriers only).
+__device__ __forceinline__ void tiled_g2s_pair(uint32_t dst, const CUtensorMap* map, int row, uint32_t pair_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(pair_bar) : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // One value into another CTA's shared memory; the barrier there counts its four bytes once they are there.
 __device__ __forceinline__ void send_to(uint32_t address, uint32_t bar, float v) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(address), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
-// The cluster's barrier in two halves.  An arrival orders nothing; who has waited knows that all have arrived.
+// The cluster's barrier in two halves.  An arrival orders nothing; who has waited knows that all have arrived.  Who leaves after it, or reads what was
+// written before it, needs cluster_sync: behind an arrival that orders nothing, a read of another CTA's memory or an arrival there may still be on its way.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
