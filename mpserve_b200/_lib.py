@@ -32,10 +32,11 @@ class BucketTensor(C.Structure):
     ]
 
 
-# struct mps_mx4_norm and struct mps_mx4_linear, packed in the order of their fields: their calls take a few microseconds, of which filling a
+# struct mps_mx4_norm, mps_mx4_linear and mps_mx4_mlp, packed in the order of their fields: their calls take a few microseconds, of which filling a
 # C.Structure would be one.
 MX4_NORM = struct.Struct("@7P7q6i2f")
 MX4_LINEAR = struct.Struct("@5P5q4i")
+MX4_MLP = struct.Struct("@7P3q5i2f4x")
 
 
 class Mx4Mlp(C.Structure):

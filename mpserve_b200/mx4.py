@@ -256,24 +256,27 @@ def product_timed_out(device: torch.device | None = None) -> bool:
 
 # ---- norms, gate and residual ------------------------------------------------------------------------------
 
-def _gain(t, name: str, cols: int, index: int) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.numel() != cols:
+def _gain(t, name: str, cols: int, index: int) -> tuple[int, int]:
+    """(pointer, dtype) of a norm's weight."""
+    dtype = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if dtype is None or t.dim() != 1 or t.numel() != cols:
         raise ValueError(f"{name} must be a bfloat16, float16 or float32 vector of {cols} values")
     if t.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    return t.data_ptr(), dtype
 
 
 def _gains(post_weight, next_weight, cols: int, index: int):
     """(pointers or 0, the dtype that the two share)."""
     post = nxt = dtype = 0
     if post_weight is not None:
-        post, dtype = _gain(post_weight, "post_weight", cols, index), _DTYPES[post_weight.dtype]
+        post, dtype = _gain(post_weight, "post_weight", cols, index)
     if next_weight is not None:
-        nxt, dtype = _gain(next_weight, "next_weight", cols, index), _DTYPES[next_weight.dtype]
-        if post_weight is not None and post_weight.dtype != next_weight.dtype:
+        post_dtype = dtype
+        nxt, dtype = _gain(next_weight, "next_weight", cols, index)
+        if post_weight is not None and post_dtype != dtype:
             raise ValueError("post_weight and next_weight must have the same dtype")
     return post, nxt, dtype
 
@@ -301,10 +304,10 @@ def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype:
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
     index = h.get_device()
-    w = _gain(weight, "weight", cols, index)
+    w, w_dtype = _gain(weight, "weight", cols, index)
     n, n_ptr, n_dtype = _normed(h, rows, cols, dtype, quantized)
     args = _lib.MX4_NORM.pack(0, h.data_ptr(), 0, 0, w, 0, n_ptr, rows, cols, 0, stride, 0, cols, 0, 0, 0, _DTYPES[h.dtype], n_dtype, 0,
-                              _DTYPES[weight.dtype], eps, 1.0)
+                              w_dtype, eps, 1.0)
     _launch(index, "mps_mx4_norm_rows", args)
     return n
 
@@ -371,45 +374,58 @@ class GatedMlp:
     """A gated MLP block in 4 bits: ``rms_norm`` -> ``gated_linear`` -> ``linear`` -> ``block_join``.
 
     ``gate_proj`` and ``up_proj`` ``[inter, hidden]``, ``down_proj`` ``[hidden, inter]`` are ``Mx4Tensor``; ``post_weight``, ``gate``,
-    ``residual_scale`` and ``next_weight`` are as for ``block_join``.  ``forward(h)`` returns ``(h', n)``."""
+    ``residual_scale`` and ``next_weight`` are as for ``block_join``.  ``forward(h)`` returns ``(h', n)``.  All of them are attributes that may be
+    replaced, and a tensor's storage with them: a call takes them as they are then, and refuses what does not fit."""
 
     def __init__(self, gate_proj: Mx4Tensor, up_proj: Mx4Tensor, down_proj: Mx4Tensor, *, pre_weight: torch.Tensor,
                  post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
                  next_weight: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "silu"):
-        for q, name in ((gate_proj, "gate_proj"), (up_proj, "up_proj"), (down_proj, "down_proj")):
-            _check_mx4(q, name)
-            if q.device != gate_proj.device:
-                raise ValueError("all tensors must be on the same CUDA device")
-        inter, hidden = gate_proj.rows, gate_proj.cols
-        if inter == 0 or (up_proj.rows, up_proj.cols) != (inter, hidden) or (down_proj.rows, down_proj.cols) != (hidden, inter):
-            raise ValueError("gate_proj and up_proj must be [inter, hidden], down_proj [hidden, inter]")
-        if activation not in _ACTIVATIONS:
-            raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
-        _check_norm_cols(hidden)
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self.pre_weight, self.post_weight, self.gate, self.next_weight = pre_weight, post_weight, gate, next_weight
-        self.hidden, self.inter = hidden, inter
-        index = self._index = gate_proj.data.get_device()
-        b = self._block = _lib.Mx4Mlp()
-        b.gate_proj, b.up_proj, b.down_proj = (q.data.data_ptr() for q in (gate_proj, up_proj, down_proj))
-        b.pre_weight, b.pre_dtype = _gain(pre_weight, "pre_weight", hidden, index), _DTYPES[pre_weight.dtype]
-        b.post_weight, b.next_weight, b.weight_dtype = _gains(post_weight, next_weight, hidden, index)
-        b.hidden, b.inter, b.activation, b.eps, b.residual_scale = hidden, inter, _ACTIVATIONS[activation], eps, residual_scale
-        self._gate_per_call = gate is not None and (not isinstance(gate, torch.Tensor) or gate.dim() != 1 or gate.numel() != hidden)
-        if gate is not None and not self._gate_per_call:
-            b.gate, b.gate_dtype, b.gate_row_stride, b.gate_col_stride = _gate(gate, pre_weight, 1, hidden)
+        self.residual_scale, self.eps, self.activation = residual_scale, eps, activation
+        _, hidden, _, _, _ = self._operands()
+        if gate is not None and isinstance(gate, torch.Tensor) and gate.dim() == 1 and gate.numel() == hidden:
+            _gate(gate, pre_weight, 1, hidden)      # a value per row or per element has to fit the tokens, which come with a call
+
+    @property
+    def hidden(self) -> int:
+        return self.gate_proj.cols
+
+    @property
+    def inter(self) -> int:
+        return self.gate_proj.rows
+
+    def _operands(self):
+        """What the attributes hold now: (device index, hidden, inter, pointers, (dtype of pre_weight, of the other two, activation))."""
+        g, u, d = self.gate_proj, self.up_proj, self.down_proj
+        for q, name in ((g, "gate_proj"), (u, "up_proj"), (d, "down_proj")):
+            _check_mx4(q, name)
+        index = g.data.get_device()
+        if u.data.get_device() != index or d.data.get_device() != index:
+            raise ValueError("all tensors must be on the same CUDA device")
+        inter, hidden = g.rows, g.cols
+        if inter == 0 or u.rows != inter or u.cols != hidden or d.rows != hidden or d.cols != inter:
+            raise ValueError("gate_proj and up_proj must be [inter, hidden], down_proj [hidden, inter]")
+        if self.activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
+        _check_norm_cols(hidden)
+        pre, pre_dtype = _gain(self.pre_weight, "pre_weight", hidden, index)
+        post, nxt, dtype = _gains(self.post_weight, self.next_weight, hidden, index)
+        return index, hidden, inter, (g.data.data_ptr(), u.data.data_ptr(), d.data.data_ptr(), pre, post, nxt), (
+            pre_dtype, dtype, _ACTIVATIONS[self.activation])
 
     def forward(self, h: torch.Tensor, *, inplace: bool = False):
+        index, hidden, inter, (g, u, d, pre, post, nxt), (pre_dtype, dtype, activation) = self._operands()
         rows, cols, stride = _matrix(h, "h")
-        if cols != self.hidden:
-            raise ValueError(f"h has {cols} columns, the block {self.hidden}")
-        index = self._index
+        if cols != hidden:
+            raise ValueError(f"h has {cols} columns, the block {hidden}")
         if h.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
-        block = self._block
-        if self._gate_per_call:      # a value per row or per element: it has to fit this h
-            block = _lib.Mx4Mlp.from_buffer_copy(block)
-            block.gate, block.gate_dtype, block.gate_row_stride, block.gate_col_stride = _gate(self.gate, h, rows, cols)
+        gate = gate_dtype = gate_row = gate_col = 0
+        if self.gate is not None:
+            gate, gate_dtype, gate_row, gate_col = _gate(self.gate, h, rows, cols)
+        block = _lib.MX4_MLP.pack(g, u, d, pre, post, gate, nxt, hidden, inter, gate_row, gate_col, gate_dtype, pre_dtype, dtype, activation, self.eps,
+                                  self.residual_scale)
         h_dtype = _DTYPES[h.dtype]
         if inplace:
             joined, out_stride = h, stride
@@ -418,11 +434,11 @@ class GatedMlp:
         else:
             joined, out_stride = h.new_empty(*h.shape), cols
         n = None
-        if block.next_weight:
+        if nxt:
             n = h.new_empty(*h.shape, dtype=torch.bfloat16) if h_dtype == 2 else h.new_empty(*h.shape)
-        scratch_bytes = _tile_bytes(rows, cols) + _tile_bytes(rows, self.inter) + rows * cols * 2
-        scratch = self.gate_proj.data.new_empty(scratch_bytes)      # of this call: freed on return, and not handed to another stream before it is done
-        args = (C.byref(block), h.data_ptr(), h_dtype, stride, rows, joined.data_ptr(), out_stride, None if n is None else n.data_ptr(),
+        scratch_bytes = _tile_bytes(rows, cols) + _tile_bytes(rows, inter) + rows * cols * 2
+        scratch = h.new_empty(scratch_bytes, dtype=torch.uint8)      # of this call: freed on return, and not handed to another stream before it is done
+        args = (_lib.Mx4Mlp.from_buffer_copy(block), h.data_ptr(), h_dtype, stride, rows, joined.data_ptr(), out_stride, None if n is None else n.data_ptr(),
                 0 if h_dtype == 2 else h_dtype, scratch.data_ptr(), scratch_bytes)
         if _current_device() == index:
             self._run(args, index)
