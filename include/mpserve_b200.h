@@ -374,7 +374,8 @@ typedef struct mps_mx4_norm {
 MPS_API int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream);
 
 /* out[t, r] = sum_k x[t, k] w[r, k], or with w_up act(sum_k x w) * (sum_k x w_up): tokens x rows, summed in FP32.  x: MXFP4 tiles
- * (x_dtype MPS_MX4), or a matrix that the call quantises into x_tiles (mps_mx4_bytes(tokens, cols) bytes) first.
+ * (x_dtype MPS_MX4), or a matrix that the call quantises: more than MPS_MX4_TOKENS_INSIDE tokens into x_tiles, mps_mx4_bytes(tokens, cols) bytes of
+ * the caller's that nobody else uses until the call's kernels are done.
  * out_dtype: MPS_BF16, MPS_F16, or with w_up also MPS_MX4 (tiles of tokens x rows). */
 typedef struct mps_mx4_linear {
     const void* x;
@@ -387,8 +388,8 @@ typedef struct mps_mx4_linear {
     int32_t x_dtype, out_dtype, activation;
     int32_t weights_ready;              /* the kernel before in the stream writes no weight: they may be read before it is done */
 } mps_mx4_linear;
-/* Scratch of the products: zero-filled once, one per stream that may run them concurrently, 256-byte aligned.  x_tiles may be null
- * where mps_mx4_bytes(tokens, cols) fits into it (8 MB). */
+enum { MPS_MX4_TOKENS_INSIDE = 8 };
+/* What the products record a wait in that ran out: zero-filled once, 256-byte aligned; any number of streams and threads may share one. */
 MPS_API int64_t mps_mx4_workspace_bytes(void);
 MPS_API int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
 /* A gated MLP block, everything but the tokens: h_out, n_out = block_join(product(gated(rms_norm(h, pre_weight)))), what passes between in MXFP4
@@ -410,8 +411,8 @@ MPS_API int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_
 MPS_API int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out,
                               int64_t h_out_stride, void* n_out, int32_t n_dtype, void* scratch, int64_t scratch_bytes, void* workspace,
                               int64_t workspace_bytes, void* stream);
-/* Every wait inside the products is bounded: waits for the stream, tells whether any since the last query gave up (its outputs are
- * then incomplete), and clears the record. */
+/* Every wait inside the products is bounded: waits for the stream, tells whether any with this workspace gave up since the last query (its
+ * outputs are then incomplete), and clears the record. */
 MPS_API int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out);
 
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of

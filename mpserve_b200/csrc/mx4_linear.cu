@@ -12,8 +12,7 @@ namespace mps {
 constexpr uint32_t kMx4SpinLimit = 1u << 20;
 constexpr int kMx4SmemMost = 232448;           // 227 KB
 
-// Workspace: word 0 records a wait that ran out; from byte 1024 on, the tokens of a call that quantises them in a kernel of its own.
-constexpr int64_t kMx4ScratchOffset = 1024, kMx4WorkspaceBytes = kMx4ScratchOffset + (int64_t)480 * kMx4TileBytes;
+constexpr int64_t kMx4WorkspaceBytes = 256;    // word 0 records a wait that ran out
 
 struct ProductArgs {
     const uint8_t* x;        // tiles, or (stream kernel with QUANTIZE) the tokens as they came
@@ -93,7 +92,8 @@ struct StreamShape {
 };
 // Tokens that the kernel quantises itself.  us, inside | by a kernel before it: 14336 x 4096, 1 token 7.7 | 8.8, 8: 9.2 | 9.5, 9: 9.9 | 9.6, 16: 12.3 | 9.7
 // (1024 x 4096 3.1 | 4.6, 3.8 | 5.2, 4.2 | 5.2, 5.3 | 5.3); and a launch less for the host.
-constexpr int kMostQuantizedInside = 8;
+constexpr int kMostQuantizedInside = MPS_MX4_TOKENS_INSIDE;
+static_assert(kMostQuantizedInside <= 16, "the kernel that quantises has 16 tokens");
 constexpr int kMostParts = 4;                  // CTAs of a cluster
 
 // One token of a tile's 128 features, four neighbouring ones a lane (`up` too where the pair is gated), into the output.
@@ -758,14 +758,9 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     const bool quantized = a.x_dtype == MPS_MX4, inside = !quantized && a.tokens <= kMostQuantizedInside;
     const void* tiles = a.x;
     if (!quantized && !inside) {
+        // not in the workspace: of two threads on one stream, one's tokens could come between the other's two kernels
         tiles = a.x_tiles;
-        if (!tiles) {
-            if (mps_mx4_bytes(a.tokens, a.cols) > kMx4WorkspaceBytes - kMx4ScratchOffset) {
-                set_error("mps_mx4_product: x_tiles missing");
-                return MPS_ERR_WORKSPACE;
-            }
-            tiles = static_cast<uint8_t*>(workspace) + kMx4ScratchOffset;
-        }
+        if (!tiles) { set_error("mps_mx4_product: x_tiles missing"); return MPS_ERR_WORKSPACE; }
     }
     if (((reinterpret_cast<uintptr_t>(inside ? nullptr : tiles) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.w_up) |
           (a.out_dtype == MPS_MX4 ? reinterpret_cast<uintptr_t>(a.out) : 0)) & 15u) || (reinterpret_cast<uintptr_t>(workspace) & 255u)) {

@@ -5,8 +5,8 @@ MXFP4 (``quantize``), or MXFP4 weights are taken from a checkpoint as they are (
 the residual stream (``rms_norm``), multiplies (``linear``, ``gated_linear``) and joins the block's result to the stream
 (``block_join``).  ``GatedMlp`` is a whole block of these.  What passes between the operators may stay in MXFP4.
 
-Every call is asynchronous on the current CUDA stream of its inputs' device; scratch is kept per device and stream, as the decoder
-keeps its own.  Inference only: nothing here has a gradient.  There is no CPU path: without the built library
+Every call is asynchronous on the current CUDA stream of its inputs' device and may be made from any thread, or captured in a graph; scratch is of the
+call.  Inference only: nothing here has a gradient.  There is no CPU path: without the built library
 or a CUDA device the calls raise.  The reference has no counterpart; it multiplies decoded weights in BF16.
 """
 from __future__ import annotations
@@ -26,20 +26,23 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 _MOST_NORM_COLS = 32768
 
-# Of the products' workspace, what x_tiles may take (include/mpserve_b200.h).
-_SCRATCH = 480 * 17408
+# Tokens up to which a product quantises them itself; more of them need x_tiles (include/mpserve_b200.h).
+_TOKENS_INSIDE = 8
 
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_workspaces: dict[int, torch.Tensor] = {}
 _stream_of = torch._C._cuda_getCurrentRawStream      # the current stream's handle by device index, without an object around it
 _current_device = torch._C._cuda_getDevice
 
 
-def _workspace(index: int, stream: int) -> torch.Tensor:
-    """Scratch of the products, one per (device, stream), as they hand it back."""
-    ws = _workspaces.get((index, stream))
+def _workspace(index: int) -> torch.Tensor:
+    """Where products record a wait that ran out, one per device.  Nothing else outlives a call: what passes between a call's kernels is in memory of
+    that call, so that host threads on one stream, and graphs captured on it, do not share any."""
+    ws = _workspaces.get(index)
     if ws is None:
         ws = torch.zeros(int(_lib.load().mps_mx4_workspace_bytes()), dtype=torch.uint8, device=torch.device("cuda", index))
-        _workspaces[index, stream] = ws
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(index).synchronize()      # other streams use it next
+        ws = _workspaces.setdefault(index, ws)
     return ws
 
 
@@ -128,6 +131,7 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
     block with an infinity or a NaN becomes NaN."""
     rows, cols, stride = _matrix(x, "x")
     data = x.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
+    _workspace(x.get_device())      # there before the first product, which may be captured
     _launch(x.get_device(), "mps_mx4_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr())
     return Mx4Tensor(data, rows, cols, x.shape)
 
@@ -161,6 +165,7 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
         raise ValueError("codes and scales must have the same rows and device")
     rows = codes.shape[0]
     data = codes.new_empty(_tile_bytes(rows, cols))
+    _workspace(codes.get_device())
     _launch(codes.get_device(), "mps_mx4_pack", codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr())
     return Mx4Tensor(data, rows, cols)
 
@@ -168,9 +173,8 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
 # ---- products --------------------------------------------------------------------------------------------
 
 def _run_product(args, index: int) -> None:
-    stream = _stream_of(index)
-    ws = _workspace(index, stream)
-    rc = _lib.load().mps_mx4_product(args, ws.data_ptr(), ws.numel(), stream)
+    ws = _workspace(index)
+    rc = _lib.load().mps_mx4_product(args, ws.data_ptr(), ws.numel(), _stream_of(index))
     if rc:
         _lib.check(rc)
 
@@ -197,8 +201,8 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool):
         data, x_dtype = x, _DTYPES[x.dtype]
         if dtype is None:
             dtype = torch.bfloat16 if x_dtype == 2 else x.dtype
-        if _tile_bytes(rows, cols) > _SCRATCH:
-            tiles = w.data.new_empty(_tile_bytes(rows, cols))
+        if rows > _TOKENS_INSIDE:
+            tiles = w.data.new_empty(_tile_bytes(rows, cols))      # of this call: freed on return, and not handed to another stream before it is done
     if cols != w_cols:
         raise ValueError(f"x has {cols} columns, the weight {w_cols}")
     if data.get_device() != index:
@@ -242,15 +246,15 @@ def gated_linear(x, w_gate: Mx4Tensor, w_up: Mx4Tensor, *, activation: str = "si
 
 
 def product_timed_out(device: torch.device | None = None) -> bool:
-    """Waits for the current stream and tells whether a product launched on it since the last call gave up on one of its bounded
-    waits (its outputs are then incomplete).  Always False in normal operation."""
+    """Waits for the device's current stream and tells whether a product on the device, a replayed graph's included, gave up on one of its bounded waits
+    since the last call (its outputs are then incomplete).  Of other streams' products, those that have ended count.  Always False in
+    normal operation."""
     dev = torch.device("cuda") if device is None else torch.device(device)
     index = torch.cuda.current_device() if dev.index is None else dev.index
     with torch.cuda.device(index):
-        stream = _stream_of(index)
-        ws = _workspace(index, stream)
+        ws = _workspace(index)
         flag = C.c_int32(0)
-        _lib.check(_lib.load().mps_mx4_status(ws.data_ptr(), ws.numel(), stream, C.byref(flag)))
+        _lib.check(_lib.load().mps_mx4_status(ws.data_ptr(), ws.numel(), _stream_of(index), C.byref(flag)))
     return bool(flag.value)
 
 
@@ -451,8 +455,7 @@ class GatedMlp:
 
     @staticmethod
     def _run(args, index: int) -> None:
-        stream = _stream_of(index)
-        ws = _workspace(index, stream)
-        rc = _lib.load().mps_mx4_gated_mlp(*args, ws.data_ptr(), ws.numel(), stream)
+        ws = _workspace(index)
+        rc = _lib.load().mps_mx4_gated_mlp(*args, ws.data_ptr(), ws.numel(), _stream_of(index))
         if rc:
             _lib.check(rc)

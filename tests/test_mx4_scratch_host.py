@@ -1,0 +1,24 @@
+"""No scratch of a product outlives its call: what the C entry takes and refuses, without a launch."""
+import pytest
+
+from mpserve_b200 import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mpserve_b200 import build
+
+    build.build()
+    return _lib.load()
+
+
+def test_the_workspace_holds_a_record_and_no_tokens(lib):
+    assert 4 <= lib.mps_mx4_workspace_bytes() < 17408
+
+
+@pytest.mark.parametrize("tokens", [9, 64, 100000])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_tokens_to_quantise_come_with_a_place_of_their_own(lib, tokens, dtype):
+    args = _lib.MX4_LINEAR.pack(256, 0, 256, 0, 256, tokens, 256, 128, 256, 128, dtype, 0, 0, 0)
+    assert lib.mps_mx4_product(args, 256, 1 << 30, None) == _lib.MPS_ERR_WORKSPACE
+    assert b"x_tiles" in lib.mps_last_error()
