@@ -12,6 +12,7 @@ or a CUDA device the calls raise.  The reference has no counterpart; it multipli
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -91,13 +92,28 @@ def _tile_bytes(rows: int, cols: int) -> int:
 
 class Mx4Tensor:
     """A ``rows`` x ``cols`` matrix in MXFP4: E2M1 codes and one power-of-two scale per 32 columns, in the tiles that the tensor
-    cores read (``data``).  ``shape`` is the shape of the tensor it was made of."""
+    cores read (``data``, a flat uint8 tensor).  ``shape`` is the shape of the tensor it was made of.  None of them can be replaced."""
 
-    __slots__ = ("data", "rows", "cols", "shape")
+    __slots__ = ("_data", "_rows", "_cols", "_shape", "_bytes")
 
     def __init__(self, data: torch.Tensor, rows: int, cols: int, shape=None):
-        self.data, self.rows, self.cols = data, rows, cols
-        self.shape = (rows, cols) if shape is None else shape
+        rows, cols = int(rows), int(cols)
+        shape = (rows, cols) if shape is None else tuple(int(n) for n in shape)
+        if rows < 0 or cols < 1:
+            raise ValueError("an MXFP4 matrix has at least one column and no negative number of rows")
+        if len(shape) == 0 or shape[-1] != cols or min(shape) < 0 or math.prod(shape[:-1]) != rows:
+            raise ValueError(f"shape {shape} is not that of {rows} rows of {cols} columns")
+        need = _tile_bytes(rows, cols)
+        if not isinstance(data, torch.Tensor) or data.dtype != torch.uint8 or data.dim() != 1 or not data.is_contiguous():
+            raise ValueError("data must be a flat, contiguous uint8 tensor")
+        if data.numel() < need:
+            raise ValueError(f"data has {data.numel()} bytes, the tiles of {rows} x {cols} {need}")
+        self._data, self._rows, self._cols, self._shape, self._bytes = data, rows, cols, shape, need
+
+    data = property(lambda self: self._data)
+    rows = property(lambda self: self._rows)
+    cols = property(lambda self: self._cols)
+    shape = property(lambda self: self._shape)
 
     @property
     def device(self) -> torch.device:
@@ -112,6 +128,7 @@ class Mx4Tensor:
     def parts(self) -> tuple[torch.Tensor, torch.Tensor]:
         """As checkpoints store it: codes ``uint8 [rows, ceil(cols / 2)]``, the even column in a byte's low half, and E8M0 scales
         ``uint8 [rows, ceil(cols / 32)]``."""
+        _check_mx4(self, "this matrix")
         dev = self.device
         codes = torch.empty((self.rows, (self.cols + 1) // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty((self.rows, -(-self.cols // BLOCK)), dtype=torch.uint8, device=dev)
@@ -119,9 +136,24 @@ class Mx4Tensor:
         return codes, scales
 
 
-def _check_mx4(q, name: str) -> None:
+def _mx4(data: torch.Tensor, rows: int, cols: int, shape) -> Mx4Tensor:
+    """One whose fields are known to fit: the checks of the public way would be two microseconds of a call's ten."""
+    q = Mx4Tensor.__new__(Mx4Tensor)
+    q._data, q._rows, q._cols, q._shape, q._bytes = data, rows, cols, shape, data.numel()
+    return q
+
+
+def _check_mx4(q, name: str) -> int:
+    """The index of ``q``'s device.  A tensor can be moved or cut off after it was checked; what the kernels read has to be there now."""
     if not isinstance(q, Mx4Tensor):
         raise ValueError(f"{name} must be an Mx4Tensor (see quantize and from_parts)")
+    data = q._data
+    index = data.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if data.numel() < q._bytes:
+        raise ValueError(f"{name} has lost a part of its data")
+    return index
 
 
 def quantize(x: torch.Tensor) -> Mx4Tensor:
@@ -133,16 +165,17 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
     data = x.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
     _workspace(x.get_device())      # there before the first product, which may be captured
     _launch(x.get_device(), "mps_mx4_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, data.data_ptr())
-    return Mx4Tensor(data, rows, cols, x.shape)
+    return _mx4(data, rows, cols, x.shape)
 
 
 def dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that ``q`` stands for.  Exact in BF16 and F32; F16 rounds, and overflows beyond 65504."""
-    _check_mx4(q, "q")
+    index = _check_mx4(q, "q")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
-    out = q.data.new_empty(*q.shape, dtype=dtype)
-    _launch(out.get_device(), "mps_mx4_dequantize", q.data.data_ptr(), q.rows, q.cols, _DTYPES[dtype], out.data_ptr())
+    data = q._data
+    out = data.new_empty(*q._shape, dtype=dtype)
+    _launch(index, "mps_mx4_dequantize", data.data_ptr(), q._rows, q._cols, _DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -167,7 +200,7 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx4Tenso
     data = codes.new_empty(_tile_bytes(rows, cols))
     _workspace(codes.get_device())
     _launch(codes.get_device(), "mps_mx4_pack", codes.data_ptr(), scales.data_ptr(), rows, cols, data.data_ptr())
-    return Mx4Tensor(data, rows, cols)
+    return _mx4(data, rows, cols, (rows, cols))
 
 
 # ---- products --------------------------------------------------------------------------------------------
@@ -180,20 +213,20 @@ def _run_product(args, index: int) -> None:
 
 
 def _product(x, w, w_up, activation: int, dtype, quantized: bool):
-    _check_mx4(w, "w" if w_up is None else "w_gate")
-    out_cols, w_cols, index, up = w.rows, w.cols, w.data.get_device(), 0
+    index = _check_mx4(w, "w" if w_up is None else "w_gate")
+    w_data, out_cols, w_cols, up = w._data, w._rows, w._cols, 0
     if w_up is not None:
-        _check_mx4(w_up, "w_up")
-        if w_up.rows != out_cols or w_up.cols != w_cols:
-            raise ValueError("w_gate and w_up must have the same shape")
-        if w_up.data.get_device() != index:
+        if _check_mx4(w_up, "w_up") != index:
             raise ValueError("all tensors must be on the same CUDA device")
-        up = w_up.data.data_ptr()
+        if w_up._rows != out_cols or w_up._cols != w_cols:
+            raise ValueError("w_gate and w_up must have the same shape")
+        up = w_up._data.data_ptr()
     if out_cols == 0:
         raise ValueError("a weight must have at least one row")
     tiles, stride = None, 0
     if isinstance(x, Mx4Tensor):
-        rows, cols, x_dtype, data = x.rows, x.cols, _MX4, x.data
+        _check_mx4(x, "x")
+        rows, cols, x_dtype, data = x._rows, x._cols, _MX4, x._data
         if dtype is None:
             dtype = torch.bfloat16
     else:
@@ -202,21 +235,21 @@ def _product(x, w, w_up, activation: int, dtype, quantized: bool):
         if dtype is None:
             dtype = torch.bfloat16 if x_dtype == 2 else x.dtype
         if rows > _TOKENS_INSIDE:
-            tiles = w.data.new_empty(_tile_bytes(rows, cols))      # of this call: freed on return, and not handed to another stream before it is done
+            tiles = w_data.new_empty(_tile_bytes(rows, cols))      # of this call: freed on return, and not handed to another stream before it is done
     if cols != w_cols:
         raise ValueError(f"x has {cols} columns, the weight {w_cols}")
     if data.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
     shape = (*x.shape[:-1], out_cols)
     if quantized:
-        out = w.data.new_empty(_tile_bytes(rows, out_cols))
-        out_dtype, result = _MX4, Mx4Tensor(out, rows, out_cols, shape)
+        out = w_data.new_empty(_tile_bytes(rows, out_cols))
+        out_dtype, result = _MX4, _mx4(out, rows, out_cols, shape)
     else:
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError("a product's dtype must be bfloat16 or float16")
         out = result = data.new_empty(*shape) if data.dtype is dtype else data.new_empty(*shape, dtype=dtype)
         out_dtype = _DTYPES[dtype]
-    args = _lib.MX4_LINEAR.pack(data.data_ptr(), 0 if tiles is None else tiles.data_ptr(), w.data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
+    args = _lib.MX4_LINEAR.pack(data.data_ptr(), 0 if tiles is None else tiles.data_ptr(), w_data.data_ptr(), up, out.data_ptr(), rows, cols, out_cols,
                                 stride, out_cols, x_dtype, out_dtype, activation, 0)
     if _current_device() == index:
         _run_product(args, index)
@@ -294,7 +327,7 @@ def _normed(like, rows, cols, dtype, quantized: bool):
     """Where a norm's result goes, in ``like``'s shape: (what the caller gets, pointer, dtype)."""
     if quantized:
         data = like.new_empty(_tile_bytes(rows, cols), dtype=torch.uint8)
-        return Mx4Tensor(data, rows, cols, like.shape), data.data_ptr(), _MX4
+        return _mx4(data, rows, cols, like.shape), data.data_ptr(), _MX4
     n = like.new_empty(*like.shape) if like.dtype is dtype else like.new_empty(*like.shape, dtype=dtype)
     return n, n.data_ptr(), _DTYPES[dtype]
 
@@ -402,20 +435,18 @@ class GatedMlp:
     def _operands(self):
         """What the attributes hold now: (device index, hidden, inter, pointers, (dtype of pre_weight, of the other two, activation))."""
         g, u, d = self.gate_proj, self.up_proj, self.down_proj
-        for q, name in ((g, "gate_proj"), (u, "up_proj"), (d, "down_proj")):
-            _check_mx4(q, name)
-        index = g.data.get_device()
-        if u.data.get_device() != index or d.data.get_device() != index:
+        index = _check_mx4(g, "gate_proj")
+        if _check_mx4(u, "up_proj") != index or _check_mx4(d, "down_proj") != index:
             raise ValueError("all tensors must be on the same CUDA device")
-        inter, hidden = g.rows, g.cols
-        if inter == 0 or u.rows != inter or u.cols != hidden or d.rows != hidden or d.cols != inter:
+        inter, hidden = g._rows, g._cols
+        if inter == 0 or u._rows != inter or u._cols != hidden or d._rows != hidden or d._cols != inter:
             raise ValueError("gate_proj and up_proj must be [inter, hidden], down_proj [hidden, inter]")
         if self.activation not in _ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
         _check_norm_cols(hidden)
         pre, pre_dtype = _gain(self.pre_weight, "pre_weight", hidden, index)
         post, nxt, dtype = _gains(self.post_weight, self.next_weight, hidden, index)
-        return index, hidden, inter, (g.data.data_ptr(), u.data.data_ptr(), d.data.data_ptr(), pre, post, nxt), (
+        return index, hidden, inter, (g._data.data_ptr(), u._data.data_ptr(), d._data.data_ptr(), pre, post, nxt), (
             pre_dtype, dtype, _ACTIVATIONS[self.activation])
 
     def forward(self, h: torch.Tensor, *, inplace: bool = False):
