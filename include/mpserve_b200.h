@@ -376,7 +376,7 @@ MPS_API int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream);
 /* out[t, r] = sum_k x[t, k] w[r, k], or with w_up act(sum_k x w) * (sum_k x w_up): tokens x rows, summed in FP32.  x: MXFP4 tiles
  * (x_dtype MPS_MX4), or a matrix that the call quantises: more than MPS_MX4_TOKENS_INSIDE tokens into x_tiles, mps_mx4_bytes(tokens, cols) bytes of
  * the caller's that nobody else uses until the call's kernels are done.
- * out_dtype: MPS_BF16, MPS_F16, or with w_up also MPS_MX4 (tiles of tokens x rows). */
+ * out_dtype: MPS_BF16, MPS_F16, without w_up also MPS_F32, with it also MPS_MX4 (tiles of tokens x rows). */
 typedef struct mps_mx4_linear {
     const void* x;
     void* x_tiles;
@@ -393,8 +393,8 @@ enum { MPS_MX4_TOKENS_INSIDE = 8 };
 MPS_API int64_t mps_mx4_workspace_bytes(void);
 MPS_API int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
 /* A gated MLP block, everything but the tokens: h_out, n_out = block_join(product(gated(rms_norm(h, pre_weight)))), what passes between in MXFP4
- * but the block's result, which has h's type (BF16 where that is FP32).  Fields as above; scratch: 256-byte aligned, contents
- * irrelevant before and after. */
+ * but the block's result y: rounded to h's type (BF16 where that is FP32; beyond F16's range as it is), or with wide_result not at all.  Fields
+ * as above; scratch: 256-byte aligned, contents irrelevant before and after. */
 typedef struct mps_mx4_mlp {
     const void* gate_proj;              /* MXFP4 tiles of inter x hidden, as up_proj; down_proj of hidden x inter */
     const void* up_proj;
@@ -406,6 +406,7 @@ typedef struct mps_mx4_mlp {
     int64_t hidden, inter, gate_row_stride;
     int32_t gate_col_stride, gate_dtype, pre_dtype, weight_dtype, activation;
     float eps, residual_scale;
+    int32_t wide_result;                /* the block's result is held in FP32 */
 } mps_mx4_mlp;
 MPS_API int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_t inter);
 MPS_API int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out,

@@ -36,7 +36,7 @@ class BucketTensor(C.Structure):
 # C.Structure would be one.
 MX4_NORM = struct.Struct("@7P7q6i2f")
 MX4_LINEAR = struct.Struct("@5P5q4i")
-MX4_MLP = struct.Struct("@7P3q5i2f4x")
+MX4_MLP = struct.Struct("@7P3q5i2fi")
 
 
 class Mx4Mlp(C.Structure):
@@ -46,7 +46,7 @@ class Mx4Mlp(C.Structure):
         ("gate_proj", _p), ("up_proj", _p), ("down_proj", _p), ("pre_weight", _p), ("post_weight", _p), ("gate", _p), ("next_weight", _p),
         ("hidden", _i64), ("inter", _i64), ("gate_row_stride", _i64),
         ("gate_col_stride", _i32), ("gate_dtype", _i32), ("pre_dtype", _i32), ("weight_dtype", _i32), ("activation", _i32),
-        ("eps", C.c_float), ("residual_scale", C.c_float),
+        ("eps", C.c_float), ("residual_scale", C.c_float), ("wide_result", _i32),
     ]
 
 

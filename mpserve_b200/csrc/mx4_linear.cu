@@ -27,7 +27,8 @@ struct ProductArgs {
     int32_t row_tiles, token_tiles, parts;
     int32_t x_dtype, out_dtype, activation;
     bool x_vec;
-    bool even;               // rows of a 16-bit output begin at multiples of 16 bytes
+    bool even;               // rows of an output that is not MXFP4 begin at multiples of 16 bytes
+    bool half_values;        // an FP32 output takes F16's values where F16 has them
     bool early;              // the kernel before writes no weight: weights may be read before it is done
 };
 
@@ -37,6 +38,12 @@ struct ProductArgs {
 __device__ __forceinline__ float act(float g, bool silu) {
     const float t = silu ? g : 1.5957691216057308f * g * fmaf(0.044715f * g, g, 1.f);
     return __fdividef(g, 1.f + __expf(-t));
+}
+
+// What F16 holds of a value, and the value itself where that would be an infinity: F16's precision with FP32's range.
+__device__ __forceinline__ float half_value(float v) {
+    const float h = __half2float(__float2half_rn(v));
+    return isinf(h) ? v : h;
 }
 
 // A wait that gives up when another one has.  CLUSTER: what it waits for comes from another CTA, too.
@@ -126,6 +133,20 @@ __device__ __forceinline__ void finish(const ProductArgs& p, int row_tile, int l
             // the second half of the last tile lies beyond the last feature and is filled up with zeros
             *reinterpret_cast<uint16_t*>(tile + mx4_code_offset(row, block + 4) + (lane & 7) * 2) = 0;
             if (lane == 0) *reinterpret_cast<uint32_t*>(tile + mx4_scale_offset(row, 1)) = 0u;
+        }
+        return;
+    }
+    if (!GATED && p.out_dtype == MPS_F32) {
+        float* out = static_cast<float*>(p.out) + token * p.out_stride + first;
+        if (p.half_values) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = half_value(f[i]);
+        }
+        if (valid >= 4 && p.even) {
+            *reinterpret_cast<float4*>(out) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < valid) out[i] = f[i];
         }
         return;
     }
@@ -446,7 +467,8 @@ __device__ __forceinline__ void store_rows(uint32_t buffer, int lane, const uint
     }
 }
 
-template <bool GATED>
+// OUT32: an FP32 output, of a product that is not gated.  Its rows go out as rows of twice as many 16-bit halves.
+template <bool GATED, bool OUT32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWideThreads, 1)
 mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
     using S = WideShape;
@@ -563,7 +585,7 @@ mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
             const WideTile t = wide_tile(tile, p.token_tiles);
             const int64_t token0 = ((int64_t)2 * t.token + rank) * kMx4Rows + quarter * 32, tokens = p.tokens - token0;   // this warp's
             const uint32_t acc = tmem + ((uint32_t)quarter << 21), buffer = ring + S::kStageRows + (warp - 2) * 2048;
-            uint16_t* rows = static_cast<uint16_t*>(p.out) + token0 * p.out_stride;
+            uint16_t* rows = static_cast<uint16_t*>(p.out) + token0 * p.out_stride * (OUT32 ? 2 : 1);
             const auto release = [&] {
                 tensor_fence_before();
                 __syncwarp();
@@ -605,6 +627,20 @@ mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
                     for (int i = 0; i < 32; ++i) w[i] = pack2(g[2 * i], g[2 * i + 1], p.out_dtype);
 #pragma unroll
                     for (int c = 0; c < 64; c += 32) store_rows(buffer, lane, w + c / 2, rows + first + c, p.out_stride, tokens, valid - c, p.even);
+                }
+            } else if (OUT32) {
+                float v[128];
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) tmem_load32(acc + half * 128 + c, v + c);
+                release();
+                if (p.half_values) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) v[i] = half_value(v[i]);
+                }
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) {
+                    const int first = t.feature * 256 + half * 128 + c;
+                    store_rows(buffer, lane, reinterpret_cast<const uint32_t*>(v + c), rows + 2 * (int64_t)first, 2 * p.out_stride, tokens, 2 * (p.rows - first), p.even);
                 }
             } else {
                 uint32_t w[64];
@@ -719,7 +755,7 @@ static int wide_maps(WideMaps& m, const ProductArgs& p) {
     return rc;
 }
 
-template <bool GATED>
+template <bool GATED, bool OUT32 = false>
 static int launch_wide(ProductArgs p, const Device& d, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     WideMaps maps = {};
@@ -728,26 +764,17 @@ static int launch_wide(ProductArgs p, const Device& d, cudaStream_t st) {
     p.token_tiles = (int)((p.tokens + 255) / 256);
     const int64_t tiles = (int64_t)p.token_tiles * (GATED ? p.row_tiles : (p.row_tiles + 1) / 2);
     const int pairs = (int)(tiles < d.sms / 2 ? tiles : d.sms / 2);
-    return launch_product(mx4_wide_kernel<GATED>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p, maps);
+    return launch_product(mx4_wide_kernel<GATED, OUT32>, ready, d, WideShape::kSmem, kWideThreads, 2 * pairs, 1, st, p, maps);
 }
 
-}  // namespace mps
-
-using namespace mps;
-
-extern "C" {
-
-int64_t mps_mx4_workspace_bytes(void) { return kMx4WorkspaceBytes; }
-
-int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (!args) { set_error("mps_mx4_product: null arguments"); return MPS_ERR_INVALID; }
-    const mps_mx4_linear& a = *args;
+// `half_values`: of an FP32 output (ProductArgs).
+static int product(const mps_mx4_linear& a, bool half_values, void* workspace, int64_t workspace_bytes, void* stream) {
     if (a.tokens < 0 || a.tokens > kMx4MostRows || a.rows <= 0 || a.rows > kMx4MostCols || a.cols <= 0 || a.cols > kMx4MostCols) {
         set_error("mps_mx4_product: tokens must be in [0, %lld], rows and cols in [1, %lld]", (long long)kMx4MostRows, (long long)kMx4MostCols);
         return MPS_ERR_INVALID;
     }
-    if (a.out_dtype != MPS_BF16 && a.out_dtype != MPS_F16 && !(a.out_dtype == MPS_MX4 && a.w_up)) {
-        set_error("mps_mx4_product: the output is BF16 or F16, or MXFP4 where the product is gated");
+    if (a.out_dtype != MPS_BF16 && a.out_dtype != MPS_F16 && a.out_dtype != (a.w_up ? MPS_MX4 : MPS_F32)) {
+        set_error("mps_mx4_product: the output is BF16 or F16, or MXFP4 where the product is gated and FP32 where it is not");
         return MPS_ERR_INVALID;
     }
     if (a.x_dtype != MPS_MX4 && !mx4_dtype_ok(a.x_dtype)) { set_error("mps_mx4_product: unknown dtype %d", (int)a.x_dtype); return MPS_ERR_INVALID; }
@@ -793,6 +820,7 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     p.activation = a.activation;
     p.x_vec = inside && mx4_vec_ok(a.x, a.x_stride, a.x_dtype);
     p.even = a.out_dtype != MPS_MX4 && a.out_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+    p.half_values = half_values;
     p.early = (!quantized && !inside) || a.weights_ready;
     if (a.w_up) {
         if (inside) return launch_stream<16, true, true>(p, d, st);
@@ -806,12 +834,26 @@ int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspa
     if (a.tokens <= 32) return launch_stream<32, false>(p, d, st);
     if (a.tokens <= 64) return launch_stream<64, false>(p, d, st);
     if (stream_pays(p, d.sms)) return launch_stream<128, false>(p, d, st);
-    return launch_wide<false>(p, d, st);
+    return a.out_dtype == MPS_F32 ? launch_wide<false, true>(p, d, st) : launch_wide<false>(p, d, st);
+}
+
+}  // namespace mps
+
+using namespace mps;
+
+extern "C" {
+
+int64_t mps_mx4_workspace_bytes(void) { return kMx4WorkspaceBytes; }
+
+int mps_mx4_product(const mps_mx4_linear* args, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!args) { set_error("mps_mx4_product: null arguments"); return MPS_ERR_INVALID; }
+    return product(*args, false, workspace, workspace_bytes, stream);
 }
 
 int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_t inter) {
-    const int64_t x = mps_mx4_bytes(tokens, hidden), a = mps_mx4_bytes(tokens, inter);
-    return x < 0 || a < 0 ? -1 : x + a + tokens * hidden * 2;      // both are multiples of 256
+    const int64_t x = mps_mx4_bytes(tokens, hidden), a = mps_mx4_bytes(tokens, inter), y = tokens * hidden;
+    if (x < 0 || a < 0) return -1;
+    return a + (x + y * 2 > y * 4 ? x + y * 2 : y * 4);      // x and a are multiples of 256
 }
 
 int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out, int64_t h_out_stride,
@@ -821,10 +863,14 @@ int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, 
     if (need < 0) { set_error("mps_mx4_gated_mlp: sizes out of range"); return MPS_ERR_INVALID; }
     if (tokens == 0) return MPS_OK;
     if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 255u)) { set_error("mps_mx4_gated_mlp: scratch missing, too small or unaligned"); return MPS_ERR_WORKSPACE; }
-    uint8_t* x = static_cast<uint8_t*>(scratch);
-    uint8_t* a = x + mps_mx4_bytes(tokens, block->hidden);
-    uint8_t* y = a + mps_mx4_bytes(tokens, block->inter);
-    const int32_t y_dtype = h_dtype == MPS_F32 ? MPS_BF16 : h_dtype;
+    // The block's result is held in 16 bits, as mps_mx4_product would give it to mps_mx4_norm_rows: 2048 tokens of an 8B layer take 169 us, in FP32
+    // 175 (512 tokens 62.5 and 63.1, fewer the same).  Of a stream in F16 it is F16's value, but in FP32 (180 us): what lies beyond 65504 would be an infinity,
+    // and its row NaN behind the norm, where the stream is in range.
+    const bool half = h_dtype == MPS_F16 && !block->wide_result;
+    const int32_t y_dtype = h_dtype == MPS_F16 || block->wide_result ? MPS_F32 : MPS_BF16;
+    uint8_t* a = static_cast<uint8_t*>(scratch);
+    uint8_t* x = a + mps_mx4_bytes(tokens, block->inter);
+    uint8_t* y = y_dtype == MPS_F32 ? x : x + mps_mx4_bytes(tokens, block->hidden);      // x has been multiplied when y comes
 
     mps_mx4_norm norm = {};
     norm.h = h;
@@ -841,28 +887,29 @@ int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, 
     int rc = mps_mx4_norm_rows(&norm, stream);
     if (rc) return rc;
 
-    mps_mx4_linear product = {};
-    product.x = x;
-    product.w = block->gate_proj;
-    product.w_up = block->up_proj;
-    product.out = a;
-    product.tokens = tokens;
-    product.cols = block->hidden;
-    product.rows = block->inter;
-    product.x_dtype = product.out_dtype = MPS_MX4;
-    product.activation = block->activation;
-    product.weights_ready = 1;          // the kernel before each of the two is this block's own
-    rc = mps_mx4_product(&product, workspace, workspace_bytes, stream);
+    mps_mx4_linear gated = {};
+    gated.x = x;
+    gated.w = block->gate_proj;
+    gated.w_up = block->up_proj;
+    gated.out = a;
+    gated.tokens = tokens;
+    gated.cols = block->hidden;
+    gated.rows = block->inter;
+    gated.x_dtype = gated.out_dtype = MPS_MX4;
+    gated.activation = block->activation;
+    gated.weights_ready = 1;          // the kernel before each of the two is this block's own
+    rc = product(gated, false, workspace, workspace_bytes, stream);
     if (rc) return rc;
 
-    product.x = a;
-    product.w = block->down_proj;
-    product.w_up = nullptr;
-    product.out = y;
-    product.cols = block->inter;
-    product.rows = product.out_stride = block->hidden;
-    product.out_dtype = y_dtype;
-    rc = mps_mx4_product(&product, workspace, workspace_bytes, stream);
+    mps_mx4_linear down = gated;
+    down.x = a;
+    down.w = block->down_proj;
+    down.w_up = nullptr;
+    down.out = y;
+    down.cols = block->inter;
+    down.rows = down.out_stride = block->hidden;
+    down.out_dtype = y_dtype;
+    rc = product(down, half, workspace, workspace_bytes, stream);
     if (rc) return rc;
 
     norm.y = y;

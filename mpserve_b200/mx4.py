@@ -411,15 +411,19 @@ class GatedMlp:
     """A gated MLP block in 4 bits: ``rms_norm`` -> ``gated_linear`` -> ``linear`` -> ``block_join``.
 
     ``gate_proj`` and ``up_proj`` ``[inter, hidden]``, ``down_proj`` ``[hidden, inter]`` are ``Mx4Tensor``; ``post_weight``, ``gate``,
-    ``residual_scale`` and ``next_weight`` are as for ``block_join``.  ``forward(h)`` returns ``(h', n)``.  All of them are attributes that may be
+    ``residual_scale`` and ``next_weight`` are as for ``block_join``.  ``forward(h)`` returns ``(h', n)``.
+
+    Between ``linear`` and ``block_join`` the block's result is rounded to ``h``'s type (BF16 beside an FP32 stream; beyond F16's range it stays what it
+    is), and ``n`` has that type too.  With ``result_dtype=torch.float32`` it is not rounded, and ``n`` has ``h``'s type.  All of these are attributes that may be
     replaced, and a tensor's storage with them: a call takes them as they are then, and refuses what does not fit."""
 
     def __init__(self, gate_proj: Mx4Tensor, up_proj: Mx4Tensor, down_proj: Mx4Tensor, *, pre_weight: torch.Tensor,
                  post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, residual_scale: float = 1.0,
-                 next_weight: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "silu"):
+                 next_weight: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "silu",
+                 result_dtype: torch.dtype | None = None):
         self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
         self.pre_weight, self.post_weight, self.gate, self.next_weight = pre_weight, post_weight, gate, next_weight
-        self.residual_scale, self.eps, self.activation = residual_scale, eps, activation
+        self.residual_scale, self.eps, self.activation, self.result_dtype = residual_scale, eps, activation, result_dtype
         _, hidden, _, _, _ = self._operands()
         if gate is not None and isinstance(gate, torch.Tensor) and gate.dim() == 1 and gate.numel() == hidden:
             _gate(gate, pre_weight, 1, hidden)      # a value per row or per element has to fit the tokens, which come with a call
@@ -443,6 +447,8 @@ class GatedMlp:
             raise ValueError("gate_proj and up_proj must be [inter, hidden], down_proj [hidden, inter]")
         if self.activation not in _ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
+        if self.result_dtype is not None and self.result_dtype is not torch.float32:
+            raise ValueError("result_dtype must be None or float32")
         _check_norm_cols(hidden)
         pre, pre_dtype = _gain(self.pre_weight, "pre_weight", hidden, index)
         post, nxt, dtype = _gains(self.post_weight, self.next_weight, hidden, index)
@@ -460,8 +466,9 @@ class GatedMlp:
         if self.gate is not None:
             gate, gate_dtype, gate_row, gate_col = _gate(self.gate, h, rows, cols)
         block = _lib.MX4_MLP.pack(g, u, d, pre, post, gate, nxt, hidden, inter, gate_row, gate_col, gate_dtype, pre_dtype, dtype, activation, self.eps,
-                                  self.residual_scale)
+                                  self.residual_scale, self.result_dtype is not None)
         h_dtype = _DTYPES[h.dtype]
+        n_dtype = 0 if h_dtype == 2 and self.result_dtype is None else h_dtype
         if inplace:
             joined, out_stride = h, stride
             if rows > 1 and stride < cols:
@@ -470,11 +477,11 @@ class GatedMlp:
             joined, out_stride = h.new_empty(*h.shape), cols
         n = None
         if nxt:
-            n = h.new_empty(*h.shape, dtype=torch.bfloat16) if h_dtype == 2 else h.new_empty(*h.shape)
-        scratch_bytes = _tile_bytes(rows, cols) + _tile_bytes(rows, inter) + rows * cols * 2
+            n = h.new_empty(*h.shape) if n_dtype == h_dtype else h.new_empty(*h.shape, dtype=torch.bfloat16)
+        scratch_bytes = _tile_bytes(rows, inter) + max(_tile_bytes(rows, cols) + rows * cols * 2, rows * cols * 4)
         scratch = h.new_empty(scratch_bytes, dtype=torch.uint8)      # of this call: freed on return, and not handed to another stream before it is done
         args = (_lib.Mx4Mlp.from_buffer_copy(block), h.data_ptr(), h_dtype, stride, rows, joined.data_ptr(), out_stride, None if n is None else n.data_ptr(),
-                0 if h_dtype == 2 else h_dtype, scratch.data_ptr(), scratch_bytes)
+                n_dtype, scratch.data_ptr(), scratch_bytes)
         if _current_device() == index:
             self._run(args, index)
         else:
