@@ -289,7 +289,8 @@ inline bool mx4_vec_ok(const void* p, int64_t row_stride, int dtype) {
 }
 // Row and column counts that every entry point accepts: tile counts and launch grids stay within 31 bits.
 constexpr int64_t kMx4MostRows = int64_t(1) << 31, kMx4MostCols = int64_t(1) << 24;
-
+// And the norms: a CTA a row, 512 threads x 8 steps x 8 columns.
+constexpr int64_t kMx4MostNormRows = 0x7FFFFFFF, kMx4MostNormCols = 32768;
 
 struct Device { int ordinal, sms; };
 int current_device(Device& d);

@@ -858,11 +858,23 @@ int64_t mps_mx4_mlp_scratch_bytes(int64_t tokens, int64_t hidden, int64_t inter)
 
 int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h_dtype, int64_t h_stride, int64_t tokens, void* h_out, int64_t h_out_stride,
                       void* n_out, int32_t n_dtype, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* stream) {
-    if (!block || !block->gate_proj || !block->up_proj || !block->down_proj || !block->pre_weight) { set_error("mps_mx4_gated_mlp: null argument"); return MPS_ERR_INVALID; }
+    // whatever would be refused on the way is refused here, before the first kernel
+    const auto refuse = [](const char* why) { set_error("mps_mx4_gated_mlp: %s", why); return MPS_ERR_INVALID; };
+    if (!block || !block->gate_proj || !block->up_proj || !block->down_proj || !block->pre_weight) return refuse("null argument");
+    if (block->hidden > kMx4MostNormCols) return refuse("hidden out of a norm's range");
+    if (!mx4_dtype_ok(h_dtype) || !mx4_dtype_ok(block->pre_dtype) || (block->gate && !mx4_dtype_ok(block->gate_dtype)) ||
+        ((block->post_weight || block->next_weight) && !mx4_dtype_ok(block->weight_dtype)) || (block->next_weight && n_dtype != MPS_MX4 && !mx4_dtype_ok(n_dtype)))
+        return refuse("unknown dtype");
+    if (block->activation != MPS_SILU && block->activation != MPS_GELU_TANH) return refuse("unknown activation");
+    if ((reinterpret_cast<uintptr_t>(block->gate_proj) | reinterpret_cast<uintptr_t>(block->up_proj) | reinterpret_cast<uintptr_t>(block->down_proj) |
+         (n_dtype == MPS_MX4 ? reinterpret_cast<uintptr_t>(n_out) : 0)) & 15u) return refuse("tiles must be 16-byte aligned");
     const int64_t need = mps_mx4_mlp_scratch_bytes(tokens, block->hidden, block->inter);
     if (need < 0) { set_error("mps_mx4_gated_mlp: sizes out of range"); return MPS_ERR_INVALID; }
     if (tokens == 0) return MPS_OK;
+    if (!h || !h_out || (block->next_weight && !n_out)) return refuse("null pointer");
+    if (tokens > kMx4MostNormRows) return refuse("more tokens than a norm has rows");
     if (!scratch || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 255u)) { set_error("mps_mx4_gated_mlp: scratch missing, too small or unaligned"); return MPS_ERR_WORKSPACE; }
+    if (!workspace || workspace_bytes < kMx4WorkspaceBytes || (reinterpret_cast<uintptr_t>(workspace) & 255u)) { set_error("mps_mx4_gated_mlp: workspace missing, too small or unaligned"); return MPS_ERR_WORKSPACE; }
     // The block's result is held in 16 bits, as mps_mx4_product would give it to mps_mx4_norm_rows: 2048 tokens of an 8B layer take 169 us, in FP32
     // 175 (512 tokens 62.5 and 63.1, fewer the same).  Of a stream in F16 it is F16's value, but in FP32 (180 us): what lies beyond 65504 would be an infinity,
     // and its row NaN behind the norm, where the stream is in range.

@@ -15,7 +15,6 @@ namespace mps {
 
 constexpr int kNormThreads = 256, kNormMostThreads = 512;
 constexpr int64_t kNormManyRows = 512;
-constexpr int kNormMostCols = 32768;    // 512 threads x 8 steps x 8 columns
 
 struct NormArgs {
     mps_mx4_norm a;
@@ -252,8 +251,8 @@ extern "C" int mps_mx4_norm_rows(const mps_mx4_norm* args, void* stream) {
     NormArgs p;
     p.a = *args;
     const mps_mx4_norm& a = p.a;
-    if (a.rows < 0 || a.rows > 0x7FFFFFFFLL || a.cols <= 0 || a.cols > kNormMostCols) {
-        set_error("mps_mx4_norm_rows: rows must be below 2^31, cols in [1, %d]", kNormMostCols);
+    if (a.rows < 0 || a.rows > kMx4MostNormRows || a.cols <= 0 || a.cols > kMx4MostNormCols) {
+        set_error("mps_mx4_norm_rows: rows must be below 2^31, cols in [1, %d]", (int)kMx4MostNormCols);
         return MPS_ERR_INVALID;
     }
     if (!mx4_dtype_ok(a.h_dtype) || (a.y && !mx4_dtype_ok(a.y_dtype)) || (a.gate && !mx4_dtype_ok(a.gate_dtype)) ||
