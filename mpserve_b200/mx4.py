@@ -349,6 +349,32 @@ def rms_norm(h: torch.Tensor, weight: torch.Tensor, *, eps: float = 1e-5, dtype:
     return n
 
 
+def _check_inplace(h, rows: int, cols: int, stride: int, others) -> None:
+    """Refuses an ``h`` that cannot be written row by row while ``others`` (name, tensor, rows, columns, row stride) are read: a CTA reads a row of each
+    and writes that row, in no order.  One that is ``h`` itself, element by element, is read where it is written and does no harm."""
+    if rows > 1 and stride < cols:
+        raise ValueError("h has rows that share memory and cannot be updated in place")
+    if rows == 0:
+        return
+    start, size = h.data_ptr(), h.element_size()
+    pitch, width = stride * size, cols * size
+    end = start + (rows - 1) * pitch + width
+    for name, t, t_rows, t_cols, t_stride in others:
+        if t is None:
+            continue
+        t_start, t_size = t.data_ptr(), t.element_size()
+        t_pitch, t_width = t_stride * t_size, t_cols * t_size
+        if t_start >= end or t_start + (t_rows - 1) * t_pitch + t_width <= start:
+            continue
+        if t_start == start and t_width == width and t_size == size and t_rows == rows and (rows == 1 or t_pitch == pitch):
+            continue
+        # columns of one wider matrix: rows of the same pitch that lie beside one another
+        beside = (t_start - start) % pitch
+        if t_rows > 1 and t_pitch == pitch and beside >= width and beside + t_width <= pitch:
+            continue
+        raise ValueError(f"{name} shares memory with h, which cannot be updated in place")
+
+
 def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                residual_scale: float = 1.0, next_weight: torch.Tensor | None = None, eps: float = 1e-5,
                quantized: bool = False, inplace: bool = False):
@@ -374,9 +400,9 @@ def block_join(y: torch.Tensor, h: torch.Tensor, *, post_weight: torch.Tensor | 
     if gate is not None:
         g, g_dtype, g_row, g_col = _gate(gate, y, rows, cols)
     if inplace:
+        _check_inplace(h, rows, cols, h_stride, (("y", y, rows, cols, y_stride), ("gate", gate, *_gate_extent(gate, g_row, rows, cols)),
+                                                 ("post_weight", post_weight, 1, cols, cols), ("next_weight", next_weight, 1, cols, cols)))
         joined, out_stride = h, h_stride
-        if rows > 1 and h_stride < cols:
-            raise ValueError("h has rows that share memory and cannot be updated in place")
     else:
         joined, out_stride = h.new_empty(*shape), cols
     if nxt:
@@ -405,6 +431,13 @@ def _gate(gate, y, rows: int, cols: int):
             if shape[:-1] == tuple(y.shape[:-1]):
                 return gate.data_ptr(), _DTYPES[gate.dtype], last, per_column
     raise ValueError("gate must be contiguous and have one value per column, per row or per element of y")
+
+
+def _gate_extent(gate, row_stride: int, rows: int, cols: int) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of what ``_gate`` has found."""
+    if gate is None:
+        return 0, 0, 0
+    return (rows, row_stride, row_stride) if row_stride else (1, gate.numel(), gate.numel())
 
 
 class GatedMlp:
@@ -470,9 +503,9 @@ class GatedMlp:
         h_dtype = _DTYPES[h.dtype]
         n_dtype = 0 if h_dtype == 2 and self.result_dtype is None else h_dtype
         if inplace:
+            _check_inplace(h, rows, cols, stride, (("gate", self.gate, *_gate_extent(self.gate, gate_row, rows, cols)),
+                                                   ("post_weight", self.post_weight, 1, cols, cols), ("next_weight", self.next_weight, 1, cols, cols)))
             joined, out_stride = h, stride
-            if rows > 1 and stride < cols:
-                raise ValueError("h has rows that share memory and cannot be updated in place")
         else:
             joined, out_stride = h.new_empty(*h.shape), cols
         n = None
