@@ -72,10 +72,10 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // where every CTA adds up a share of the tokens, always in the same order.  Up to 32 tokens (16 with a gate) each sends its parts to where they are
 // added, as they come out of the accumulator, and a barrier there counts them: nothing but that barrier is waited for (1 token through 14336 x 4096
 // 7.4 us).  More would take stages from the ring; they take its place, and the adding CTA fetches them between two barriers of the whole cluster
-// (1 token 7.7 us that way; 64 tokens through 4096 x 14336 9.5 us, sent 10.1).
+// (1 token 7.9 us that way; 64 tokens through 4096 x 14336 9.8 us, sent 10.2).
 //
 // Warps: 0 copies, 1 multiplies, the next four or eight take the accumulator over, one or two on each quarter of its lanes (four launch a little
-// sooner, 1 token 7.4 us and with eight 7.6; eight are done sooner where there are more tokens, the gated pair for 64 17.2 us and with four 18.1); all of them add the
+// sooner, 1 token 7.4 us and with eight 7.6; eight are done sooner where there are more tokens, the gated pair for 64 17.4 us and with four 18.4); all of them add the
 // parts up.  With QUANTIZE, one more for every stage of the ring quantises the tokens' columns on their way into it, instead of a kernel before this one.
 template <int TOKENS, bool GATED>
 struct StreamShape {
@@ -97,8 +97,8 @@ struct StreamShape {
     static_assert(kStageBytes % 1024 == 0, "the swizzle counts from multiples of 1024 bytes");
     static_assert(kAcc * 128 * 4 <= kReceived, "a part of the accumulator takes the ring's place");
 };
-// Tokens that the kernel quantises itself.  us, inside | by a kernel before it: 14336 x 4096, 1 token 7.7 | 8.8, 8: 9.2 | 9.5, 9: 9.9 | 9.6, 16: 12.3 | 9.7
-// (1024 x 4096 3.1 | 4.6, 3.8 | 5.2, 4.2 | 5.2, 5.3 | 5.3); and a launch less for the host.
+// Tokens that the kernel quantises itself.  us, inside | by a kernel before it: 14336 x 4096, 1 token 7.7 | 8.8, 8: 9.2 | 9.6, 9: 9.9 | 9.6, 16: 12.3 | 9.7
+// (1024 x 4096 3.1 | 4.7, 3.9 | 5.2, 4.2 | 5.2, 5.3 | 5.3); and a launch and a buffer less for the host.
 constexpr int kMostQuantizedInside = MPS_MX4_TOKENS_INSIDE;
 static_assert(kMostQuantizedInside <= 16, "the kernel that quantises has 16 tokens");
 constexpr int kMostParts = 4;                  // CTAs of a cluster
@@ -391,7 +391,7 @@ mx4_stream_kernel(const ProductArgs p) {
 //
 // The copies of both CTAs count at the first one's barrier, whose thread issues the multiplications, so they are tiled copies: a tile is 17 rows of 1 KB,
 // the scales the first, and box and coordinates say which are wanted.  (With untiled copies, which count at their own CTA's barriers, the second
-// CTA has to hand every stage on with a release at cluster scope: 4096 x 4096 x 14336 took 164 us that way.)
+// CTA has to hand every stage on with a release at cluster scope: 4096 x 4096 x 14336 took 164 us that way, and takes 98.5.)
 //
 // Warps: 0 copies, 1 multiplies (first CTA) or waits for the end (second), 2 to 9 take the accumulator over, two
 // on each quarter of the lanes, one on each half of the columns.
@@ -716,9 +716,11 @@ static int launch_stream(ProductArgs p, const Device& d, cudaStream_t st) {
                           (int)tiles * p.parts, p.parts, st, p);
 }
 
-// Whether 128 tokens a tile with the weights on the lanes take less time than 256 with the tokens on the lanes, by what a tile of K, a round of CTAs
-// and a launch cost in each, us.  Measured, stream | wide: 14336 x 4096, 64 tokens 9.7 | 10.7, 128: 11.6 | 11.5, 512: 25.2 | 17.8; 4096 x 14336,
-// 128: 11.8 | 26.0, 512: 18.3 | 26.0, 1024: 29.7 | 26.5; 4096 x 4096, 256: 10.2 | 10.4, 1024: 13.1 | 10.7; 517 x 1000, 1024: 7.3 | 8.8.
+// Whether 128 tokens a tile with the weights on the lanes take less time than 256 with the tokens on the lanes, by an estimate of both: so much for a launch,
+// a tile of K and a further round of CTAs.  It is there to be compared, not to be read: where a cluster adds parts up the streaming kernel takes up to
+// 1.6 times as long.  Measured, stream | wide, us: 14336 x 4096, 128 tokens 12.0 | 12.1, 160: 14.1 | 12.1, 384: 24.3 | 18.8, 512: 25.8 | 18.9; 4096 x 14336,
+// 128: 12.1 | 25.0, 512: 19.0 | 25.3, 1024: 29.9 | 26.1; 4096 x 4096, 256: 10.0 | 10.6, 1024: 13.2 | 11.3; 517 x 1000, 1024: 7.4 | 9.2.  It takes the shorter
+// one at each of these.
 static bool stream_pays(const ProductArgs& p, int sms) {
     const int64_t tiles = (int64_t)p.row_tiles * ((p.tokens + 127) / 128), wide = (int64_t)((p.row_tiles + 1) / 2) * ((p.tokens + 255) / 256);
     const int parts = parts_of(tiles, p.chunks, sms);

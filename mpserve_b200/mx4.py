@@ -169,7 +169,8 @@ def quantize(x: torch.Tensor) -> Mx4Tensor:
 
 
 def dequantize(q: Mx4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that ``q`` stands for.  Exact in BF16 and F32; F16 rounds, and overflows beyond 65504."""
+    """The values that ``q`` stands for.  Exact in BF16 and F32, up to their range, which a checkpoint's scale above 2^125 may pass; F16 rounds, and overflows
+    beyond 65504."""
     index = _check_mx4(q, "q")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bfloat16, float16 or float32")
