@@ -9,7 +9,7 @@ namespace mps {
 
 // ---- what the kernels share -------------------------------------------------------------------------
 
-constexpr uint32_t kMx4SpinLimit = 1u << 20;
+constexpr uint32_t kMx4SpinLimit = 1u << 20;   // a poll lasts 4 us where nothing comes: 4 s in all
 constexpr int kMx4SmemMost = 232448;           // 227 KB
 
 constexpr int64_t kMx4WorkspaceBytes = 256;    // word 0 records a wait that ran out
@@ -393,7 +393,7 @@ mx4_stream_kernel(const ProductArgs p) {
 // the scales the first, and box and coordinates say which are wanted.  (With untiled copies, which count at their own CTA's barriers, the second
 // CTA has to hand every stage on with a release at cluster scope: 4096 x 4096 x 14336 took 164 us that way, and takes 98.5.)
 //
-// Warps: 0 copies, 1 multiplies (first CTA) or waits for the end (second), 2 to 9 take the accumulator over, two
+// Warps: 0 copies, 1 multiplies (first CTA only), 2 to 9 take the accumulator over, two
 // on each quarter of the lanes, one on each half of the columns.
 struct WideMaps { CUtensorMap x, w_scales, w_codes, up_scales, up_codes; };
 constexpr int kMx4MapRow = 1024, kMx4TileMapRows = kMx4TileBytes / kMx4MapRow;
@@ -534,16 +534,14 @@ mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
                 }
             }
             // Copies that nobody multiplied come all the same, before this CTA is gone.  (The second CTA's count at the other's barrier: its own is never
-            // arrived at, and the wait there lasts for the limit of polls, a thousand times what a copy takes.)
+            // arrived at, and the wait there lasts for its 1024 polls, 4 ms, a thousand times what a copy takes.)
             for (int64_t j = i > S::kStages ? i - S::kStages : 0; j < i; ++j) {
                 const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
-                if (!bar_wait<true>(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), rank ? 0u : parity, kMx4SpinLimit);
+                if (!bar_wait<true>(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), rank ? 0u : parity, rank ? 1024u : kMx4SpinLimit);
             }
         }
     } else if (warp == 1) {
-        if (rank == 1) {
-            warp_wait<true>(drained, 0, &failed);
-        } else {
+        if (rank == 0) {
             const uint32_t lead = elect_one();
             int s = 0;
             uint32_t parity = 0, round = 0;
@@ -572,7 +570,7 @@ mx4_wide_kernel(const ProductArgs p, const __grid_constant__ WideMaps maps) {
                 }
                 if (ok) tensor_commit_pair(lead, acc_full);
             }
-            tensor_commit_pair(lead, drained);
+            tensor_commit_pair<1>(lead, drained);      // the second CTA leaves when the first does; a wait of its own would have to outlast the kernel
             warp_wait(drained, 0, &failed);
         }
     } else {

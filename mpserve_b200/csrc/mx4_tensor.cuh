@@ -77,11 +77,12 @@ __device__ __forceinline__ void tensor_commit(uint32_t lead, uint32_t bar) {
 __device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// The same for a pair of CTAs: at this place in the shared memory of both.
+// The same for a pair of CTAs: at this place in the shared memory of those that CTAS, a bit each, names.
+template <int CTAS = 3>
 __device__ __forceinline__ void tensor_commit_pair(uint32_t lead, uint32_t bar) {
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %2, 0;\n\t"
                  "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
-                 ::"r"(bar), "h"((uint16_t)3), "r"(lead) : "memory");
+                 ::"r"(bar), "h"((uint16_t)CTAS), "r"(lead) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;

@@ -28,7 +28,10 @@ def test_waits_for_another_cta_acquire_at_cluster_scope():
     waits = re.findall(r"(?:bar|warp)_wait(<true>)?\((\w+)", wide)
     assert {bar for _, bar in waits} == {"empty", "full", "acc_empty", "acc_full", "drained"}
     assert all(scope for scope, bar in waits if bar in ("empty", "acc_empty", "acc_full"))
-    assert "warp_wait<true>(full(s)" in wide and "warp_wait<true>(drained" in wide
+    assert "warp_wait<true>(full(s)" in wide
+    # bounded waits begin when what they wait for is under way: the end of all multiplications is waited for by who issued them, and told to nobody else
+    assert "tensor_commit_pair<1>(lead, drained);" in wide
+    assert wide.index("if (rank == 0) {\n            const uint32_t lead") < wide.index("drained, 0, &failed")
 
 
 def test_copies_of_a_pair_count_at_the_barrier_that_is_waited_at():
