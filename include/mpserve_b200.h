@@ -416,6 +416,79 @@ MPS_API int mps_mx4_gated_mlp(const mps_mx4_mlp* block, const void* h, int32_t h
  * outputs are then incomplete), and clears the record. */
 MPS_API int mps_mx4_status(void* workspace, int64_t workspace_bytes, void* stream, int32_t* timed_out);
 
+/* The attention half of a decoding step -----------------------------------------------------------
+ * No counterpart in the reference.  Types: MPS_BF16, MPS_F16, where said MPS_F32. */
+
+/* INT4 weights: codes [rows, cols], one a byte as the AWQ entries take them, a 16-bit scale and a zero point (0 to 15; zeros null: 8) per row and `group` columns
+ * (32, 64 or 128; the last group may be cut short): value = (code - zero) * scale.  mps_int4_pack lays a weight out once, in mps_int4_bytes() device
+ * bytes, 16-byte aligned (-1 for sizes that are not served); csrc/int4.cu says what is in them. */
+MPS_API int64_t mps_int4_bytes(int64_t rows, int64_t cols, int32_t group);
+MPS_API int mps_int4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t rows, int64_t cols, int32_t group, void* data,
+                          void* stream);
+MPS_API int mps_int4_dequantize(const void* data, int64_t rows, int64_t cols, int32_t group, int32_t scale_dtype, int32_t dtype, void* out, void* stream);
+/* out[t, r] = sum_k x[t, k] value[r, k], summed in FP32, rounded once. */
+typedef struct mps_int4_linear {
+    const void* x;
+    const void* w;
+    void* out;
+    int64_t tokens, cols, rows;
+    int64_t x_stride, out_stride;       /* of rows, in elements */
+    int32_t group, x_dtype, scale_dtype, out_dtype;
+} mps_int4_linear;
+enum { MPS_INT4_MOST_TOKENS = 1 << 21 };
+MPS_API int mps_int4_product(const mps_int4_linear* args, void* stream);
+
+/* Queries and keys [tokens, heads, dim], normalised over each head where a weight is given, and rotated by their positions: pair j of the first `rotated` values
+ * of a head, (j, j + rotated / 2) or `interleaved` (2 j, 2 j + 1), by positions[axis[j]][token] * turns[j] whole turns, times `scale`.  q_out [tokens, q_heads,
+ * dim] is contiguous; k_out too, or with slots they are the pages of a cache, that k and v are written into: token t at slot slots[t] % page_size
+ * of page slots[t] / page_size; slots outside the cache are not written.  Strides in elements; dim up to 256. */
+typedef struct mps_head_rotate {
+    const void* q;
+    const void* k;
+    const void* v;                      /* with slots */
+    void* q_out;
+    void* k_out;
+    void* v_out;                        /* with slots */
+    const void* q_weight;               /* [dim], or null */
+    const void* k_weight;
+    const void* positions;              /* int32 or int64 [axes, tokens] */
+    const double* turns;                /* [rotated / 2]: whole turns for a step of one position */
+    const uint8_t* axis;                /* [rotated / 2], or null: 0 */
+    const int64_t* slots;               /* [tokens], or null */
+    int64_t tokens;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_cache_head_stride, v_page_stride, v_slot_stride, v_cache_head_stride;
+    int64_t pages, page_size;
+    int32_t q_heads, kv_heads, dim, rotated, interleaved, wide_positions, dtype, weight_dtype;
+    float eps, scale;
+} mps_head_rotate;
+enum { MPS_MOST_HEADS = 1024, MPS_MOST_SEQUENCES = 1 << 16 };
+MPS_API int mps_head_rotate_rows(const mps_head_rotate* args, void* stream);
+
+/* One query per sequence and head against a prefix that all sequences share and tokens of their own, both in a paged cache [pages, page_size, kv_heads, dim]:
+ * out = softmax(scale q k^T) v over prefix_length keys of prefix_table's pages and lengths[b] keys of row b of tables.  out [batch, q_heads, dim] and lse
+ * [batch, q_heads] (or null; natural logarithm) are contiguous.  Nothing to attend to: zeros, and minus infinity.  Lengths below 0 count as 0, above what a table holds as that; keys
+ * of a page outside the cache as absent.  dim 64 or 128; page_size a power of two, 16 at least. */
+typedef struct mps_prefix_attend {
+    const void* q;
+    const void* k_pages;
+    const void* v_pages;
+    void* out;
+    float* lse;
+    const int32_t* tables;              /* [batch, table_columns] */
+    const int32_t* lengths;             /* [batch] */
+    const int32_t* prefix_table;
+    int64_t batch, table_columns, prefix_length, pages, page_size;
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int32_t q_heads, kv_heads, dim, dtype;
+    float scale;
+} mps_prefix_attend;
+#define MPS_MOST_KEYS (INT64_C(1) << 30)
+/* Of these sizes on the current device (pointers and strides do not matter), or -1; 256-byte aligned, contents irrelevant before and after. */
+MPS_API int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args);
+MPS_API int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* stream);
+
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of
  * (pattern * (index+1)) -- what ranks all-reduce after a sharded decode.  result_dev: device
  * uint64[2], accumulated into (zero it first). */

@@ -37,6 +37,10 @@ class BucketTensor(C.Structure):
 MX4_NORM = struct.Struct("@7P7q6i2f")
 MX4_LINEAR = struct.Struct("@5P5q4i")
 MX4_MLP = struct.Struct("@7P3q5i2fi")
+# struct mps_int4_linear, mps_head_rotate and mps_prefix_attend, likewise.
+INT4_LINEAR = struct.Struct("@3P5q4i")
+HEAD_ROTATE = struct.Struct("@12P15q8i2f")
+PREFIX_ATTEND = struct.Struct("@8P13q4if4x")
 
 
 class Mx4Mlp(C.Structure):
@@ -91,6 +95,13 @@ _PROTOS = {
     "mps_mx4_mlp_scratch_bytes": (_i64, [_i64, _i64, _i64]),
     "mps_mx4_gated_mlp": (C.c_int, [C.POINTER(Mx4Mlp), _p, _i32, _i64, _i64, _p, _i64, _p, _i32, _p, _i64, _p, _i64, _p]),
     "mps_mx4_status": (C.c_int, [_p, _i64, _p, C.POINTER(_i32)]),
+    "mps_int4_bytes": (_i64, [_i64, _i64, _i32]),
+    "mps_int4_pack": (C.c_int, [_p, _p, _p, _i64, _i64, _i32, _p, _p]),
+    "mps_int4_dequantize": (C.c_int, [_p, _i64, _i64, _i32, _i32, _i32, _p, _p]),
+    "mps_int4_product": (C.c_int, [C.c_char_p, _p]),
+    "mps_head_rotate_rows": (C.c_int, [C.c_char_p, _p]),
+    "mps_prefix_attend_scratch_bytes": (_i64, [C.c_char_p]),
+    "mps_prefix_attend_tokens": (C.c_int, [C.c_char_p, _p, _i64, _p]),
     "mps_checksum_u16": (C.c_int, [_p, _i64, _p, _p]),
     "mps_build_workspace_bytes": (C.c_size_t, [_i64, _i64]),
     "mps_build_analyze": (C.c_int, [_p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _i64, _p, C.c_size_t, _p,

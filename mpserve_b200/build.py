@@ -18,11 +18,12 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "lib" / "libmpserve_b200.so"
 OBJ = PKG / "lib" / "obj"
-SOURCES = ["decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu", "mx4_convert.cu", "mx4_norm.cu", "mx4_linear.cu"]
+SOURCES = ["decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu", "mx4_convert.cu", "mx4_norm.cu", "mx4_linear.cu",
+           "int4.cu", "attn_rotate.cu", "attn_shared.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-std=c++17", "-lineinfo", *ARCH_FLAGS, "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 # The codec has no arithmetic but on integers and bit patterns.  The 4-bit operators keep subnormals (a scale goes down to 2^-127); where a fast function is
-# good enough (their activations) it is called by its name.
+# good enough (their activations) it is called by its name.  So it is with the operators of attention.
 FAST_MATH = {"decode_bucket.cu", "decode_shared.cu", "encode.cu", "plan_order.cu"}
 
 

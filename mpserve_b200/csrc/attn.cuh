@@ -1,0 +1,107 @@
+// What the kernels of the attention behind a shared prefix have in common: their arguments, and how the sequences' own keys are split.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+
+#include "mx4.cuh"
+#include "stream_common.cuh"
+#include "warp_mma.cuh"
+
+namespace mps {
+
+struct AttendArgs {
+    const uint16_t* q;
+    const uint16_t* k;                 // the cache's pages
+    const uint16_t* v;
+    uint16_t* out;
+    float* lse;
+    const int32_t* tables;
+    const int32_t* lengths;
+    const int32_t* prefix_table;
+    float* prefix_o;                   // [split][key head][row][dim], and the same of (m, l)
+    float2* prefix_ml;
+    float* own_o;                      // [item][key head][query head of the group][dim]
+    float2* own_ml;
+    int64_t q_token, q_head, k_page, k_slot, k_head, v_page, v_slot, v_head;      // strides
+    int64_t table_columns, most_own, prefix, prefix_step, own_items, page_mask;
+    int32_t pages, page_shift, prefix_splits, batch, kv_heads, group;
+    float scale_log2;
+};
+
+// A sequence's own keys are cut into stretches of a length that is the same for all, such that no more come of it than there are places for: with
+// T keys in all, B sequences and P places, stretches of at least T / (P - B) are at most T / (T / (P - B)) + B.  How long sequences are is known on the
+// GPU only, so every CTA finds its stretch for itself, from the lengths.
+constexpr int64_t kOwnLeast = 128;         // keys of a stretch, at least
+
+__device__ __forceinline__ int64_t own_length(const AttendArgs& p, int b) { return min(max((int64_t)p.lengths[b], (int64_t)0), p.most_own); }
+
+__device__ __forceinline__ int64_t warp_total(int64_t v) {
+#pragma unroll
+    for (int x = 16; x; x >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, x);
+    return v;
+}
+// By a whole warp.
+__device__ __forceinline__ int64_t own_step(const AttendArgs& p) {
+    int64_t total = 0;
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) total += own_length(p, b);
+    total = warp_total(total);
+    const int64_t places = p.own_items - p.batch;
+    return max(kOwnLeast, ((total + places - 1) / places + 63) / 64 * 64);
+}
+
+struct OwnItem { int64_t sequence, first, last; };      // keys first to last - 1; sequence -1: none
+// By a whole warp, the same in every lane.
+__device__ __forceinline__ OwnItem own_item(const AttendArgs& p, int64_t item) {
+    const int lane = threadIdx.x & 31;
+    const int64_t step = own_step(p);
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int b = b0 + lane;
+        const int64_t length = b < p.batch ? own_length(p, b) : 0, count = (length + step - 1) / step;
+        int64_t before = count;
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) {
+            const int64_t v = __shfl_up_sync(0xFFFFFFFFu, before, x);
+            if (lane >= x) before += v;
+        }
+        const int64_t all = __shfl_sync(0xFFFFFFFFu, before, 31);
+        before -= count;
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, item >= before && item < before + count);
+        if (here) {
+            const int from = __ffs(here) - 1;
+            const int64_t first = __shfl_sync(0xFFFFFFFFu, (item - before) * step, from), end = __shfl_sync(0xFFFFFFFFu, length, from);
+            return {b0 + from, first, min(first + step, end)};
+        }
+        item -= all;
+    }
+    return {-1, 0, 0};
+}
+
+struct OwnItems { int64_t first; int count; };
+// The stretches of a sequence, by a whole warp.
+__device__ __forceinline__ OwnItems own_items(const AttendArgs& p, int sequence) {
+    if (p.own_items == 0) return {0, 0};
+    const int64_t step = own_step(p);
+    int64_t before = 0;
+    for (int b = threadIdx.x & 31; b < sequence; b += 32) before += (own_length(p, b) + step - 1) / step;
+    return {warp_total(before), (int)((own_length(p, sequence) + step - 1) / step)};
+}
+
+// A launch with dynamic shared memory that may overlap the end of the kernel before it.
+template <typename... Params, typename... Args>
+inline int launch_overlapping_smem(const char* what, void (*kernel)(Params...), unsigned int ctas, dim3 threads, int smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas);
+    config.blockDim = threads;
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = st;
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
+}
+
+}  // namespace mps

@@ -1,0 +1,400 @@
+// Attention of a batch of single tokens that share a prefix: every sequence's query attends to the prefix, which all have in common, and to tokens of its own.
+//
+//   out = sum_k softmax_k(scale q . key_k) value_k      over the prefix's keys and those of the sequence's own table
+//
+// Both lie in one paged cache.  A part of the keys gives, for a query, the largest logit m, l = sum_k 2^(logit_k - m) and o = sum_k 2^(logit_k - m) value_k (logits
+// in units of log 2); parts join as
+//   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
+// whatever the keys were split into, so that the prefix is read once for many queries and every sequence's own keys once, each in as many parts as fill the GPU.
+#include "attn.cuh"
+
+namespace mps {
+
+// ---- own tokens: keys on the rows of the products ------------------------------------------------------
+//
+// A CTA has a stretch of one sequence's keys for one key head; its four warps take blocks of 16 keys in turn, each through a ring of its own that
+// nobody else waits for.  Logits are computed as K q^T, 16 keys by 8 query heads, and the result as V^T P^T, so that the eight columns are the query
+// heads that share the key head, and none of the tensor cores' rows idles.  Bound: memory; four warps with two blocks of 16 keys on their way, and two
+// such CTAs on an SM, have 128 KB under way.
+constexpr int kFewWarps = 4, kFewStages = 3, kFewColumns = 8;
+
+template <int DIM>
+struct FewShape {
+    static constexpr int kRow = DIM * 2, kBlock = 16 * kRow, kStage = 2 * kBlock;      // 16 keys, then their values
+    static constexpr int kRing = kFewStages * kStage;
+    static constexpr int kSmem = kFewWarps * kRing;
+    static_assert(kRing >= kFewColumns * DIM * 4, "a warp's result takes its ring's place");
+};
+
+// 16-byte piece `piece` of row `row`: rows of 256 (128) bytes, pieces XORed with the row, so that eight rows' pieces lie in different banks.
+template <int DIM>
+__device__ __forceinline__ uint32_t few_place(int row, int piece) { return row * (DIM * 2) + ((piece ^ (row & 7)) << 4); }
+
+struct KeyRange { const int32_t* table; int64_t first, last; };      // keys first to last - 1 of a table
+
+// Columns: `base` + column heads of query pointers; `live` of them.
+template <int DIM, bool BF16>
+__device__ __forceinline__ void attend_few(const AttendArgs& p, uint8_t* smem, const KeyRange range, int kv_head, const uint16_t* query, int live, float* part_o,
+                                           float2* part_ml) {
+    using S = FewShape<DIM>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+    const int blocks = (int)((range.last - range.first + 15) >> 4);
+    constexpr int kPieces = DIM / 8;       // of a row
+
+    uint32_t q[DIM / 16][2];
+#pragma unroll
+    for (int d = 0; d < DIM / 16; ++d) {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(query + d * 16 + 2 * t);
+        q[d][0] = g < live ? at[0] : 0u;
+        q[d][1] = g < live ? at[4] : 0u;
+    }
+    const auto page_of = [&](int block) {      // of the pool, or one that is outside
+        return block < blocks ? range.table[(range.first + block * 16) >> p.page_shift] : -1;
+    };
+    // keys of the block that are there
+    const auto present = [&](int block, int page) {
+        return block < blocks && (uint32_t)page < (uint32_t)p.pages ? (int)min((int64_t)16, range.last - range.first - block * 16) : 0;
+    };
+    const auto load = [&](int block, int page, int stage) {
+        const int keys = present(block, page);
+        const int64_t slot = (range.first + block * 16) & p.page_mask;
+        const uint16_t* k = p.k + (keys ? (int64_t)page * p.k_page + slot * p.k_slot + (int64_t)kv_head * p.k_head : 0);
+        const uint16_t* v = p.v + (keys ? (int64_t)page * p.v_page + slot * p.v_slot + (int64_t)kv_head * p.v_head : 0);
+        const uint32_t to = ring + stage * S::kStage;
+#pragma unroll
+        for (int i = 0; i < kPieces / 2; ++i) {
+            const int row = i * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
+            const bool there = row < keys;      // others become zeros: a value that is not there must not be a NaN, which 0 does not multiply away
+            cp_async_16_or_zero(to + few_place<DIM>(row, piece), k + (there ? row * p.k_slot + piece * 8 : 0), there);
+            cp_async_16_or_zero(to + S::kBlock + few_place<DIM>(row, piece), v + (there ? row * p.v_slot + piece * 8 : 0), there);
+        }
+    };
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DIM / 16][4];
+#pragma unroll
+    for (int d = 0; d < DIM / 16; ++d) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f; }
+
+    int pages[kFewStages];      // of the blocks in the ring
+#pragma unroll
+    for (int s = 0; s < kFewStages - 1; ++s) {
+        pages[s] = page_of(warp + s * kFewWarps);
+        if (warp + s * kFewWarps < blocks) load(warp + s * kFewWarps, pages[s], s);
+        cp_async_commit();
+    }
+    int ahead = page_of(warp + (kFewStages - 1) * kFewWarps), stage = 0;
+    for (int b = warp; b < blocks; b += kFewWarps) {
+        const int next = b + (kFewStages - 1) * kFewWarps;
+        pages[kFewStages - 1] = ahead;
+        if (next < blocks) load(next, ahead, stage == 0 ? kFewStages - 1 : stage - 1);
+        cp_async_commit();
+        ahead = page_of(next + kFewWarps);
+        cp_async_wait<kFewStages - 1>();
+        __syncwarp();
+        const uint32_t at = ring + stage * S::kStage;
+        const int keys = present(b, pages[0]);
+        // K q^T
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DIM / 16; ++d) {
+            uint32_t a[4];
+            load_matrices(a, at + few_place<DIM>(lane & 15, 2 * d + (lane >> 4)));
+            multiply<BF16>(s, a, q[d][0], q[d][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = g + 8 * (i >> 1) < keys ? s[i] * p.scale_log2 : -INFINITY;
+        float up[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float top = fmaxf(s[i], s[i + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+            top = fmaxf(top, m[i]);
+            const float base = top == -INFINITY ? 0.f : top;
+            up[i] = exp2f(m[i] - base);
+            m[i] = top;
+            s[i] = exp2f(s[i] - base);
+            s[i + 2] = exp2f(s[i + 2] - base);
+            l[i] = fmaf(l[i], up[i], s[i] + s[i + 2]);
+        }
+        const uint32_t p0 = transpose8(pack_pair<BF16>(s[0], s[1])), p1 = transpose8(pack_pair<BF16>(s[2], s[3]));
+        // V^T P^T
+#pragma unroll
+        for (int d = 0; d < DIM / 16; ++d) {
+            uint32_t a[4];
+            load_matrices_transposed(a, at + S::kBlock + few_place<DIM>((lane & 7) + ((lane >> 4) << 3), 2 * d + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] *= up[i & 1];
+            multiply<BF16>(o[d], a, p0, p1);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i + 1 < kFewStages; ++i) pages[i] = pages[i + 1];
+        if (++stage == kFewStages) stage = 0;
+    }
+    cp_async_wait<0>();
+    __shared__ float ms[kFewWarps][kFewColumns], ls[kFewWarps][kFewColumns];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], x);
+        if (g == 0) { ms[warp][2 * t + i] = m[i]; ls[warp][2 * t + i] = l[i]; }
+    }
+    __syncthreads();
+    // the four warps' results, each in its own ring, by columns
+    float* own = reinterpret_cast<float*>(smem + warp * S::kRing);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = 2 * t + i;
+        float top = ms[0][c];
+#pragma unroll
+        for (int w = 1; w < kFewWarps; ++w) top = fmaxf(top, ms[w][c]);
+        const float f = exp2f(m[i] - (top == -INFINITY ? 0.f : top));      // 0 for a warp that had nothing; a NaN stays one
+#pragma unroll
+        for (int d = 0; d < DIM / 16; ++d) {
+            own[c * DIM + d * 16 + g] = o[d][i] * f;
+            own[c * DIM + d * 16 + g + 8] = o[d][i + 2] * f;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < live * DIM; i += kFewWarps * 32) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) v += reinterpret_cast<const float*>(smem + w * S::kRing)[i];
+        part_o[i] = v;
+    }
+    if (threadIdx.x < live) {
+        const int c = threadIdx.x;
+        float top = ms[0][c], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kFewWarps; ++w) top = fmaxf(top, ms[w][c]);
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) sum = fmaf(ls[w][c], exp2f(ms[w][c] - (top == -INFINITY ? 0.f : top)), sum);
+        part_ml[c] = make_float2(top, sum);
+    }
+}
+
+template <int DIM, bool BF16>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_own_kernel(const AttendArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    griddep_wait();
+    griddep_launch();
+    const int column_tiles = (p.group + kFewColumns - 1) / kFewColumns;
+    const int kv_head = blockIdx.x % p.kv_heads, columns = blockIdx.x / p.kv_heads % column_tiles, item = blockIdx.x / p.kv_heads / column_tiles;
+    const OwnItem own = own_item(p, item);
+    if (own.sequence < 0) return;
+    const int first = columns * kFewColumns, live = min(kFewColumns, p.group - first), g = (threadIdx.x & 31) >> 2;
+    const uint16_t* query = p.q + own.sequence * p.q_token + (int64_t)(kv_head * p.group + first + (g < live ? g : 0)) * p.q_head;
+    const int64_t part = ((int64_t)item * p.kv_heads + kv_head) * p.group + first;
+    attend_few<DIM, BF16>(p, smem, {p.tables + own.sequence * p.table_columns, own.first, own.last}, kv_head, query, live, p.own_o + part * DIM, p.own_ml + part);
+}
+
+// The prefix, eight rows (queries of a key head) at a time.
+template <int DIM, bool BF16>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_prefix_kernel(const AttendArgs p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    griddep_wait();
+    griddep_launch();
+    const int rows = p.batch * p.group, row_tiles = (rows + kFewColumns - 1) / kFewColumns;
+    const int tile = blockIdx.x % row_tiles, kv_head = blockIdx.x / row_tiles % p.kv_heads, split = blockIdx.x / row_tiles / p.kv_heads;
+    const int first = tile * kFewColumns, live = min(kFewColumns, rows - first), g = (threadIdx.x & 31) >> 2, row = first + (g < live ? g : 0);
+    const uint16_t* query = p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head;
+    const int64_t part = ((int64_t)split * p.kv_heads + kv_head) * rows + first, begin = (int64_t)split * p.prefix_step;
+    attend_few<DIM, BF16>(p, smem, {p.prefix_table, begin, min(p.prefix, begin + p.prefix_step)}, kv_head, query, live, p.prefix_o + part * DIM, p.prefix_ml + part);
+}
+
+// ---- the parts of a query joined -----------------------------------------------------------------------
+//
+// A CTA has a sequence, a warp a head at a time: its lanes share the parts' weights first, then each has its columns of all parts.
+constexpr int kJoinWarps = 8;
+template <int DIM, bool BF16>
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
+    griddep_wait();
+    griddep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sequence = blockIdx.x;
+    const OwnItems own = own_items(p, sequence);
+    const int splits = p.prefix_splits, count = splits + own.count;
+    const int64_t rows = (int64_t)p.batch * p.group;
+    constexpr int kColumns = DIM / 32;
+    for (int head = warp; head < p.kv_heads * p.group; head += kJoinWarps) {
+        const int kv_head = head / p.group, in_group = head % p.group;
+        const auto place = [&](int i) {
+            return i < splits ? ((int64_t)i * p.kv_heads + kv_head) * rows + (int64_t)sequence * p.group + in_group
+                              : ((own.first + i - splits) * p.kv_heads + kv_head) * p.group + in_group;
+        };
+        float top = -INFINITY, sum = 0.f, out[kColumns];
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
+        for (int first = 0; first < count; first += 32) {
+            const int i = first + lane;
+            const float2 ml = i < count ? (i < splits ? p.prefix_ml : p.own_ml)[place(i)] : make_float2(-INFINITY, 0.f);
+            float high = ml.x;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, x));
+            high = fmaxf(high, top);
+            const float base = high == -INFINITY ? 0.f : high, up = exp2f(top - base), weight = exp2f(ml.x - base);
+            top = high;
+            float part = ml.y * weight;
+#pragma unroll
+            for (int x = 16; x; x >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, x);
+            sum = fmaf(sum, up, part);
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) out[c] *= up;
+            for (int j = 0; j < min(32, count - first); ++j) {
+                const float w = __shfl_sync(0xFFFFFFFFu, weight, j);
+                const float* from = (first + j < splits ? p.prefix_o : p.own_o) + place(first + j) * DIM + lane * kColumns;
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) out[c] = fmaf(w, from[c], out[c]);
+            }
+        }
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query with nothing to attend to gets zeros
+        uint16_t* to = p.out + ((int64_t)sequence * p.kv_heads * p.group + head) * DIM + lane * kColumns;
+#pragma unroll
+        for (int c = 0; c < kColumns; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_pair<BF16>(out[c] * inverse, out[c + 1] * inverse);
+        if (p.lse && lane == 0) p.lse[(int64_t)sequence * p.kv_heads * p.group + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------
+
+struct AttendPlan {
+    int64_t prefix_step;          // keys of a part of the prefix
+    int prefix_splits;
+    int64_t own_items;            // at most
+    int64_t floats(int64_t rows, int64_t kv_heads, int64_t group, int64_t dim) const {      // of the scratch
+        return (prefix_splits * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
+    }
+};
+static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
+    AttendPlan plan = {};
+    const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group, row_tiles = (rows + kFewColumns - 1) / kFewColumns;
+    if (a.prefix_length > 0) {
+        const int64_t wanted = (2 * sms + row_tiles * a.kv_heads - 1) / (row_tiles * a.kv_heads);
+        plan.prefix_step = ((a.prefix_length + wanted - 1) / wanted + 63) / 64 * 64;
+        plan.prefix_splits = (int)((a.prefix_length + plan.prefix_step - 1) / plan.prefix_step);
+    }
+    const int64_t most = a.table_columns * a.page_size;
+    if (most > 0) {
+        const int64_t tiles = a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
+        const int64_t extra = std::min((4 * sms + tiles - 1) / tiles, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
+        plan.own_items = a.batch + extra;
+    }
+    return plan;
+}
+
+static int check_attend(const mps_prefix_attend& a) {
+    if (a.batch < 0 || a.batch > MPS_MOST_SEQUENCES || a.q_heads <= 0 || a.kv_heads <= 0 || a.q_heads > MPS_MOST_HEADS || a.q_heads % a.kv_heads) {
+        set_error("mps_prefix_attend_tokens: batch must be in [0, %d], query heads a multiple of the key heads and at most %d", (int)MPS_MOST_SEQUENCES, (int)MPS_MOST_HEADS);
+        return MPS_ERR_INVALID;
+    }
+    if (a.dim != 64 && a.dim != 128) { set_error("mps_prefix_attend_tokens: dim must be 64 or 128"); return MPS_ERR_INVALID; }
+    if (a.dtype != MPS_BF16 && a.dtype != MPS_F16) { set_error("mps_prefix_attend_tokens: dtype must be BF16 or F16"); return MPS_ERR_INVALID; }
+    if (a.pages < 0 || a.pages > 0x7FFFFFFF || a.page_size < 16 || a.page_size > 1 << 20 || (a.page_size & (a.page_size - 1))) {
+        set_error("mps_prefix_attend_tokens: the size of a page must be a power of two from 16 to 2^20, pages below 2^31");
+        return MPS_ERR_INVALID;
+    }
+    if (a.table_columns < 0 || a.table_columns * a.page_size > MPS_MOST_KEYS || a.prefix_length < 0 || a.prefix_length > MPS_MOST_KEYS) {
+        set_error("mps_prefix_attend_tokens: a table and the prefix may have at most %lld keys", (long long)MPS_MOST_KEYS);
+        return MPS_ERR_INVALID;
+    }
+    return MPS_OK;
+}
+
+template <int DIM, bool BF16>
+static int attend(const AttendArgs& p, int64_t prefix_ctas, int64_t own_ctas, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    Device d;
+    int rc = current_device(d);
+    if (rc) return rc;
+    if (!(ready.load(std::memory_order_acquire) >> (d.ordinal & 63) & 1)) {
+        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_own_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<DIM>::kSmem));
+        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_prefix_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<DIM>::kSmem));
+        ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
+    }
+    if (prefix_ctas) {
+        rc = launch_overlapping_smem("attend_prefix_kernel", attend_prefix_kernel<DIM, BF16>, (unsigned int)prefix_ctas, dim3(kFewWarps * 32), FewShape<DIM>::kSmem, st, p);
+        if (rc) return rc;
+    }
+    if (own_ctas) {
+        rc = launch_overlapping_smem("attend_own_kernel", attend_own_kernel<DIM, BF16>, (unsigned int)own_ctas, dim3(kFewWarps * 32), FewShape<DIM>::kSmem, st, p);
+        if (rc) return rc;
+    }
+    return launch_overlapping("attend_join_kernel", attend_join_kernel<DIM, BF16>, (unsigned int)p.batch, dim3(kJoinWarps * 32), st, p);
+}
+
+}  // namespace mps
+
+using namespace mps;
+
+extern "C" int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args) {
+    if (!args || check_attend(*args)) return -1;
+    Device d;
+    if (current_device(d)) return -1;
+    const int64_t group = args->q_heads / args->kv_heads;
+    return attend_plan(*args, d.sms).floats(args->batch * group, args->kv_heads, group, args->dim) * 4 + 64;
+}
+
+extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* stream) {
+    if (!args) { set_error("mps_prefix_attend_tokens: null arguments"); return MPS_ERR_INVALID; }
+    const mps_prefix_attend& a = *args;
+    int rc = check_attend(a);
+    if (rc) return rc;
+    if (a.batch == 0) return MPS_OK;
+    if (!a.q || !a.out || (a.pages && (!a.k_pages || !a.v_pages)) || (a.table_columns && (!a.tables || !a.lengths)) || (a.prefix_length && !a.prefix_table)) {
+        set_error("mps_prefix_attend_tokens: missing pointer");
+        return MPS_ERR_INVALID;
+    }
+    if (((reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages)) & 15u) || (a.k_page_stride | a.k_slot_stride | a.k_head_stride) % 8 ||
+        (a.v_page_stride | a.v_slot_stride | a.v_head_stride) % 8) {
+        set_error("mps_prefix_attend_tokens: pages must be 16-byte aligned, their strides multiples of 8 elements");
+        return MPS_ERR_INVALID;
+    }
+    if ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out)) & 15u || (a.q_token_stride | a.q_head_stride) % 8) {
+        set_error("mps_prefix_attend_tokens: queries must be 16-byte aligned, their strides multiples of 8 elements");
+        return MPS_ERR_INVALID;
+    }
+    Device d;
+    rc = current_device(d);
+    if (rc) return rc;
+    AttendArgs p = {};
+    const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group;
+    const AttendPlan plan = attend_plan(a, d.sms);
+    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15u) || scratch_bytes < plan.floats(rows, a.kv_heads, group, a.dim) * 4) {
+        set_error("mps_prefix_attend_tokens: scratch missing, unaligned or too small");
+        return MPS_ERR_WORKSPACE;
+    }
+    p.q = static_cast<const uint16_t*>(a.q);
+    p.k = static_cast<const uint16_t*>(a.k_pages);
+    p.v = static_cast<const uint16_t*>(a.v_pages);
+    p.out = static_cast<uint16_t*>(a.out);
+    p.lse = a.lse;
+    p.tables = a.tables;
+    p.lengths = a.lengths;
+    p.prefix_table = a.prefix_table;
+    p.q_token = a.q_token_stride; p.q_head = a.q_head_stride;
+    p.k_page = a.k_page_stride; p.k_slot = a.k_slot_stride; p.k_head = a.k_head_stride;
+    p.v_page = a.v_page_stride; p.v_slot = a.v_slot_stride; p.v_head = a.v_head_stride;
+    p.table_columns = a.table_columns;
+    p.most_own = a.table_columns * a.page_size;
+    p.prefix = a.prefix_length;
+    p.prefix_step = plan.prefix_step;
+    p.prefix_splits = plan.prefix_splits;
+    p.own_items = plan.own_items;
+    p.pages = (int32_t)a.pages;
+    p.page_shift = __builtin_ctzll((unsigned long long)a.page_size);
+    p.page_mask = a.page_size - 1;
+    p.batch = (int32_t)a.batch;
+    p.kv_heads = a.kv_heads;
+    p.group = (int32_t)group;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    const int64_t prefix_parts = plan.prefix_splits * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
+    p.prefix_o = static_cast<float*>(scratch);
+    p.own_o = p.prefix_o + prefix_parts * a.dim;
+    p.prefix_ml = reinterpret_cast<float2*>(p.own_o + own_parts * a.dim);
+    p.own_ml = p.prefix_ml + prefix_parts;
+    const int64_t prefix_ctas = plan.prefix_splits * a.kv_heads * ((rows + kFewColumns - 1) / kFewColumns);
+    const int64_t own_ctas = plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
+    if (prefix_ctas > 0x7FFFFFFF || own_ctas > 0x7FFFFFFF) { set_error("mps_prefix_attend_tokens: too much work for one launch"); return MPS_ERR_INVALID; }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, prefix_ctas, own_ctas, st) : attend<64, false>(p, prefix_ctas, own_ctas, st);
+    return a.dtype == MPS_BF16 ? attend<128, true>(p, prefix_ctas, own_ctas, st) : attend<128, false>(p, prefix_ctas, own_ctas, st);
+}

@@ -1,0 +1,50 @@
+// The tensor cores' warp-wide products of 16-bit operands, and how their fragments come from shared memory.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace mps {
+
+// d[16 x 8] += a[16 x 16] b[16 x 8], sums in FP32.  Lane 4 g + t: d has rows g and g + 8 (words 0, 1 and 2, 3), columns 2 t and 2 t + 1; a's words rows g, g + 8, g,
+// g + 8 at columns 2 t (the first two) and 2 t + 8; b's words rows 2 t and 2 t + 8 of column g, each with the row after.
+template <bool BF16>
+__device__ __forceinline__ void multiply(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four 8 x 8 matrices: lane i names row i % 8 of matrix i / 8, and gets of each the two values at row g, columns 2 t and 2 t + 1 (transposed: column g, rows 2 t ...).
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t row) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&r)[4], uint32_t row) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row) : "memory");
+}
+// An 8 x 8 matrix that a warp holds, two values of row g a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    if (BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// 16 bytes into shared memory, of this source or zeros.
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+}  // namespace mps
