@@ -487,7 +487,8 @@ typedef struct mps_prefix_attend {
 #define MPS_MOST_KEYS (INT64_C(1) << 30)
 /* Of these sizes on the current device (pointers and strides do not matter), or -1; 256-byte aligned, contents irrelevant before and after. */
 MPS_API int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args);
-MPS_API int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* stream);
+/* workspace: mps_mx4_workspace_bytes() bytes as for the MXFP4 products, which may be theirs; mps_mx4_status tells of waits that ran out. */
+MPS_API int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of
  * (pattern * (index+1)) -- what ranks all-reduce after a sharded decode.  result_dev: device

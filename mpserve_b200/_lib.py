@@ -101,7 +101,7 @@ _PROTOS = {
     "mps_int4_product": (C.c_int, [C.c_char_p, _p]),
     "mps_head_rotate_rows": (C.c_int, [C.c_char_p, _p]),
     "mps_prefix_attend_scratch_bytes": (_i64, [C.c_char_p]),
-    "mps_prefix_attend_tokens": (C.c_int, [C.c_char_p, _p, _i64, _p]),
+    "mps_prefix_attend_tokens": (C.c_int, [C.c_char_p, _p, _i64, _p, _i64, _p]),
     "mps_checksum_u16": (C.c_int, [_p, _i64, _p, _p]),
     "mps_build_workspace_bytes": (C.c_size_t, [_i64, _i64]),
     "mps_build_analyze": (C.c_int, [_p, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _i32, _i64, _p, C.c_size_t, _p,

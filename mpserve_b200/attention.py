@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .mx4 import _DTYPES, _current_device, _launch, _stream_of
+from .mx4 import _DTYPES, _current_device, _launch, _stream_of, _workspace
 
 __all__ = ["Rotary", "KvCache", "norm_rotate", "norm_rotate_append", "shared_prefix_attention"]
 
@@ -287,13 +287,14 @@ def shared_prefix_attention(q: torch.Tensor, cache: KvCache, tables: torch.Tenso
         kind = _DTYPES[dtype]
         need = _scratch_bytes(index, batch, columns, prefix_length, page_size, q_heads, kv_heads, dim, kind)
         scratch = q.new_empty(need, dtype=torch.uint8)      # of this call: freed on return, and not handed to another stream before it is done
+        ws = _workspace(index)
         args = _lib.PREFIX_ATTEND.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                        tables.data_ptr(), lengths.data_ptr(), prefix_ptr, batch, columns, prefix_length, pages, page_size, q_token, q_head,
                                        *_strides(k_pages)[:3], *_strides(v_pages)[:3], q_heads, kv_heads, dim, kind, dim ** -0.5 if scale is None else scale)
         if _current_device() == index:
-            rc = _lib.load().mps_prefix_attend_tokens(args, scratch.data_ptr(), need, _stream_of(index))
+            rc = _lib.load().mps_prefix_attend_tokens(args, scratch.data_ptr(), need, ws.data_ptr(), ws.numel(), _stream_of(index))
             if rc:
                 _lib.check(rc)
         else:
-            _launch(index, "mps_prefix_attend_tokens", args, scratch.data_ptr(), need)
+            _launch(index, "mps_prefix_attend_tokens", args, scratch.data_ptr(), need, ws.data_ptr(), ws.numel())
     return (out, lse) if return_lse else out

@@ -26,8 +26,22 @@ struct AttendArgs {
     int64_t q_token, q_head, k_page, k_slot, k_head, v_page, v_slot, v_head;      // strides
     int64_t table_columns, most_own, prefix, prefix_step, own_items, page_mask;
     int32_t pages, page_shift, prefix_splits, batch, kv_heads, group;
-    float scale_log2;
+    int32_t q_factor;                  // 1, -1 or 0: what queries are multiplied by, exactly
+    float scale_log2;                  // positive
+    uint32_t* workspace;               // word 0 records a wait that ran out
 };
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t times_zero(uint32_t pair) {      // 0, or NaN for what is not finite
+    uint32_t r;
+    if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(0u));
+    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(0u));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t query_pair(uint32_t pair, int factor) {
+    return factor == 1 ? pair : factor == -1 ? pair ^ 0x80008000u : times_zero<BF16>(pair);
+}
 
 // A sequence's own keys are cut into stretches of a length that is the same for all, such that no more come of it than there are places for: with
 // T keys in all, B sequences and P places, stretches of at least T / (P - B) are at most T / (T / (P - B)) + B.  How long sequences are is known on the

@@ -1,0 +1,342 @@
+// The shared prefix: 128 queries of a key head at a time on the tensor cores.
+//
+// A query of the batch is a row: row b * group + g of key head h is query head h * group + g of sequence b.  A CTA has one stretch of the prefix for up to 256 rows, in
+// two groups of four warps; keys and values come 128 at a time into a ring in shared memory, page by page as tiled copies.
+//   S = Q K^T   128 x 128 in tensor memory, operands from shared memory;
+//   P = 2^(S - m) in the cache's type, which takes S's place: a thread has a row, so that maxima and sums need no other thread;
+//   O += P V    128 x dim in tensor memory, P from there.
+// While one group makes its P, the tensor cores work for the other.  With more than 128 rows each group has 128 of them and both use the same keys; with no more
+// (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of keys in turn, and their results are two parts.
+//
+// O is scaled anew only where a row's largest logit has grown by more than 2^8 since it last was: P is then at most 2^8, which is far from the end of
+// either type's range, and what m a part refers to does not matter when parts are joined.  P is rounded to 16 bits, as the tensor cores take it: a relative
+// 2^-8 (BF16) of every weight by itself, below what the result is rounded by.  Sums are of P as it was before.
+// Bounds: for many rows the tensor cores and the exponentials alike (128 x 128 logits are 1024 cycles of each per group at the nominal rates), for few the memory.
+#pragma once
+
+#include <cuda.h>
+
+#include "attn.cuh"
+#include "mx4_tensor.cuh"
+
+namespace mps {
+
+constexpr int kPrefixKeys = 128, kPrefixRows = 128, kPrefixThreads = 384;      // the last two warps have nothing to do but to complete a group of four
+constexpr float kRescale = 8.f;      // in powers of two
+
+template <int DIM>
+struct PrefixShape {
+    static constexpr int kHalf = kPrefixKeys * 128, kHalves = DIM / 64;      // 64 columns of a tile, rows of 128 bytes
+    static constexpr int kStage = kHalves * kHalf, kStages = DIM == 128 ? 5 : 8;
+    static constexpr int kRing = 2 * kStage;                                  // behind two tiles of queries
+    static constexpr int kBars = kRing + kStages * kStage;
+    static constexpr int kSmem = kBars + (2 * kStages + 5) * 8 + 16;
+    static constexpr int kColumns = 512;                                      // S, S, O, O
+    static_assert(kSmem <= 232448, "shared memory");
+};
+struct PrefixMaps { CUtensorMap k, v; };
+
+// A box: 64 columns of neighbouring slots of one page.  A page outside the cache gives zeros.
+__device__ __forceinline__ void page_box(uint32_t dst, const CUtensorMap* map, int column, int slot, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(column), "r"(slot), "r"(head), "r"(page), "r"(bar) : "memory");
+}
+// 2^x, off by 2^-22 of itself: far below what P is rounded by.  (Results below 2^-126 become 0.)
+__device__ __forceinline__ float fast_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+template <int DIM, bool BF16>
+__global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const AttendArgs p, const __grid_constant__ PrefixMaps maps) {
+    using S = PrefixShape<DIM>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem), ring = base + S::kRing, bar0 = base + S::kBars;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + S::kSmem - 16);
+    volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 12);
+    volatile uint32_t& absent = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 8);      // pages of this stretch lie outside the cache
+    const auto full = [&](int s) { return bar0 + 8u * s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    const auto s_full = [&](int g) { return bar0 + 8u * (2 * S::kStages + g); };
+    const auto p_ready = [&](int g) { return bar0 + 8u * (2 * S::kStages + 2 + g); };
+    const uint32_t done = bar0 + 8u * (2 * S::kStages + 4);
+
+    const int rows = p.batch * p.group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows, pairs = row_tiles / 2, wide_tiles = (row_tiles + 1) / 2;
+    const int x = blockIdx.x % wide_tiles, kv_head = blockIdx.x / wide_tiles % p.kv_heads, split = blockIdx.x / wide_tiles / p.kv_heads;
+    const bool paired = x < pairs;             // else the groups take the keys in turn
+    const int64_t key0 = (int64_t)split * p.prefix_step, key_end = min(p.prefix, key0 + p.prefix_step);
+    const int tiles = (int)((key_end - key0 + kPrefixKeys - 1) / kPrefixKeys);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g), 4); }
+        mbar_init(done, 1);
+        failed = 0u;
+        absent = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    if (warp == 9 && lane == 0) { prefetch_map(&maps.k); prefetch_map(&maps.v); }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch();
+
+    // the queries, as the tensor cores read them: 16-byte pieces XORed with the row
+    for (int i = threadIdx.x; i < (paired ? 2 : 1) * kPrefixRows * (DIM / 8); i += kPrefixThreads) {
+        const int r = i / (DIM / 8), piece = i % (DIM / 8), row = x * 2 * kPrefixRows + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head + piece * 8);
+        v = make_uint4(query_pair<BF16>(v.x, p.q_factor), query_pair<BF16>(v.y, p.q_factor), query_pair<BF16>(v.z, p.q_factor), query_pair<BF16>(v.w, p.q_factor));
+        const int in_tile = r % kPrefixRows;
+        *reinterpret_cast<uint4*>(smem + r / kPrefixRows * S::kStage + piece / 8 * S::kHalf + in_tile * 128 + (((piece & 7) ^ (in_tile & 7)) << 4)) = v;
+    }
+    {
+        const int64_t first = key0 >> p.page_shift, last = (key_end - 1) >> p.page_shift;
+        for (int64_t i = first + threadIdx.x; i <= last; i += kPrefixThreads)
+            if ((uint32_t)p.prefix_table[i] >= (uint32_t)p.pages) absent = 1u;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written here
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    const uint32_t s_at = tmem, o_at = tmem + 256;      // and 128 columns on for the second group
+
+    // tiles come as K0, K1, V0, K2, V1, ...: number in that order
+    const auto key_number = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
+    const auto value_number = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
+
+    // a row's 128 logits want more registers than a 384th of them: the four warps that copy and multiply give up theirs (256 x 208 + 128 x 88 = 384 x 168)
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 9) {
+            const int box = (int)min(p.page_mask + 1, (int64_t)kPrefixKeys), boxes = kPrefixKeys / box;
+            // this lane's box of a tile: its page (the one behind the last, which gives zeros, for one outside), or -1
+            const auto page_of = [&](int j) {
+                const int64_t key = key0 + (int64_t)j * kPrefixKeys + lane * box;
+                if (j >= tiles || lane >= boxes || key >= key_end) return -1;
+                const int page = p.prefix_table[key >> p.page_shift];
+                return (uint32_t)page < (uint32_t)p.pages ? page : p.pages;
+            };
+            int ahead = page_of(0), keys = -1, values = -1, n = 0;
+            bool ok = true;
+            for (; n < 2 * tiles; ++n) {
+                const bool is_key = n == 0 || ((n & 1) && (n + 1) / 2 < tiles);
+                const int j = n == 0 ? 0 : is_key ? (n + 1) / 2 : n & 1 ? tiles - 1 : n / 2 - 1, s = n % S::kStages;
+                if (is_key) {
+                    values = keys;
+                    keys = ahead;
+                    ahead = page_of(j + 1);
+                } else if (n == 2 * tiles - 1) {
+                    values = keys;
+                }
+                const int page = is_key ? keys : values;
+                if (n >= S::kStages && !(ok = warp_wait(empty(s), (uint32_t)(n / S::kStages - 1) & 1u, &failed))) break;
+                const uint32_t live = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0));
+                if (lane == 0) mbar_expect_tx(full(s), live * box * 128 * S::kHalves);
+                __syncwarp();
+                if (page >= 0) {
+                    const int slot = (int)((key0 + (int64_t)j * kPrefixKeys + lane * box) & p.page_mask);
+    #pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h)
+                        page_box(ring + s * S::kStage + h * S::kHalf + lane * box * 128, is_key ? &maps.k : &maps.v, h * 64, slot, kv_head, page, full(s));
+                }
+                __syncwarp();
+            }
+            // no copy and no arrival may come after this CTA is gone
+            for (int i = max(0, n - S::kStages); i < n; ++i) {
+                const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
+                if (!warp_wait(empty(i % S::kStages), parity, &failed)) mbar_wait(full(i % S::kStages), parity, kMx4SpinLimit);
+            }
+        } else if (warp == 8) {
+            const uint32_t lead = elect_one();
+            const uint32_t qk = half_instruction(BF16, kPrefixKeys, false), pv = half_instruction(BF16, DIM, true);
+            bool ok = true;
+            const auto arrived = [&](int n) { ok = ok && warp_wait(full(n % S::kStages), (uint32_t)(n / S::kStages) & 1u, &failed); };
+            const auto logits = [&](int g, int j) {
+                const uint32_t q = base + (paired ? g : 0) * S::kStage, k = ring + key_number(j) % S::kStages * S::kStage;
+    #pragma unroll
+                for (int h = 0; h < S::kHalves; ++h)
+    #pragma unroll
+                    for (int i = 0; i < 4; ++i)      // 32 bytes on: two in the descriptors' unit
+                        half_multiply(lead, s_at + g * 128, operand_desc(q + h * S::kHalf) + 2 * i, operand_desc(k + h * S::kHalf) + 2 * i, qk, h + i ? 1u : 0u);
+                tensor_commit(lead, s_full(g));
+            };
+            const auto results = [&](int g, int j, uint32_t add) {
+                const uint32_t v = ring + value_number(j) % S::kStages * S::kStage;
+    #pragma unroll
+                for (int i = 0; i < kPrefixKeys / 16; ++i)      // 16 keys on: two groups of eight rows
+                    half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i ? 1u : add);
+            };
+            // values behind the prefix's last are what the page holds, which may be NaN: rows of zeros instead
+            const auto values = [&](int j) {
+                arrived(value_number(j));
+                const int valid = (int)min((int64_t)kPrefixKeys, key_end - key0 - (int64_t)j * kPrefixKeys);
+                if (ok && valid < kPrefixKeys) {
+                    uint8_t* v = smem + S::kRing + value_number(j) % S::kStages * S::kStage;
+    #pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h)
+                        for (int i = valid * 8 + lane; i < kPrefixKeys * 8; i += 32) *reinterpret_cast<uint4*>(v + h * S::kHalf + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+            };
+            const auto weights = [&](int g, int turn) {
+                ok = ok && warp_wait(p_ready(g), (uint32_t)turn & 1u, &failed);
+                tensor_fence_after();
+            };
+            arrived(0);
+            if (ok) {
+                logits(0, 0);
+                if (paired) logits(1, 0);
+                tensor_commit(lead, empty(0));
+            }
+            if (!paired && tiles > 1) {
+                arrived(key_number(1));
+                if (ok) {
+                    logits(1, 1);
+                    tensor_commit(lead, empty(key_number(1) % S::kStages));
+                }
+            }
+            for (int j = 0; j < tiles && ok; ++j) {
+                values(j);
+                if (paired) {
+                    if (j + 1 < tiles) arrived(key_number(j + 1));
+                    for (int g = 0; g < 2 && ok; ++g) {
+                        weights(g, j);
+                        if (!ok) break;
+                        results(g, j, j ? 1u : 0u);
+                        if (g) tensor_commit(lead, empty(value_number(j) % S::kStages));
+                        if (j + 1 < tiles) {
+                            logits(g, j + 1);
+                            if (g) tensor_commit(lead, empty(key_number(j + 1) % S::kStages));
+                        }
+                    }
+                } else {
+                    weights(j & 1, j >> 1);
+                    if (!ok) break;
+                    results(j & 1, j, j > 1 ? 1u : 0u);
+                    tensor_commit(lead, empty(value_number(j) % S::kStages));
+                    if (j + 2 < tiles) {
+                        arrived(key_number(j + 2));
+                        if (!ok) break;
+                        logits(j & 1, j + 2);
+                        tensor_commit(lead, empty(key_number(j + 2) % S::kStages));
+                    }
+                }
+            }
+            tensor_commit(lead, done);
+            warp_wait(done, 0, &failed);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int g = warp >> 2, row = (x * 2 + (paired ? g : 0)) * kPrefixRows + (warp & 3) * 32 + lane;
+        const bool some = row - lane < rows;         // of the warp's rows are queries
+        const uint32_t mine = (uint32_t)(warp & 3) << 21, s_mine = s_at + g * 128 + mine, o_mine = o_at + g * 128 + mine;
+        const int turns = paired ? tiles : (tiles - g + 1) / 2;
+        float m = -INFINITY;
+        float2 sum = make_float2(0.f, 0.f);
+        bool ok = true;
+        for (int turn = 0; turn < turns; ++turn) {
+            ok = warp_wait(s_full(g), (uint32_t)turn & 1u, &failed);
+            if (!ok) break;
+            tensor_fence_after();
+            if (some) {
+                const int j = paired ? turn : 2 * turn + g;
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ask32(s_mine + c * 32, s[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_arrived(s[c]);
+                const int64_t left = key_end - key0 - (int64_t)j * kPrefixKeys;
+                if (left < kPrefixKeys) {
+#pragma unroll
+                    for (int i = 0; i < kPrefixKeys; ++i) s[i >> 5][i & 31] = i < (int)left ? s[i >> 5][i & 31] : 0xFF800000u;
+                }
+                if (absent) {
+#pragma unroll
+                    for (int b = 0; b < kPrefixKeys / 16; ++b) {
+                        const int64_t key = key0 + (int64_t)j * kPrefixKeys + b * 16;
+                        const bool there = key < key_end && (uint32_t)p.prefix_table[key >> p.page_shift] < (uint32_t)p.pages;
+#pragma unroll
+                        for (int i = b * 16; i < b * 16 + 16; ++i) s[i >> 5][i & 31] = there ? s[i >> 5][i & 31] : 0xFF800000u;
+                    }
+                }
+                float top[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                }
+                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+                if (turn == 0) {
+                    m = high;
+                } else if (__any_sync(0xFFFFFFFFu, high > m + kRescale)) {
+                    const float next = fmaxf(m, high), up = fast_exp2(m - (next == -INFINITY ? 0.f : next));
+                    m = next;
+                    sum.x *= up;
+                    sum.y *= up;
+#pragma unroll
+                    for (int c = 0; c < DIM / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ask32(o_mine + c * 32, o);
+                        tmem_arrived(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
+                        tmem_store32(o_mine + c * 32, o);
+                    }
+                }
+                const float from = m == -INFINITY ? 0.f : m;
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), from2 = make_float2(-from, -from), one2 = make_float2(1.f, 1.f);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = c * 64 + 2 * i;
+                        float2 v = fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), scale2, from2);
+                        v.x = fast_exp2(v.x);
+                        v.y = fast_exp2(v.y);
+                        sum = fma2(v, one2, sum);
+                        w[i] = pack_pair<BF16>(v.x, v.y);
+                    }
+                    tmem_store32(s_mine + c * 32, w);
+                }
+                tmem_stored();
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready(g));
+        }
+        ok = ok && warp_wait(done, 0, &failed);
+        tensor_fence_after();
+        if (ok && some) {
+            const int64_t part = ((int64_t)(paired ? split : 2 * split + g) * p.kv_heads + kv_head) * rows + row;
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) {
+                uint32_t o[32];
+                tmem_ask32(o_mine + c * 32, o);
+                tmem_arrived(o);
+                if (row < rows) {
+                    float4* to = reinterpret_cast<float4*>(p.prefix_o + part * DIM + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        to[i] = turns ? make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]))
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+            if (row < rows) p.prefix_ml[part] = make_float2(m, sum.x + sum.y);
+        }
+    }
+    __syncwarp();
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
+    if (warp == 8) tmem_free<1>(tmem, S::kColumns);
+}
+
+}  // namespace mps

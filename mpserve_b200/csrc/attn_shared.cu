@@ -6,7 +6,7 @@
 // in units of log 2); parts join as
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
 // whatever the keys were split into, so that the prefix is read once for many queries and every sequence's own keys once, each in as many parts as fill the GPU.
-#include "attn.cuh"
+#include "attn_prefix.cuh"
 
 namespace mps {
 
@@ -46,8 +46,8 @@ __device__ __forceinline__ void attend_few(const AttendArgs& p, uint8_t* smem, c
 #pragma unroll
     for (int d = 0; d < DIM / 16; ++d) {
         const uint32_t* at = reinterpret_cast<const uint32_t*>(query + d * 16 + 2 * t);
-        q[d][0] = g < live ? at[0] : 0u;
-        q[d][1] = g < live ? at[4] : 0u;
+        q[d][0] = g < live ? query_pair<BF16>(at[0], p.q_factor) : 0u;
+        q[d][1] = g < live ? query_pair<BF16>(at[4], p.q_factor) : 0u;
     }
     const auto page_of = [&](int block) {      // of the pool, or one that is outside
         return block < blocks ? range.table[(range.first + block * 16) >> p.page_shift] : -1;
@@ -188,20 +188,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_own_kernel(const Att
     attend_few<DIM, BF16>(p, smem, {p.tables + own.sequence * p.table_columns, own.first, own.last}, kv_head, query, live, p.own_o + part * DIM, p.own_ml + part);
 }
 
-// The prefix, eight rows (queries of a key head) at a time.
-template <int DIM, bool BF16>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_prefix_kernel(const AttendArgs p) {
-    extern __shared__ __align__(1024) uint8_t smem[];
-    griddep_wait();
-    griddep_launch();
-    const int rows = p.batch * p.group, row_tiles = (rows + kFewColumns - 1) / kFewColumns;
-    const int tile = blockIdx.x % row_tiles, kv_head = blockIdx.x / row_tiles % p.kv_heads, split = blockIdx.x / row_tiles / p.kv_heads;
-    const int first = tile * kFewColumns, live = min(kFewColumns, rows - first), g = (threadIdx.x & 31) >> 2, row = first + (g < live ? g : 0);
-    const uint16_t* query = p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head;
-    const int64_t part = ((int64_t)split * p.kv_heads + kv_head) * rows + first, begin = (int64_t)split * p.prefix_step;
-    attend_few<DIM, BF16>(p, smem, {p.prefix_table, begin, min(p.prefix, begin + p.prefix_step)}, kv_head, query, live, p.prefix_o + part * DIM, p.prefix_ml + part);
-}
-
 // ---- the parts of a query joined -----------------------------------------------------------------------
 //
 // A CTA has a sequence, a warp a head at a time: its lanes share the parts' weights first, then each has its columns of all parts.
@@ -212,11 +198,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sequence = blockIdx.x;
     const OwnItems own = own_items(p, sequence);
-    const int splits = p.prefix_splits, count = splits + own.count;
-    const int64_t rows = (int64_t)p.batch * p.group;
+    const int64_t rows = (int64_t)p.batch * p.group, twice = (rows + kPrefixRows - 1) / kPrefixRows / 2 * 2 * kPrefixRows;
     constexpr int kColumns = DIM / 32;
     for (int head = warp; head < p.kv_heads * p.group; head += kJoinWarps) {
         const int kv_head = head / p.group, in_group = head % p.group;
+        // rows from `twice` on have two parts of each stretch of the prefix
+        const int splits = (int64_t)sequence * p.group + in_group < twice ? p.prefix_splits : 2 * p.prefix_splits, count = splits + own.count;
         const auto place = [&](int i) {
             return i < splits ? ((int64_t)i * p.kv_heads + kv_head) * rows + (int64_t)sequence * p.group + in_group
                               : ((own.first + i - splits) * p.kv_heads + kv_head) * p.group + in_group;
@@ -257,20 +244,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 // ---- host side -------------------------------------------------------------------------------------------
 
 struct AttendPlan {
-    int64_t prefix_step;          // keys of a part of the prefix
+    int64_t prefix_step;          // keys of a stretch of the prefix
     int prefix_splits;
+    int prefix_parts;             // of a row
+    int wide_tiles;               // CTAs for a stretch and a key head
     int64_t own_items;            // at most
     int64_t floats(int64_t rows, int64_t kv_heads, int64_t group, int64_t dim) const {      // of the scratch
-        return (prefix_splits * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
+        return (prefix_parts * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
     }
 };
 static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
     AttendPlan plan = {};
-    const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group, row_tiles = (rows + kFewColumns - 1) / kFewColumns;
+    const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows;
+    plan.wide_tiles = (int)((row_tiles + 1) / 2);
     if (a.prefix_length > 0) {
-        const int64_t wanted = (2 * sms + row_tiles * a.kv_heads - 1) / (row_tiles * a.kv_heads);
-        plan.prefix_step = ((a.prefix_length + wanted - 1) / wanted + 63) / 64 * 64;
+        // a CTA an SM, as long as there are tiles of keys
+        const int64_t wanted = std::max<int64_t>(1, sms / ((int64_t)plan.wide_tiles * a.kv_heads)), tiles = (a.prefix_length + kPrefixKeys - 1) / kPrefixKeys;
+        plan.prefix_step = (tiles + wanted - 1) / wanted * kPrefixKeys;
         plan.prefix_splits = (int)((a.prefix_length + plan.prefix_step - 1) / plan.prefix_step);
+        plan.prefix_parts = plan.prefix_splits * (row_tiles % 2 ? 2 : 1);
     }
     const int64_t most = a.table_columns * a.page_size;
     if (most > 0) {
@@ -299,19 +291,49 @@ static int check_attend(const mps_prefix_attend& a) {
     return MPS_OK;
 }
 
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+static int page_map(CUtensorMap& map, EncodeTiled encode, const void* pages, const mps_prefix_attend& a, int64_t slot, int64_t head, int64_t page) {
+    const cuuint64_t size[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.page_size, (cuuint64_t)a.kv_heads, (cuuint64_t)a.pages};
+    // of a dimension of one the stride is never used, but may not be 0
+    const auto bytes = [&](int64_t stride) { return (cuuint64_t)(stride ? stride : a.dim) * 2; };
+    const cuuint64_t stride[3] = {bytes(slot), bytes(head), bytes(page)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(a.page_size, (int64_t)kPrefixKeys), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode(&map, a.dtype == MPS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pages), size, stride, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
+}
+static int page_maps(PrefixMaps& maps, const mps_prefix_attend& a) {
+    static std::atomic<EncodeTiled> known{nullptr};
+    EncodeTiled encode = known.load(std::memory_order_relaxed);
+    if (!encode) {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        MPS_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !entry) { set_error("the driver has no cuTensorMapEncodeTiled"); return MPS_ERR_UNSUPPORTED; }
+        encode = reinterpret_cast<EncodeTiled>(entry);
+        known.store(encode, std::memory_order_relaxed);
+    }
+    const int rc = page_map(maps.k, encode, a.k_pages, a, a.k_slot_stride, a.k_head_stride, a.k_page_stride);
+    return rc ? rc : page_map(maps.v, encode, a.v_pages, a, a.v_slot_stride, a.v_head_stride, a.v_page_stride);
+}
+
 template <int DIM, bool BF16>
-static int attend(const AttendArgs& p, int64_t prefix_ctas, int64_t own_ctas, cudaStream_t st) {
+static int attend(const AttendArgs& p, const mps_prefix_attend& a, int64_t prefix_ctas, int64_t own_ctas, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     Device d;
     int rc = current_device(d);
     if (rc) return rc;
     if (!(ready.load(std::memory_order_acquire) >> (d.ordinal & 63) & 1)) {
         MPS_CUDA_TRY(cudaFuncSetAttribute(attend_own_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<DIM>::kSmem));
-        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_prefix_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<DIM>::kSmem));
+        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_prefix_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixShape<DIM>::kSmem));
         ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
     }
     if (prefix_ctas) {
-        rc = launch_overlapping_smem("attend_prefix_kernel", attend_prefix_kernel<DIM, BF16>, (unsigned int)prefix_ctas, dim3(kFewWarps * 32), FewShape<DIM>::kSmem, st, p);
+        PrefixMaps maps;
+        rc = page_maps(maps, a);
+        if (rc) return rc;
+        rc = launch_overlapping_smem("attend_prefix_kernel", attend_prefix_kernel<DIM, BF16>, (unsigned int)prefix_ctas, dim3(kPrefixThreads), PrefixShape<DIM>::kSmem, st, p,
+                                     maps);
         if (rc) return rc;
     }
     if (own_ctas) {
@@ -333,12 +355,14 @@ extern "C" int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args
     return attend_plan(*args, d.sms).floats(args->batch * group, args->kv_heads, group, args->dim) * 4 + 64;
 }
 
-extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* stream) {
+extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
     if (!args) { set_error("mps_prefix_attend_tokens: null arguments"); return MPS_ERR_INVALID; }
-    const mps_prefix_attend& a = *args;
+    mps_prefix_attend a = *args;
     int rc = check_attend(a);
     if (rc) return rc;
     if (a.batch == 0) return MPS_OK;
+    if (a.pages == 0) a.prefix_length = a.table_columns = 0;      // no key is there
     if (!a.q || !a.out || (a.pages && (!a.k_pages || !a.v_pages)) || (a.table_columns && (!a.tables || !a.lengths)) || (a.prefix_length && !a.prefix_table)) {
         set_error("mps_prefix_attend_tokens: missing pointer");
         return MPS_ERR_INVALID;
@@ -362,6 +386,11 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
         set_error("mps_prefix_attend_tokens: scratch missing, unaligned or too small");
         return MPS_ERR_WORKSPACE;
     }
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < mps_mx4_workspace_bytes()) {
+        set_error("mps_prefix_attend_tokens: workspace missing, unaligned or too small");
+        return MPS_ERR_WORKSPACE;
+    }
+    p.workspace = static_cast<uint32_t*>(workspace);
     p.q = static_cast<const uint16_t*>(a.q);
     p.k = static_cast<const uint16_t*>(a.k_pages);
     p.v = static_cast<const uint16_t*>(a.v_pages);
@@ -385,16 +414,18 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     p.batch = (int32_t)a.batch;
     p.kv_heads = a.kv_heads;
     p.group = (int32_t)group;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
-    const int64_t prefix_parts = plan.prefix_splits * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
+    // a negative scale is the queries' sign, one of 0 makes them zeros: what multiplies the logits is positive, and the largest stays the largest
+    p.q_factor = a.scale > 0.f ? 1 : a.scale < 0.f ? -1 : a.scale == 0.f ? 0 : 1;
+    p.scale_log2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
+    const int64_t prefix_parts = plan.prefix_parts * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
     p.prefix_o = static_cast<float*>(scratch);
     p.own_o = p.prefix_o + prefix_parts * a.dim;
     p.prefix_ml = reinterpret_cast<float2*>(p.own_o + own_parts * a.dim);
     p.own_ml = p.prefix_ml + prefix_parts;
-    const int64_t prefix_ctas = plan.prefix_splits * a.kv_heads * ((rows + kFewColumns - 1) / kFewColumns);
+    const int64_t prefix_ctas = (int64_t)plan.prefix_splits * a.kv_heads * plan.wide_tiles;
     const int64_t own_ctas = plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
     if (prefix_ctas > 0x7FFFFFFF || own_ctas > 0x7FFFFFFF) { set_error("mps_prefix_attend_tokens: too much work for one launch"); return MPS_ERR_INVALID; }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, prefix_ctas, own_ctas, st) : attend<64, false>(p, prefix_ctas, own_ctas, st);
-    return a.dtype == MPS_BF16 ? attend<128, true>(p, prefix_ctas, own_ctas, st) : attend<128, false>(p, prefix_ctas, own_ctas, st);
+    if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, a, prefix_ctas, own_ctas, st) : attend<64, false>(p, a, prefix_ctas, own_ctas, st);
+    return a.dtype == MPS_BF16 ? attend<128, true>(p, a, prefix_ctas, own_ctas, st) : attend<128, false>(p, a, prefix_ctas, own_ctas, st);
 }

@@ -9,7 +9,6 @@ namespace mps {
 
 // ---- what the kernels share -------------------------------------------------------------------------
 
-constexpr uint32_t kMx4SpinLimit = 1u << 20;   // a poll lasts 4 us where nothing comes: 4 s in all
 constexpr int kMx4SmemMost = 232448;           // 227 KB
 
 constexpr int64_t kMx4WorkspaceBytes = 256;    // word 0 records a wait that ran out
@@ -44,24 +43,6 @@ __device__ __forceinline__ float act(float g, bool silu) {
 __device__ __forceinline__ float half_value(float v) {
     const float h = __half2float(__float2half_rn(v));
     return isinf(h) ? v : h;
-}
-
-// A wait that gives up when another one has.  CLUSTER: what it waits for comes from another CTA, too.
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-#pragma unroll 1
-    for (uint32_t i = 0; i < kMx4SpinLimit; ++i) {
-        if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 63u && *failed) return false;
-    }
-    *failed = 1u;
-    return false;
-}
-
-// The same for a whole warp: the same answer in every lane.
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    return __all_sync(0xFFFFFFFFu, bar_wait<CLUSTER>(bar, parity, failed));
 }
 
 // ---- few tokens: weights on the accumulator's lanes -------------------------------------------------

@@ -1,8 +1,10 @@
-// The tensor-core side of the MXFP4 products: descriptors, scale copies, block-scaled multiplications and accumulator reads.
+// The tensor-core side of the MXFP4 products and of attention: descriptors, scale copies, multiplications, accumulator reads and bounded waits.
 #pragma once
 
 #include <cuda.h>
 #include <stdint.h>
+
+#include "stream_common.cuh"
 
 namespace mps {
 
@@ -69,6 +71,25 @@ __device__ __forceinline__ void mx4_multiply(uint32_t lead, uint32_t d, uint64_t
             "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
             ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(sfa), "r"(sfb), "r"(add), "r"(lead) : "memory");
 }
+// 16-bit operands of one type, FP32 accumulator of 128 x n: both from shared memory, or the left one from tensor memory, two values a column.
+// `wide_b`: the right operand has its n dimension innermost.
+__device__ __forceinline__ uint32_t half_instruction(bool bf16, uint32_t n, bool wide_b) {
+    return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)wide_b << 16 | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void half_multiply(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instruction), "r"(add), "r"(lead) : "memory");
+}
+__device__ __forceinline__ void half_multiply_kept(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t instruction, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(instruction), "r"(add), "r"(lead) : "memory");
+}
+// Shared-memory operand whose rows of 128 bytes lie along the product's sum: 64 columns to a row, eight rows 1024 bytes, the next 64 columns `next` bytes on.
+__device__ __forceinline__ uint64_t wide_operand_desc(uint32_t smem, uint32_t next) {
+    return (uint64_t)((smem >> 4) & 0x3FFFu) | (uint64_t)(next >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
 // The barrier gets an arrival when everything that lane has issued to the tensor core is done.
 __device__ __forceinline__ void tensor_commit(uint32_t lead, uint32_t bar) {
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.u32 e, %1, 0;\n\t@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
@@ -103,6 +124,26 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+constexpr uint32_t kMx4SpinLimit = 1u << 20;   // a poll lasts 4 us where nothing comes: 4 s in all
+
+// A wait that gives up when another one has.  CLUSTER: what it waits for comes from another CTA, too.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kMx4SpinLimit; ++i) {
+        if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 63u && *failed) return false;
+    }
+    *failed = 1u;
+    return false;
+}
+
+// The same for a whole warp: the same answer in every lane.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+    return __all_sync(0xFFFFFFFFu, bar_wait<CLUSTER>(bar, parity, failed));
+}
+
 // Another CTA's shared memory, at the place that has this address in one's own.
 __device__ __forceinline__ uint32_t peer_address(uint32_t smem, int rank) {
     uint32_t a;
@@ -163,5 +204,35 @@ __device__ __forceinline__ void tmem_load32(uint32_t tmem, float* v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+
+// Thirty-two columns asked for, without a wait; tmem_arrived waits for all that were, and nothing that they are kept in may be used before.
+__device__ __forceinline__ void tmem_ask32(uint32_t tmem, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(tmem) : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+          "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+          "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+          "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+// Thirty-two columns stored, without a wait; tmem_stored waits for all that were.
+__device__ __forceinline__ void tmem_store32(uint32_t tmem, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+          "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(tmem) : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 }  // namespace mps

@@ -50,7 +50,7 @@ def test_errors_come_back_from_the_c_entries(lib):
     bad = _lib.MPS_ERR_INVALID
     linear = lambda *a: lib.mps_int4_product(_lib.INT4_LINEAR.pack(*a), None)  # noqa: E731
     rotate = lambda **kw: lib.mps_head_rotate_rows(_rotate(**kw), None)  # noqa: E731
-    attend = lambda **kw: lib.mps_prefix_attend_tokens(_attend(**kw), None, 0, None)  # noqa: E731
+    attend = lambda **kw: lib.mps_prefix_attend_tokens(_attend(**kw), None, 0, None, 0, None)  # noqa: E731
     for call, text in (
             (lambda: lib.mps_int4_product(None, None), b"null"), (lambda: linear(16, 16, 16, 1, 64, 8, 64, 8, 100, 0, 0, 0), b"group"),
             (lambda: linear(16, 16, 16, 1, 64, 0, 64, 8, 64, 0, 0, 0), b"rows"), (lambda: linear(16, 16, 16, -1, 64, 8, 64, 8, 64, 0, 0, 0), b"tokens"),
@@ -63,7 +63,7 @@ def test_errors_come_back_from_the_c_entries(lib):
             (lambda: rotate(rotated=63), b"even"), (lambda: rotate(dtype=3), b"dtype"), (lambda: rotate(qw=16, weight_dtype=3), b"dtype"), (lambda: rotate(q_heads=1025), b"heads"),
             (lambda: rotate(q=0), b"missing"), (lambda: rotate(positions=0), b"missing"), (lambda: rotate(v=16), b"missing"), (lambda: rotate(slots=16), b"missing"),
             (lambda: rotate(slots=16, v=16, v_out=16, pages=2, page=24), b"power of two"),
-            (lambda: lib.mps_prefix_attend_tokens(None, None, 0, None), b"null"), (lambda: attend(dim=96), b"64 or 128"), (lambda: attend(dtype=2), b"BF16 or F16"),
+            (lambda: lib.mps_prefix_attend_tokens(None, None, 0, None, 0, None), b"null"), (lambda: attend(dim=96), b"64 or 128"), (lambda: attend(dtype=2), b"BF16 or F16"),
             (lambda: attend(page=8), b"power of two"), (lambda: attend(page=48), b"power of two"), (lambda: attend(q_heads=3, kv_heads=2), b"multiple"),
             (lambda: attend(batch=-1), b"batch"), (lambda: attend(prefix_length=(1 << 30) + 1), b"keys"), (lambda: attend(columns=1 << 27), b"keys"),
             (lambda: attend(q=0), b"missing"), (lambda: attend(prefix=0), b"missing"), (lambda: attend(tables=0), b"missing"), (lambda: attend(k=8), b"aligned"),
