@@ -190,55 +190,88 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) attend_own_kernel(const Att
 
 // ---- the parts of a query joined -----------------------------------------------------------------------
 //
-// A CTA has a sequence, a warp a head at a time: its lanes share the parts' weights first, then each has its columns of all parts.
-constexpr int kJoinWarps = 8;
-template <int DIM, bool BF16>
+// A warp has a head of a sequence, its lanes the columns, eight parts at a time under way; with many parts of few heads four warps share them.  (One after the
+// other, a warp to a head, the parts of four sequences behind 1024 took 43 us.)
+constexpr int kJoinWarps = 4, kJoinAhead = 8;
+constexpr int64_t kJoinFewHeads = 1024;
+template <int DIM, bool BF16, int SHARE>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
+    constexpr int kColumns = DIM / 32, kHeads = kJoinWarps / SHARE;
+    __shared__ float ms[kJoinWarps], ls[kJoinWarps], os[SHARE == 1 ? 1 : kJoinWarps][DIM];
     griddep_wait();
     griddep_launch();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sequence = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q_heads = p.kv_heads * p.group, tiles = (q_heads + kHeads - 1) / kHeads;
+    const int sequence = blockIdx.x / tiles, head = blockIdx.x % tiles * kHeads + warp / SHARE, share = warp % SHARE;
     const OwnItems own = own_items(p, sequence);
-    const int64_t rows = (int64_t)p.batch * p.group, twice = (rows + kPrefixRows - 1) / kPrefixRows / 2 * 2 * kPrefixRows;
-    constexpr int kColumns = DIM / 32;
-    for (int head = warp; head < p.kv_heads * p.group; head += kJoinWarps) {
-        const int kv_head = head / p.group, in_group = head % p.group;
-        // rows from `twice` on have two parts of each stretch of the prefix
-        const int splits = (int64_t)sequence * p.group + in_group < twice ? p.prefix_splits : 2 * p.prefix_splits, count = splits + own.count;
-        const auto place = [&](int i) {
-            return i < splits ? ((int64_t)i * p.kv_heads + kv_head) * rows + (int64_t)sequence * p.group + in_group
-                              : ((own.first + i - splits) * p.kv_heads + kv_head) * p.group + in_group;
-        };
-        float top = -INFINITY, sum = 0.f, out[kColumns];
+    if (SHARE == 1 && head >= q_heads) return;
+    const int kv_head = head / p.group, in_group = head % p.group;
+    const int64_t rows = (int64_t)p.batch * p.group, twice = (rows + kPrefixRows - 1) / kPrefixRows / 2 * 2 * kPrefixRows, row = (int64_t)sequence * p.group + in_group;
+    // rows from `twice` on have two parts of each stretch of the prefix
+    const int splits = row < twice ? p.prefix_splits : 2 * p.prefix_splits, count = splits + own.count;
+    const int64_t prefix_step = p.kv_heads * rows, prefix_first = kv_head * rows + row, own_step = (int64_t)p.kv_heads * p.group;
+    const int64_t own_first = (own.first * p.kv_heads + kv_head) * p.group + in_group;
+    float top = -INFINITY, sum = 0.f, out[kColumns];
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
-        for (int first = 0; first < count; first += 32) {
-            const int i = first + lane;
-            const float2 ml = i < count ? (i < splits ? p.prefix_ml : p.own_ml)[place(i)] : make_float2(-INFINITY, 0.f);
-            float high = ml.x;
+    for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
+    for (int first = share; first < count; first += kJoinAhead * SHARE) {
+        float2 ml[kJoinAhead];
+        float o[kJoinAhead][kColumns];
 #pragma unroll
-            for (int x = 16; x; x >>= 1) high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, x));
-            high = fmaxf(high, top);
-            const float base = high == -INFINITY ? 0.f : high, up = exp2f(top - base), weight = exp2f(ml.x - base);
-            top = high;
-            float part = ml.y * weight;
-#pragma unroll
-            for (int x = 16; x; x >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, x);
-            sum = fmaf(sum, up, part);
-#pragma unroll
-            for (int c = 0; c < kColumns; ++c) out[c] *= up;
-            for (int j = 0; j < min(32, count - first); ++j) {
-                const float w = __shfl_sync(0xFFFFFFFFu, weight, j);
-                const float* from = (first + j < splits ? p.prefix_o : p.own_o) + place(first + j) * DIM + lane * kColumns;
-#pragma unroll
-                for (int c = 0; c < kColumns; ++c) out[c] = fmaf(w, from[c], out[c]);
+        for (int j = 0; j < kJoinAhead; ++j) {
+            const int i = first + j * SHARE;
+            const bool prefix = i < splits, there = i < count;
+            const int64_t at = prefix ? prefix_first + i * prefix_step : own_first + (i - splits) * own_step;
+            ml[j] = there ? (prefix ? p.prefix_ml : p.own_ml)[at] : make_float2(-INFINITY, 0.f);
+            const float* from = (prefix ? p.prefix_o : p.own_o) + at * DIM + lane * kColumns;
+            if (kColumns == 4) {
+                const float4 v = there ? *reinterpret_cast<const float4*>(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+                o[j][0] = v.x; o[j][1] = v.y; o[j][kColumns - 2] = v.z; o[j][kColumns - 1] = v.w;
+            } else {
+                const float2 v = there ? *reinterpret_cast<const float2*>(from) : make_float2(0.f, 0.f);
+                o[j][0] = v.x; o[j][1] = v.y;
             }
         }
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query with nothing to attend to gets zeros
-        uint16_t* to = p.out + ((int64_t)sequence * p.kv_heads * p.group + head) * DIM + lane * kColumns;
+        float high = top;
 #pragma unroll
-        for (int c = 0; c < kColumns; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_pair<BF16>(out[c] * inverse, out[c + 1] * inverse);
-        if (p.lse && lane == 0) p.lse[(int64_t)sequence * p.kv_heads * p.group + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        for (int j = 0; j < kJoinAhead; ++j) high = fmaxf(high, ml[j].x);
+        const float base = high == -INFINITY ? 0.f : high, up = exp2f(top - base);
+        top = high;
+        sum *= up;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) out[c] *= up;
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j) {
+            const float w = exp2f(ml[j].x - base);
+            sum = fmaf(ml[j].y, w, sum);
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) out[c] = fmaf(o[j][c], w, out[c]);
+        }
     }
+    if (SHARE > 1) {
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) os[warp][lane * kColumns + c] = out[c];
+        if (lane == 0) { ms[warp] = top; ls[warp] = sum; }
+        __syncthreads();
+        if (share || head >= q_heads) return;
+#pragma unroll
+        for (int w = 1; w < SHARE; ++w) top = fmaxf(top, ms[warp + w]);
+        const float base = top == -INFINITY ? 0.f : top;
+        sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
+#pragma unroll
+        for (int w = 0; w < SHARE; ++w) {
+            const float f = exp2f(ms[warp + w] - base);
+            sum = fmaf(ls[warp + w], f, sum);
+#pragma unroll
+            for (int c = 0; c < kColumns; ++c) out[c] = fmaf(os[SHARE == 1 ? 0 : warp + w][lane * kColumns + c], f, out[c]);
+        }
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // a query with nothing to attend to gets zeros
+    uint16_t* to = p.out + ((int64_t)sequence * q_heads + head) * DIM + lane * kColumns;
+#pragma unroll
+    for (int c = 0; c < kColumns; c += 2) *reinterpret_cast<uint32_t*>(to + c) = pack_pair<BF16>(out[c] * inverse, out[c + 1] * inverse);
+    if (p.lse && lane == 0) p.lse[(int64_t)sequence * q_heads + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ---- host side -------------------------------------------------------------------------------------------
@@ -340,7 +373,10 @@ static int attend(const AttendArgs& p, const mps_prefix_attend& a, int64_t prefi
         rc = launch_overlapping_smem("attend_own_kernel", attend_own_kernel<DIM, BF16>, (unsigned int)own_ctas, dim3(kFewWarps * 32), FewShape<DIM>::kSmem, st, p);
         if (rc) return rc;
     }
-    return launch_overlapping("attend_join_kernel", attend_join_kernel<DIM, BF16>, (unsigned int)p.batch, dim3(kJoinWarps * 32), st, p);
+    const int64_t q_heads = (int64_t)p.kv_heads * p.group;
+    if (a.batch * q_heads <= kJoinFewHeads)
+        return launch_overlapping("attend_join_kernel", attend_join_kernel<DIM, BF16, kJoinWarps>, (unsigned int)(a.batch * q_heads), dim3(kJoinWarps * 32), st, p);
+    return launch_overlapping("attend_join_kernel", attend_join_kernel<DIM, BF16, 1>, (unsigned int)(a.batch * ((q_heads + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), st, p);
 }
 
 }  // namespace mps
