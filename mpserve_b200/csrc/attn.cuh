@@ -25,7 +25,7 @@ struct AttendArgs {
     float2* own_ml;
     int64_t q_token, q_head, k_page, k_slot, k_head, v_page, v_slot, v_head;      // strides
     int64_t table_columns, most_own, prefix, prefix_step, own_items, page_mask;
-    int32_t pages, page_shift, prefix_splits, batch, kv_heads, group;
+    int32_t pages, page_shift, prefix_splits, prefix_units, batch, kv_heads, group;
     int32_t q_factor;                  // 1, -1 or 0: what queries are multiplied by, exactly
     float scale_log2;                  // positive
     uint32_t* workspace;               // word 0 records a wait that ran out
@@ -45,10 +45,10 @@ __device__ __forceinline__ uint32_t query_pair(uint32_t pair, int factor) {
 
 // A sequence's own keys are cut into stretches of a length that is the same for all, such that no more come of it than there are places for: with
 // T keys in all, B sequences and P places, stretches of at least T / (P - B) are at most T / (T / (P - B)) + B.  How long sequences are is known on the
-// GPU only, so every CTA finds its stretch for itself, from the lengths.
-constexpr int64_t kOwnLeast = 128;         // keys of a stretch, at least
+// GPU only, so whoever works on stretches finds them for itself, from the lengths.  Lengths are at most 2^30.
+constexpr int kOwnLeast = 128;         // keys of a stretch, at least
 
-__device__ __forceinline__ int64_t own_length(const AttendArgs& p, int b) { return min(max((int64_t)p.lengths[b], (int64_t)0), p.most_own); }
+__device__ __forceinline__ int own_length(const AttendArgs& p, int b) { return min(max(p.lengths[b], 0), (int)p.most_own); }
 
 __device__ __forceinline__ int64_t warp_total(int64_t v) {
 #pragma unroll
@@ -56,49 +56,51 @@ __device__ __forceinline__ int64_t warp_total(int64_t v) {
     return v;
 }
 // By a whole warp.
-__device__ __forceinline__ int64_t own_step(const AttendArgs& p) {
+__device__ __forceinline__ int own_step(const AttendArgs& p) {
     int64_t total = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) total += own_length(p, b);
     total = warp_total(total);
     const int64_t places = p.own_items - p.batch;
-    return max(kOwnLeast, ((total + places - 1) / places + 63) / 64 * 64);
+    return (int)max((int64_t)kOwnLeast, ((total + places - 1) / places + 63) / 64 * 64);
 }
 
-struct OwnItem { int64_t sequence, first, last; };      // keys first to last - 1; sequence -1: none
-// By a whole warp, the same in every lane.
-__device__ __forceinline__ OwnItem own_item(const AttendArgs& p, int64_t item) {
-    const int lane = threadIdx.x & 31;
-    const int64_t step = own_step(p);
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const int64_t length = b < p.batch ? own_length(p, b) : 0, count = (length + step - 1) / step;
-        int64_t before = count;
+// Stretches in the order of their numbers, by a whole warp: 32 sequences at a time.
+struct OwnFinder {
+    int step, first_sequence, before;      // stretches of the sequences before first_sequence
+    int sequence, first, last;             // what was found: keys first to last - 1; sequence -1: none
+    __device__ __forceinline__ void find(const AttendArgs& p, int item) {
+        const int lane = threadIdx.x & 31;
+        for (; first_sequence < p.batch; first_sequence += 32) {
+            const int b = first_sequence + lane, length = b < p.batch ? own_length(p, b) : 0, count = (length + step - 1) / step;
+            int behind = count;
 #pragma unroll
-        for (int x = 1; x < 32; x *= 2) {
-            const int64_t v = __shfl_up_sync(0xFFFFFFFFu, before, x);
-            if (lane >= x) before += v;
+            for (int x = 1; x < 32; x *= 2) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, behind, x);
+                if (lane >= x) behind += v;
+            }
+            const int all = __shfl_sync(0xFFFFFFFFu, behind, 31), number = item - before - (behind - count);
+            const uint32_t here = __ballot_sync(0xFFFFFFFFu, number >= 0 && number < count);
+            if (here) {
+                const int from = __ffs(here) - 1;
+                sequence = first_sequence + from;
+                first = __shfl_sync(0xFFFFFFFFu, number, from) * step;
+                last = min(first + step, __shfl_sync(0xFFFFFFFFu, length, from));
+                return;
+            }
+            before += all;
         }
-        const int64_t all = __shfl_sync(0xFFFFFFFFu, before, 31);
-        before -= count;
-        const uint32_t here = __ballot_sync(0xFFFFFFFFu, item >= before && item < before + count);
-        if (here) {
-            const int from = __ffs(here) - 1;
-            const int64_t first = __shfl_sync(0xFFFFFFFFu, (item - before) * step, from), end = __shfl_sync(0xFFFFFFFFu, length, from);
-            return {b0 + from, first, min(first + step, end)};
-        }
-        item -= all;
+        sequence = -1;
     }
-    return {-1, 0, 0};
-}
+};
 
-struct OwnItems { int64_t first; int count; };
+struct OwnItems { int first, count; };
 // The stretches of a sequence, by a whole warp.
 __device__ __forceinline__ OwnItems own_items(const AttendArgs& p, int sequence) {
     if (p.own_items == 0) return {0, 0};
-    const int64_t step = own_step(p);
+    const int step = own_step(p);
     int64_t before = 0;
     for (int b = threadIdx.x & 31; b < sequence; b += 32) before += (own_length(p, b) + step - 1) / step;
-    return {warp_total(before), (int)((own_length(p, sequence) + step - 1) / step)};
+    return {(int)warp_total(before), (own_length(p, sequence) + step - 1) / step};
 }
 
 // A launch with dynamic shared memory that may overlap the end of the kernel before it.

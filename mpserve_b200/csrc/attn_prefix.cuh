@@ -16,21 +16,22 @@
 
 #include <cuda.h>
 
-#include "attn.cuh"
+#include "attn_own.cuh"
 #include "mx4_tensor.cuh"
 
 namespace mps {
 
-constexpr int kPrefixKeys = 128, kPrefixRows = 128, kPrefixThreads = 384;      // the last two warps have nothing to do but to complete a group of four
+constexpr int kPrefixKeys = 128, kPrefixRows = 128, kPrefixThreads = 512;
 constexpr float kRescale = 8.f;      // in powers of two
 
 template <int DIM>
 struct PrefixShape {
     static constexpr int kHalf = kPrefixKeys * 128, kHalves = DIM / 64;      // 64 columns of a tile, rows of 128 bytes
-    static constexpr int kStage = kHalves * kHalf, kStages = DIM == 128 ? 5 : 8;
+    static constexpr int kStage = kHalves * kHalf, kStages = DIM == 128 ? 3 : 6;
     static constexpr int kRing = 2 * kStage;                                  // behind two tiles of queries
-    static constexpr int kBars = kRing + kStages * kStage;
-    static constexpr int kSmem = kBars + (2 * kStages + 5) * 8 + 16;
+    static constexpr int kOwn = kRing + kStages * kStage;                     // the rings of those who have the sequences' own keys
+    static constexpr int kBars = kOwn + FewShape<DIM>::kSmem;
+    static constexpr int kSmem = kBars + (2 * kStages + 7) * 8 + 16;
     static constexpr int kColumns = 512;                                      // S, S, O, O
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -48,8 +49,26 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return r;
 }
 
+// The largest of three; NaN where there is one.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// Logits of 32 keys from `key` on: minus infinity for keys behind the stretch's last, and for those of pages outside the cache.
+__device__ __forceinline__ void leave_gaps(const AttendArgs& p, int key, int key_end, uint32_t (&v)[32]) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int first = key + b * 16;
+        const int keys = first < key_end && (uint32_t)p.prefix_table[first >> p.page_shift] < (uint32_t)p.pages ? min(key_end - first, 16) : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[b * 16 + i] = i < keys ? v[b * 16 + i] : 0xFF800000u;
+    }
+}
+
+// Warps: 0 to 3 and 4 to 7 a group's rows, 8 multiplies, 9 copies (10 and 11 complete a group of four), 12 to 15 the sequences' own keys.
 template <int DIM, bool BF16>
-__global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const AttendArgs p, const __grid_constant__ PrefixMaps maps) {
+__global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendArgs p, const __grid_constant__ PrefixMaps maps) {
     using S = PrefixShape<DIM>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -60,47 +79,31 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
     const auto full = [&](int s) { return bar0 + 8u * s; };
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
     const auto s_full = [&](int g) { return bar0 + 8u * (2 * S::kStages + g); };
-    const auto p_ready = [&](int g) { return bar0 + 8u * (2 * S::kStages + 2 + g); };
-    const uint32_t done = bar0 + 8u * (2 * S::kStages + 4);
+    const auto p_ready = [&](int g, int half) { return bar0 + 8u * (2 * S::kStages + 2 + 2 * g + half); };      // of 64 keys
+    const uint32_t done = bar0 + 8u * (2 * S::kStages + 6);
+    const bool some_prefix = blockIdx.x < p.prefix_units;
 
     const int rows = p.batch * p.group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows, pairs = row_tiles / 2, wide_tiles = (row_tiles + 1) / 2;
     const int x = blockIdx.x % wide_tiles, kv_head = blockIdx.x / wide_tiles % p.kv_heads, split = blockIdx.x / wide_tiles / p.kv_heads;
     const bool paired = x < pairs;             // else the groups take the keys in turn
-    const int64_t key0 = (int64_t)split * p.prefix_step, key_end = min(p.prefix, key0 + p.prefix_step);
-    const int tiles = (int)((key_end - key0 + kPrefixKeys - 1) / kPrefixKeys);
+    const int key0 = split * (int)p.prefix_step, key_end = min((int)p.prefix, key0 + (int)p.prefix_step);      // at most 2^30
+    const int tiles = (key_end - key0 + kPrefixKeys - 1) / kPrefixKeys;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g), 4); }
+        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g, 0), 4); mbar_init(p_ready(g, 1), 4); }
         mbar_init(done, 1);
         failed = 0u;
         absent = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
-    if (warp == 9 && lane == 0) { prefetch_map(&maps.k); prefetch_map(&maps.v); }
-    __syncthreads();
-    griddep_wait();
-    griddep_launch();
-
-    // the queries, as the tensor cores read them: 16-byte pieces XORed with the row
-    for (int i = threadIdx.x; i < (paired ? 2 : 1) * kPrefixRows * (DIM / 8); i += kPrefixThreads) {
-        const int r = i / (DIM / 8), piece = i % (DIM / 8), row = x * 2 * kPrefixRows + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head + piece * 8);
-        v = make_uint4(query_pair<BF16>(v.x, p.q_factor), query_pair<BF16>(v.y, p.q_factor), query_pair<BF16>(v.z, p.q_factor), query_pair<BF16>(v.w, p.q_factor));
-        const int in_tile = r % kPrefixRows;
-        *reinterpret_cast<uint4*>(smem + r / kPrefixRows * S::kStage + piece / 8 * S::kHalf + in_tile * 128 + (((piece & 7) ^ (in_tile & 7)) << 4)) = v;
-    }
-    {
-        const int64_t first = key0 >> p.page_shift, last = (key_end - 1) >> p.page_shift;
-        for (int64_t i = first + threadIdx.x; i <= last; i += kPrefixThreads)
-            if ((uint32_t)p.prefix_table[i] >= (uint32_t)p.pages) absent = 1u;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written here
+    if (warp == 8 && some_prefix) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    if (warp == 9 && lane == 0 && some_prefix) { prefetch_map(&maps.k); prefetch_map(&maps.v); }
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
+    griddep_wait();
+    griddep_launch();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
     const uint32_t s_at = tmem, o_at = tmem + 256;      // and 128 columns on for the second group
 
@@ -108,14 +111,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
     const auto key_number = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
     const auto value_number = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
 
-    // a row's 128 logits want more registers than a 384th of them: the four warps that copy and multiply give up theirs (256 x 208 + 128 x 88 = 384 x 168)
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 9) {
+    // What the softmax warps and the multiplying one wait for: the queries in shared memory, and whether pages are absent.
+    const auto prepared = [&]() { asm volatile("bar.sync 1, 288;" ::: "memory"); };
+
+    // a row's 128 logits want more registers than a 512th of them: the four warps that copy and multiply give up theirs (256 x 160 + 128 x 64 + 128 x 128 = 512 x 128)
+    if (warp >= 12) {
+        if (p.own_items) attend_own<DIM, BF16>(p, base + S::kOwn + (warp - 12) * FewShape<DIM>::kRing, blockIdx.x * kFewWarps + warp - 12, gridDim.x * kFewWarps);
+    } else if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 9 && some_prefix) {
             const int box = (int)min(p.page_mask + 1, (int64_t)kPrefixKeys), boxes = kPrefixKeys / box;
             // this lane's box of a tile: its page (the one behind the last, which gives zeros, for one outside), or -1
             const auto page_of = [&](int j) {
-                const int64_t key = key0 + (int64_t)j * kPrefixKeys + lane * box;
+                const int key = key0 + j * kPrefixKeys + lane * box;
                 if (j >= tiles || lane >= boxes || key >= key_end) return -1;
                 const int page = p.prefix_table[key >> p.page_shift];
                 return (uint32_t)page < (uint32_t)p.pages ? page : p.pages;
@@ -138,8 +146,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
                 if (lane == 0) mbar_expect_tx(full(s), live * box * 128 * S::kHalves);
                 __syncwarp();
                 if (page >= 0) {
-                    const int slot = (int)((key0 + (int64_t)j * kPrefixKeys + lane * box) & p.page_mask);
-    #pragma unroll
+                    const int slot = (key0 + j * kPrefixKeys + lane * box) & (int)p.page_mask;
+#pragma unroll
                     for (int h = 0; h < S::kHalves; ++h)
                         page_box(ring + s * S::kStage + h * S::kHalf + lane * box * 128, is_key ? &maps.k : &maps.v, h * 64, slot, kv_head, page, full(s));
                 }
@@ -150,42 +158,47 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
                 const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
                 if (!warp_wait(empty(i % S::kStages), parity, &failed)) mbar_wait(full(i % S::kStages), parity, kMx4SpinLimit);
             }
-        } else if (warp == 8) {
+        } else if (warp == 8 && some_prefix) {
+            prepared();
+            tensor_fence_after();
             const uint32_t lead = elect_one();
             const uint32_t qk = half_instruction(BF16, kPrefixKeys, false), pv = half_instruction(BF16, DIM, true);
             bool ok = true;
             const auto arrived = [&](int n) { ok = ok && warp_wait(full(n % S::kStages), (uint32_t)(n / S::kStages) & 1u, &failed); };
             const auto logits = [&](int g, int j) {
                 const uint32_t q = base + (paired ? g : 0) * S::kStage, k = ring + key_number(j) % S::kStages * S::kStage;
-    #pragma unroll
+#pragma unroll
                 for (int h = 0; h < S::kHalves; ++h)
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < 4; ++i)      // 32 bytes on: two in the descriptors' unit
                         half_multiply(lead, s_at + g * 128, operand_desc(q + h * S::kHalf) + 2 * i, operand_desc(k + h * S::kHalf) + 2 * i, qk, h + i ? 1u : 0u);
                 tensor_commit(lead, s_full(g));
             };
-            const auto results = [&](int g, int j, uint32_t add) {
+            // half by half, as the weights come
+            const auto results = [&](int g, int j, int turn) {
                 const uint32_t v = ring + value_number(j) % S::kStages * S::kStage;
-    #pragma unroll
-                for (int i = 0; i < kPrefixKeys / 16; ++i)      // 16 keys on: two groups of eight rows
-                    half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i ? 1u : add);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && warp_wait(p_ready(g, half), (uint32_t)turn & 1u, &failed);
+                    if (!ok) return;
+                    tensor_fence_after();
+#pragma unroll
+                    for (int i = half * 4; i < half * 4 + 4; ++i)      // 16 keys on: two groups of eight rows
+                        half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i || turn ? 1u : 0u);
+                }
             };
             // values behind the prefix's last are what the page holds, which may be NaN: rows of zeros instead
             const auto values = [&](int j) {
                 arrived(value_number(j));
-                const int valid = (int)min((int64_t)kPrefixKeys, key_end - key0 - (int64_t)j * kPrefixKeys);
+                const int valid = min(kPrefixKeys, key_end - key0 - j * kPrefixKeys);
                 if (ok && valid < kPrefixKeys) {
                     uint8_t* v = smem + S::kRing + value_number(j) % S::kStages * S::kStage;
-    #pragma unroll
+#pragma unroll
                     for (int h = 0; h < S::kHalves; ++h)
                         for (int i = valid * 8 + lane; i < kPrefixKeys * 8; i += 32) *reinterpret_cast<uint4*>(v + h * S::kHalf + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-            };
-            const auto weights = [&](int g, int turn) {
-                ok = ok && warp_wait(p_ready(g), (uint32_t)turn & 1u, &failed);
-                tensor_fence_after();
             };
             arrived(0);
             if (ok) {
@@ -205,9 +218,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
                 if (paired) {
                     if (j + 1 < tiles) arrived(key_number(j + 1));
                     for (int g = 0; g < 2 && ok; ++g) {
-                        weights(g, j);
+                        results(g, j, j);
                         if (!ok) break;
-                        results(g, j, j ? 1u : 0u);
                         if (g) tensor_commit(lead, empty(value_number(j) % S::kStages));
                         if (j + 1 < tiles) {
                             logits(g, j + 1);
@@ -215,9 +227,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
                         }
                     }
                 } else {
-                    weights(j & 1, j >> 1);
+                    results(j & 1, j, j >> 1);
                     if (!ok) break;
-                    results(j & 1, j, j > 1 ? 1u : 0u);
                     tensor_commit(lead, empty(value_number(j) % S::kStages));
                     if (j + 2 < tiles) {
                         arrived(key_number(j + 2));
@@ -231,7 +242,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
             warp_wait(done, 0, &failed);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        if (some_prefix) {
+        // the queries, as the tensor cores read them: 16-byte pieces XORed with the row; eight at a time under way
+        constexpr int kAhead = DIM / 16;      // pieces of a row by 256 threads
+        for (int tile = 0; tile < (paired ? 2 : 1); ++tile) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int r = (i * 256 + threadIdx.x) / (DIM / 8), piece = threadIdx.x % (DIM / 8), row = (x * 2 + tile) * kPrefixRows + r;
+                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (row < rows) v[i] = *reinterpret_cast<const uint4*>(p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head + piece * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int r = (i * 256 + threadIdx.x) / (DIM / 8), piece = threadIdx.x % (DIM / 8);
+                *reinterpret_cast<uint4*>(smem + tile * S::kStage + piece / 8 * S::kHalf + r * 128 + (((piece & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(query_pair<BF16>(v[i].x, p.q_factor), query_pair<BF16>(v[i].y, p.q_factor), query_pair<BF16>(v[i].z, p.q_factor),
+                               query_pair<BF16>(v[i].w, p.q_factor));
+            }
+        }
+        {
+            const int first = key0 >> p.page_shift, last = (key_end - 1) >> p.page_shift;
+            for (int i = first + threadIdx.x; i <= last; i += 256)
+                if ((uint32_t)p.prefix_table[i] >= (uint32_t)p.pages) absent = 1u;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written here
+        prepared();
         const int g = warp >> 2, row = (x * 2 + (paired ? g : 0)) * kPrefixRows + (warp & 3) * 32 + lane;
         const bool some = row - lane < rows;         // of the warp's rows are queries
         const uint32_t mine = (uint32_t)(warp & 3) << 21, s_mine = s_at + g * 128 + mine, o_mine = o_at + g * 128 + mine;
@@ -244,42 +281,41 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
             if (!ok) break;
             tensor_fence_after();
             if (some) {
+                // The logits are read twice, 32 columns at a time and the next ones on their way: for the largest, and to be replaced by the weights.
                 const int j = paired ? turn : 2 * turn + g;
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ask32(s_mine + c * 32, s[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_arrived(s[c]);
-                const int64_t left = key_end - key0 - (int64_t)j * kPrefixKeys;
-                if (left < kPrefixKeys) {
-#pragma unroll
-                    for (int i = 0; i < kPrefixKeys; ++i) s[i >> 5][i & 31] = i < (int)left ? s[i >> 5][i & 31] : 0xFF800000u;
-                }
-                if (absent) {
-#pragma unroll
-                    for (int b = 0; b < kPrefixKeys / 16; ++b) {
-                        const int64_t key = key0 + (int64_t)j * kPrefixKeys + b * 16;
-                        const bool there = key < key_end && (uint32_t)p.prefix_table[key >> p.page_shift] < (uint32_t)p.pages;
-#pragma unroll
-                        for (int i = b * 16; i < b * 16 + 16; ++i) s[i >> 5][i & 31] = there ? s[i >> 5][i & 31] : 0xFF800000u;
-                    }
-                }
+                const int left = key_end - key0 - j * kPrefixKeys;
+                const bool gaps = left < kPrefixKeys || absent;
+                uint32_t s[2][32];
+                tmem_ask32(s_mine, s[0]);
                 float top[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    top[c] = __uint_as_float(s[c][0]);
+                    uint32_t(&v)[32] = s[c & 1];
+                    tmem_arrived(v);
+                    tmem_ask32(s_mine + (c + 1) % 4 * 32, s[(c + 1) & 1]);
+                    if (gaps) leave_gaps(p, key0 + j * kPrefixKeys + c * 32, key_end, v);
+                    if (c == 0) {
 #pragma unroll
-                    for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(v[i]);
+                    }
+#pragma unroll
+                    for (int i = c ? 0 : 4; i < 32; i += 8) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (i + k + 4 < 32) top[k] = max3(top[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + k + 4]));
+                            else top[k] = max3(top[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + k]));
+                    }
                 }
-                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+                const float high = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
                 if (turn == 0) {
                     m = high;
-                } else if (__any_sync(0xFFFFFFFFu, high > m + kRescale)) {
-                    const float next = fmaxf(m, high), up = fast_exp2(m - (next == -INFINITY ? 0.f : next));
+                } else if (__any_sync(0xFFFFFFFFu, !(high <= m + kRescale))) {
+                    const float next = max3(m, high, high), up = fast_exp2(m - (next == -INFINITY ? 0.f : next));
                     m = next;
                     sum.x *= up;
                     sum.y *= up;
-#pragma unroll
+                    tmem_arrived(s[0]);
+#pragma unroll 1
                     for (int c = 0; c < DIM / 32; ++c) {
                         uint32_t o[32];
                         tmem_ask32(o_mine + c * 32, o);
@@ -292,43 +328,64 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
                 const float from = m == -INFINITY ? 0.f : m;
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), from2 = make_float2(-from, -from), one2 = make_float2(1.f, 1.f);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int half = 0; half < 2; ++half) {
                     uint32_t w[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int at = c * 64 + 2 * i;
-                        float2 v = fma2(make_float2(__uint_as_float(s[at >> 5][at & 31]), __uint_as_float(s[at >> 5][(at & 31) + 1])), scale2, from2);
-                        v.x = fast_exp2(v.x);
-                        v.y = fast_exp2(v.y);
-                        sum = fma2(v, one2, sum);
-                        w[i] = pack_pair<BF16>(v.x, v.y);
+                    for (int part = 0; part < 2; ++part) {
+                        const int c = half * 2 + part;
+                        uint32_t(&v)[32] = s[c & 1];
+                        tmem_arrived(v);
+                        if (c < 3) tmem_ask32(s_mine + (c + 1) * 32, s[(c + 1) & 1]);
+                        if (gaps) leave_gaps(p, key0 + j * kPrefixKeys + c * 32, key_end, v);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, from2);
+                            e.x = fast_exp2(e.x);
+                            e.y = fast_exp2(e.y);
+                            sum = fma2(e, one2, sum);
+                            w[part * 16 + i] = pack_pair<BF16>(e.x, e.y);
+                        }
                     }
-                    tmem_store32(s_mine + c * 32, w);
+                    tmem_store32(s_mine + half * 32, w);
+                    tmem_stored();
+                    tensor_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready(g, half));
                 }
-                tmem_stored();
+            } else if (lane == 0) {
+                mbar_arrive(p_ready(g, 0));
+                mbar_arrive(p_ready(g, 1));
             }
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready(g));
         }
         ok = ok && warp_wait(done, 0, &failed);
         tensor_fence_after();
         if (ok && some) {
             const int64_t part = ((int64_t)(paired ? split : 2 * split + g) * p.kv_heads + kv_head) * rows + row;
+            // by way of the ring, whose tiles have been multiplied: straight from the registers every store would touch 32 rows
+            const uint32_t rows_at = ring + warp * (32 * 128);      // 32 rows of 32 columns, pieces XORed with the row
+            const int64_t first_part = part - lane;
 #pragma unroll
             for (int c = 0; c < DIM / 32; ++c) {
                 uint32_t o[32];
                 tmem_ask32(o_mine + c * 32, o);
                 tmem_arrived(o);
-                if (row < rows) {
-                    float4* to = reinterpret_cast<float4*>(p.prefix_o + part * DIM + c * 32);
+                __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        to[i] = turns ? make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]))
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rows_at + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(turns ? o[4 * i] : 0u),
+                                 "r"(turns ? o[4 * i + 1] : 0u), "r"(turns ? o[4 * i + 2] : 0u), "r"(turns ? o[4 * i + 3] : 0u) : "memory");
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 4 + (lane >> 3), piece = lane & 7;
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(rows_at + r * 128 + ((piece ^ (r & 7)) << 4)) : "memory");
+                    if (row - lane + r < rows) *reinterpret_cast<uint4*>(p.prefix_o + (first_part + r) * DIM + c * 32 + piece * 4) = v;
                 }
             }
             if (row < rows) p.prefix_ml[part] = make_float2(m, sum.x + sum.y);
+        }
         }
     }
     __syncwarp();
@@ -336,7 +393,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_prefix_kernel(const 
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
-    if (warp == 8) tmem_free<1>(tmem, S::kColumns);
+    if (warp == 8 && some_prefix) tmem_free<1>(tmem, S::kColumns);
 }
 
 }  // namespace mps

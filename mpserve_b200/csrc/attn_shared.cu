@@ -10,184 +10,6 @@
 
 namespace mps {
 
-// ---- own tokens: keys on the rows of the products ------------------------------------------------------
-//
-// A CTA has a stretch of one sequence's keys for one key head; its four warps take blocks of 16 keys in turn, each through a ring of its own that
-// nobody else waits for.  Logits are computed as K q^T, 16 keys by 8 query heads, and the result as V^T P^T, so that the eight columns are the query
-// heads that share the key head, and none of the tensor cores' rows idles.  Bound: memory; four warps with two blocks of 16 keys on their way, and two
-// such CTAs on an SM, have 128 KB under way.
-constexpr int kFewWarps = 4, kFewStages = 3, kFewColumns = 8;
-
-template <int DIM>
-struct FewShape {
-    static constexpr int kRow = DIM * 2, kBlock = 16 * kRow, kStage = 2 * kBlock;      // 16 keys, then their values
-    static constexpr int kRing = kFewStages * kStage;
-    static constexpr int kSmem = kFewWarps * kRing;
-    static_assert(kRing >= kFewColumns * DIM * 4, "a warp's result takes its ring's place");
-};
-
-// 16-byte piece `piece` of row `row`: rows of 256 (128) bytes, pieces XORed with the row, so that eight rows' pieces lie in different banks.
-template <int DIM>
-__device__ __forceinline__ uint32_t few_place(int row, int piece) { return row * (DIM * 2) + ((piece ^ (row & 7)) << 4); }
-
-struct KeyRange { const int32_t* table; int64_t first, last; };      // keys first to last - 1 of a table
-
-// Columns: `base` + column heads of query pointers; `live` of them.
-template <int DIM, bool BF16>
-__device__ __forceinline__ void attend_few(const AttendArgs& p, uint8_t* smem, const KeyRange range, int kv_head, const uint16_t* query, int live, float* part_o,
-                                           float2* part_ml) {
-    using S = FewShape<DIM>;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * S::kRing;
-    const int blocks = (int)((range.last - range.first + 15) >> 4);
-    constexpr int kPieces = DIM / 8;       // of a row
-
-    uint32_t q[DIM / 16][2];
-#pragma unroll
-    for (int d = 0; d < DIM / 16; ++d) {
-        const uint32_t* at = reinterpret_cast<const uint32_t*>(query + d * 16 + 2 * t);
-        q[d][0] = g < live ? query_pair<BF16>(at[0], p.q_factor) : 0u;
-        q[d][1] = g < live ? query_pair<BF16>(at[4], p.q_factor) : 0u;
-    }
-    const auto page_of = [&](int block) {      // of the pool, or one that is outside
-        return block < blocks ? range.table[(range.first + block * 16) >> p.page_shift] : -1;
-    };
-    // keys of the block that are there
-    const auto present = [&](int block, int page) {
-        return block < blocks && (uint32_t)page < (uint32_t)p.pages ? (int)min((int64_t)16, range.last - range.first - block * 16) : 0;
-    };
-    const auto load = [&](int block, int page, int stage) {
-        const int keys = present(block, page);
-        const int64_t slot = (range.first + block * 16) & p.page_mask;
-        const uint16_t* k = p.k + (keys ? (int64_t)page * p.k_page + slot * p.k_slot + (int64_t)kv_head * p.k_head : 0);
-        const uint16_t* v = p.v + (keys ? (int64_t)page * p.v_page + slot * p.v_slot + (int64_t)kv_head * p.v_head : 0);
-        const uint32_t to = ring + stage * S::kStage;
-#pragma unroll
-        for (int i = 0; i < kPieces / 2; ++i) {
-            const int row = i * (32 / kPieces) + lane / kPieces, piece = lane % kPieces;
-            const bool there = row < keys;      // others become zeros: a value that is not there must not be a NaN, which 0 does not multiply away
-            cp_async_16_or_zero(to + few_place<DIM>(row, piece), k + (there ? row * p.k_slot + piece * 8 : 0), there);
-            cp_async_16_or_zero(to + S::kBlock + few_place<DIM>(row, piece), v + (there ? row * p.v_slot + piece * 8 : 0), there);
-        }
-    };
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DIM / 16][4];
-#pragma unroll
-    for (int d = 0; d < DIM / 16; ++d) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f; }
-
-    int pages[kFewStages];      // of the blocks in the ring
-#pragma unroll
-    for (int s = 0; s < kFewStages - 1; ++s) {
-        pages[s] = page_of(warp + s * kFewWarps);
-        if (warp + s * kFewWarps < blocks) load(warp + s * kFewWarps, pages[s], s);
-        cp_async_commit();
-    }
-    int ahead = page_of(warp + (kFewStages - 1) * kFewWarps), stage = 0;
-    for (int b = warp; b < blocks; b += kFewWarps) {
-        const int next = b + (kFewStages - 1) * kFewWarps;
-        pages[kFewStages - 1] = ahead;
-        if (next < blocks) load(next, ahead, stage == 0 ? kFewStages - 1 : stage - 1);
-        cp_async_commit();
-        ahead = page_of(next + kFewWarps);
-        cp_async_wait<kFewStages - 1>();
-        __syncwarp();
-        const uint32_t at = ring + stage * S::kStage;
-        const int keys = present(b, pages[0]);
-        // K q^T
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = 0; d < DIM / 16; ++d) {
-            uint32_t a[4];
-            load_matrices(a, at + few_place<DIM>(lane & 15, 2 * d + (lane >> 4)));
-            multiply<BF16>(s, a, q[d][0], q[d][1]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = g + 8 * (i >> 1) < keys ? s[i] * p.scale_log2 : -INFINITY;
-        float up[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float top = fmaxf(s[i], s[i + 2]);
-#pragma unroll
-            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-            top = fmaxf(top, m[i]);
-            const float base = top == -INFINITY ? 0.f : top;
-            up[i] = exp2f(m[i] - base);
-            m[i] = top;
-            s[i] = exp2f(s[i] - base);
-            s[i + 2] = exp2f(s[i + 2] - base);
-            l[i] = fmaf(l[i], up[i], s[i] + s[i + 2]);
-        }
-        const uint32_t p0 = transpose8(pack_pair<BF16>(s[0], s[1])), p1 = transpose8(pack_pair<BF16>(s[2], s[3]));
-        // V^T P^T
-#pragma unroll
-        for (int d = 0; d < DIM / 16; ++d) {
-            uint32_t a[4];
-            load_matrices_transposed(a, at + S::kBlock + few_place<DIM>((lane & 7) + ((lane >> 4) << 3), 2 * d + ((lane >> 3) & 1)));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] *= up[i & 1];
-            multiply<BF16>(o[d], a, p0, p1);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i + 1 < kFewStages; ++i) pages[i] = pages[i + 1];
-        if (++stage == kFewStages) stage = 0;
-    }
-    cp_async_wait<0>();
-    __shared__ float ms[kFewWarps][kFewColumns], ls[kFewWarps][kFewColumns];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int x = 4; x < 32; x *= 2) l[i] += __shfl_xor_sync(0xFFFFFFFFu, l[i], x);
-        if (g == 0) { ms[warp][2 * t + i] = m[i]; ls[warp][2 * t + i] = l[i]; }
-    }
-    __syncthreads();
-    // the four warps' results, each in its own ring, by columns
-    float* own = reinterpret_cast<float*>(smem + warp * S::kRing);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int c = 2 * t + i;
-        float top = ms[0][c];
-#pragma unroll
-        for (int w = 1; w < kFewWarps; ++w) top = fmaxf(top, ms[w][c]);
-        const float f = exp2f(m[i] - (top == -INFINITY ? 0.f : top));      // 0 for a warp that had nothing; a NaN stays one
-#pragma unroll
-        for (int d = 0; d < DIM / 16; ++d) {
-            own[c * DIM + d * 16 + g] = o[d][i] * f;
-            own[c * DIM + d * 16 + g + 8] = o[d][i + 2] * f;
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < live * DIM; i += kFewWarps * 32) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) v += reinterpret_cast<const float*>(smem + w * S::kRing)[i];
-        part_o[i] = v;
-    }
-    if (threadIdx.x < live) {
-        const int c = threadIdx.x;
-        float top = ms[0][c], sum = 0.f;
-#pragma unroll
-        for (int w = 1; w < kFewWarps; ++w) top = fmaxf(top, ms[w][c]);
-#pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) sum = fmaf(ls[w][c], exp2f(ms[w][c] - (top == -INFINITY ? 0.f : top)), sum);
-        part_ml[c] = make_float2(top, sum);
-    }
-}
-
-template <int DIM, bool BF16>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) attend_own_kernel(const AttendArgs p) {
-    extern __shared__ __align__(1024) uint8_t smem[];
-    griddep_wait();
-    griddep_launch();
-    const int column_tiles = (p.group + kFewColumns - 1) / kFewColumns;
-    const int kv_head = blockIdx.x % p.kv_heads, columns = blockIdx.x / p.kv_heads % column_tiles, item = blockIdx.x / p.kv_heads / column_tiles;
-    const OwnItem own = own_item(p, item);
-    if (own.sequence < 0) return;
-    const int first = columns * kFewColumns, live = min(kFewColumns, p.group - first), g = (threadIdx.x & 31) >> 2;
-    const uint16_t* query = p.q + own.sequence * p.q_token + (int64_t)(kv_head * p.group + first + (g < live ? g : 0)) * p.q_head;
-    const int64_t part = ((int64_t)item * p.kv_heads + kv_head) * p.group + first;
-    attend_few<DIM, BF16>(p, smem, {p.tables + own.sequence * p.table_columns, own.first, own.last}, kv_head, query, live, p.own_o + part * DIM, p.own_ml + part);
-}
-
 // ---- the parts of a query joined -----------------------------------------------------------------------
 //
 // A warp has a head of a sequence, its lanes the columns, eight parts at a time under way; with many parts of few heads four warps share them.  (One after the
@@ -209,7 +31,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     // rows from `twice` on have two parts of each stretch of the prefix
     const int splits = row < twice ? p.prefix_splits : 2 * p.prefix_splits, count = splits + own.count;
     const int64_t prefix_step = p.kv_heads * rows, prefix_first = kv_head * rows + row, own_step = (int64_t)p.kv_heads * p.group;
-    const int64_t own_first = (own.first * p.kv_heads + kv_head) * p.group + in_group;
+    const int64_t own_first = ((int64_t)own.first * p.kv_heads + kv_head) * p.group + in_group;
     float top = -INFINITY, sum = 0.f, out[kColumns];
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
@@ -299,8 +121,9 @@ static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
     }
     const int64_t most = a.table_columns * a.page_size;
     if (most > 0) {
+        // eight stretches for each of the warps that have them, where the tables hold so many
         const int64_t tiles = a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
-        const int64_t extra = std::min((4 * sms + tiles - 1) / tiles, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
+        const int64_t extra = std::min<int64_t>((8 * kFewWarps * sms + tiles - 1) / tiles, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
         plan.own_items = a.batch + extra;
     }
     return plan;
@@ -351,26 +174,19 @@ static int page_maps(PrefixMaps& maps, const mps_prefix_attend& a) {
 }
 
 template <int DIM, bool BF16>
-static int attend(const AttendArgs& p, const mps_prefix_attend& a, int64_t prefix_ctas, int64_t own_ctas, cudaStream_t st) {
+static int attend(const AttendArgs& p, const mps_prefix_attend& a, unsigned int ctas, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
     Device d;
     int rc = current_device(d);
     if (rc) return rc;
     if (!(ready.load(std::memory_order_acquire) >> (d.ordinal & 63) & 1)) {
-        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_own_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, FewShape<DIM>::kSmem));
-        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_prefix_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixShape<DIM>::kSmem));
+        MPS_CUDA_TRY(cudaFuncSetAttribute(attend_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixShape<DIM>::kSmem));
         ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
     }
-    if (prefix_ctas) {
-        PrefixMaps maps;
-        rc = page_maps(maps, a);
-        if (rc) return rc;
-        rc = launch_overlapping_smem("attend_prefix_kernel", attend_prefix_kernel<DIM, BF16>, (unsigned int)prefix_ctas, dim3(kPrefixThreads), PrefixShape<DIM>::kSmem, st, p,
-                                     maps);
-        if (rc) return rc;
-    }
-    if (own_ctas) {
-        rc = launch_overlapping_smem("attend_own_kernel", attend_own_kernel<DIM, BF16>, (unsigned int)own_ctas, dim3(kFewWarps * 32), FewShape<DIM>::kSmem, st, p);
+    if (ctas) {
+        PrefixMaps maps = {};
+        if (p.prefix_units) rc = page_maps(maps, a);
+        if (!rc) rc = launch_overlapping_smem("attend_kernel", attend_kernel<DIM, BF16>, ctas, dim3(kPrefixThreads), PrefixShape<DIM>::kSmem, st, p, maps);
         if (rc) return rc;
     }
     const int64_t q_heads = (int64_t)p.kv_heads * p.group;
@@ -458,10 +274,11 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     p.own_o = p.prefix_o + prefix_parts * a.dim;
     p.prefix_ml = reinterpret_cast<float2*>(p.own_o + own_parts * a.dim);
     p.own_ml = p.prefix_ml + prefix_parts;
-    const int64_t prefix_ctas = (int64_t)plan.prefix_splits * a.kv_heads * plan.wide_tiles;
-    const int64_t own_ctas = plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
-    if (prefix_ctas > 0x7FFFFFFF || own_ctas > 0x7FFFFFFF) { set_error("mps_prefix_attend_tokens: too much work for one launch"); return MPS_ERR_INVALID; }
+    const int64_t units = (int64_t)plan.prefix_splits * a.kv_heads * plan.wide_tiles, own_units = plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
+    if (units > 0x7FFFFFFF || own_units > 0x7FFFFFFF) { set_error("mps_prefix_attend_tokens: too much work for one launch"); return MPS_ERR_INVALID; }
+    p.prefix_units = (int32_t)units;
+    const unsigned int ctas = (unsigned int)std::max(units, std::min<int64_t>(d.sms, (own_units + kFewWarps - 1) / kFewWarps));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, a, prefix_ctas, own_ctas, st) : attend<64, false>(p, a, prefix_ctas, own_ctas, st);
-    return a.dtype == MPS_BF16 ? attend<128, true>(p, a, prefix_ctas, own_ctas, st) : attend<128, false>(p, a, prefix_ctas, own_ctas, st);
+    if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, a, ctas, st) : attend<64, false>(p, a, ctas, st);
+    return a.dtype == MPS_BF16 ? attend<128, true>(p, a, ctas, st) : attend<128, false>(p, a, ctas, st);
 }
