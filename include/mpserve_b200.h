@@ -426,9 +426,11 @@ MPS_API int64_t mps_int4_bytes(int64_t rows, int64_t cols, int32_t group);
 MPS_API int mps_int4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t rows, int64_t cols, int32_t group, void* data,
                           void* stream);
 MPS_API int mps_int4_dequantize(const void* data, int64_t rows, int64_t cols, int32_t group, int32_t scale_dtype, int32_t dtype, void* out, void* stream);
-/* out[t, r] = sum_k x[t, k] value[r, k], summed in FP32, rounded once. */
+/* out[t, r] = sum_k x[t, k] value[r, k], summed in FP32, rounded once.  Tokens whose rows do not begin at multiples of 16 bytes (or overlap) are copied first, into
+ * x_rows: tokens x cols, a row filled up to a multiple of 8, of the caller's that nobody else uses until the call's kernels are done, 16-byte aligned. */
 typedef struct mps_int4_linear {
     const void* x;
+    void* x_rows;                       /* or null, where they do */
     const void* w;
     void* out;
     int64_t tokens, cols, rows;
@@ -436,7 +438,8 @@ typedef struct mps_int4_linear {
     int32_t group, x_dtype, scale_dtype, out_dtype;
 } mps_int4_linear;
 enum { MPS_INT4_MOST_TOKENS = 1 << 21 };
-MPS_API int mps_int4_product(const mps_int4_linear* args, void* stream);
+/* workspace: mps_mx4_workspace_bytes() bytes as for the MXFP4 products, which may be theirs; mps_mx4_status tells of waits that ran out. */
+MPS_API int mps_int4_product(const mps_int4_linear* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Queries and keys [tokens, heads, dim], normalised over each head where a weight is given, and rotated by their positions: pair j of the first `rotated` values
  * of a head, (j, j + rotated / 2) or `interleaved` (2 j, 2 j + 1), by positions[axis[j]][token] * turns[j] whole turns, times `scale`.  q_out [tokens, q_heads,
@@ -487,7 +490,7 @@ typedef struct mps_prefix_attend {
 #define MPS_MOST_KEYS (INT64_C(1) << 30)
 /* Of these sizes on the current device (pointers and strides do not matter), or -1; 256-byte aligned, contents irrelevant before and after. */
 MPS_API int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args);
-/* workspace: mps_mx4_workspace_bytes() bytes as for the MXFP4 products, which may be theirs; mps_mx4_status tells of waits that ran out. */
+/* workspace: as for mps_int4_product. */
 MPS_API int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Checksum of a decoded tensor: sum of the 16-bit patterns (mod 2^64) and an XOR fold of

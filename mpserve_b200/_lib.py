@@ -38,7 +38,7 @@ MX4_NORM = struct.Struct("@7P7q6i2f")
 MX4_LINEAR = struct.Struct("@5P5q4i")
 MX4_MLP = struct.Struct("@7P3q5i2fi")
 # struct mps_int4_linear, mps_head_rotate and mps_prefix_attend, likewise.
-INT4_LINEAR = struct.Struct("@3P5q4i")
+INT4_LINEAR = struct.Struct("@4P5q4i")
 HEAD_ROTATE = struct.Struct("@12P15q8i2f")
 PREFIX_ATTEND = struct.Struct("@8P13q4if4x")
 
@@ -98,7 +98,7 @@ _PROTOS = {
     "mps_int4_bytes": (_i64, [_i64, _i64, _i32]),
     "mps_int4_pack": (C.c_int, [_p, _p, _p, _i64, _i64, _i32, _p, _p]),
     "mps_int4_dequantize": (C.c_int, [_p, _i64, _i64, _i32, _i32, _i32, _p, _p]),
-    "mps_int4_product": (C.c_int, [C.c_char_p, _p]),
+    "mps_int4_product": (C.c_int, [C.c_char_p, _p, _i64, _p]),
     "mps_head_rotate_rows": (C.c_int, [C.c_char_p, _p]),
     "mps_prefix_attend_scratch_bytes": (_i64, [C.c_char_p]),
     "mps_prefix_attend_tokens": (C.c_int, [C.c_char_p, _p, _i64, _p, _i64, _p]),

@@ -103,21 +103,4 @@ __device__ __forceinline__ OwnItems own_items(const AttendArgs& p, int sequence)
     return {(int)warp_total(before), (own_length(p, sequence) + step - 1) / step};
 }
 
-// A launch with dynamic shared memory that may overlap the end of the kernel before it.
-template <typename... Params, typename... Args>
-inline int launch_overlapping_smem(const char* what, void (*kernel)(Params...), unsigned int ctas, dim3 threads, int smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas);
-    config.blockDim = threads;
-    config.dynamicSmemBytes = (size_t)smem;
-    config.stream = st;
-    cudaLaunchAttribute overlap;
-    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &overlap;
-    config.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
-    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
-}
-
 }  // namespace mps

@@ -7,9 +7,9 @@
 // frequency, in revolutions, is an FP64 product, whose whole part is dropped in FP64; what is left is below half a revolution and its sine and cosine
 // are FP32's.  All other arithmetic is FP32, rounded once to the output's type.
 //
-// A CTA has one token: its first threads make the token's cosines and sines, once for all heads, while every thread's share of the heads is on its way; a
-// share is eight neighbouring values, so that four to 32 lanes have a head, and neighbours' halves of a pair change lanes by shuffles.  Bounds: memory,
-// for a few tokens the launch.
+// Eight values of a head are a lane's, four and the four that they are paired with, so that four to 32 lanes have a head and a pair never changes lanes.  With few
+// tokens a CTA has one, all heads at once, and its first threads make the token's cosines and sines while the heads are on their way; with many a warp has
+// one, makes them for itself and goes through the heads with four of them on their way, without a barrier.  Bounds: memory, for a few tokens the launch.
 #include <initializer_list>
 
 #include "mx4.cuh"
@@ -17,6 +17,7 @@
 namespace mps {
 
 constexpr int kHeadMostDim = 256;
+constexpr int64_t kRotateFewTokens = 148;
 
 struct RotateArgs {
     mps_head_rotate a;
@@ -28,7 +29,7 @@ struct RotateArgs {
 struct HeadPlace {
     const void* in;
     void* out;           // null: nowhere
-    int64_t in_at, out_at;
+    int64_t in_at, out_at, out_stride;      // out_stride: of the next head of its kind
     const void* weight;
     bool turned;         // not a value
 };
@@ -40,7 +41,7 @@ __device__ __forceinline__ HeadPlace head_place(const RotateArgs& p, int64_t tok
     r.turned = true;
     if (h < a.q_heads) {
         r.in = a.q; r.in_at = token * a.q_token_stride + (int64_t)h * a.q_head_stride;
-        r.out = a.q_out; r.out_at = (token * a.q_heads + h) * a.dim;
+        r.out = a.q_out; r.out_at = (token * a.q_heads + h) * a.dim; r.out_stride = a.dim;
         r.weight = a.q_weight;
         return r;
     }
@@ -52,27 +53,29 @@ __device__ __forceinline__ HeadPlace head_place(const RotateArgs& p, int64_t tok
     r.in = key ? a.k : a.v;
     r.in_at = key ? token * a.k_token_stride + (int64_t)h * a.k_head_stride : token * a.v_token_stride + (int64_t)h * a.v_head_stride;
     if (!a.slots) {
-        r.out = a.k_out; r.out_at = (token * a.kv_heads + h) * a.dim;
+        r.out = a.k_out; r.out_at = (token * a.kv_heads + h) * a.dim; r.out_stride = a.dim;
     } else {
         r.out = page < 0 ? nullptr : key ? a.k_out : a.v_out;
+        r.out_stride = key ? a.k_cache_head_stride : a.v_cache_head_stride;
         r.out_at = key ? page * a.k_page_stride + offset * a.k_slot_stride + (int64_t)h * a.k_cache_head_stride
                        : page * a.v_page_stride + offset * a.v_slot_stride + (int64_t)h * a.v_cache_head_stride;
     }
     return r;
 }
 
-// The token's cosines and sines, times the rotation's scale, by the CTA's threads.
+// Cosine and sine of a token's pair j, times the rotation's scale.
+__device__ __forceinline__ void pair_angle(const mps_head_rotate& a, int64_t token, int j, float& cosine, float& sine) {
+    const int64_t at = (a.axis ? (int64_t)a.axis[j] * a.tokens : 0) + token;
+    const double position = a.wide_positions ? (double)static_cast<const int64_t*>(a.positions)[at] : (double)static_cast<const int32_t*>(a.positions)[at];
+    const double turns = position * a.turns[j];
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    cosine = c * a.scale;
+    sine = s * a.scale;
+}
+// Those of all its pairs, by the CTA's threads.
 __device__ __forceinline__ void token_angles(const RotateArgs& p, int64_t token, float* cosines, float* sines) {
-    const mps_head_rotate& a = p.a;
-    for (int j = threadIdx.x; j < a.rotated / 2; j += blockDim.x) {
-        const int64_t at = (a.axis ? (int64_t)a.axis[j] * a.tokens : 0) + token;
-        const double position = a.wide_positions ? (double)static_cast<const int64_t*>(a.positions)[at] : (double)static_cast<const int32_t*>(a.positions)[at];
-        const double turns = position * a.turns[j];
-        float s, c;
-        sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-        cosines[j] = c * a.scale;
-        sines[j] = s * a.scale;
-    }
+    for (int j = threadIdx.x; j < p.a.rotated / 2; j += blockDim.x) pair_angle(p.a, token, j, cosines[j], sines[j]);
 }
 
 __device__ __forceinline__ void token_slot(const RotateArgs& p, int64_t token, int64_t& page, int64_t& offset) {
@@ -87,7 +90,91 @@ __device__ __forceinline__ void token_slot(const RotateArgs& p, int64_t token, i
     }
 }
 
-// Rows of whole eights, aligned.  LANES (a power of two) have a head; STEPS heads a thread; WIDE: FP32.
+// Which eight values of a head are lane u's: a to a + 3 and b to b + 3; their pairs, where they are turned, are 4 u to 4 u + 3.
+struct RotateLane {
+    int a, b;
+    bool live, turned;
+    __device__ __forceinline__ RotateLane(const mps_head_rotate& r, int u) {
+        live = u < r.dim / 8;
+        turned = u < r.rotated / 8;
+        const bool halves = turned && !r.interleaved;
+        a = halves ? 4 * u : 8 * u;
+        b = halves ? r.rotated / 2 + 4 * u : 8 * u + 4;
+    }
+};
+template <bool WIDE>
+struct RotateRaw {       // as they were loaded
+    uint4 a, b;          // of a 16-bit type the first two words each
+    __device__ __forceinline__ void load(const void* base, int64_t at, const RotateLane& l) {
+        if (WIDE) {
+            const float* p = static_cast<const float*>(base) + at;
+            a = *reinterpret_cast<const uint4*>(p + l.a);
+            b = *reinterpret_cast<const uint4*>(p + l.b);
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+            const uint2 x = *reinterpret_cast<const uint2*>(p + l.a), y = *reinterpret_cast<const uint2*>(p + l.b);
+            a.x = x.x; a.y = x.y; b.x = y.x; b.y = y.y;
+        }
+    }
+    __device__ __forceinline__ void values(int dtype, Pairs& v) const {
+        Raw8 r;
+        r.a = WIDE ? a : make_uint4(a.x, a.y, b.x, b.y);
+        r.b = WIDE ? b : r.a;
+        unpack8(r, WIDE ? MPS_F32 : dtype == MPS_BF16 ? MPS_BF16 : MPS_F16, v.each());
+    }
+    static __device__ __forceinline__ void store(void* base, int dtype, int64_t at, const RotateLane& l, const Pairs& v) {
+        if (WIDE) {
+            float* p = static_cast<float*>(base) + at;
+            *reinterpret_cast<float4*>(p + l.a) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+            *reinterpret_cast<float4*>(p + l.b) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
+        } else {
+            uint16_t* p = static_cast<uint16_t*>(base) + at;
+            *reinterpret_cast<uint2*>(p + l.a) = make_uint2(pack2(v.p[0].x, v.p[0].y, dtype), pack2(v.p[1].x, v.p[1].y, dtype));
+            *reinterpret_cast<uint2*>(p + l.b) = make_uint2(pack2(v.p[2].x, v.p[2].y, dtype), pack2(v.p[3].x, v.p[3].y, dtype));
+        }
+    }
+};
+// A norm's weight at a lane's places.
+__device__ __forceinline__ void rotate_gain(const mps_head_rotate& r, const void* weight, const RotateLane& l, Pairs& v) {
+    if (!weight || !l.live) return;
+    if (r.weight_dtype == MPS_F32) {
+        RotateRaw<true> raw;
+        raw.load(weight, 0, l);
+        raw.values(MPS_F32, v);
+    } else {
+        RotateRaw<false> raw;
+        raw.load(weight, 0, l);
+        raw.values(r.weight_dtype, v);
+    }
+}
+// A lane's values, normalised (all LANES of the head, `mates`, together) and turned.
+template <int LANES>
+__device__ __forceinline__ void rotate8(const RotateArgs& p, Pairs& v, bool normed, const Pairs& gain, bool turned, const float (&c)[4], const float (&s)[4], uint32_t mates) {
+    if (normed) {
+        float2 two = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) two = fma2(v.p[i], v.p[i], two);
+        float sum = two.x + two.y;
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
+        v = times(times(v, rsqrtf(fmaf(sum, p.inv_dim, p.a.eps))), gain);
+    }
+    if (!turned) return;
+    if (p.a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v.p[i] = fma2(make_float2(v.p[i].y, v.p[i].x), make_float2(-s[i], s[i]), mul2(v.p[i], make_float2(c[i], c[i])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 x = v.p[i], y = v.p[i + 2], c2 = make_float2(c[2 * i], c[2 * i + 1]), s2 = make_float2(s[2 * i], s[2 * i + 1]);
+            v.p[i] = fma2(y, make_float2(-s2.x, -s2.y), mul2(x, c2));
+            v.p[i + 2] = fma2(x, s2, mul2(y, c2));
+        }
+    }
+}
+
+// Few tokens.  LANES (a power of two) have a head; STEPS heads a thread; WIDE: FP32.
 template <int LANES, int STEPS, bool WIDE>
 __global__ void __launch_bounds__(STEPS == 1 ? 1024 : 512) rotate_kernel(const RotateArgs p) {
     __shared__ __align__(16) float cosines[kHeadMostDim / 2], sines[kHeadMostDim / 2];
@@ -95,78 +182,96 @@ __global__ void __launch_bounds__(STEPS == 1 ? 1024 : 512) rotate_kernel(const R
     griddep_launch();
     const mps_head_rotate& a = p.a;
     const int64_t token = blockIdx.x;
-    const int u = threadIdx.x % LANES, units = a.dim / 8, per_pass = blockDim.x / LANES, heads = a.q_heads + (a.v ? 2 : 1) * a.kv_heads;
+    const int u = threadIdx.x % LANES, per_pass = blockDim.x / LANES, heads = a.q_heads + (a.v ? 2 : 1) * a.kv_heads;
     const uint32_t mates = LANES == 32 ? 0xFFFFFFFFu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));      // the lanes of a head
-    const int dtype = WIDE ? MPS_F32 : a.dtype == MPS_BF16 ? MPS_BF16 : MPS_F16;
+    const RotateLane lane(a, u);
     int64_t page, offset;
     token_slot(p, token, page, offset);
-    const auto valid = [&](int h) { return h < heads && u < units ? 8 : 0; };
-    const auto gain = [&](int h) {
-        const void* weight = h < a.q_heads ? a.q_weight : h < a.q_heads + a.kv_heads ? a.k_weight : nullptr;
-        return load_raw8(weight, a.weight_dtype, u * 8, weight ? valid(h) : 0, true);
-    };
-    uint4 raw[STEPS][WIDE ? 2 : 1];
-    Raw8 first_gain;
+    RotateRaw<WIDE> raw[STEPS];
+    Pairs gain[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int h = s * per_pass + threadIdx.x / LANES;
-        const HeadPlace place = head_place(p, token, min(h, heads - 1), page, offset);
-        const Raw8 r = load_raw8(place.in, WIDE ? MPS_F32 : MPS_BF16, place.in_at + u * 8, valid(h), true);
-        raw[s][0] = r.a;
-        if (WIDE) raw[s][WIDE ? 1 : 0] = r.b;
-        if (s == 0) first_gain = gain(h);
+        raw[s].a = raw[s].b = make_uint4(0u, 0u, 0u, 0u);
+        if (h < heads) {
+            const HeadPlace place = head_place(p, token, h, page, offset);
+            if (lane.live) raw[s].load(place.in, place.in_at, lane);
+            rotate_gain(a, place.weight, lane, gain[s]);
+        }
     }
     token_angles(p, token, cosines, sines);
     __syncthreads();
-    // this lane's pairs: those of a unit of the first halves, or (half as many) of neighbours
-    const int half = a.rotated / 16, place_of = a.interleaved ? u * 4 : (u < half ? u : u - half) * 8;
-    const int partner = u < half ? u + half : u - half;
-    const bool turned = u * 8 < a.rotated;
-    float c[8], s8[8];
+    float c[4], sn[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int at = turned ? place_of + (a.interleaved ? i >> 1 : i) : 0;
-        c[i] = cosines[at];
-        s8[i] = sines[at];
-        if (a.interleaved ? !(i & 1) : u < half) s8[i] = -s8[i];
+    for (int i = 0; i < 4; ++i) {
+        const int j = lane.turned ? 4 * u + i : 0;
+        c[i] = cosines[j];
+        sn[i] = sines[j];
     }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int h = s * per_pass + threadIdx.x / LANES;      // the same for the lanes of a head
         if (h >= heads) break;
-        float v[8];
-        Raw8 r;
-        r.a = raw[s][0];
-        r.b = raw[s][WIDE ? 1 : 0];
-        unpack8(r, dtype, v);
         const HeadPlace place = head_place(p, token, h, page, offset);
-        if (place.weight) {
-            float w[8], sum = 0.f;
-            unpack8(s == 0 ? first_gain : gain(h), a.weight_dtype, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-#pragma unroll
-            for (int o = LANES / 2; o; o >>= 1) sum += __shfl_xor_sync(mates, sum, o);
-            const float rms = rsqrtf(fmaf(sum, p.inv_dim, a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * rms * w[i];
-        }
-        if (place.turned) {
-            float other[8];
-            if (a.interleaved) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) other[i] = v[i ^ 1];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(mates, v[i], partner, LANES);
-            }
-            if (turned) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fmaf(other[i], s8[i], v[i] * c[i]);
-            }
-        }
-        if (place.out) store8(place.out, dtype, place.out_at + u * 8, valid(h), true, v);
+        Pairs v;
+        raw[s].values(a.dtype, v);
+        rotate8<LANES>(p, v, place.weight != nullptr, gain[s], place.turned && lane.turned, c, sn, mates);
+        if (place.out && lane.live) RotateRaw<WIDE>::store(place.out, a.dtype, place.out_at, lane, v);
     }
+}
+
+// Many tokens: `share` warps have one.
+constexpr int kRotateAhead = 4, kRotateWarps = 4;
+template <int LANES, bool WIDE>
+__global__ void __launch_bounds__(kRotateWarps * 32) rotate_many_kernel(const RotateArgs p, const int share) {
+    griddep_wait();
+    griddep_launch();
+    const mps_head_rotate& a = p.a;
+    const int64_t worker = (int64_t)blockIdx.x * kRotateWarps + (threadIdx.x >> 5), token = worker / share;
+    if (token >= a.tokens) return;
+    constexpr int kHeads = 32 / LANES;
+    const int l = threadIdx.x & 31, u = l % LANES, first = (int)(worker % share) * kHeads + l / LANES, step = share * kHeads;
+    const uint32_t mates = LANES == 32 ? 0xFFFFFFFFu : ((1u << (LANES & 31)) - 1u) << (l & ~(LANES - 1));      // the lanes of a head
+    const RotateLane lane(a, u);
+    int64_t page, offset;
+    token_slot(p, token, page, offset);
+    float c[4], s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane.turned) pair_angle(a, token, 4 * u + i, c[i], s[i]);
+    // heads of one kind; h0: the first one's number among all
+    const auto go = [&](int h0, int heads, int64_t in_stride) {
+        if (first >= heads) return;
+        const HeadPlace place = head_place(p, token, h0 + first, page, offset);
+        Pairs gain;
+        rotate_gain(a, place.weight, lane, gain);
+        const bool turned = place.turned && lane.turned;
+        const int64_t in_step = in_stride * step, out_step = place.out_stride * step;
+        RotateRaw<WIDE> raw[kRotateAhead];
+        int64_t in = place.in_at, out = place.out_at;
+#pragma unroll
+        for (int i = 0; i < kRotateAhead; ++i) {
+            raw[i].a = raw[i].b = make_uint4(0u, 0u, 0u, 0u);
+            if (first + i * step < heads && lane.live) raw[i].load(place.in, in, lane);
+            in += in_step;
+        }
+        for (int h = first; h < heads; h += kRotateAhead * step) {
+#pragma unroll
+            for (int i = 0; i < kRotateAhead; ++i) {
+                if (h + i * step >= heads) break;      // the same for the lanes of a head
+                Pairs v;
+                raw[i].values(a.dtype, v);
+                if (h + (i + kRotateAhead) * step < heads && lane.live) raw[i].load(place.in, in, lane);
+                in += in_step;
+                rotate8<LANES>(p, v, place.weight != nullptr, gain, turned, c, s, mates);
+                if (place.out && lane.live) RotateRaw<WIDE>::store(place.out, a.dtype, out, lane, v);
+                out += out_step;
+            }
+        }
+    };
+    go(0, a.q_heads, a.q_head_stride);
+    go(a.q_heads, a.kv_heads, a.k_head_stride);
+    if (a.v) go(a.q_heads + a.kv_heads, a.kv_heads, a.v_head_stride);
 }
 
 // Any dim, any alignment: a warp has a head, value by value, by way of shared memory.
@@ -220,10 +325,20 @@ __global__ void __launch_bounds__(kRotateAnyWarps * 32) rotate_any_kernel(const 
 template <int LANES>
 static int launch_rotate(const RotateArgs& p, cudaStream_t st) {
     const int heads = p.a.q_heads + (p.a.v ? 2 : 1) * p.a.kv_heads;
-    // few tokens: every head at once; many: 256 threads, which leave the SM room for other tokens
-    const int all = (heads * LANES + 31) / 32 * 32, most = p.a.tokens <= 148 ? 1024 : 256;
+    if (p.a.tokens > kRotateFewTokens) {
+        // as many warps for a token as there are places for on the GPU, and passes for
+        const int passes = (heads * LANES + 31) / 32;
+        int share = 1;
+        while (share < passes && p.a.tokens * share < 4096) share *= 2;
+        const int64_t ctas = (p.a.tokens * share + kRotateWarps - 1) / kRotateWarps;
+        if (ctas > 0x7FFFFFFF) { set_error("mps_head_rotate_rows: too many tokens"); return MPS_ERR_INVALID; }
+        return p.a.dtype == MPS_F32 ? launch_overlapping("rotate_many_kernel", rotate_many_kernel<LANES, true>, (unsigned int)ctas, dim3(kRotateWarps * 32), st, p, share)
+                                    : launch_overlapping("rotate_many_kernel", rotate_many_kernel<LANES, false>, (unsigned int)ctas, dim3(kRotateWarps * 32), st, p, share);
+    }
+    // every head at once, where a CTA has the threads
+    const int all = (heads * LANES + 31) / 32 * 32;
     int steps = 1;
-    while (steps < 4 && (all + steps - 1) / steps > most) ++steps;
+    while (steps < 4 && (all + steps - 1) / steps > 1024) ++steps;
     const int threads = ((heads + steps - 1) / steps * LANES + 31) / 32 * 32;
     if (threads > (steps == 1 ? 1024 : 512)) return launch_overlapping("rotate_any_kernel", rotate_any_kernel, (unsigned int)p.a.tokens, dim3(kRotateAnyWarps * 32), st, p);
     const unsigned int ctas = (unsigned int)p.a.tokens;
@@ -270,19 +385,19 @@ extern "C" int mps_head_rotate_rows(const mps_head_rotate* args, void* stream) {
     p.inv_dim = (float)(1.0 / (double)a.dim);
     p.page_shift = append ? __builtin_ctzll((unsigned long long)a.page_size) : 0;
     p.slots = append ? a.pages * a.page_size : 0;
-    // every head begins at a multiple of eight values, by pointer and strides
-    const int64_t unit = 8 * mx4_dtype_bytes(a.dtype);
-    const auto even = [&](const void* q, std::initializer_list<int64_t> strides) {
-        bool ok = reinterpret_cast<uintptr_t>(q) % unit == 0;
-        for (const int64_t s : strides) ok = ok && s % 8 == 0;
+    // fours of every head begin at multiples of four values, by pointer and strides
+    const auto even = [](const void* q, int dtype, std::initializer_list<int64_t> strides) {
+        bool ok = reinterpret_cast<uintptr_t>(q) % (4 * mx4_dtype_bytes(dtype)) == 0;
+        for (const int64_t s : strides) ok = ok && s % 4 == 0;
         return ok;
     };
-    const auto weight_even = [&](const void* q) { return reinterpret_cast<uintptr_t>(q) % (8 * mx4_dtype_bytes(a.weight_dtype)) == 0; };
-    const bool vec = a.dim % 8 == 0 && a.rotated % (a.interleaved ? 8 : 16) == 0 && even(a.q, {a.q_token_stride, a.q_head_stride}) &&
-                     even(a.k, {a.k_token_stride, a.k_head_stride}) && even(a.q_out, {}) && weight_even(a.q_weight) && weight_even(a.k_weight) &&
-                     (append ? even(a.v, {a.v_token_stride, a.v_head_stride}) && even(a.k_out, {a.k_page_stride, a.k_slot_stride, a.k_cache_head_stride}) &&
-                                   even(a.v_out, {a.v_page_stride, a.v_slot_stride, a.v_cache_head_stride})
-                             : even(a.k_out, {}));
+    const bool vec = a.dim % 8 == 0 && a.rotated % 8 == 0 && even(a.q, a.dtype, {a.q_token_stride, a.q_head_stride}) &&
+                     even(a.k, a.dtype, {a.k_token_stride, a.k_head_stride}) && even(a.q_out, a.dtype, {}) && even(a.q_weight, a.weight_dtype, {}) &&
+                     even(a.k_weight, a.weight_dtype, {}) &&
+                     (append ? even(a.v, a.dtype, {a.v_token_stride, a.v_head_stride}) &&
+                                   even(a.k_out, a.dtype, {a.k_page_stride, a.k_slot_stride, a.k_cache_head_stride}) &&
+                                   even(a.v_out, a.dtype, {a.v_page_stride, a.v_slot_stride, a.v_cache_head_stride})
+                             : even(a.k_out, a.dtype, {}));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!vec) return launch_overlapping("rotate_any_kernel", rotate_any_kernel, (unsigned int)a.tokens, dim3(kRotateAnyWarps * 32), st, p);
     if (a.dim <= 32) return launch_rotate<4>(p, st);

@@ -159,16 +159,9 @@ static int page_map(CUtensorMap& map, EncodeTiled encode, const void* pages, con
     return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
 }
 static int page_maps(PrefixMaps& maps, const mps_prefix_attend& a) {
-    static std::atomic<EncodeTiled> known{nullptr};
-    EncodeTiled encode = known.load(std::memory_order_relaxed);
-    if (!encode) {
-        void* entry = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        MPS_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found));
-        if (found != cudaDriverEntryPointSuccess || !entry) { set_error("the driver has no cuTensorMapEncodeTiled"); return MPS_ERR_UNSUPPORTED; }
-        encode = reinterpret_cast<EncodeTiled>(entry);
-        known.store(encode, std::memory_order_relaxed);
-    }
+    EncodeTiled encode;
+    const int found = tensor_map_encoder(encode);
+    if (found) return found;
     const int rc = page_map(maps.k, encode, a.k_pages, a, a.k_slot_stride, a.k_head_stride, a.k_page_stride);
     return rc ? rc : page_map(maps.v, encode, a.v_pages, a, a.v_slot_stride, a.v_head_stride, a.v_page_stride);
 }

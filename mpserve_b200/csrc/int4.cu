@@ -4,40 +4,40 @@
 // point is a whole number of at most 15, exact in BF16 and F16, so the tensor cores multiply those by the tokens as they came, a group's products are summed in
 // FP32, and the scale multiplies that sum, in FP32: nothing is rounded before the output.
 //
-// In memory a weight is an array of blocks of 16 rows x 64 columns, 512 bytes each, row of blocks after row of blocks, then a word for every group and
-// row, 16 rows together.  A block holds for every lane of a warp the 16 bytes that make its left operands of four m16n8k16 multiplications: lane 4 g + t
-// has rows g and g + 8; its word s the columns k = 32 (s / 2) + 8 t + 4 (s % 2) and the three after: codes of (g, k), (g + 8, k), (g, k + 2), (g + 8, k + 2) in
-// the four nibbles of the low half, their right neighbours in those of the high half.  A mask and a shift give a pair of codes in the two halves of a register,
-// an OR makes them 128 + q in BF16 (1024 + q in F16), and one subtraction of 128 + z takes both to q - z.  The order of columns is that in
-// which a lane reads 16 bytes of a token at a time.  Columns are filled up to a multiple of 64 and of the group with codes that equal their zero
-// point, rows to a multiple of 16 with a scale of 0.
+// In memory a weight is an array of tiles of 128 rows x 128 columns, row of tiles after row of tiles, each in one piece, so that one bulk copy brings it: 8 KB of
+// codes, then a word for every row and group, the scale in its low half and the zero point in its high one.  Codes are in sixteen blocks of 16 rows x 64 columns (two
+// for the first 16 rows, two for the next ...), and a block has 16 bytes for every lane of a warp: lane 4 g + t has rows g and g + 8; its word s the columns
+// k = 16 s + 4 t and the three after: codes of (g, k), (g + 8, k), (g, k + 2), (g + 8, k + 2) in the four nibbles of the low half, their right neighbours in those
+// of the high half.  A mask and a shift give a pair of codes in the two halves of a register, an OR makes them 128 + q in BF16 (1024 + q in
+// F16), and one subtraction of 128 + z takes both to q - z: four registers that are a lane's share of 16 rows x 16 columns in tensor memory.  What fills a tile up
+// has codes, zero points and scales of 0.
 #include "mx4.cuh"
+#include "mx4_tensor.cuh"
 #include "stream_common.cuh"
-#include "warp_mma.cuh"
+
+#include <algorithm>
+#include <atomic>
 
 namespace mps {
 
-constexpr int kInt4Rows = 16, kInt4Cols = 64, kInt4BlockBytes = 512;
+constexpr int kInt4Rows = 128, kInt4Cols = 128, kInt4CodeBytes = kInt4Rows * kInt4Cols / 2;
 constexpr int64_t kInt4MostRows = int64_t(1) << 27, kInt4MostCols = int64_t(1) << 24;
 
-struct Int4Shape {
-    int64_t row_tiles;
-    int32_t blocks;      // of a row of blocks
-    int32_t groups;      // with those that fill up
-    __host__ __device__ int64_t codes_bytes() const { return row_tiles * blocks * kInt4BlockBytes; }
-    __host__ __device__ int64_t bytes() const { return codes_bytes() + row_tiles * groups * kInt4Rows * 4; }
-};
-static __host__ __device__ inline Int4Shape int4_shape(int64_t rows, int64_t cols, int32_t group) {
-    const int unit = group > kInt4Cols ? group : kInt4Cols;
-    const int64_t wide = (cols + unit - 1) / unit * unit;
-    return {(rows + kInt4Rows - 1) / kInt4Rows, (int32_t)(wide / kInt4Cols), (int32_t)(wide / group)};
-}
+__host__ __device__ constexpr int int4_tile_bytes(int group) { return kInt4CodeBytes + kInt4Rows * (kInt4Cols / group) * 4; }
+__host__ __device__ inline int64_t int4_chunks(int64_t cols) { return (cols + kInt4Cols - 1) / kInt4Cols; }
+__host__ __device__ inline int64_t int4_row_tiles(int64_t rows) { return (rows + kInt4Rows - 1) / kInt4Rows; }
+// In a tile: the word of a row and one of its groups, after the codes; sixteen rows' words of a group lie together.
+__host__ __device__ inline int int4_scale_word(int row, int group, int groups) { return (row / 16 * groups + group) * 16 + row % 16; }
 static bool int4_size_ok(int64_t rows, int64_t cols, int32_t group) {
     return rows >= 0 && rows <= kInt4MostRows && cols > 0 && cols <= kInt4MostCols && (group == 32 || group == 64 || group == 128);
 }
 
-// Column, within a block, of the first code of nibble `i` (0 to 3) of word s of lane 4 g + t.
-__device__ __forceinline__ int int4_column(int t, int s, int i) { return 32 * (s >> 1) + 8 * t + 4 * (s & 1) + (i & 2); }
+// Row and column, within a tile, of the first code of nibble `i` (0 to 3) of code word `w`.
+__device__ __forceinline__ int int4_row(int w, int i) { return (w >> 8) * 16 + ((w >> 4) & 7) + 8 * (i & 1); }
+__device__ __forceinline__ int int4_column(int w, int i) {
+    const int s = w & 3, t = (w >> 2) & 3, block = (w >> 7) & 1;
+    return block * 64 + 16 * s + 4 * t + (i & 2);
+}
 
 // ---- laid out once, and back --------------------------------------------------------------------------
 
@@ -49,39 +49,36 @@ struct Int4Parts {
     int32_t group;
 };
 
+// A CTA a tile at a time.
 __global__ void __launch_bounds__(256) int4_pack_kernel(const Int4Parts p, uint8_t* __restrict__ data) {
     griddep_wait();
     griddep_launch();
-    const Int4Shape shape = int4_shape(p.rows, p.cols, p.group);
-    const int64_t groups = (p.cols + p.group - 1) / p.group, words = shape.codes_bytes() / 4, step = (int64_t)gridDim.x * blockDim.x;
-    uint32_t* out = reinterpret_cast<uint32_t*>(data);
-    for (int64_t w = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; w < words; w += step) {
-        const int64_t block = w >> 7, tile = block / shape.blocks;
-        const int64_t first = (block - tile * shape.blocks) * kInt4Cols;
-        const int lane = (int)(w >> 2) & 31, s = (int)w & 3;
-        uint32_t word = 0u;
+    const int64_t chunks = int4_chunks(p.cols), tiles = int4_row_tiles(p.rows) * chunks, groups = (p.cols + p.group - 1) / p.group;
+    const int in_tile = kInt4Cols / p.group;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t row0 = tile / chunks * kInt4Rows, col0 = tile % chunks * kInt4Cols;
+        uint32_t* out = reinterpret_cast<uint32_t*>(data + tile * int4_tile_bytes(p.group));
+        for (int w = threadIdx.x; w < kInt4CodeBytes / 4; w += blockDim.x) {
+            uint32_t word = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t row = tile * kInt4Rows + (lane >> 2) + 8 * (i & 1);
+            for (int i = 0; i < 4; ++i) {
+                const int64_t row = row0 + int4_row(w, i);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int64_t col = first + int4_column(lane & 3, s, i) + j, g = col / p.group;
-                uint32_t code = 0u;
-                if (row < p.rows) {
-                    if (col < p.cols) code = p.codes[row * p.cols + col];
-                    else if (g < groups) code = p.zeros ? p.zeros[row * groups + g] : 8u;
+                for (int j = 0; j < 2; ++j) {
+                    const int64_t col = col0 + int4_column(w, i) + j, g = col / p.group;
+                    uint32_t code = 0u;
+                    if (row < p.rows && g < groups) code = col < p.cols ? p.codes[row * p.cols + col] : p.zeros ? p.zeros[row * groups + g] : 8u;      // q - z = 0
+                    word |= (code & 15u) << (4 * i + 16 * j);
                 }
-                word |= (code & 15u) << (4 * i + 16 * j);
             }
+            out[w] = word;
         }
-        out[w] = word;
-    }
-    const int64_t scales = shape.row_tiles * shape.groups * kInt4Rows;
-    for (int64_t w = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; w < scales; w += step) {
-        const int64_t g = (w >> 4) % shape.groups, row = (w >> 4) / shape.groups * kInt4Rows + (w & 15);
-        uint32_t word = 0u;
-        if (row < p.rows && g < groups) word = p.scales[row * groups + g] | (p.zeros ? (uint32_t)p.zeros[row * groups + g] & 15u : 8u) << 16;
-        out[words + w] = word;
+        for (int w = threadIdx.x; w < kInt4Rows * in_tile; w += blockDim.x) {
+            const int64_t row = row0 + w % kInt4Rows, g = col0 / p.group + w / kInt4Rows;
+            uint32_t word = 0u;
+            if (row < p.rows && g < groups) word = p.scales[row * groups + g] | (p.zeros ? (uint32_t)p.zeros[row * groups + g] & 15u : 8u) << 16;
+            out[kInt4CodeBytes / 4 + int4_scale_word(w % kInt4Rows, w / kInt4Rows, in_tile)] = word;
+        }
     }
 }
 
@@ -89,51 +86,70 @@ __device__ __forceinline__ float int4_scale(uint32_t word, bool bf16) {
     return bf16 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((uint16_t)word));
 }
 
-// A thread a word: eight values.
 __global__ void __launch_bounds__(256) int4_values_kernel(const uint8_t* __restrict__ data, int64_t rows, int64_t cols, int32_t group, int scale_bf16, int dtype,
                                                           void* __restrict__ out) {
     griddep_wait();
     griddep_launch();
-    const Int4Shape shape = int4_shape(rows, cols, group);
-    const int64_t words = shape.codes_bytes() / 4, step = (int64_t)gridDim.x * blockDim.x;
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(data);
-    for (int64_t w = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; w < words; w += step) {
-        const int64_t block = w >> 7, tile = block / shape.blocks;
-        const int64_t first = (block - tile * shape.blocks) * kInt4Cols;
-        const int lane = (int)(w >> 2) & 31, s = (int)w & 3;
-        const uint32_t word = in[w];
+    const int64_t chunks = int4_chunks(cols), tiles = int4_row_tiles(rows) * chunks;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t row0 = tile / chunks * kInt4Rows, col0 = tile % chunks * kInt4Cols;
+        const uint32_t* in = reinterpret_cast<const uint32_t*>(data + tile * int4_tile_bytes(group));
+        for (int w = threadIdx.x; w < kInt4CodeBytes / 4; w += blockDim.x) {
+            const uint32_t word = in[w];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (lane >> 2) + 8 * (i & 1);
-            const int64_t row = tile * kInt4Rows + r;
-            const int64_t col = first + int4_column(lane & 3, s, i);
-            if (row >= rows) continue;
-            const uint32_t sz = in[words + (tile * shape.groups + col / group) * kInt4Rows + r];
-            const float scale = int4_scale(sz, scale_bf16);
-            const int zero = (int)(sz >> 16);
+            for (int i = 0; i < 4; ++i) {
+                const int r = int4_row(w, i), c = int4_column(w, i);
+                if (row0 + r >= rows) continue;
+                const uint32_t sz = in[kInt4CodeBytes / 4 + int4_scale_word(r, c / group, kInt4Cols / group)];
+                const float scale = int4_scale(sz, scale_bf16);
+                const int zero = (int)(sz >> 16);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (col + j >= cols) continue;
-                const float v = (float)((int)((word >> (4 * i + 16 * j)) & 15u) - zero) * scale;      // exact: 5 bits times 11
-                const int64_t at = row * cols + col + j;
-                if (dtype == MPS_F32) static_cast<float*>(out)[at] = v;
-                else static_cast<uint16_t*>(out)[at] = (uint16_t)pack2(v, 0.f, dtype);
+                for (int j = 0; j < 2; ++j) {
+                    if (col0 + c + j >= cols) continue;
+                    const float v = (float)((int)((word >> (4 * i + 16 * j)) & 15u) - zero) * scale;      // exact: 5 bits times 11
+                    const int64_t at = (row0 + r) * cols + col0 + c + j;
+                    if (dtype == MPS_F32) static_cast<float*>(out)[at] = v;
+                    else static_cast<uint16_t*>(out)[at] = (uint16_t)pack2(v, 0.f, dtype);
+                }
             }
         }
     }
 }
 
 // ---- products -------------------------------------------------------------------------------------------
+//
+// A CTA has 128 features for up to TOKENS tokens, and a share of the columns: a cluster of up to eight shares a row of tiles, as many as fill the GPU, and adds
+// its CTAs' sums up in shared memory, always in the same order.  A tile and its columns of the tokens come into a ring of some 200 KB.  Warps:
+//   0 copies;  1 multiplies: features (left operand, tensor memory) by tokens (right operand, shared memory), a group of columns into an accumulator of its own;
+//   2 to 9 take codes apart and store them in tensor memory, four warps a tile, 32 rows each: two tiles at a time, since what one takes is mostly waits in a row;
+//   10 to 13 add the groups' accumulators up, times their scales: a thread has a feature, its tokens are in registers.
+// Bound: memory; and taking codes apart, some 100 instructions for 16 rows of a tile, 200 cycles of an SM's issue slots for 8.5 KB.
+constexpr int kInt4Workers = 8, kInt4Adders = 4, kInt4Threads = (2 + kInt4Workers + kInt4Adders) * 32;
+constexpr int kInt4Buffers = 4, kInt4Sums = 4, kInt4MostParts = 8;
+constexpr int kInt4Smem = 227 << 10;
 
 struct Int4Args {
-    const void* x;
     const uint8_t* w;
     void* out;
-    int64_t x_stride, out_stride, tokens;
-    int64_t rows;
-    int32_t cols, group, blocks, groups;
+    int64_t out_stride, tokens, rows;
+    int32_t chunks, parts, token_tiles;
     int32_t out_dtype;
-    bool scale_bf16, x_vec;
+    bool scale_bf16;
+    uint32_t* workspace;     // word 0 records a wait that ran out
+};
+
+template <int TOKENS, int GROUP>
+struct Int4Tensor {
+    static constexpr int kGroups = kInt4Cols / GROUP, kTile = int4_tile_bytes(GROUP);
+    static constexpr int kX = TOKENS * kInt4Cols * 2;                                // two halves of 64 columns
+    static constexpr int kStage = (kX + kTile + 1023) / 1024 * 1024;                 // the tokens, then the tile
+    static constexpr int kStages = std::min(18, (kInt4Smem - 1024) / kStage);
+    static constexpr int kBars = kStages * kStage;
+    static constexpr int kSmem = kBars + (2 * kStages + 2 * kInt4Buffers + 2 * kInt4Sums + 1) * 8 + 16;
+    static constexpr int kSumColumns = kInt4Buffers * 64, kColumns = 512;            // tensor memory: left operands, then accumulators
+    static_assert(kSumColumns + kInt4Sums * TOKENS <= kColumns, "tensor memory");
+    static_assert(kSmem <= kInt4Smem && kX % 1024 == 0, "shared memory");
+    static_assert(TOKENS * kInt4Rows * 4 <= kStages * kStage, "sums take the ring's place");
 };
 
 template <bool BF16>
@@ -143,7 +159,6 @@ __device__ __forceinline__ uint32_t subtract2(uint32_t a, uint32_t b) {
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-
 // Two codes, nibble i of both halves of `w`, minus their zero point: `zero` is 128 + z in BF16 (1024 + z in F16), twice.
 template <bool BF16>
 __device__ __forceinline__ uint32_t int4_pair(uint32_t w, int i, uint32_t zero) {
@@ -154,100 +169,307 @@ __device__ __forceinline__ uint32_t int4_zero(uint32_t word) {
     const uint32_t z = word >> 16;
     return (z | z << 16) | (BF16 ? 0x43004300u : 0x64006400u);
 }
+// Sixteen lanes of tensor memory x 64 columns: lane 4 g + t has, of every eight columns, 2 t and 2 t + 1 of lanes g (two words) and g + 8.
+__device__ __forceinline__ void tmem_store_fragments(uint32_t tmem, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+          "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+          "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(tmem) : "memory");
+}
 
-// A CTA of eight warps has 16 features; the warps share their columns, a group (64 columns at least) in turn.
-constexpr int kInt4Warps = 8;
+// 64 columns of TOKENS tokens, zeros beyond both.
+__device__ __forceinline__ void token_box(uint32_t dst, const CUtensorMap* map, int column, int token, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(column), "r"(token), "r"(bar) : "memory");
+}
 
-template <int TILES, bool BF16>
-__global__ void __launch_bounds__(kInt4Warps * 32) int4_few_kernel(const Int4Args p) {
-    __shared__ float parts[kInt4Warps][TILES * 8][kInt4Rows + 1];
+template <int TOKENS, int GROUP, bool BF16>
+__global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4Args p, const __grid_constant__ CUtensorMap x_map) {
+    using S = Int4Tensor<TOKENS, GROUP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem), bar0 = base + S::kBars;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + S::kSmem - 16);
+    volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 12);
+    const auto full = [&](int s) { return bar0 + 8u * s; };                                     // a tile and its tokens have come
+    const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    const auto ready = [&](int b) { return bar0 + 8u * (2 * S::kStages + b); };                 // a tile is in tensor memory
+    const auto used = [&](int b) { return bar0 + 8u * (2 * S::kStages + kInt4Buffers + b); };
+    const auto summed = [&](int d) { return bar0 + 8u * (2 * S::kStages + 2 * kInt4Buffers + d); };      // a group's accumulator
+    const auto taken = [&](int d) { return bar0 + 8u * (2 * S::kStages + 2 * kInt4Buffers + kInt4Sums + d); };
+    const uint32_t drained = bar0 + 8u * (2 * S::kStages + 2 * kInt4Buffers + 2 * kInt4Sums);
+
+    const int part = blockIdx.x % p.parts;
+    const int64_t at = blockIdx.x / p.parts, token0 = at % p.token_tiles * TOKENS, row_tile = at / p.token_tiles;
+    const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
+    const int k0 = (int)((int64_t)p.chunks * part / p.parts), count = (int)((int64_t)p.chunks * (part + 1) / p.parts) - k0;      // this CTA's tiles
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kInt4Workers / 2 + kInt4Adders + 1); }
+        for (int b = 0; b < kInt4Buffers; ++b) { mbar_init(ready(b), kInt4Workers / 2); mbar_init(used(b), 1); }
+        for (int d = 0; d < kInt4Sums; ++d) { mbar_init(summed(d), 1); mbar_init(taken(d), kInt4Adders); }
+        mbar_init(drained, 1);
+        failed = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    if (warp == 0 && lane == 0) prefetch_map(&x_map);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
     griddep_wait();
     griddep_launch();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t tile = blockIdx.x, token0 = (int64_t)blockIdx.y * (TILES * 8);
-    const int tokens = (int)min((int64_t)(TILES * 8), p.tokens - token0);
-    const uint4* codes = reinterpret_cast<const uint4*>(p.w + tile * p.blocks * kInt4BlockBytes) + lane;
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(p.w + (int64_t)gridDim.x * p.blocks * kInt4BlockBytes) + tile * p.groups * kInt4Rows;
-    const uint16_t* x = static_cast<const uint16_t*>(p.x) + token0 * p.x_stride;
-    const int unit = max(p.group, kInt4Cols), units = p.blocks * kInt4Cols / unit;
 
-    float acc[TILES][4];
+    float acc[TOKENS];      // of the adding warps
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
+            int i = 0;
+            for (; i < count; ++i) {
+                const int s = i % S::kStages;
+                if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
+                const uint32_t to = base + s * S::kStage;
+                mbar_expect_tx(full(s), S::kX + S::kTile);
+                bulk_g2s(to + S::kX, w + (int64_t)i * S::kTile, S::kTile, full(s));
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
-    for (int u = warp; u < units; u += kInt4Warps) {
-        // a unit is one group of 128 (two blocks), one of 64, or two of 32 (half a block each)
-        float part[TILES][4];
-        uint32_t lo = 0u, hi = 0u;
-#pragma unroll 1
-        for (int h = 0; h < unit / 32; ++h) {
-            const int k = u * unit + h * 32;
-            if ((k & (p.group - 1)) == 0) {
-                lo = scales[(k / p.group) * kInt4Rows + g];
-                hi = scales[(k / p.group) * kInt4Rows + g + 8];
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) { part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f; }
+                for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
             }
-            const uint2 w = reinterpret_cast<const uint2*>(codes + (k >> 6) * 32)[(k >> 5) & 1];
-            const uint32_t zlo = int4_zero<BF16>(lo), zhi = int4_zero<BF16>(hi);
-            uint32_t a[2][4];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint32_t v = s ? w.y : w.x;
-                a[s][0] = int4_pair<BF16>(v, 0, zlo);
-                a[s][1] = int4_pair<BF16>(v, 1, zhi);
-                a[s][2] = int4_pair<BF16>(v, 2, zlo);
-                a[s][3] = int4_pair<BF16>(v, 3, zhi);
+            // no copy and no arrival may come after this CTA is gone
+            for (int j = max(0, i - S::kStages); j < i; ++j) {
+                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
+                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
             }
+        }
+    } else if (warp == 1) {
+        const uint32_t lead = elect_one(), instruction = half_instruction(BF16, TOKENS, false);
+        bool ok = true;
+        int n = 0;      // groups so far
+        for (int i = 0; i < count && ok; ++i) {
+            const int b = i % kInt4Buffers, s = i % S::kStages;
+            ok = warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed) && warp_wait(ready(b), (uint32_t)(i / kInt4Buffers) & 1u, &failed);
+            if (!ok) break;
+            const uint32_t x = base + s * S::kStage;
 #pragma unroll
-            for (int n = 0; n < TILES; ++n) {
-                const int token = n * 8 + g;
-                const Raw8 b = load_raw8(x, MPS_BF16, token * p.x_stride + k + 8 * t, token < tokens ? p.cols - (k + 8 * t) : 0, p.x_vec);
-                multiply<BF16>(part[n], a[0], b.a.x, b.a.y);
-                multiply<BF16>(part[n], a[1], b.a.z, b.a.w);
+            for (int g = 0; g < S::kGroups; ++g, ++n) {
+                const int d = n % kInt4Sums;
+                if (n >= kInt4Sums) ok = ok && warp_wait(taken(d), (uint32_t)(n / kInt4Sums - 1) & 1u, &failed);
+                if (!ok) break;
+                tensor_fence_after();
+#pragma unroll
+                for (int k = g * (GROUP / 16); k < (g + 1) * (GROUP / 16); ++k)      // 16 columns: eight of tensor memory, 32 bytes of a token's row
+                    half_multiply_kept(lead, tmem + S::kSumColumns + d * TOKENS, tmem + b * 64 + k * 8, operand_desc(x + k / 4 * (TOKENS * 128)) + 2 * (k & 3), instruction,
+                                       k > g * (GROUP / 16) ? 1u : 0u);
+                tensor_commit(lead, summed(d));
             }
-            if (((k + 32) & (p.group - 1)) == 0) {
-                const float slo = int4_scale(lo, p.scale_bf16), shi = int4_scale(hi, p.scale_bf16);
+            if (ok) {
+                tensor_commit(lead, used(b));
+                tensor_commit(lead, empty(s));
+            }
+        }
+        tensor_commit(lead, drained);
+        warp_wait(drained, 0, &failed);
+    } else if (warp < 2 + kInt4Workers) {
+        // a quarter of tensor memory's lanes: sixteen rows, and sixteen more
+        const int quarter = warp & 3, g = lane >> 2;
+        for (int i = warp >= 6; i < count; i += 2) {
+            const int b = i % kInt4Buffers, s = i % S::kStages;
+            if (!warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+            const uint8_t* tile = smem + s * S::kStage + S::kX;
+            const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
+            const uint4 w[4] = {codes[0], codes[32], codes[64], codes[96]};
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + quarter * (S::kGroups * 32) + g;
+            uint32_t zeros[2][S::kGroups][2];      // of rows g and g + 8
 #pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-                    acc[n][0] = fmaf(slo, part[n][0], acc[n][0]);
-                    acc[n][1] = fmaf(slo, part[n][1], acc[n][1]);
-                    acc[n][2] = fmaf(shi, part[n][2], acc[n][2]);
-                    acc[n][3] = fmaf(shi, part[n][3], acc[n][3]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < S::kGroups; ++j) {
+                    zeros[h][j][0] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16]);
+                    zeros[h][j][1] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16 + 8]);
                 }
+            if (i >= kInt4Buffers && !warp_wait(used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
+            tensor_fence_after();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t r[32];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {      // 16 columns of the product
+                    const uint4& v4 = w[h * 2 + (k >> 2)];
+                    const uint32_t v = (k & 3) == 0 ? v4.x : (k & 3) == 1 ? v4.y : (k & 3) == 2 ? v4.z : v4.w;
+                    const uint32_t(&z)[2] = zeros[h][k * 16 / GROUP];
+                    r[4 * k] = int4_pair<BF16>(v, 0, z[0]);
+                    r[4 * k + 1] = int4_pair<BF16>(v, 2, z[0]);
+                    r[4 * k + 2] = int4_pair<BF16>(v, 1, z[1]);
+                    r[4 * k + 3] = int4_pair<BF16>(v, 3, z[1]);
+                }
+                tmem_store_fragments(tmem + ((uint32_t)(quarter * 32 + h * 16) << 16) + b * 64, r);
+            }
+            tmem_stored();
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(ready(b));
+                mbar_arrive(empty(s));
+            }
+        }
+    } else {
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + S::kSumColumns;
+#pragma unroll
+        for (int t = 0; t < TOKENS; ++t) acc[t] = 0.f;
+        bool ok = true;
+        int n = 0;
+        for (int i = 0; i < count && ok; ++i) {
+            const int s = i % S::kStages;
+            ok = warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed);
+            if (!ok) break;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(smem + s * S::kStage + S::kX + kInt4CodeBytes);
+            float scale[S::kGroups];
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g) scale[g] = int4_scale(words[int4_scale_word(row, g, S::kGroups)], p.scale_bf16);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+#pragma unroll
+            for (int g = 0; g < S::kGroups; ++g, ++n) {
+                const int d = n % kInt4Sums;
+                ok = ok && warp_wait(summed(d), (uint32_t)(n / kInt4Sums) & 1u, &failed);
+                if (!ok) break;
+                tensor_fence_after();
+                constexpr int kStep = TOKENS < 32 ? TOKENS : 32;
+#pragma unroll
+                for (int c = 0; c < TOKENS; c += kStep) {
+                    if (c < tokens) {
+                        float v[kStep];
+                        if constexpr (kStep == 16) tmem_load16(from + d * TOKENS + c, v);
+                        else tmem_load32(from + d * TOKENS + c, v);
+                        const float2 s2 = make_float2(scale[g], scale[g]);
+#pragma unroll
+                        for (int t = 0; t < kStep; t += 2) {
+                            const float2 sum = fma2(s2, make_float2(v[t], v[t + 1]), make_float2(acc[c + t], acc[c + t + 1]));
+                            acc[c + t] = sum.x;
+                            acc[c + t + 1] = sum.y;
+                        }
+                    }
+                }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(taken(d));
             }
         }
     }
+    const bool adds = warp >= 2 + kInt4Workers;
+    const int own_row = (warp & 3) * 32 + lane;
+    const int64_t feature = row_tile * kInt4Rows;
+    const auto put = [&](int token, int row, float v) {
+        if (feature + row < p.rows) static_cast<uint16_t*>(p.out)[(token0 + token) * p.out_stride + feature + row] = (uint16_t)pack2(v, 0.f, p.out_dtype);
+    };
+    __syncwarp();
+    tensor_fence_before();
+    if (p.parts == 1) {
+        if (adds && !failed) {
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) {
-        parts[warp][n * 8 + 2 * t][g] = acc[n][0];
-        parts[warp][n * 8 + 2 * t + 1][g] = acc[n][1];
-        parts[warp][n * 8 + 2 * t][g + 8] = acc[n][2];
-        parts[warp][n * 8 + 2 * t + 1][g + 8] = acc[n][3];
+            for (int t = 0; t < TOKENS; ++t)
+                if (t < tokens) put(t, own_row, acc[t]);
+        }
+    } else {
+        float* sums = reinterpret_cast<float*>(smem);      // [token][row]: whatever the ring held has been used
+        __syncthreads();
+        if (adds) {
+#pragma unroll
+            for (int t = 0; t < TOKENS; ++t)
+                if (t < tokens) sums[t * kInt4Rows + own_row] = acc[t];
+        }
+        cluster_sync();
+        if (!failed) {
+            // every parts-th token is this CTA's, a warp has 128 rows of one at a time
+            for (int t = part + warp * p.parts; t < tokens; t += kInt4Threads / 32 * p.parts) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int g = 0; g < kInt4MostParts; ++g)
+                    if (g < p.parts) add4(v, load_peer(peer_address(base + t * (kInt4Rows * 4) + lane * 16, g)));
+                put(t, lane * 4, v.x);
+                put(t, lane * 4 + 1, v.y);
+                put(t, lane * 4 + 2, v.z);
+                put(t, lane * 4 + 3, v.w);
+            }
+        }
+        cluster_sync();      // nobody leaves while his sums are read
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < tokens * kInt4Rows; i += kInt4Warps * 32) {
-        const int token = i / kInt4Rows, r = i % kInt4Rows;
-        const int64_t row = tile * kInt4Rows + r;
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kInt4Warps; ++w) v += parts[w][token][r];
-        if (row < p.rows) static_cast<uint16_t*>(p.out)[(token0 + token) * p.out_stride + row] = (uint16_t)pack2(v, 0.f, p.out_dtype);
-    }
+    tensor_fence_after();
+    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
+    if (warp == 1) tmem_free<1>(tmem, S::kColumns);
 }
 
-template <int TILES>
-static int launch_few(const Int4Args& p, bool bf16, cudaStream_t st) {
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+// The tokens as boxes of 64 columns x `box` rows; rows begin at multiples of 16 bytes.
+static int token_map(CUtensorMap& map, const void* x, int64_t tokens, int64_t cols, int64_t stride, bool bf16, int box) {
+    EncodeTiled encode;
+    const int rc = tensor_map_encoder(encode);
+    if (rc) return rc;
+    const cuuint64_t size[2] = {(cuuint64_t)cols, (cuuint64_t)tokens}, pitch[1] = {(cuuint64_t)(tokens > 1 ? stride : (cols + 7) / 8 * 8) * 2};
+    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, step[2] = {1, 1};
+    const CUresult r = encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x), size, pitch, boxes, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
+}
+
+struct Int4Tokens { const void* x; int64_t cols, stride; };
+
+template <int TOKENS, int GROUP, bool BF16>
+static int launch_tensor(Int4Args p, const Int4Tokens& x, const Device& d, cudaStream_t st) {
+    using S = Int4Tensor<TOKENS, GROUP>;
+    static std::atomic<uint64_t> ready{0};
+    if (!(ready.load(std::memory_order_acquire) >> (d.ordinal & 63) & 1)) {
+        MPS_CUDA_TRY(cudaFuncSetAttribute(int4_tensor_kernel<TOKENS, GROUP, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
+    }
+    CUtensorMap map;
+    const int rc = token_map(map, x.x, p.tokens, x.cols, x.stride, BF16, TOKENS);
+    if (rc) return rc;
+    p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
+    const int64_t tiles = int4_row_tiles(p.rows) * p.token_tiles;
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kInt4MostParts, p.chunks), d.sms / tiles));
+    if (tiles * p.parts > 0x7FFFFFFF) { set_error("mps_int4_product: too many tiles for one launch"); return MPS_ERR_INVALID; }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned int)((p.rows + kInt4Rows - 1) / kInt4Rows), (unsigned int)((p.tokens + TILES * 8 - 1) / (TILES * 8)));
-    config.blockDim = dim3(kInt4Warps * 32);
+    config.gridDim = dim3((unsigned int)(tiles * p.parts));
+    config.blockDim = dim3(kInt4Threads);
+    config.dynamicSmemBytes = S::kSmem;
     config.stream = st;
-    cudaLaunchAttribute overlap;
-    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &overlap;
-    config.numAttrs = 1;
-    const cudaError_t e = bf16 ? cudaLaunchKernelEx(&config, int4_few_kernel<TILES, true>, p) : cudaLaunchKernelEx(&config, int4_few_kernel<TILES, false>, p);
-    return e == cudaSuccess ? MPS_OK : cuda_fail(e, "int4_few_kernel");
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = (unsigned int)p.parts;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&config, int4_tensor_kernel<TOKENS, GROUP, BF16>, p, map);
+    return e == cudaSuccess ? MPS_OK : cuda_fail(e, "int4_tensor_kernel");
+}
+template <int TOKENS, bool BF16>
+static int launch_tokens(const Int4Args& p, const Int4Tokens& x, int group, const Device& d, cudaStream_t st) {
+    return group == 128 ? launch_tensor<TOKENS, 128, BF16>(p, x, d, st) : group == 64 ? launch_tensor<TOKENS, 64, BF16>(p, x, d, st)
+                                                                                      : launch_tensor<TOKENS, 32, BF16>(p, x, d, st);
+}
+template <bool BF16>
+static int launch_product(const Int4Args& p, const Int4Tokens& x, int group, const Device& d, cudaStream_t st) {
+    return p.tokens <= 16 ? launch_tokens<16, BF16>(p, x, group, d, st) : p.tokens <= 32 ? launch_tokens<32, BF16>(p, x, group, d, st)
+                                                                                         : launch_tokens<64, BF16>(p, x, group, d, st);
+}
+
+// Tokens whose rows do not begin at multiples of 16 bytes, as tiled copies want them, or lie over one another: copied into rows that do.
+__global__ void __launch_bounds__(256) int4_align_kernel(const uint16_t* __restrict__ x, int64_t stride, int64_t tokens, int32_t cols, int32_t wide, uint16_t* __restrict__ out) {
+    griddep_wait();
+    griddep_launch();
+    const int64_t all = tokens * wide, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += step) {
+        const int64_t token = i / wide, col = i - token * wide;
+        out[i] = col < cols ? x[token * stride + col] : (uint16_t)0;
+    }
 }
 
 }  // namespace mps
@@ -255,7 +477,7 @@ static int launch_few(const Int4Args& p, bool bf16, cudaStream_t st) {
 using namespace mps;
 
 extern "C" int64_t mps_int4_bytes(int64_t rows, int64_t cols, int32_t group) {
-    return int4_size_ok(rows, cols, group) ? int4_shape(rows, cols, group).bytes() : -1;
+    return int4_size_ok(rows, cols, group) ? int4_row_tiles(rows) * int4_chunks(cols) * int4_tile_bytes(group) : -1;
 }
 
 extern "C" int mps_int4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t rows, int64_t cols, int32_t group, void* data,
@@ -264,8 +486,8 @@ extern "C" int mps_int4_pack(const uint8_t* codes, const uint16_t* scales, const
     if (rows == 0) return MPS_OK;
     if (!codes || !scales || !data) { set_error("mps_int4_pack: null pointer"); return MPS_ERR_INVALID; }
     if (reinterpret_cast<uintptr_t>(data) & 15u) { set_error("mps_int4_pack: unaligned data"); return MPS_ERR_INVALID; }
-    const int64_t words = int4_shape(rows, cols, group).codes_bytes() / 4;
-    return launch_overlapping("int4_pack_kernel", int4_pack_kernel, (unsigned int)min((words + 255) / 256, int64_t(1) << 20), dim3(256),
+    const int64_t tiles = int4_row_tiles(rows) * int4_chunks(cols);
+    return launch_overlapping("int4_pack_kernel", int4_pack_kernel, (unsigned int)std::min(tiles, int64_t(1) << 20), dim3(256),
                               static_cast<cudaStream_t>(stream), Int4Parts{codes, scales, zeros, rows, cols, group}, static_cast<uint8_t*>(data));
 }
 
@@ -275,12 +497,12 @@ extern "C" int mps_int4_dequantize(const void* data, int64_t rows, int64_t cols,
     if (rows == 0) return MPS_OK;
     if (!data || !out) { set_error("mps_int4_dequantize: null pointer"); return MPS_ERR_INVALID; }
     if (reinterpret_cast<uintptr_t>(data) & 15u) { set_error("mps_int4_dequantize: unaligned data"); return MPS_ERR_INVALID; }
-    const int64_t words = int4_shape(rows, cols, group).codes_bytes() / 4;
-    return launch_overlapping("int4_values_kernel", int4_values_kernel, (unsigned int)min((words + 255) / 256, int64_t(1) << 20), dim3(256),
+    const int64_t tiles = int4_row_tiles(rows) * int4_chunks(cols);
+    return launch_overlapping("int4_values_kernel", int4_values_kernel, (unsigned int)std::min(tiles, int64_t(1) << 20), dim3(256),
                               static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(data), rows, cols, group, (int)(scale_dtype == MPS_BF16), (int)dtype, out);
 }
 
-extern "C" int mps_int4_product(const mps_int4_linear* args, void* stream) {
+extern "C" int mps_int4_product(const mps_int4_linear* args, void* workspace, int64_t workspace_bytes, void* stream) {
     if (!args) { set_error("mps_int4_product: null arguments"); return MPS_ERR_INVALID; }
     const mps_int4_linear& a = *args;
     if (a.rows <= 0 || !int4_size_ok(a.rows, a.cols, a.group)) { set_error("mps_int4_product: rows, cols or group out of range"); return MPS_ERR_INVALID; }
@@ -293,26 +515,33 @@ extern "C" int mps_int4_product(const mps_int4_linear* args, void* stream) {
     if (a.tokens == 0) return MPS_OK;
     if (!a.x || !a.w || !a.out) { set_error("mps_int4_product: null pointer"); return MPS_ERR_INVALID; }
     if (reinterpret_cast<uintptr_t>(a.w) & 15u) { set_error("mps_int4_product: unaligned weight"); return MPS_ERR_INVALID; }
-    const Int4Shape shape = int4_shape(a.rows, a.cols, a.group);
-    Int4Args p;
-    p.x = a.x;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < mps_mx4_workspace_bytes()) {
+        set_error("mps_int4_product: workspace missing, unaligned or too small");
+        return MPS_ERR_WORKSPACE;
+    }
+    Device d;
+    const int rc = current_device(d);
+    if (rc) return rc;
+    Int4Args p = {};
+    p.workspace = static_cast<uint32_t*>(workspace);
     p.w = static_cast<const uint8_t*>(a.w);
     p.out = a.out;
-    p.x_stride = a.x_stride;
     p.out_stride = a.out_stride;
     p.tokens = a.tokens;
     p.rows = a.rows;
-    p.cols = (int32_t)a.cols;
-    p.group = a.group;
-    p.blocks = shape.blocks;
-    p.groups = shape.groups;
+    p.chunks = (int32_t)int4_chunks(a.cols);
     p.out_dtype = a.out_dtype;
     p.scale_bf16 = a.scale_dtype == MPS_BF16;
-    p.x_vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.x_stride % 8 == 0 || a.tokens == 1);
-    const bool bf16 = a.x_dtype == MPS_BF16;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.tokens <= 8) return launch_few<1>(p, bf16, st);
-    if (a.tokens <= 16) return launch_few<2>(p, bf16, st);
-    if (a.tokens <= 32) return launch_few<4>(p, bf16, st);
-    return launch_few<8>(p, bf16, st);
+    Int4Tokens x = {a.x, a.cols, a.x_stride};
+    if (reinterpret_cast<uintptr_t>(a.x) % 16 || (a.tokens > 1 && (a.x_stride % 8 || a.x_stride < a.cols))) {
+        if (!a.x_rows || reinterpret_cast<uintptr_t>(a.x_rows) % 16) { set_error("mps_int4_product: x_rows missing or unaligned"); return MPS_ERR_WORKSPACE; }
+        const int64_t wide = (a.cols + 7) / 8 * 8;
+        const int rc2 = launch_overlapping("int4_align_kernel", int4_align_kernel, (unsigned int)std::min((a.tokens * wide + 255) / 256, int64_t(1) << 16), dim3(256), st,
+                                           static_cast<const uint16_t*>(a.x), a.x_stride, a.tokens, (int32_t)a.cols, (int32_t)wide, static_cast<uint16_t*>(a.x_rows));
+        if (rc2) return rc2;
+        x.x = a.x_rows;
+        x.stride = wide;
+    }
+    return a.x_dtype == MPS_BF16 ? launch_product<true>(p, x, a.group, d, st) : launch_product<false>(p, x, a.group, d, st);
 }

@@ -13,6 +13,7 @@
 // codes of the least scale; rows beyond the last are never read as values (they are what the memory holds).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -294,6 +295,8 @@ constexpr int64_t kMx4MostNormRows = 0x7FFFFFFF, kMx4MostNormCols = 32768;
 
 struct Device { int ordinal, sms; };
 int current_device(Device& d);
+// The driver's encoder of tensor maps (mx4_linear.cu).
+int tensor_map_encoder(decltype(&cuTensorMapEncodeTiled)& encode);
 
 // A launch that may overlap the end of the kernel before it.
 template <typename... Params, typename... Args>
@@ -301,6 +304,23 @@ inline int launch_overlapping(const char* what, void (*kernel)(Params...), unsig
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(ctas);
     config.blockDim = threads;
+    config.stream = st;
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
+}
+
+// A launch with dynamic shared memory that may overlap the end of the kernel before it.
+template <typename... Params, typename... Args>
+inline int launch_overlapping_smem(const char* what, void (*kernel)(Params...), unsigned int ctas, dim3 threads, int smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas);
+    config.blockDim = threads;
+    config.dynamicSmemBytes = (size_t)smem;
     config.stream = st;
     cudaLaunchAttribute overlap;
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;

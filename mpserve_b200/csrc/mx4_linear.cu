@@ -717,9 +717,9 @@ static int tile_map(CUtensorMap& map, EncodeTiled encode, const void* tiles, int
                               CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
 }
-static int wide_maps(WideMaps& m, const ProductArgs& p) {
+int tensor_map_encoder(EncodeTiled& encode) {
     static std::atomic<EncodeTiled> known{nullptr};
-    EncodeTiled encode = known.load(std::memory_order_relaxed);
+    encode = known.load(std::memory_order_relaxed);
     if (!encode) {
         void* entry = nullptr;
         cudaDriverEntryPointQueryResult found;
@@ -728,6 +728,12 @@ static int wide_maps(WideMaps& m, const ProductArgs& p) {
         encode = reinterpret_cast<EncodeTiled>(entry);
         known.store(encode, std::memory_order_relaxed);
     }
+    return MPS_OK;
+}
+static int wide_maps(WideMaps& m, const ProductArgs& p) {
+    EncodeTiled encode;
+    const int found = tensor_map_encoder(encode);
+    if (found) return found;
     int rc = tile_map(m.x, encode, p.x, mx4_row_tiles(p.tokens), p.chunks, kMx4TileMapRows);
     if (!rc) rc = tile_map(m.w_scales, encode, p.w, p.row_tiles, p.chunks, 1);
     if (!rc) rc = tile_map(m.w_codes, encode, p.w, p.row_tiles, p.chunks, kMx4TileMapRows - 1);

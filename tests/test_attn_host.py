@@ -14,16 +14,14 @@ def lib():
 
 
 def test_packed_arguments_have_the_sizes_of_their_structs():
-    assert _lib.INT4_LINEAR.size == 3 * 8 + 5 * 8 + 4 * 4
+    assert _lib.INT4_LINEAR.size == 4 * 8 + 5 * 8 + 4 * 4
     assert _lib.HEAD_ROTATE.size == 12 * 8 + 15 * 8 + 8 * 4 + 2 * 4
     assert _lib.PREFIX_ATTEND.size == 8 * 8 + 13 * 8 + 4 * 4 + 4 + 4      # the last four fill up to a multiple of 8
 
 
 @pytest.mark.parametrize("rows,cols,group", [(0, 1, 32), (1, 1, 128), (16, 64, 64), (17, 65, 32), (14336, 4096, 128), (1 << 27, 1 << 24, 32)])
 def test_bytes_of_a_weight(lib, rows, cols, group):
-    unit = max(group, 64)
-    wide = -(-cols // unit) * unit
-    want = -(-rows // 16) * 16 * (wide // 2 + wide // group * 4)
+    want = -(-rows // 128) * -(-cols // 128) * (128 * 128 // 2 + 128 * (128 // group) * 4)
     assert lib.mps_int4_bytes(rows, cols, group) == want == int4._bytes(rows, cols, group)
 
 
@@ -48,11 +46,11 @@ def _attend(**kw):
 
 def test_errors_come_back_from_the_c_entries(lib):
     bad = _lib.MPS_ERR_INVALID
-    linear = lambda *a: lib.mps_int4_product(_lib.INT4_LINEAR.pack(*a), None)  # noqa: E731
+    linear = lambda x, *a: lib.mps_int4_product(_lib.INT4_LINEAR.pack(x, 0, *a), None, 0, None)  # noqa: E731
     rotate = lambda **kw: lib.mps_head_rotate_rows(_rotate(**kw), None)  # noqa: E731
     attend = lambda **kw: lib.mps_prefix_attend_tokens(_attend(**kw), None, 0, None, 0, None)  # noqa: E731
     for call, text in (
-            (lambda: lib.mps_int4_product(None, None), b"null"), (lambda: linear(16, 16, 16, 1, 64, 8, 64, 8, 100, 0, 0, 0), b"group"),
+            (lambda: lib.mps_int4_product(None, None, 0, None), b"null"), (lambda: linear(16, 16, 16, 1, 64, 8, 64, 8, 100, 0, 0, 0), b"group"),
             (lambda: linear(16, 16, 16, 1, 64, 0, 64, 8, 64, 0, 0, 0), b"rows"), (lambda: linear(16, 16, 16, -1, 64, 8, 64, 8, 64, 0, 0, 0), b"tokens"),
             (lambda: linear(16, 16, 16, 1, 64, 8, 64, 8, 64, 2, 0, 0), b"dtypes"), (lambda: linear(16, 16, 16, 1, 64, 8, 64, 8, 64, 0, 0, 2), b"dtypes"),
             (lambda: linear(0, 16, 16, 1, 64, 8, 64, 8, 64, 0, 0, 0), b"null"), (lambda: linear(16, 8, 16, 1, 64, 8, 64, 8, 64, 0, 0, 0), b"unaligned"),
