@@ -14,6 +14,7 @@
 #include "mx4.cuh"
 #include "mx4_tensor.cuh"
 #include "stream_common.cuh"
+#include "warp_mma.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -118,15 +119,13 @@ __global__ void __launch_bounds__(256) int4_values_kernel(const uint8_t* __restr
 
 // ---- products -------------------------------------------------------------------------------------------
 //
-// A CTA has 128 features for up to TOKENS tokens, and a share of the columns: a cluster of up to eight shares a row of tiles, as many as fill the GPU, and adds
-// its CTAs' sums up in shared memory, always in the same order.  A tile and its columns of the tokens come into a ring of some 200 KB.  Warps:
-//   0 copies;  1 multiplies: features (left operand, tensor memory) by tokens (right operand, shared memory), a group of columns into an accumulator of its own;
-//   2 to 9 take codes apart and store them in tensor memory, four warps a tile, 32 rows each: two tiles at a time, since what one takes is mostly waits in a row;
-//   10 to 13 add the groups' accumulators up, times their scales: a thread has a feature, its tokens are in registers.
-// Bound: memory; and taking codes apart, some 100 instructions for 16 rows of a tile, 200 cycles of an SM's issue slots for 8.5 KB.
+// Two kernels.  In both a CTA has 128 features for up to TOKENS tokens, and a share of the columns: a cluster of up to eight shares a row of tiles, as many as fill the
+// GPU, and adds its CTAs' sums up in shared memory, always in the same order.  A tile and its columns of the tokens come into a ring of some 200 KB: tiles as one
+// bulk copy each (to issue one costs a thread some 100 cycles: with 1 KB copies that was what the kernel took), the tokens by a warp of their own.
 constexpr int kInt4Workers = 8, kInt4Adders = 4, kInt4Threads = (2 + kInt4Workers + kInt4Adders) * 32;
 constexpr int kInt4Buffers = 4, kInt4Sums = 4, kInt4MostParts = 8;
 constexpr int kInt4Smem = 227 << 10;
+constexpr int kInt4FewTokens = 32;
 
 struct Int4Args {
     const uint8_t* w;
@@ -135,6 +134,7 @@ struct Int4Args {
     int32_t chunks, parts, token_tiles;
     int32_t out_dtype;
     bool scale_bf16;
+    bool even;               // rows of the output begin at multiples of 8 bytes
     uint32_t* workspace;     // word 0 records a wait that ran out
 };
 
@@ -180,12 +180,183 @@ __device__ __forceinline__ void tmem_store_fragments(uint32_t tmem, const uint32
           "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(tmem) : "memory");
 }
 
+// The sums of a cluster's CTAs, [token][row] at the start of each one's shared memory, into the output: every parts-th token is this CTA's, a warp has 128 rows of
+// one at a time.  All threads take part; nobody leaves while his sums are read.
+__device__ __forceinline__ void finish_tile(const Int4Args& p, uint32_t sums, int64_t row_tile, int64_t token0, int tokens, int part, int warp, int lane, int warps, bool failed) {
+    if (p.parts > 1) cluster_sync(); else __syncthreads();
+    if (!failed) {
+        const int64_t feature = row_tile * kInt4Rows + lane * 4;
+        for (int t = part + warp * p.parts; t < tokens; t += warps * p.parts) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < kInt4MostParts; ++g) {
+                const uint32_t at = sums + t * (kInt4Rows * 4) + lane * 16;
+                if (g < p.parts) add4(v, load_peer(p.parts > 1 ? peer_address(at, g) : at));
+            }
+            uint16_t* to = static_cast<uint16_t*>(p.out) + (token0 + t) * p.out_stride + feature;
+            const uint32_t lo = pack2(v.x, v.y, p.out_dtype), hi = pack2(v.z, v.w, p.out_dtype);
+            if (p.even && feature + 4 <= p.rows) {
+                *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
+            } else {
+                if (feature < p.rows) to[0] = (uint16_t)lo;
+                if (feature + 1 < p.rows) to[1] = (uint16_t)(lo >> 16);
+                if (feature + 2 < p.rows) to[2] = (uint16_t)hi;
+                if (feature + 3 < p.rows) to[3] = (uint16_t)(hi >> 16);
+            }
+        }
+    }
+    __syncwarp();
+    if (p.parts > 1) cluster_sync();
+}
+
 // 64 columns of TOKENS tokens, zeros beyond both.
 __device__ __forceinline__ void token_box(uint32_t dst, const CUtensorMap* map, int column, int token, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(column), "r"(token), "r"(bar) : "memory");
 }
 
+// ---- up to 32 tokens: codes stay in registers -----------------------------------------------------------
+//
+// Sixteen warps, two sets of eight that take tiles in turn, a warp 16 rows: a code word becomes the left operand of an m16n8k16 where it is, and a group's products
+// are multiplied by its scale in registers.  Bound: memory; taking codes apart (11 instructions for eight codes, half of them on a pipe that takes two a
+// cycle) some 220 cycles an SM for 8.5 KB, the products of eight tokens 130.
+constexpr int kFewWarps = 16, kFewThreads = (2 + kFewWarps) * 32;
+template <int TOKENS, int GROUP>
+struct Int4Few {
+    static constexpr int kGroups = kInt4Cols / GROUP, kTile = int4_tile_bytes(GROUP);
+    static constexpr int kX = TOKENS * kInt4Cols * 2;
+    static constexpr int kStage = (kX + kTile + 1023) / 1024 * 1024;
+    static constexpr int kStages = std::min(18, (kInt4Smem - 1024) / kStage);
+    static constexpr int kBars = kStages * kStage;
+    static constexpr int kSmem = kBars + 2 * kStages * 8 + 16;
+    static_assert(kSmem <= kInt4Smem && kX % 1024 == 0, "shared memory");
+    static_assert(2 * TOKENS * kInt4Rows * 4 <= kBars, "sums take the ring's place");
+};
+
+template <int TOKENS, int GROUP, bool BF16>
+__global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args p, const __grid_constant__ CUtensorMap x_map) {
+    using S = Int4Few<TOKENS, GROUP>;
+    constexpr int kTiles = TOKENS / 8;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem), bar0 = base + S::kBars;
+    volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 12);
+    const auto full = [&](int s) { return bar0 + 8u * s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    const int part = blockIdx.x % p.parts;
+    const int64_t at = blockIdx.x / p.parts, token0 = at % p.token_tiles * TOKENS, row_tile = at / p.token_tiles;
+    const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
+    const int k0 = (int)((int64_t)p.chunks * part / p.parts), count = (int)((int64_t)p.chunks * (part + 1) / p.parts) - k0;      // this CTA's tiles
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 2); mbar_init(empty(s), kFewWarps / 2); }
+        failed = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch();
+    float acc[kTiles][4];
+    if (warp < 2) {
+        if (lane == 0) {
+            const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
+            int i = 0;
+            for (; i < count; ++i) {
+                const int s = i % S::kStages;
+                if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
+                const uint32_t to = base + s * S::kStage;
+                if (warp == 0) {
+                    mbar_expect_tx(full(s), S::kTile);
+                    bulk_g2s(to + S::kX, w + (int64_t)i * S::kTile, S::kTile, full(s));
+                } else {
+                    mbar_expect_tx(full(s), S::kX);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
+                }
+            }
+            // no copy may come after this CTA is gone
+            for (int j = max(0, i - S::kStages); j < i; ++j) {
+                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
+                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
+            }
+        }
+    } else {
+        const int rows16 = warp - 2 & 7, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
+        // four columns of token g, 16 k + 4 t on: piece 2 k + t / 2 of the row's eight, XORed with the row
+        const auto x_at = [&](int n, int k) {
+            return (k >> 2) * (TOKENS * 128) + (n * 8 + g) * 128 + (((2 * (k & 3) + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
+        };
+        for (int i = warp >= 10; i < count; i += 2) {
+            const int s = i % S::kStages;
+            if (!warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+            const uint8_t* x = smem + s * S::kStage;
+            const uint8_t* tile = x + S::kX;
+            const uint4* codes = reinterpret_cast<const uint4*>(tile + rows16 * 1024) + lane;
+            const uint4 w[2] = {codes[0], codes[32]};
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + rows16 * (S::kGroups * 16) + g;
+            uint32_t lo[S::kGroups], hi[S::kGroups];
+#pragma unroll
+            for (int j = 0; j < S::kGroups; ++j) {
+                lo[j] = words[j * 16];
+                hi[j] = words[j * 16 + 8];
+            }
+            // products of 64 columns (32 in groups of 32) do not wait for those of the next
+            constexpr int kParts = GROUP == 32 ? 4 : 2;
+            float part_sum[kTiles][kParts][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int j = k * 16 / GROUP, c = k * kParts / 8;
+                const uint32_t zlo = int4_zero<BF16>(lo[j]), zhi = int4_zero<BF16>(hi[j]);
+                const uint4& v4 = w[k >> 2];
+                const uint32_t v = (k & 3) == 0 ? v4.x : (k & 3) == 1 ? v4.y : (k & 3) == 2 ? v4.z : v4.w;
+                const uint32_t a[4] = {int4_pair<BF16>(v, 0, zlo), int4_pair<BF16>(v, 1, zhi), int4_pair<BF16>(v, 2, zlo), int4_pair<BF16>(v, 3, zhi)};
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    if (k * kParts % 8 == 0) part_sum[n][c][0] = part_sum[n][c][1] = part_sum[n][c][2] = part_sum[n][c][3] = 0.f;
+                    const uint2 b = *reinterpret_cast<const uint2*>(x + x_at(n, k));
+                    multiply<BF16>(part_sum[n][c], a, b.x, b.y);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+#pragma unroll
+            for (int j = 0; j < S::kGroups; ++j) {
+                const float slo = int4_scale(lo[j], p.scale_bf16), shi = int4_scale(hi[j], p.scale_bf16);
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float sum = GROUP == 128 ? part_sum[n][0][e] + part_sum[n][1][e] : part_sum[n][j][e];
+                        acc[n][e] = fmaf(e < 2 ? slo : shi, sum, acc[n][e]);
+                    }
+            }
+        }
+    }
+    __syncwarp();
+    __syncthreads();      // whatever the ring held has been used
+    if (warp >= 2) {
+        // the two sets' sums beside one another, then added
+        float* sums = reinterpret_cast<float*>(smem) + (warp >= 10 ? TOKENS * kInt4Rows : 0) + (warp - 2 & 7) * 16 + (lane >> 2);
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * (lane & 3) + (e & 1)) * kInt4Rows + (e >> 1) * 8] = acc[n][e];
+    }
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(smem);
+    for (int i = threadIdx.x; i < tokens * kInt4Rows; i += kFewThreads) sums[i] += sums[TOKENS * kInt4Rows + i];
+    finish_tile(p, base, row_tile, token0, tokens, part, warp, lane, kFewThreads / 32, failed != 0u);
+    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
+}
+
+// ---- more tokens: codes go to tensor memory ---------------------------------------------------------------
+//
+// Warps:
+//   0 copies;  1 multiplies: features (left operand, tensor memory) by tokens (right operand, shared memory), a group of columns into an accumulator of its own;
+//   2 to 9 take codes apart and store them in tensor memory, four warps a tile, 32 rows each: two tiles at a time, since what one takes is mostly waits in a row;
+//   10 to 13 add the groups' accumulators up, times their scales: a thread has a feature, its tokens are in registers.
+// Bound: the left operand: its 32 KB of a tile cost the tensor core some 700 cycles, however few tokens there are.
 template <int TOKENS, int GROUP, bool BF16>
 __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4Args p, const __grid_constant__ CUtensorMap x_map) {
     using S = Int4Tensor<TOKENS, GROUP>;
@@ -250,13 +421,15 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         int n = 0;      // groups so far
         for (int i = 0; i < count && ok; ++i) {
             const int b = i % kInt4Buffers, s = i % S::kStages;
-            ok = warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed) && warp_wait(ready(b), (uint32_t)(i / kInt4Buffers) & 1u, &failed);
+            // of a tile that is in tensor memory the tokens have come, too: those who put it there have seen it.  A sum's first place is free from the start: the phase
+            // before the first counts as over.
+            ok = warp_wait2(ready(b), (uint32_t)(i / kInt4Buffers) & 1u, taken(n % kInt4Sums), (uint32_t)(n / kInt4Sums - 1) & 1u, &failed);
             if (!ok) break;
             const uint32_t x = base + s * S::kStage;
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g, ++n) {
                 const int d = n % kInt4Sums;
-                if (n >= kInt4Sums) ok = ok && warp_wait(taken(d), (uint32_t)(n / kInt4Sums - 1) & 1u, &failed);
+                if (g) ok = ok && warp_wait(taken(d), (uint32_t)(n / kInt4Sums - 1) & 1u, &failed);
                 if (!ok) break;
                 tensor_fence_after();
 #pragma unroll
@@ -277,7 +450,8 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         const int quarter = warp & 3, g = lane >> 2;
         for (int i = warp >= 6; i < count; i += 2) {
             const int b = i % kInt4Buffers, s = i % S::kStages;
-            if (!warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+            if (!warp_wait2(full(s), (uint32_t)(i / S::kStages) & 1u, used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
+            tensor_fence_after();
             const uint8_t* tile = smem + s * S::kStage + S::kX;
             const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
             const uint4 w[4] = {codes[0], codes[32], codes[64], codes[96]};
@@ -290,8 +464,6 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
                     zeros[h][j][0] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16]);
                     zeros[h][j][1] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16 + 8]);
                 }
-            if (i >= kInt4Buffers && !warp_wait(used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
-            tensor_fence_after();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t r[32];
@@ -324,18 +496,16 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         int n = 0;
         for (int i = 0; i < count && ok; ++i) {
             const int s = i % S::kStages;
-            ok = warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed);
+            ok = warp_wait2(full(s), (uint32_t)(i / S::kStages) & 1u, summed(n % kInt4Sums), (uint32_t)(n / kInt4Sums) & 1u, &failed);
             if (!ok) break;
             const uint32_t* words = reinterpret_cast<const uint32_t*>(smem + s * S::kStage + S::kX + kInt4CodeBytes);
             float scale[S::kGroups];
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g) scale[g] = int4_scale(words[int4_scale_word(row, g, S::kGroups)], p.scale_bf16);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty(s));
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g, ++n) {
                 const int d = n % kInt4Sums;
-                ok = ok && warp_wait(summed(d), (uint32_t)(n / kInt4Sums) & 1u, &failed);
+                if (g) ok = ok && warp_wait(summed(d), (uint32_t)(n / kInt4Sums) & 1u, &failed);
                 if (!ok) break;
                 tensor_fence_after();
                 constexpr int kStep = TOKENS < 32 ? TOKENS : 32;
@@ -358,46 +528,19 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
                 __syncwarp();
                 if (lane == 0) mbar_arrive(taken(d));
             }
+            if (lane == 0 && ok) mbar_arrive(empty(s));
         }
     }
-    const bool adds = warp >= 2 + kInt4Workers;
-    const int own_row = (warp & 3) * 32 + lane;
-    const int64_t feature = row_tile * kInt4Rows;
-    const auto put = [&](int token, int row, float v) {
-        if (feature + row < p.rows) static_cast<uint16_t*>(p.out)[(token0 + token) * p.out_stride + feature + row] = (uint16_t)pack2(v, 0.f, p.out_dtype);
-    };
     __syncwarp();
     tensor_fence_before();
-    if (p.parts == 1) {
-        if (adds && !failed) {
+    __syncthreads();      // whatever the ring held has been used
+    if (warp >= 2 + kInt4Workers) {
+        float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-            for (int t = 0; t < TOKENS; ++t)
-                if (t < tokens) put(t, own_row, acc[t]);
-        }
-    } else {
-        float* sums = reinterpret_cast<float*>(smem);      // [token][row]: whatever the ring held has been used
-        __syncthreads();
-        if (adds) {
-#pragma unroll
-            for (int t = 0; t < TOKENS; ++t)
-                if (t < tokens) sums[t * kInt4Rows + own_row] = acc[t];
-        }
-        cluster_sync();
-        if (!failed) {
-            // every parts-th token is this CTA's, a warp has 128 rows of one at a time
-            for (int t = part + warp * p.parts; t < tokens; t += kInt4Threads / 32 * p.parts) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int g = 0; g < kInt4MostParts; ++g)
-                    if (g < p.parts) add4(v, load_peer(peer_address(base + t * (kInt4Rows * 4) + lane * 16, g)));
-                put(t, lane * 4, v.x);
-                put(t, lane * 4 + 1, v.y);
-                put(t, lane * 4 + 2, v.z);
-                put(t, lane * 4 + 3, v.w);
-            }
-        }
-        cluster_sync();      // nobody leaves while his sums are read
+        for (int t = 0; t < TOKENS; ++t)
+            if (t < tokens) sums[t * kInt4Rows + (warp & 3) * 32 + lane] = acc[t];
     }
+    finish_tile(p, base, row_tile, token0, tokens, part, warp, lane, kInt4Threads / 32, failed != 0u);
     __syncthreads();
     tensor_fence_after();
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
@@ -419,16 +562,15 @@ static int token_map(CUtensorMap& map, const void* x, int64_t tokens, int64_t co
 
 struct Int4Tokens { const void* x; int64_t cols, stride; };
 
-template <int TOKENS, int GROUP, bool BF16>
-static int launch_tensor(Int4Args p, const Int4Tokens& x, const Device& d, cudaStream_t st) {
-    using S = Int4Tensor<TOKENS, GROUP>;
-    static std::atomic<uint64_t> ready{0};
+template <int TOKENS, typename Kernel>
+static int launch_kernel(const char* what, Kernel kernel, int smem, int threads, std::atomic<uint64_t>& ready, Int4Args p, const Int4Tokens& x, bool bf16, const Device& d,
+                         cudaStream_t st) {
     if (!(ready.load(std::memory_order_acquire) >> (d.ordinal & 63) & 1)) {
-        MPS_CUDA_TRY(cudaFuncSetAttribute(int4_tensor_kernel<TOKENS, GROUP, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        MPS_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
     }
     CUtensorMap map;
-    const int rc = token_map(map, x.x, p.tokens, x.cols, x.stride, BF16, TOKENS);
+    const int rc = token_map(map, x.x, p.tokens, x.cols, x.stride, bf16, TOKENS);
     if (rc) return rc;
     p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
     const int64_t tiles = int4_row_tiles(p.rows) * p.token_tiles;
@@ -436,8 +578,8 @@ static int launch_tensor(Int4Args p, const Int4Tokens& x, const Device& d, cudaS
     if (tiles * p.parts > 0x7FFFFFFF) { set_error("mps_int4_product: too many tiles for one launch"); return MPS_ERR_INVALID; }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned int)(tiles * p.parts));
-    config.blockDim = dim3(kInt4Threads);
-    config.dynamicSmemBytes = S::kSmem;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
     config.stream = st;
     cudaLaunchAttribute attributes[2];
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -447,18 +589,26 @@ static int launch_tensor(Int4Args p, const Int4Tokens& x, const Device& d, cudaS
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&config, int4_tensor_kernel<TOKENS, GROUP, BF16>, p, map);
-    return e == cudaSuccess ? MPS_OK : cuda_fail(e, "int4_tensor_kernel");
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p, map);
+    return e == cudaSuccess ? MPS_OK : cuda_fail(e, what);
+}
+template <int TOKENS, int GROUP, bool BF16>
+static int launch_group(const Int4Args& p, const Int4Tokens& x, const Device& d, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    if constexpr (TOKENS <= kInt4FewTokens)
+        return launch_kernel<TOKENS>("int4_few_kernel", int4_few_kernel<TOKENS, GROUP, BF16>, Int4Few<TOKENS, GROUP>::kSmem, kFewThreads, ready, p, x, BF16, d, st);
+    else
+        return launch_kernel<TOKENS>("int4_tensor_kernel", int4_tensor_kernel<TOKENS, GROUP, BF16>, Int4Tensor<TOKENS, GROUP>::kSmem, kInt4Threads, ready, p, x, BF16, d, st);
 }
 template <int TOKENS, bool BF16>
 static int launch_tokens(const Int4Args& p, const Int4Tokens& x, int group, const Device& d, cudaStream_t st) {
-    return group == 128 ? launch_tensor<TOKENS, 128, BF16>(p, x, d, st) : group == 64 ? launch_tensor<TOKENS, 64, BF16>(p, x, d, st)
-                                                                                      : launch_tensor<TOKENS, 32, BF16>(p, x, d, st);
+    return group == 128 ? launch_group<TOKENS, 128, BF16>(p, x, d, st) : group == 64 ? launch_group<TOKENS, 64, BF16>(p, x, d, st)
+                                                                                     : launch_group<TOKENS, 32, BF16>(p, x, d, st);
 }
 template <bool BF16>
 static int launch_product(const Int4Args& p, const Int4Tokens& x, int group, const Device& d, cudaStream_t st) {
-    return p.tokens <= 16 ? launch_tokens<16, BF16>(p, x, group, d, st) : p.tokens <= 32 ? launch_tokens<32, BF16>(p, x, group, d, st)
-                                                                                         : launch_tokens<64, BF16>(p, x, group, d, st);
+    return p.tokens <= 8 ? launch_tokens<8, BF16>(p, x, group, d, st) : p.tokens <= 16 ? launch_tokens<16, BF16>(p, x, group, d, st)
+         : p.tokens <= 32 ? launch_tokens<32, BF16>(p, x, group, d, st) : launch_tokens<64, BF16>(p, x, group, d, st);
 }
 
 // Tokens whose rows do not begin at multiples of 16 bytes, as tiled copies want them, or lie over one another: copied into rows that do.
@@ -532,6 +682,7 @@ extern "C" int mps_int4_product(const mps_int4_linear* args, void* workspace, in
     p.chunks = (int32_t)int4_chunks(a.cols);
     p.out_dtype = a.out_dtype;
     p.scale_bf16 = a.scale_dtype == MPS_BF16;
+    p.even = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.out_stride % 4 == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Int4Tokens x = {a.x, a.cols, a.x_stride};
     if (reinterpret_cast<uintptr_t>(a.x) % 16 || (a.tokens > 1 && (a.x_stride % 8 || a.x_stride < a.cols))) {

@@ -146,6 +146,14 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xFFFFFFFFu, bar_wait<CLUSTER>(bar, parity, failed));
 }
 
+// For two barriers, polled together.
+__device__ __forceinline__ bool warp_wait2(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, volatile uint32_t* failed) {
+    const bool first = mbar_try_wait(a, a_parity), second = mbar_try_wait(b, b_parity);
+    if (__all_sync(0xFFFFFFFFu, first && second)) return true;
+    const bool ok = bar_wait(a, a_parity, failed) && bar_wait(b, b_parity, failed);
+    return __all_sync(0xFFFFFFFFu, ok);
+}
+
 // Another CTA's shared memory, at the place that has this address in one's own.
 __device__ __forceinline__ uint32_t peer_address(uint32_t smem, int rank) {
     uint32_t a;
