@@ -159,16 +159,23 @@ __device__ __forceinline__ uint32_t subtract2(uint32_t a, uint32_t b) {
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// Two codes, nibble i of both halves of `w`, minus their zero point: `zero` is 128 + z in BF16 (1024 + z in F16), twice.
+// What codes are masked and completed with.  From registers: an instruction takes one of the two as it is, and the compiler, which knows both, would make two
+// instructions of one (one token through 14336 x 4096 took 12.5 us that way).
 template <bool BF16>
-__device__ __forceinline__ uint32_t int4_pair(uint32_t w, int i, uint32_t zero) {
-    return subtract2<BF16>(((w >> (4 * i)) & 0x000F000Fu) | (BF16 ? 0x43004300u : 0x64006400u), zero);
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t int4_zero(uint32_t word) {
-    const uint32_t z = word >> 16;
-    return (z | z << 16) | (BF16 ? 0x43004300u : 0x64006400u);
-}
+struct Int4Masks {
+    uint32_t mask, magic;
+    __device__ __forceinline__ Int4Masks() {
+        asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(mask));
+        asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300 : 0x64006400));
+    }
+    // Two codes, nibble i of both halves of `w`, minus their zero point: `zero` is 128 + z in BF16 (1024 + z in F16), twice.
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int i, uint32_t zero) const {
+        uint32_t r;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w >> (4 * i)), "r"(mask), "r"(magic));      // and, or
+        return subtract2<BF16>(r, zero);
+    }
+    __device__ __forceinline__ uint32_t zero(uint32_t word) const { return __byte_perm(word, 0u, 0x3232) | magic; }
+};
 // Sixteen lanes of tensor memory x 64 columns: lane 4 g + t has, of every eight columns, 2 t and 2 t + 1 of lanes g (two words) and g + 8.
 __device__ __forceinline__ void tmem_store_fragments(uint32_t tmem, const uint32_t (&r)[32]) {
     asm volatile(
@@ -209,6 +216,13 @@ __device__ __forceinline__ void finish_tile(const Int4Args& p, uint32_t sums, in
     if (p.parts > 1) cluster_sync();
 }
 
+// ... unless a wait ran out: no copy may come after the CTA is gone, or while sums take the ring's place.
+template <int STAGES, typename Full>
+__device__ __forceinline__ void copies_end(int asked, Full full) {
+    for (int i = max(0, asked - STAGES); i < asked; ++i) mbar_wait(full(i % STAGES), (uint32_t)(i / STAGES) & 1u, kMx4SpinLimit);
+    __syncthreads();
+}
+
 // 64 columns of TOKENS tokens, zeros beyond both.
 __device__ __forceinline__ void token_box(uint32_t dst, const CUtensorMap* map, int column, int token, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -217,10 +231,10 @@ __device__ __forceinline__ void token_box(uint32_t dst, const CUtensorMap* map, 
 
 // ---- up to 32 tokens: codes stay in registers -----------------------------------------------------------
 //
-// Sixteen warps, two sets of eight that take tiles in turn, a warp 16 rows: a code word becomes the left operand of an m16n8k16 where it is, and a group's products
-// are multiplied by its scale in registers.  Bound: memory; taking codes apart (11 instructions for eight codes, half of them on a pipe that takes two a
+// Sixteen warps, four sets of four that take tiles in turn, a warp 32 rows: a code word becomes the left operand of an m16n8k16 where it is, and a group's products
+// are multiplied by its scale in registers.  Bound: memory; taking codes apart (11 instructions for eight codes, seven of them on a pipe that takes two a
 // cycle) some 220 cycles an SM for 8.5 KB, the products of eight tokens 130.
-constexpr int kFewWarps = 16, kFewThreads = (2 + kFewWarps) * 32;
+constexpr int kFewSets = 4, kFewSetWarps = 4, kFewWarps = kFewSets * kFewSetWarps, kFewThreads = (2 + kFewWarps) * 32;
 template <int TOKENS, int GROUP>
 struct Int4Few {
     static constexpr int kGroups = kInt4Cols / GROUP, kTile = int4_tile_bytes(GROUP);
@@ -230,8 +244,10 @@ struct Int4Few {
     static constexpr int kBars = kStages * kStage;
     static constexpr int kSmem = kBars + 2 * kStages * 8 + 16;
     static_assert(kSmem <= kInt4Smem && kX % 1024 == 0, "shared memory");
-    static_assert(2 * TOKENS * kInt4Rows * 4 <= kBars, "sums take the ring's place");
+    static_assert(kFewSets * TOKENS * kInt4Rows * 4 <= kBars, "sums take the ring's place");
 };
+
+__device__ __forceinline__ int few_token(int column) { return column < 4 ? 2 * column : 2 * column - 7; }      // of eight
 
 template <int TOKENS, int GROUP, bool BF16>
 __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args p, const __grid_constant__ CUtensorMap x_map) {
@@ -248,14 +264,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
     const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
     const int k0 = (int)((int64_t)p.chunks * part / p.parts), count = (int)((int64_t)p.chunks * (part + 1) / p.parts) - k0;      // this CTA's tiles
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 2); mbar_init(empty(s), kFewWarps / 2); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 2); mbar_init(empty(s), kFewSetWarps); }
         failed = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     griddep_wait();
     griddep_launch();
-    float acc[kTiles][4];
+    float acc[2][kTiles][4];      // of two times 16 rows
+    int asked = 0;      // stages that this thread has filled
     if (warp < 2) {
         if (lane == 0) {
             const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
@@ -273,79 +290,102 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
                     for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
                 }
             }
-            // no copy may come after this CTA is gone
-            for (int j = max(0, i - S::kStages); j < i; ++j) {
-                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
-                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
-            }
+            asked = i;
         }
     } else {
-        const int rows16 = warp - 2 & 7, g = lane >> 2, t = lane & 3;
+        const int quarter = (warp - 2) % kFewSetWarps, set = (warp - 2) / kFewSetWarps, g = lane >> 2, t = lane & 3;
+        const Int4Masks<BF16> masks;
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n) { acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f; }
-        // four columns of token g, 16 k + 4 t on: piece 2 k + t / 2 of the row's eight, XORed with the row
-        const auto x_at = [&](int n, int k) {
-            return (k >> 2) * (TOKENS * 128) + (n * 8 + g) * 128 + (((2 * (k & 3) + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
-        };
-        for (int i = warp >= 10; i < count; i += 2) {
-            const int s = i % S::kStages;
-            if (!warp_wait(full(s), (uint32_t)(i / S::kStages) & 1u, &failed)) break;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) { acc[h][n][0] = acc[h][n][1] = acc[h][n][2] = acc[h][n][3] = 0.f; }
+        // Four columns of a token, 16 k + 4 t on: piece 2 k + t / 2 of its row's eight, XORed with the row.  Column g of a product is token few_token(g): four rows of
+        // which half a warp reads at once then have their pieces in different banks.
+        int x_at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x_at[k] = few_token(g) * 128 + (((2 * k + (t >> 1)) ^ few_token(g)) << 4) + (t & 1) * 8;
+        int s = set;
+        uint32_t parity = 0;
+        for (int i = set; i < count; i += kFewSets) {
+            if (!warp_wait(full(s), parity, &failed)) break;
             const uint8_t* x = smem + s * S::kStage;
             const uint8_t* tile = x + S::kX;
-            const uint4* codes = reinterpret_cast<const uint4*>(tile + rows16 * 1024) + lane;
-            const uint4 w[2] = {codes[0], codes[32]};
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + rows16 * (S::kGroups * 16) + g;
-            uint32_t lo[S::kGroups], hi[S::kGroups];
-#pragma unroll
-            for (int j = 0; j < S::kGroups; ++j) {
-                lo[j] = words[j * 16];
-                hi[j] = words[j * 16 + 8];
-            }
-            // products of 64 columns (32 in groups of 32) do not wait for those of the next
-            constexpr int kParts = GROUP == 32 ? 4 : 2;
-            float part_sum[kTiles][kParts][4];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int j = k * 16 / GROUP, c = k * kParts / 8;
-                const uint32_t zlo = int4_zero<BF16>(lo[j]), zhi = int4_zero<BF16>(hi[j]);
-                const uint4& v4 = w[k >> 2];
-                const uint32_t v = (k & 3) == 0 ? v4.x : (k & 3) == 1 ? v4.y : (k & 3) == 2 ? v4.z : v4.w;
-                const uint32_t a[4] = {int4_pair<BF16>(v, 0, zlo), int4_pair<BF16>(v, 1, zhi), int4_pair<BF16>(v, 2, zlo), int4_pair<BF16>(v, 3, zhi)};
-#pragma unroll
-                for (int n = 0; n < kTiles; ++n) {
-                    if (k * kParts % 8 == 0) part_sum[n][c][0] = part_sum[n][c][1] = part_sum[n][c][2] = part_sum[n][c][3] = 0.f;
-                    const uint2 b = *reinterpret_cast<const uint2*>(x + x_at(n, k));
-                    multiply<BF16>(part_sum[n][c], a, b.x, b.y);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty(s));
-#pragma unroll
-            for (int j = 0; j < S::kGroups; ++j) {
-                const float slo = int4_scale(lo[j], p.scale_bf16), shi = int4_scale(hi[j], p.scale_bf16);
+            const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + quarter * (S::kGroups * 32) + g;
+            uint2 b[TOKENS <= 16 ? kTiles : 1][8];
+            if (TOKENS <= 16) {
 #pragma unroll
                 for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float sum = GROUP == 128 ? part_sum[n][0][e] + part_sum[n][1][e] : part_sum[n][j][e];
-                        acc[n][e] = fmaf(e < 2 ? slo : shi, sum, acc[n][e]);
-                    }
+                    for (int k = 0; k < 8; ++k) b[TOKENS <= 16 ? n : 0][k] = *reinterpret_cast<const uint2*>(x + x_at[k & 3] + (k >> 2) * (TOKENS * 128) + n * 1024);
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint4 w[2] = {codes[h * 64], codes[h * 64 + 32]};
+                uint32_t lo[S::kGroups], hi[S::kGroups];
+#pragma unroll
+                for (int j = 0; j < S::kGroups; ++j) {
+                    lo[j] = words[(h * S::kGroups + j) * 16];
+                    hi[j] = words[(h * S::kGroups + j) * 16 + 8];
+                }
+                // products of 64 columns (32 in groups of 32) do not wait for those of the next
+                constexpr int kParts = GROUP == 32 ? 4 : 2;
+                float sums[kTiles][kParts][4];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int j = k * 16 / GROUP, c = k * kParts / 8;
+                    const uint32_t zlo = masks.zero(lo[j]), zhi = masks.zero(hi[j]);
+                    const uint4& v4 = w[k >> 2];
+                    const uint32_t v = (k & 3) == 0 ? v4.x : (k & 3) == 1 ? v4.y : (k & 3) == 2 ? v4.z : v4.w;
+                    const uint32_t a[4] = {masks.pair(v, 0, zlo), masks.pair(v, 1, zhi), masks.pair(v, 2, zlo), masks.pair(v, 3, zhi)};
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) {
+                        const uint2 y = TOKENS <= 16 ? b[TOKENS <= 16 ? n : 0][k] : *reinterpret_cast<const uint2*>(x + x_at[k & 3] + (k >> 2) * (TOKENS * 128) + n * 1024);
+                        if (k * kParts % 8 == 0) multiply_first<BF16>(sums[n][c], a, y.x, y.y);
+                        else multiply<BF16>(sums[n][c], a, y.x, y.y);
+                    }
+                }
+                if (h == 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(empty(s));
+                }
+#pragma unroll
+                for (int j = 0; j < S::kGroups; ++j) {
+                    const float slo = int4_scale(lo[j], p.scale_bf16), shi = int4_scale(hi[j], p.scale_bf16);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float sum = GROUP == 128 ? sums[n][0][e] + sums[n][1][e] : sums[n][j][e];
+                            acc[h][n][e] = fmaf(e < 2 ? slo : shi, sum, acc[h][n][e]);
+                        }
+                }
+            }
+            s += kFewSets;
+            if (s >= S::kStages) { s -= S::kStages; parity ^= 1u; }
         }
     }
     __syncwarp();
-    __syncthreads();      // whatever the ring held has been used
+    __syncthreads();      // whatever the ring held has been used ...
+    if (failed) copies_end<S::kStages>(asked, full);
     if (warp >= 2) {
-        // the two sets' sums beside one another, then added
-        float* sums = reinterpret_cast<float*>(smem) + (warp >= 10 ? TOKENS * kInt4Rows : 0) + (warp - 2 & 7) * 16 + (lane >> 2);
+        // the sets' sums beside one another, then added
+        float* sums = reinterpret_cast<float*>(smem) + (warp - 2) / kFewSetWarps * (TOKENS * kInt4Rows) + (warp - 2) % kFewSetWarps * 32 + (lane >> 2);
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sums[(n * 8 + 2 * (lane & 3) + (e & 1)) * kInt4Rows + (e >> 1) * 8] = acc[n][e];
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sums[(n * 8 + few_token(2 * (lane & 3) + (e & 1))) * kInt4Rows + h * 16 + (e >> 1) * 8] = acc[h][n][e];
     }
     __syncthreads();
     float* sums = reinterpret_cast<float*>(smem);
-    for (int i = threadIdx.x; i < tokens * kInt4Rows; i += kFewThreads) sums[i] += sums[TOKENS * kInt4Rows + i];
+    for (int i = threadIdx.x; i < tokens * kInt4Rows; i += kFewThreads) {
+        float v = sums[i];
+#pragma unroll
+        for (int set = 1; set < kFewSets; ++set) v += sums[set * (TOKENS * kInt4Rows) + i];
+        sums[i] = v;
+    }
     finish_tile(p, base, row_tile, token0, tokens, part, warp, lane, kFewThreads / 32, failed != 0u);
     if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
 }
@@ -396,6 +436,7 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
     griddep_launch();
 
     float acc[TOKENS];      // of the adding warps
+    int asked = 0;          // stages that this thread has filled
     if (warp == 0) {
         if (lane == 0) {
             const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
@@ -409,11 +450,7 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
 #pragma unroll
                 for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
             }
-            // no copy and no arrival may come after this CTA is gone
-            for (int j = max(0, i - S::kStages); j < i; ++j) {
-                const uint32_t parity = (uint32_t)(j / S::kStages) & 1u;
-                if (!bar_wait(empty(j % S::kStages), parity, &failed)) mbar_wait(full(j % S::kStages), parity, kMx4SpinLimit);
-            }
+            asked = i;
         }
     } else if (warp == 1) {
         const uint32_t lead = elect_one(), instruction = half_instruction(BF16, TOKENS, false);
@@ -448,6 +485,7 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
     } else if (warp < 2 + kInt4Workers) {
         // a quarter of tensor memory's lanes: sixteen rows, and sixteen more
         const int quarter = warp & 3, g = lane >> 2;
+        const Int4Masks<BF16> masks;
         for (int i = warp >= 6; i < count; i += 2) {
             const int b = i % kInt4Buffers, s = i % S::kStages;
             if (!warp_wait2(full(s), (uint32_t)(i / S::kStages) & 1u, used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
@@ -461,8 +499,8 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < S::kGroups; ++j) {
-                    zeros[h][j][0] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16]);
-                    zeros[h][j][1] = int4_zero<BF16>(words[(h * S::kGroups + j) * 16 + 8]);
+                    zeros[h][j][0] = masks.zero(words[(h * S::kGroups + j) * 16]);
+                    zeros[h][j][1] = masks.zero(words[(h * S::kGroups + j) * 16 + 8]);
                 }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -472,10 +510,10 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
                     const uint4& v4 = w[h * 2 + (k >> 2)];
                     const uint32_t v = (k & 3) == 0 ? v4.x : (k & 3) == 1 ? v4.y : (k & 3) == 2 ? v4.z : v4.w;
                     const uint32_t(&z)[2] = zeros[h][k * 16 / GROUP];
-                    r[4 * k] = int4_pair<BF16>(v, 0, z[0]);
-                    r[4 * k + 1] = int4_pair<BF16>(v, 2, z[0]);
-                    r[4 * k + 2] = int4_pair<BF16>(v, 1, z[1]);
-                    r[4 * k + 3] = int4_pair<BF16>(v, 3, z[1]);
+                    r[4 * k] = masks.pair(v, 0, z[0]);
+                    r[4 * k + 1] = masks.pair(v, 2, z[0]);
+                    r[4 * k + 2] = masks.pair(v, 1, z[1]);
+                    r[4 * k + 3] = masks.pair(v, 3, z[1]);
                 }
                 tmem_store_fragments(tmem + ((uint32_t)(quarter * 32 + h * 16) << 16) + b * 64, r);
             }
@@ -533,7 +571,8 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
     }
     __syncwarp();
     tensor_fence_before();
-    __syncthreads();      // whatever the ring held has been used
+    __syncthreads();      // whatever the ring held has been used ...
+    if (failed) copies_end<S::kStages>(asked, full);
     if (warp >= 2 + kInt4Workers) {
         float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
