@@ -120,9 +120,11 @@ __global__ void __launch_bounds__(256) int4_values_kernel(const uint8_t* __restr
 // ---- products -------------------------------------------------------------------------------------------
 //
 // Two kernels.  In both a CTA has 128 features for up to TOKENS tokens, and a share of the columns: a cluster of up to eight shares a row of tiles, as many as fill the
-// GPU, and adds its CTAs' sums up in shared memory, always in the same order.  A tile and its columns of the tokens come into a ring of some 200 KB: tiles as one
-// bulk copy each (to issue one costs a thread some 100 cycles: with 1 KB copies that was what the kernel took), the tokens by a warp of their own.
+// GPU, and adds its CTAs' sums up in shared memory, always in the same order.  Two tiles and their columns of the tokens come at a time into a ring of some 200 KB, as
+// one copy each: how many copies an SM has to start counts, not their bytes (31 MB in copies of 4.25 KB take 18.5 to 22.6 us, of 8.5 KB 12.4, of 17 KB 8.3, as
+// plain loads 8.3).
 constexpr int kInt4Workers = 8, kInt4Adders = 4, kInt4Threads = (2 + kInt4Workers + kInt4Adders) * 32;
+constexpr int kInt4StageTiles = 2;
 constexpr int kInt4Buffers = 4, kInt4Sums = 4, kInt4MostParts = 8;
 constexpr int kInt4Smem = 227 << 10;
 constexpr int kInt4FewTokens = 32;
@@ -133,6 +135,7 @@ struct Int4Args {
     int64_t out_stride, tokens, rows;
     int32_t chunks, parts, token_tiles;
     int32_t out_dtype;
+    bool whole;              // columns are a multiple of 64: the tokens' map has a third dimension, columns by 64
     bool scale_bf16;
     bool even;               // rows of the output begin at multiples of 8 bytes
     uint32_t* workspace;     // word 0 records a wait that ran out
@@ -141,9 +144,9 @@ struct Int4Args {
 template <int TOKENS, int GROUP>
 struct Int4Tensor {
     static constexpr int kGroups = kInt4Cols / GROUP, kTile = int4_tile_bytes(GROUP);
-    static constexpr int kX = TOKENS * kInt4Cols * 2;                                // two halves of 64 columns
-    static constexpr int kStage = (kX + kTile + 1023) / 1024 * 1024;                 // the tokens, then the tile
-    static constexpr int kStages = std::min(18, (kInt4Smem - 1024) / kStage);
+    static constexpr int kX = kInt4StageTiles * TOKENS * kInt4Cols * 2;              // by 64 columns
+    static constexpr int kStage = (kX + kInt4StageTiles * kTile + 1023) / 1024 * 1024;      // the tokens, then the tiles
+    static constexpr int kStages = (kInt4Smem - 1024) / kStage;
     static constexpr int kBars = kStages * kStage;
     static constexpr int kSmem = kBars + (2 * kStages + 2 * kInt4Buffers + 2 * kInt4Sums + 1) * 8 + 16;
     static constexpr int kSumColumns = kInt4Buffers * 64, kColumns = 512;            // tensor memory: left operands, then accumulators
@@ -223,10 +226,18 @@ __device__ __forceinline__ void copies_end(int asked, Full full) {
     __syncthreads();
 }
 
-// 64 columns of TOKENS tokens, zeros beyond both.
-__device__ __forceinline__ void token_box(uint32_t dst, const CUtensorMap* map, int column, int token, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(column), "r"(token), "r"(bar) : "memory");
+// Columns of TOKENS tokens, from column 64 `block` on, 64 a row, zeros beyond both.
+template <int TOKENS>
+__device__ __forceinline__ void token_boxes(uint32_t dst, const CUtensorMap* map, int block, int token, bool whole, uint32_t bar) {
+    if (whole) {
+        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(map), "r"(0), "r"(token), "r"(block), "r"(bar) : "memory");
+    } else {
+#pragma unroll
+        for (int h = 0; h < kInt4StageTiles * 2; ++h)
+            asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                         ::"r"(dst + h * (TOKENS * 128)), "l"(map), "r"((block + h) * 64), "r"(token), "r"(bar) : "memory");
+    }
 }
 
 // ---- up to 32 tokens: codes stay in registers -----------------------------------------------------------
@@ -238,12 +249,13 @@ constexpr int kFewSets = 4, kFewSetWarps = 4, kFewWarps = kFewSets * kFewSetWarp
 template <int TOKENS, int GROUP>
 struct Int4Few {
     static constexpr int kGroups = kInt4Cols / GROUP, kTile = int4_tile_bytes(GROUP);
-    static constexpr int kX = TOKENS * kInt4Cols * 2;
-    static constexpr int kStage = (kX + kTile + 1023) / 1024 * 1024;
-    static constexpr int kStages = std::min(18, (kInt4Smem - 1024) / kStage);
+    static constexpr int kX = kInt4StageTiles * TOKENS * kInt4Cols * 2;
+    static constexpr int kStage = (kX + kInt4StageTiles * kTile + 1023) / 1024 * 1024;
+    static constexpr int kStages = (kInt4Smem - 1024) / kStage;
     static constexpr int kBars = kStages * kStage;
     static constexpr int kSmem = kBars + 2 * kStages * 8 + 16;
     static_assert(kSmem <= kInt4Smem && kX % 1024 == 0, "shared memory");
+    static_assert(kFewSets % kInt4StageTiles == 0 && kStages >= kFewSets / kInt4StageTiles, "a set's tiles are in the same place of their stages");
     static_assert(kFewSets * TOKENS * kInt4Rows * 4 <= kBars, "sums take the ring's place");
 };
 
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
     const int tokens = (int)min((int64_t)TOKENS, p.tokens - token0);
     const int k0 = (int)((int64_t)p.chunks * part / p.parts), count = (int)((int64_t)p.chunks * (part + 1) / p.parts) - k0;      // this CTA's tiles
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 2); mbar_init(empty(s), kFewSetWarps); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 2); mbar_init(empty(s), kInt4StageTiles * kFewSetWarps); }
         failed = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -277,17 +289,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
         if (lane == 0) {
             const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
             int i = 0;
-            for (; i < count; ++i) {
-                const int s = i % S::kStages;
+            for (; i * kInt4StageTiles < count; ++i) {
+                const int s = i % S::kStages, tile = i * kInt4StageTiles;
                 if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
                 const uint32_t to = base + s * S::kStage;
                 if (warp == 0) {
-                    mbar_expect_tx(full(s), S::kTile);
-                    bulk_g2s(to + S::kX, w + (int64_t)i * S::kTile, S::kTile, full(s));
+                    const uint32_t bytes = min(kInt4StageTiles, count - tile) * S::kTile;
+                    mbar_expect_tx(full(s), bytes);
+                    bulk_g2s(to + S::kX, w + (int64_t)tile * S::kTile, bytes, full(s));
                 } else {
                     mbar_expect_tx(full(s), S::kX);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
+                    token_boxes<TOKENS>(to, &x_map, (k0 + tile) * 2, (int)token0, p.whole, full(s));
                 }
             }
             asked = i;
@@ -304,12 +316,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
         int x_at[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x_at[k] = few_token(g) * 128 + (((2 * k + (t >> 1)) ^ few_token(g)) << 4) + (t & 1) * 8;
-        int s = set;
+        int s = set / kInt4StageTiles;
         uint32_t parity = 0;
         for (int i = set; i < count; i += kFewSets) {
             if (!warp_wait(full(s), parity, &failed)) break;
-            const uint8_t* x = smem + s * S::kStage;
-            const uint8_t* tile = x + S::kX;
+            const uint8_t* x = smem + s * S::kStage + set % kInt4StageTiles * (TOKENS * kInt4Cols * 2);
+            const uint8_t* tile = smem + s * S::kStage + S::kX + set % kInt4StageTiles * S::kTile;
             const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
             const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + quarter * (S::kGroups * 32) + g;
             uint2 b[TOKENS <= 16 ? kTiles : 1][8];
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
                         }
                 }
             }
-            s += kFewSets;
+            s += kFewSets / kInt4StageTiles;
             if (s >= S::kStages) { s -= S::kStages; parity ^= 1u; }
         }
     }
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
     const int k0 = (int)((int64_t)p.chunks * part / p.parts), count = (int)((int64_t)p.chunks * (part + 1) / p.parts) - k0;      // this CTA's tiles
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kInt4Workers / 2 + kInt4Adders + 1); }
+        for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), kInt4StageTiles * (kInt4Workers / 2 + kInt4Adders + 1)); }
         for (int b = 0; b < kInt4Buffers; ++b) { mbar_init(ready(b), kInt4Workers / 2); mbar_init(used(b), 1); }
         for (int d = 0; d < kInt4Sums; ++d) { mbar_init(summed(d), 1); mbar_init(taken(d), kInt4Adders); }
         mbar_init(drained, 1);
@@ -441,14 +453,13 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         if (lane == 0) {
             const uint8_t* w = p.w + (row_tile * p.chunks + k0) * S::kTile;
             int i = 0;
-            for (; i < count; ++i) {
-                const int s = i % S::kStages;
+            for (; i * kInt4StageTiles < count; ++i) {
+                const int s = i % S::kStages, tile = i * kInt4StageTiles;
                 if (i >= S::kStages && !bar_wait(empty(s), (uint32_t)(i / S::kStages - 1) & 1u, &failed)) break;
-                const uint32_t to = base + s * S::kStage;
-                mbar_expect_tx(full(s), S::kX + S::kTile);
-                bulk_g2s(to + S::kX, w + (int64_t)i * S::kTile, S::kTile, full(s));
-#pragma unroll
-                for (int h = 0; h < 2; ++h) token_box(to + h * (TOKENS * 128), &x_map, (k0 + i) * kInt4Cols + h * 64, (int)token0, full(s));
+                const uint32_t to = base + s * S::kStage, bytes = min(kInt4StageTiles, count - tile) * S::kTile;
+                mbar_expect_tx(full(s), S::kX + bytes);
+                bulk_g2s(to + S::kX, w + (int64_t)tile * S::kTile, bytes, full(s));
+                token_boxes<TOKENS>(to, &x_map, (k0 + tile) * 2, (int)token0, p.whole, full(s));
             }
             asked = i;
         }
@@ -457,12 +468,12 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         bool ok = true;
         int n = 0;      // groups so far
         for (int i = 0; i < count && ok; ++i) {
-            const int b = i % kInt4Buffers, s = i % S::kStages;
+            const int b = i % kInt4Buffers, stage = i / kInt4StageTiles, s = stage % S::kStages;
             // of a tile that is in tensor memory the tokens have come, too: those who put it there have seen it.  A sum's first place is free from the start: the phase
             // before the first counts as over.
             ok = warp_wait2(ready(b), (uint32_t)(i / kInt4Buffers) & 1u, taken(n % kInt4Sums), (uint32_t)(n / kInt4Sums - 1) & 1u, &failed);
             if (!ok) break;
-            const uint32_t x = base + s * S::kStage;
+            const uint32_t x = base + s * S::kStage + i % kInt4StageTiles * (TOKENS * kInt4Cols * 2);
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g, ++n) {
                 const int d = n % kInt4Sums;
@@ -487,10 +498,10 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         const int quarter = warp & 3, g = lane >> 2;
         const Int4Masks<BF16> masks;
         for (int i = warp >= 6; i < count; i += 2) {
-            const int b = i % kInt4Buffers, s = i % S::kStages;
-            if (!warp_wait2(full(s), (uint32_t)(i / S::kStages) & 1u, used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
+            const int b = i % kInt4Buffers, stage = i / kInt4StageTiles, s = stage % S::kStages;
+            if (!warp_wait2(full(s), (uint32_t)(stage / S::kStages) & 1u, used(b), (uint32_t)(i / kInt4Buffers - 1) & 1u, &failed)) break;
             tensor_fence_after();
-            const uint8_t* tile = smem + s * S::kStage + S::kX;
+            const uint8_t* tile = smem + s * S::kStage + S::kX + i % kInt4StageTiles * S::kTile;
             const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
             const uint4 w[4] = {codes[0], codes[32], codes[64], codes[96]};
             const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + quarter * (S::kGroups * 32) + g;
@@ -533,10 +544,10 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
         bool ok = true;
         int n = 0;
         for (int i = 0; i < count && ok; ++i) {
-            const int s = i % S::kStages;
-            ok = warp_wait2(full(s), (uint32_t)(i / S::kStages) & 1u, summed(n % kInt4Sums), (uint32_t)(n / kInt4Sums) & 1u, &failed);
+            const int stage = i / kInt4StageTiles, s = stage % S::kStages;
+            ok = warp_wait2(full(s), (uint32_t)(stage / S::kStages) & 1u, summed(n % kInt4Sums), (uint32_t)(n / kInt4Sums) & 1u, &failed);
             if (!ok) break;
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(smem + s * S::kStage + S::kX + kInt4CodeBytes);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(smem + s * S::kStage + S::kX + i % kInt4StageTiles * S::kTile + kInt4CodeBytes);
             float scale[S::kGroups];
 #pragma unroll
             for (int g = 0; g < S::kGroups; ++g) scale[g] = int4_scale(words[int4_scale_word(row, g, S::kGroups)], p.scale_bf16);
@@ -587,14 +598,16 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
 }
 
 using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
-// The tokens as boxes of 64 columns x `box` rows; rows begin at multiples of 16 bytes.
+// The tokens as boxes of 64 columns x `box` rows (x as many 64 columns as a stage has, where the columns are a multiple of 64); rows begin at multiples of 16 bytes.
 static int token_map(CUtensorMap& map, const void* x, int64_t tokens, int64_t cols, int64_t stride, bool bf16, int box) {
     EncodeTiled encode;
     const int rc = tensor_map_encoder(encode);
     if (rc) return rc;
-    const cuuint64_t size[2] = {(cuuint64_t)cols, (cuuint64_t)tokens}, pitch[1] = {(cuuint64_t)(tokens > 1 ? stride : (cols + 7) / 8 * 8) * 2};
-    const cuuint32_t boxes[2] = {64, (cuuint32_t)box}, step[2] = {1, 1};
-    const CUresult r = encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(x), size, pitch, boxes, step,
+    const bool whole = cols % 64 == 0;
+    const cuuint64_t row = (cuuint64_t)(tokens > 1 ? stride : (cols + 7) / 8 * 8) * 2;
+    const cuuint64_t size[3] = {whole ? 64 : (cuuint64_t)cols, (cuuint64_t)tokens, (cuuint64_t)(cols / 64)}, pitch[2] = {row, 128};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)box, kInt4StageTiles * 2}, step[3] = {1, 1, 1};
+    const CUresult r = encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, whole ? 3 : 2, const_cast<void*>(x), size, pitch, boxes, step,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? MPS_OK : cuda_fail(static_cast<cudaError_t>(r), "cuTensorMapEncodeTiled");      // the two count their errors alike
 }
@@ -611,6 +624,7 @@ static int launch_kernel(const char* what, Kernel kernel, int smem, int threads,
     CUtensorMap map;
     const int rc = token_map(map, x.x, p.tokens, x.cols, x.stride, bf16, TOKENS);
     if (rc) return rc;
+    p.whole = x.cols % 64 == 0;
     p.token_tiles = (int)((p.tokens + TOKENS - 1) / TOKENS);
     const int64_t tiles = int4_row_tiles(p.rows) * p.token_tiles;
     p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kInt4MostParts, p.chunks), d.sms / tiles));
