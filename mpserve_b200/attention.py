@@ -69,17 +69,12 @@ class Rotary:
         return r
 
 
-def _strides(t: torch.Tensor) -> tuple[int, ...]:
-    """In elements; of a dimension of one, 0: what torch says there means nothing."""
-    return tuple(0 if n <= 1 else s for n, s in zip(t.shape, t.stride()))
-
-
 class KvCache:
     """The pages of a paged cache: ``k_pages`` and ``v_pages`` ``[pages, page_size, kv_heads, head_dim]``, one dtype (bfloat16, float16; float32 for
     ``norm_rotate_append`` alone), the last dimension of unit stride, the others of any that keeps 16-byte alignment; no two places share memory.  The tensors are the
-    caller's; slot ``i`` is place ``i % page_size`` of page ``i // page_size``.  ``page_size`` is a power of two."""
+    caller's, and cannot be replaced; slot ``i`` is place ``i % page_size`` of page ``i // page_size``.  ``page_size`` is a power of two."""
 
-    __slots__ = ("k_pages", "v_pages")
+    __slots__ = ("_k_pages", "_v_pages")
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
         for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
@@ -100,7 +95,7 @@ class KvCache:
             if dim > 1 and t.stride(3) != 1:
                 raise ValueError(f"{name} must have unit stride along its last dimension")
             unit = 16 // t.element_size()
-            if t.data_ptr() % 16 or any(s % unit for s in _strides(t)[:3]):
+            if t.data_ptr() % 16 or any(s % unit for n, s in zip(t.shape[:3], t.stride()[:3]) if n > 1):
                 raise ValueError(f"{name} must be 16-byte aligned, with strides that keep it so")
             reach = dim
             for n, s in sorted(zip(t.shape[:3], t.stride()[:3]), key=lambda ns: ns[1]):
@@ -108,89 +103,105 @@ class KvCache:
                     raise ValueError(f"{name} has places that share memory")
                 if n > 1:
                     reach = s * (n - 1) + reach
-        self.k_pages, self.v_pages = k_pages, v_pages
+        self._k_pages, self._v_pages = k_pages, v_pages
 
+    k_pages = property(lambda self: self._k_pages)
+    v_pages = property(lambda self: self._v_pages)
     pages = property(lambda self: self.k_pages.shape[0])
     page_size = property(lambda self: self.k_pages.shape[1])
     kv_heads = property(lambda self: self.k_pages.shape[2])
     head_dim = property(lambda self: self.k_pages.shape[3])
 
 
-def _heads(t, name: str) -> tuple[int, int, int, int, int]:
-    """(tokens, heads, dim, token stride, head stride)."""
+# The checks below are written out, tensor by tensor: as functions they were a third of the ten microseconds that a call took on the host.
+
+def _refuse_heads(t, name: str):
+    """Says what is wrong with what should have been ``[tokens, heads, head_dim]`` on a GPU."""
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise ValueError(f"{name} must have the dimensions [tokens, heads, head_dim]")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be bfloat16, float16 or float32")
-    tokens, heads, dim = t.shape
-    by_token, by_head, unit = t.stride()
-    if unit != 1 and dim > 1:
-        raise ValueError(f"{name} must have unit stride along its last dimension")
-    return tokens, heads, dim, by_token if tokens > 1 else 0, by_head if heads > 1 else 0
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    raise ValueError(f"{name} must have unit stride along its last dimension")
 
 
 def _head_weight(t, name: str, dim: int, index: int) -> tuple[int, int]:
-    if t is None:
-        return 0, -1
-    dtype = _DTYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
-    if dtype is None or t.dim() != 1 or t.shape[0] != dim or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype not in _DTYPES or t.dim() != 1 or t.numel() != dim or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous bfloat16, float16 or float32 vector of {dim} values")
     if t.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
-    return t.data_ptr(), dtype
+    return t.data_ptr(), _DTYPES[t.dtype]
 
 
 def _rotate(q, k, v, positions, rotary, cache, slots, q_weight, k_weight, eps):
-    tokens, q_heads, dim, q_token, q_head = _heads(q, "q")
-    k_tokens, kv_heads, k_dim, k_token, k_head = _heads(k, "k")
-    index, dtype = q.get_device(), q.dtype
+    for t, name in ((q, "q"), (k, "k")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            _refuse_heads(t, name)
+    (tokens, q_heads, dim), (k_tokens, kv_heads, k_dim) = q.shape, k.shape
+    (q_token, q_head, q_unit), (k_token, k_head, k_unit) = q.stride(), k.stride()
+    dtype, index = q.dtype, q.get_device()
+    kind = _DTYPES.get(dtype)
+    if kind is None or index < 0 or (q_unit != 1 and dim > 1):
+        _refuse_heads(q, "q")
     if k_tokens != tokens or k_dim != dim or k.dtype is not dtype:
         raise ValueError("q and k must have the same tokens, head_dim and dtype")
-    if q_heads < 1 or kv_heads < 1 or q_heads > _MOST_HEADS or kv_heads > _MOST_HEADS or dim < 1 or dim > _MOST_DIM:
+    if k_unit != 1 and dim > 1:
+        _refuse_heads(k, "k")
+    if not 0 < q_heads <= _MOST_HEADS or not 0 < kv_heads <= _MOST_HEADS or not 0 < dim <= _MOST_DIM:
         raise ValueError(f"there must be 1 to {_MOST_HEADS} heads of 1 to {_MOST_DIM} values")
     if not isinstance(rotary, Rotary):
         raise ValueError("rotary must be a Rotary")
-    if rotary.dims > dim:
-        raise ValueError(f"rotary turns {rotary.dims} values, a head has {dim}")
-    if not isinstance(positions, torch.Tensor) or (positions.dtype is not torch.int64 and positions.dtype is not torch.int32) or not positions.is_contiguous():
+    turned, turns, axis = rotary.dims, rotary._turns, rotary._axis
+    if turned > dim:
+        raise ValueError(f"rotary turns {turned} values, a head has {dim}")
+    if not isinstance(positions, torch.Tensor) or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int32 or int64 tensor")
-    shape = positions.shape
-    if shape[-1:] != (tokens,) or len(shape) > 2 or (shape[0] if len(shape) == 2 else 1) < rotary.axes:
+    wide, shape = positions.dtype is torch.int64, positions.shape
+    if not wide and positions.dtype is not torch.int32:
+        raise ValueError("positions must be a contiguous int32 or int64 tensor")
+    if len(shape) not in (1, 2) or shape[-1] != tokens or (shape[0] if len(shape) == 2 else 1) < rotary.axes:
         raise ValueError(f"positions must be [{tokens}] or, with a row for each of {rotary.axes} axes, [axes, {tokens}]")
-    if k.get_device() != index or positions.get_device() != index or rotary._turns.get_device() != index:
+    if k.get_device() != index or positions.get_device() != index or turns.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
-    qw, qw_dtype = _head_weight(q_weight, "q_weight", dim, index)
-    kw, kw_dtype = _head_weight(k_weight, "k_weight", dim, index)
-    if qw and kw and qw_dtype != kw_dtype:
-        raise ValueError("q_weight and k_weight must have the same dtype")
-    q_out = q.new_empty(tokens, q_heads, dim)
+    qw = kw = weight_kind = 0
+    if q_weight is not None:
+        qw, weight_kind = _head_weight(q_weight, "q_weight", dim, index)
+    if k_weight is not None:
+        q_kind = weight_kind
+        kw, weight_kind = _head_weight(k_weight, "k_weight", dim, index)
+        if qw and q_kind != weight_kind:
+            raise ValueError("q_weight and k_weight must have the same dtype")
     if cache is None:
         k_out = k.new_empty(tokens, kv_heads, dim)
         k_ptr, v_ptr, v_out, slots_ptr = k_out.data_ptr(), 0, 0, 0
-        rest = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        v_token = v_head = k_page = k_slot = k_place = v_page = v_slot = v_place = pages = page_size = 0
     else:
         if not isinstance(cache, KvCache):
             raise ValueError("cache must be a KvCache")
-        v_tokens, v_heads, v_dim, v_token, v_head = _heads(v, "v")
-        if v_tokens != tokens or v_heads != kv_heads or v_dim != dim or v.dtype is not dtype:
+        if not isinstance(v, torch.Tensor) or v.dim() != 3:
+            _refuse_heads(v, "v")
+        if v.shape != k.shape or v.dtype is not dtype:
             raise ValueError("k and v must have the same shape and dtype")
-        k_out, v_pages = cache.k_pages, cache.v_pages
+        v_token, v_head, v_unit = v.stride()
+        if v_unit != 1 and dim > 1:
+            _refuse_heads(v, "v")
+        k_out, v_pages = cache._k_pages, cache._v_pages
         pages, page_size, cache_heads, cache_dim = k_out.shape
         if cache_heads != kv_heads or cache_dim != dim or k_out.dtype is not dtype:
             raise ValueError("the cache must have the heads, head_dim and dtype of k")
-        if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.shape != (tokens,) or not slots.is_contiguous():
+        k_page, k_slot, k_place, _ = k_out.stride()
+        v_page, v_slot, v_place, _ = v_pages.stride()
+        if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or slots.dim() != 1 or slots.numel() != tokens or not slots.is_contiguous():
             raise ValueError(f"slots must be a contiguous int64 vector of {tokens} values")
         if v.get_device() != index or k_out.get_device() != index or slots.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
         k_ptr, v_ptr, v_out, slots_ptr = k_out.data_ptr(), v.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
-        rest = (v_token, v_head, *_strides(k_out)[:3], *_strides(v_pages)[:3], pages, page_size)
-    axis = rotary._axis
-    args = _lib.HEAD_ROTATE.pack(q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), k_ptr, v_out, qw, kw, positions.data_ptr(), rotary._turns.data_ptr(),
-                                 0 if axis is None else axis.data_ptr(), slots_ptr, tokens, q_token, q_head, k_token, k_head, *rest, q_heads, kv_heads,
-                                 dim, rotary.dims, rotary.interleaved, positions.dtype is torch.int64, _DTYPES[dtype], max(qw_dtype, kw_dtype, 0), eps,
-                                 rotary.scale)
+    q_out = q.new_empty(tokens, q_heads, dim)
+    args = _lib.HEAD_ROTATE.pack(q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), k_ptr, v_out, qw, kw, positions.data_ptr(), turns.data_ptr(),
+                                 0 if axis is None else axis.data_ptr(), slots_ptr, tokens, q_token, q_head, k_token, k_head, v_token, v_head, k_page, k_slot,
+                                 k_place, v_page, v_slot, v_place, pages, page_size, q_heads, kv_heads, dim, turned, rotary.interleaved, wide, kind, weight_kind,
+                                 eps, rotary.scale)
     if _current_device() == index:
         rc = _lib.load().mps_head_rotate_rows(args, _stream_of(index))
         if rc:
@@ -242,12 +253,17 @@ def shared_prefix_attention(q: torch.Tensor, cache: KvCache, tables: torch.Tenso
     A length below 0 counts as 0, one beyond its table as the table; keys of a page outside the cache are absent.  A query with nothing to attend to gets zeros.
     Softmax and sums are FP32; the weights of the values are rounded to the cache's dtype before they multiply them.
     With ``return_lse`` also the FP32 logarithms of the softmax's denominators, ``[batch, q_heads]``."""
-    batch, q_heads, dim, q_token, q_head = _heads(q, "q")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        _refuse_heads(q, "q")
+    batch, q_heads, dim = q.shape
+    q_token, q_head, q_unit = q.stride()
+    dtype, index = q.dtype, q.get_device()
+    if index < 0 or q_unit != 1:
+        _refuse_heads(q, "q")
     if not isinstance(cache, KvCache):
         raise ValueError("cache must be a KvCache")
-    k_pages, v_pages = cache.k_pages, cache.v_pages
+    k_pages, v_pages = cache._k_pages, cache._v_pages
     pages, page_size, kv_heads, cache_dim = k_pages.shape
-    dtype, index = q.dtype, q.get_device()
     if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError("q must be bfloat16 or float16")
     if k_pages.dtype is not dtype or cache_dim != dim:
@@ -260,17 +276,19 @@ def shared_prefix_attention(q: torch.Tensor, cache: KvCache, tables: torch.Tenso
         raise ValueError(f"q_heads must be a multiple of the cache's {kv_heads} heads, at most {_MOST_HEADS}")
     if batch > _MOST_SEQUENCES:
         raise ValueError(f"a batch has at most {_MOST_SEQUENCES} sequences")
-    if not isinstance(tables, torch.Tensor) or tables.dtype is not torch.int32 or tables.dim() != 2 or tables.shape[0] != batch or not tables.is_contiguous():
+    if not isinstance(tables, torch.Tensor) or tables.dtype is not torch.int32 or tables.dim() != 2 or not tables.is_contiguous():
         raise ValueError(f"tables must be a contiguous int32 matrix of {batch} rows")
-    if not isinstance(lengths, torch.Tensor) or lengths.dtype is not torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
+    table_rows, columns = tables.shape
+    if table_rows != batch:
+        raise ValueError(f"tables must be a contiguous int32 matrix of {batch} rows")
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.numel() != batch or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 vector of {batch} values")
-    prefix_length = int(prefix_length)
-    columns, prefix_ptr = tables.shape[1], 0
+    prefix_length, prefix_ptr = int(prefix_length), 0
     if prefix_length < 0:
         raise ValueError("prefix_length must not be negative")
     if prefix_length:
         if (not isinstance(prefix_table, torch.Tensor) or prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous()
-                or prefix_table.shape[0] * page_size < prefix_length):
+                or prefix_table.numel() * page_size < prefix_length):
             raise ValueError(f"prefix_table must be a contiguous int32 vector with the pages of {prefix_length} tokens")
         if prefix_table.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
@@ -279,8 +297,11 @@ def shared_prefix_attention(q: torch.Tensor, cache: KvCache, tables: torch.Tenso
         raise ValueError("a table and the prefix may have at most 2^30 tokens")
     if k_pages.get_device() != index or tables.get_device() != index or lengths.get_device() != index:
         raise ValueError("all tensors must be on the same CUDA device")
-    if (q_token | q_head) % 8 or q.data_ptr() % 16:
+    at = q.data_ptr()
+    if at % 16 or (q_token % 8 and batch > 1) or (q_head % 8 and q_heads > 1):
         raise ValueError("q must be 16-byte aligned, with strides that keep it so")
+    k_page, k_slot, k_place, _ = k_pages.stride()
+    v_page, v_slot, v_place, _ = v_pages.stride()
     out = q.new_empty(batch, q_heads, dim)
     lse = q.new_empty(batch, q_heads, dtype=torch.float32) if return_lse else None
     if batch:
@@ -288,9 +309,9 @@ def shared_prefix_attention(q: torch.Tensor, cache: KvCache, tables: torch.Tenso
         need = _scratch_bytes(index, batch, columns, prefix_length, page_size, q_heads, kv_heads, dim, kind)
         scratch = q.new_empty(need, dtype=torch.uint8)      # of this call: freed on return, and not handed to another stream before it is done
         ws = _workspace(index)
-        args = _lib.PREFIX_ATTEND.pack(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        args = _lib.PREFIX_ATTEND.pack(at, k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                        tables.data_ptr(), lengths.data_ptr(), prefix_ptr, batch, columns, prefix_length, pages, page_size, q_token, q_head,
-                                       *_strides(k_pages)[:3], *_strides(v_pages)[:3], q_heads, kv_heads, dim, kind, dim ** -0.5 if scale is None else scale)
+                                       k_page, k_slot, k_place, v_page, v_slot, v_place, q_heads, kv_heads, dim, kind, dim ** -0.5 if scale is None else scale)
         if _current_device() == index:
             rc = _lib.load().mps_prefix_attend_tokens(args, scratch.data_ptr(), need, ws.data_ptr(), ws.numel(), _stream_of(index))
             if rc:

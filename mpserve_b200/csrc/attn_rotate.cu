@@ -360,7 +360,14 @@ extern "C" int mps_head_rotate_rows(const mps_head_rotate* args, void* stream) {
     if (!args) { set_error("mps_head_rotate_rows: null arguments"); return MPS_ERR_INVALID; }
     RotateArgs p;
     p.a = *args;
+    mps_head_rotate& own = p.a;
     const mps_head_rotate& a = p.a;
+    // strides of dimensions of one mean nothing
+    if (a.tokens == 1) own.q_token_stride = own.k_token_stride = own.v_token_stride = 0;
+    if (a.q_heads == 1) own.q_head_stride = 0;
+    if (a.kv_heads == 1) own.k_head_stride = own.v_head_stride = own.k_cache_head_stride = own.v_cache_head_stride = 0;
+    if (a.pages == 1) own.k_page_stride = own.v_page_stride = 0;
+    if (a.page_size == 1) own.k_slot_stride = own.v_slot_stride = 0;
     if (a.tokens < 0 || a.tokens > 0x7FFFFFFF || a.q_heads < 0 || a.kv_heads < 0 || a.q_heads > MPS_MOST_HEADS || a.kv_heads > MPS_MOST_HEADS ||
         a.q_heads + a.kv_heads == 0) {
         set_error("mps_head_rotate_rows: tokens must be below 2^31, heads at most %d", (int)MPS_MOST_HEADS);

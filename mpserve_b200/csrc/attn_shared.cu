@@ -208,6 +208,11 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     if (rc) return rc;
     if (a.batch == 0) return MPS_OK;
     if (a.pages == 0) a.prefix_length = a.table_columns = 0;      // no key is there
+    // strides of dimensions of one mean nothing
+    if (a.batch == 1) a.q_token_stride = 0;
+    if (a.q_heads == 1) a.q_head_stride = 0;
+    if (a.kv_heads == 1) a.k_head_stride = a.v_head_stride = 0;
+    if (a.pages == 1) a.k_page_stride = a.v_page_stride = 0;
     if (!a.q || !a.out || (a.pages && (!a.k_pages || !a.v_pages)) || (a.table_columns && (!a.tables || !a.lengths)) || (a.prefix_length && !a.prefix_table)) {
         set_error("mps_prefix_attend_tokens: missing pointer");
         return MPS_ERR_INVALID;

@@ -65,7 +65,7 @@ def test_errors_come_back_from_the_c_entries(lib):
             (lambda: attend(page=8), b"power of two"), (lambda: attend(page=48), b"power of two"), (lambda: attend(q_heads=3, kv_heads=2), b"multiple"),
             (lambda: attend(batch=-1), b"batch"), (lambda: attend(prefix_length=(1 << 30) + 1), b"keys"), (lambda: attend(columns=1 << 27), b"keys"),
             (lambda: attend(q=0), b"missing"), (lambda: attend(prefix=0), b"missing"), (lambda: attend(tables=0), b"missing"), (lambda: attend(k=8), b"aligned"),
-            (lambda: attend(stride=4), b"aligned")):
+            (lambda: attend(stride=4, batch=2), b"aligned")):
         assert call() == bad
         assert text in lib.mps_last_error()
     # nothing to do is no error, and touches nothing
