@@ -24,8 +24,12 @@ struct AttendArgs {
     float* own_o;                      // [item][key head][query head of the group][dim]
     float2* own_ml;
     int64_t q_token, q_head, k_page, k_slot, k_head, v_page, v_slot, v_head;      // strides
-    int64_t table_columns, most_own, prefix, prefix_step, own_items, page_mask;
-    int32_t pages, page_shift, prefix_splits, prefix_units, batch, kv_heads, group;
+    int32_t* plan;                     // [0]: stretches of the prefix; from [1] on: the stretches of own keys before each sequence's first, and after the last's
+    int64_t table_columns, most_own, page_mask;
+    int32_t prefix, pages, page_shift, batch, kv_heads, group;
+    int32_t wide_tiles;                // CTAs for a stretch of the prefix and a key head
+    int32_t most_splits, own_items;    // places for stretches: of the prefix, of own keys
+    int32_t own_ctas;                  // where the host has settled who does what; else -1
     int32_t q_factor;                  // 1, -1 or 0: what queries are multiplied by, exactly
     float scale_log2;                  // positive
     uint32_t* workspace;               // word 0 records a wait that ran out
@@ -43,11 +47,20 @@ __device__ __forceinline__ uint32_t query_pair(uint32_t pair, int factor) {
     return factor == 1 ? pair : factor == -1 ? pair ^ 0x80008000u : times_zero<BF16>(pair);
 }
 
-// A sequence's own keys are cut into stretches of a length that is the same for all, such that no more come of it than there are places for: with
-// T keys in all, B sequences and P places, stretches of at least T / (P - B) are at most T / (T / (P - B)) + B.  How long sequences are is known on the
-// GPU only, so whoever works on stretches finds them for itself, from the lengths.  Lengths are at most 2^30.
-constexpr int kOwnLeast = 128;         // keys of a stretch, at least
+// How the work is split.  The prefix is cut into stretches that a CTA has for up to 256 rows of a key head; the other CTAs have the sequences' own keys, cut into stretches of
+// a length that is the same for all.  How long sequences are is known on the GPU only, so every CTA finds the split for itself, from the lengths: of all numbers
+// of stretches of the prefix that leave a CTA for the sequences, the one with which the slower side is soonest done.  What a side takes, in cycles, from
+// measurements at 1.9 GHz: a CTA that has a part of the prefix, its start and end and 128 keys for 256 rows or for 128; one that has sequences, its start and a
+// byte (some 95 GB/s an SM).
+constexpr int kPrefixKeys = 128, kPrefixRows = 128;
+constexpr int kPrefixStart = 9000, kPrefixPaired = 3000, kPrefixSingle = 1800, kOwnStart = 6000, kOwnBytesPerCycle = 50;
+constexpr int kOwnWarps = 14;              // that have own keys, of a CTA
+constexpr int kOwnLeast = 64;              // keys of a stretch, at least
+constexpr int kFewColumns = 8;             // query heads of a key head that go together
 
+struct AttendSplit { int splits, step, own_ctas, own_step; };      // of the prefix: stretches, and tiles of one; of own keys: CTAs, and keys of a stretch
+
+// Lengths are at most 2^30.
 __device__ __forceinline__ int own_length(const AttendArgs& p, int b) { return min(max(p.lengths[b], 0), (int)p.most_own); }
 
 __device__ __forceinline__ int64_t warp_total(int64_t v) {
@@ -55,13 +68,64 @@ __device__ __forceinline__ int64_t warp_total(int64_t v) {
     for (int x = 16; x; x >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, x);
     return v;
 }
-// By a whole warp.
-__device__ __forceinline__ int own_step(const AttendArgs& p) {
-    int64_t total = 0;
-    for (int b = threadIdx.x & 31; b < p.batch; b += 32) total += own_length(p, b);
-    total = warp_total(total);
-    const int64_t places = p.own_items - p.batch;
-    return (int)max((int64_t)kOwnLeast, ((total + places - 1) / places + 63) / 64 * 64);
+// By a whole warp, the same in every lane.  With T own keys in all, B sequences and P places beyond B, stretches of at least T / P are at most T / (T / P) + B.
+template <int DIM>
+__device__ __forceinline__ AttendSplit split_work(const AttendArgs& p, int ctas) {
+    const int lane = threadIdx.x & 31, units = p.kv_heads * p.wide_tiles, tiles = (p.prefix + kPrefixKeys - 1) / kPrefixKeys;
+    const int heads = p.kv_heads * ((p.group + kFewColumns - 1) / kFewColumns);
+    int64_t keys = 0;
+    if (p.own_items) {
+        for (int b = lane; b < p.batch; b += 32) keys += own_length(p, b);
+        keys = warp_total(keys);
+    }
+    AttendSplit r = {0, 0, ctas, kOwnLeast};
+    if (tiles && p.own_ctas >= 0) {
+        r = {1, tiles, p.own_ctas, kOwnLeast};
+    } else if (tiles) {
+        const int tile_cycles = (p.batch * p.group + kPrefixRows - 1) / kPrefixRows > 1 ? kPrefixPaired : kPrefixSingle;
+        const float own_cycles = (float)keys * (float)heads * (float)(DIM * 4 / kOwnBytesPerCycle);
+        int best = 0x7FFFFFFF, best_splits = 1;
+        for (int s = lane + 1; s <= p.most_splits; s += 32) {
+            const int left = ctas - units * s;
+            if (keys && left < 1) break;
+            const float cost = fmaxf((float)(kPrefixStart + (tiles + s - 1) / s * tile_cycles), keys ? kOwnStart + own_cycles / (float)left : 0.f);
+            const int rounded = (int)fminf(cost, 2e9f);
+            if (rounded < best) { best = rounded; best_splits = s; }
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1) {
+            const int cost = __shfl_xor_sync(0xFFFFFFFFu, best, x), s = __shfl_xor_sync(0xFFFFFFFFu, best_splits, x);
+            if (cost < best || (cost == best && s < best_splits)) { best = cost; best_splits = s; }
+        }
+        r.step = (tiles + best_splits - 1) / best_splits;
+        r.splits = (tiles + r.step - 1) / r.step;
+        r.own_ctas = ctas - units * r.splits;
+    }
+    if (p.own_items) {
+        // four stretches for each of the warps that have them
+        const int64_t places = min((int64_t)(p.own_items - p.batch), max((int64_t)1, ((int64_t)r.own_ctas * (4 * kOwnWarps) + heads - 1) / heads));
+        r.own_step = (int)max((int64_t)kOwnLeast, ((keys + places - 1) / places + 63) / 64 * 64);
+    }
+    return r;
+}
+
+// The numbers of stretches before each sequence's first, for who joins them; by a whole warp.
+__device__ __forceinline__ void write_plan(const AttendArgs& p, const AttendSplit& split) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    if (lane == 0) p.plan[0] = split.splits;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int b = b0 + lane, count = p.own_items && b < p.batch ? (own_length(p, b) + split.own_step - 1) / split.own_step : 0;
+        int behind = count;
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, behind, x);
+            if (lane >= x) behind += v;
+        }
+        if (b < p.batch) p.plan[1 + b] = before + behind - count;
+        before += __shfl_sync(0xFFFFFFFFu, behind, 31);
+    }
+    if (lane == 0) p.plan[1 + p.batch] = before;
 }
 
 // Stretches in the order of their numbers, by a whole warp: 32 sequences at a time.
@@ -92,15 +156,5 @@ struct OwnFinder {
         sequence = -1;
     }
 };
-
-struct OwnItems { int first, count; };
-// The stretches of a sequence, by a whole warp.
-__device__ __forceinline__ OwnItems own_items(const AttendArgs& p, int sequence) {
-    if (p.own_items == 0) return {0, 0};
-    const int step = own_step(p);
-    int64_t before = 0;
-    for (int b = threadIdx.x & 31; b < sequence; b += 32) before += (own_length(p, b) + step - 1) / step;
-    return {(int)warp_total(before), (own_length(p, sequence) + step - 1) / step};
-}
 
 }  // namespace mps

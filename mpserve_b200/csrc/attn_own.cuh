@@ -2,22 +2,20 @@
 //
 // A warp has a stretch of one sequence's keys for one key head, 16 keys at a time, through a ring of its own.  Logits are computed as K q^T, 16 keys by 8 query
 // heads, and the result as V^T P^T, so that the eight columns are the query heads that share the key head, and none of the tensor cores' rows idles.
-// Bound: memory.  Four warps of a CTA do this beside those that have the prefix; their rings are 64 KB under way on an SM, which is what 6.5 TB/s need at a latency of
-// 1.4 us, so a warp's stretches follow one another without a gap: the next one's first keys are asked for while the last ones of this are multiplied.
+// Bound: memory.  A CTA's rings are 224 KB, and a warp's stretches follow one another without a gap: the next one's first keys are asked for while the last ones of this are
+// multiplied.
 #pragma once
 
 #include "attn.cuh"
 
 namespace mps {
 
-constexpr int kFewWarps = 4, kFewColumns = 8;
-
 template <int DIM>
 struct FewShape {
     static constexpr int kRow = DIM * 2, kBlock = 16 * kRow, kStage = 2 * kBlock;      // 16 keys, then their values
     static constexpr int kStages = 256 / DIM;                                          // 16 KB a warp
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kSmem = kFewWarps * kRing;
+    static constexpr int kSmem = kOwnWarps * kRing;
 };
 
 // 16-byte piece `piece` of row `row`: rows of 256 (128) bytes, pieces XORed with the row, so that eight rows' pieces lie in different banks.
@@ -32,13 +30,13 @@ struct FewBlock {
 
 // Every workers-th unit is this warp's.  `ring`: its shared memory.
 template <int DIM, bool BF16>
-__device__ __forceinline__ void attend_own(const AttendArgs& p, uint32_t ring, int worker, int workers) {
+__device__ __forceinline__ void attend_own(const AttendArgs& p, int own_step, uint32_t ring, int worker, int workers) {
     using S = FewShape<DIM>;
     constexpr int kPieces = DIM / 8;       // of a row
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int column_tiles = (p.group + kFewColumns - 1) / kFewColumns, per_item = p.kv_heads * column_tiles, units = (int)p.own_items * per_item;
+    const int column_tiles = (p.group + kFewColumns - 1) / kFewColumns, per_item = p.kv_heads * column_tiles, units = p.own_items * per_item;
     OwnFinder find;
-    find.step = own_step(p);
+    find.step = own_step;
     find.first_sequence = find.before = find.first = find.last = 0;
     find.sequence = 0;
 

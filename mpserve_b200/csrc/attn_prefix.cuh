@@ -21,17 +21,17 @@
 
 namespace mps {
 
-constexpr int kPrefixKeys = 128, kPrefixRows = 128, kPrefixThreads = 512;
+constexpr int kAttendThreads = 512;
 constexpr float kRescale = 8.f;      // in powers of two
 
 template <int DIM>
 struct PrefixShape {
     static constexpr int kHalf = kPrefixKeys * 128, kHalves = DIM / 64;      // 64 columns of a tile, rows of 128 bytes
-    static constexpr int kStage = kHalves * kHalf, kStages = DIM == 128 ? 3 : 6;
+    static constexpr int kStage = kHalves * kHalf, kStages = DIM == 128 ? 5 : 12;
     static constexpr int kRing = 2 * kStage;                                  // behind two tiles of queries
-    static constexpr int kOwn = kRing + kStages * kStage;                     // the rings of those who have the sequences' own keys
-    static constexpr int kBars = kOwn + FewShape<DIM>::kSmem;
-    static constexpr int kSmem = kBars + (2 * kStages + 7) * 8 + 16;
+    static constexpr int kBars = kRing + kStages * kStage;
+    static_assert(FewShape<DIM>::kSmem <= kBars, "the sequences' own keys take the same place in the CTAs that have them");
+    static constexpr int kSmem = kBars + (2 * kStages + 7) * 8 + 32;
     static constexpr int kColumns = 512;                                      // S, S, O, O
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -66,13 +66,15 @@ __device__ __forceinline__ void leave_gaps(const AttendArgs& p, int key, int key
     }
 }
 
-// Warps: 0 to 3 and 4 to 7 a group's rows, 8 multiplies, 9 copies (10 and 11 complete a group of four), 12 to 15 the sequences' own keys.
+// Warps of a CTA that has a part of the prefix: 0 to 3 and 4 to 7 a group's rows, 8 multiplies, 9 copies (the others complete groups of four).  Of one that has the sequences'
+// own keys: 0 to 13, each for itself.
 template <int DIM, bool BF16>
-__global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendArgs p, const __grid_constant__ PrefixMaps maps) {
+__global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendArgs p, const __grid_constant__ PrefixMaps maps) {
     using S = PrefixShape<DIM>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem), ring = base + S::kRing, bar0 = base + S::kBars;
+    AttendSplit& shared_split = *reinterpret_cast<AttendSplit*>(smem + S::kSmem - 32);
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + S::kSmem - 16);
     volatile uint32_t& failed = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 12);
     volatile uint32_t& absent = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 8);      // pages of this stretch lie outside the cache
@@ -81,13 +83,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
     const auto s_full = [&](int g) { return bar0 + 8u * (2 * S::kStages + g); };
     const auto p_ready = [&](int g, int half) { return bar0 + 8u * (2 * S::kStages + 2 + 2 * g + half); };      // of 64 keys
     const uint32_t done = bar0 + 8u * (2 * S::kStages + 6);
-    const bool some_prefix = blockIdx.x < p.prefix_units;
-
-    const int rows = p.batch * p.group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows, pairs = row_tiles / 2, wide_tiles = (row_tiles + 1) / 2;
-    const int x = blockIdx.x % wide_tiles, kv_head = blockIdx.x / wide_tiles % p.kv_heads, split = blockIdx.x / wide_tiles / p.kv_heads;
-    const bool paired = x < pairs;             // else the groups take the keys in turn
-    const int key0 = split * (int)p.prefix_step, key_end = min((int)p.prefix, key0 + (int)p.prefix_step);      // at most 2^30
-    const int tiles = (key_end - key0 + kPrefixKeys - 1) / kPrefixKeys;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
@@ -97,14 +92,35 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
         absent = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8 && some_prefix) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
-    if (warp == 9 && lane == 0 && some_prefix) { prefetch_map(&maps.k); prefetch_map(&maps.v); }
+    if (warp == 8 && p.prefix) tmem_alloc<1>(smem_u32(&tmem_slot), S::kColumns);
+    if (warp == 9 && lane == 0 && p.prefix) { prefetch_map(&maps.k); prefetch_map(&maps.v); }
+    griddep_wait();
+    griddep_launch();
+    if (warp == 0) {
+        const AttendSplit split = split_work<DIM>(p, (int)gridDim.x);
+        if (lane == 0) shared_split = split;
+    }
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
-    griddep_wait();
-    griddep_launch();
-    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    const AttendSplit split = shared_split;
+    const int prefix_ctas = p.kv_heads * p.wide_tiles * split.splits;
+    if (blockIdx.x == gridDim.x - 1 && warp == 15) write_plan(p, split);      // it has own keys, and this warp none of them
+    const uint32_t tmem = p.prefix ? __shfl_sync(0xFFFFFFFFu, tmem_slot, 0) : 0u;
+    if ((int)blockIdx.x >= prefix_ctas) {
+        if (p.own_items && warp < kOwnWarps)
+            attend_own<DIM, BF16>(p, split.own_step, base + warp * FewShape<DIM>::kRing, ((int)blockIdx.x - prefix_ctas) * kOwnWarps + warp, split.own_ctas * kOwnWarps);
+        __syncthreads();
+        if (warp == 8 && p.prefix) tmem_free<1>(tmem, S::kColumns);
+        return;
+    }
+
+    const int rows = p.batch * p.group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows, pairs = row_tiles / 2;
+    const int x = blockIdx.x % p.wide_tiles, kv_head = blockIdx.x / p.wide_tiles % p.kv_heads, stretch = blockIdx.x / p.wide_tiles / p.kv_heads;
+    const bool paired = x < pairs;             // else the groups take the keys in turn
+    const int key0 = stretch * split.step * kPrefixKeys, key_end = min(p.prefix, key0 + split.step * kPrefixKeys);
+    const int tiles = (key_end - key0 + kPrefixKeys - 1) / kPrefixKeys;
+    int asked = 0;                             // tiles that this warp has asked for
     const uint32_t s_at = tmem, o_at = tmem + 256;      // and 128 columns on for the second group
 
     // tiles come as K0, K1, V0, K2, V1, ...: number in that order
@@ -114,12 +130,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
     // What the softmax warps and the multiplying one wait for: the queries in shared memory, and whether pages are absent.
     const auto prepared = [&]() { asm volatile("bar.sync 1, 288;" ::: "memory"); };
 
-    // a row's 128 logits want more registers than a 512th of them: the four warps that copy and multiply give up theirs (256 x 160 + 128 x 64 + 128 x 128 = 512 x 128)
-    if (warp >= 12) {
-        if (p.own_items) attend_own<DIM, BF16>(p, base + S::kOwn + (warp - 12) * FewShape<DIM>::kRing, blockIdx.x * kFewWarps + warp - 12, gridDim.x * kFewWarps);
-    } else if (warp >= 8) {
+    // a row's 128 logits want more registers than a 512th of them: the other warps give up theirs (256 x 192 + 128 x 64 + 128 x 64 = 512 x 128)
+    if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 9 && some_prefix) {
+        if (warp == 9) {
             const int box = (int)min(p.page_mask + 1, (int64_t)kPrefixKeys), boxes = kPrefixKeys / box;
             // this lane's box of a tile: its page (the one behind the last, which gives zeros, for one outside), or -1
             const auto page_of = [&](int j) {
@@ -153,12 +167,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
                 }
                 __syncwarp();
             }
-            // no copy and no arrival may come after this CTA is gone
-            for (int i = max(0, n - S::kStages); i < n; ++i) {
-                const uint32_t parity = (uint32_t)(i / S::kStages) & 1u;
-                if (!warp_wait(empty(i % S::kStages), parity, &failed)) mbar_wait(full(i % S::kStages), parity, kMx4SpinLimit);
-            }
-        } else if (warp == 8 && some_prefix) {
+            asked = n;
+        } else if (warp == 8) {
             prepared();
             tensor_fence_after();
             const uint32_t lead = elect_one();
@@ -242,8 +252,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
             warp_wait(done, 0, &failed);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-        if (some_prefix) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // the queries, as the tensor cores read them: 16-byte pieces XORed with the row; eight at a time under way
         constexpr int kAhead = DIM / 16;      // pieces of a row by 256 threads
         for (int tile = 0; tile < (paired ? 2 : 1); ++tile) {
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
         ok = ok && warp_wait(done, 0, &failed);
         tensor_fence_after();
         if (ok && some) {
-            const int64_t part = ((int64_t)(paired ? split : 2 * split + g) * p.kv_heads + kv_head) * rows + row;
+            const int64_t part = ((int64_t)(paired ? stretch : 2 * stretch + g) * p.kv_heads + kv_head) * rows + row;
             // by way of the ring, whose tiles have been multiplied: straight from the registers every store would touch 32 rows
             const uint32_t rows_at = ring + warp * (32 * 128);      // 32 rows of 32 columns, pieces XORed with the row
             const int64_t first_part = part - lane;
@@ -386,14 +395,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) attend_kernel(const AttendA
             }
             if (row < rows) p.prefix_ml[part] = make_float2(m, sum.x + sum.y);
         }
-        }
     }
     __syncwarp();
     tensor_fence_before();
-    __syncthreads();
+    __syncthreads();      // what was copied has been multiplied, unless a wait ran out
     tensor_fence_after();
-    if (threadIdx.x == 0 && failed) atomicExch(p.workspace, 1u);
-    if (warp == 8 && some_prefix) tmem_free<1>(tmem, S::kColumns);
+    if (failed) {
+        // no copy may come after this CTA is gone
+        for (int i = max(0, asked - S::kStages); i < asked; ++i) mbar_wait(full(i % S::kStages), (uint32_t)(i / S::kStages) & 1u, kMx4SpinLimit);
+        if (threadIdx.x == 0) atomicExch(p.workspace, 1u);
+        __syncthreads();
+    }
+    if (warp == 8) tmem_free<1>(tmem, S::kColumns);
 }
 
 }  // namespace mps

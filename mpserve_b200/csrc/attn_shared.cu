@@ -24,14 +24,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q_heads = p.kv_heads * p.group, tiles = (q_heads + kHeads - 1) / kHeads;
     const int sequence = blockIdx.x / tiles, head = blockIdx.x % tiles * kHeads + warp / SHARE, share = warp % SHARE;
-    const OwnItems own = own_items(p, sequence);
+    const int stretches = p.plan[0], own_before = p.plan[1 + sequence], own_count = p.plan[2 + sequence] - own_before;
     if (SHARE == 1 && head >= q_heads) return;
     const int kv_head = head / p.group, in_group = head % p.group;
     const int64_t rows = (int64_t)p.batch * p.group, twice = (rows + kPrefixRows - 1) / kPrefixRows / 2 * 2 * kPrefixRows, row = (int64_t)sequence * p.group + in_group;
     // rows from `twice` on have two parts of each stretch of the prefix
-    const int splits = row < twice ? p.prefix_splits : 2 * p.prefix_splits, count = splits + own.count;
+    const int splits = row < twice ? stretches : 2 * stretches, count = splits + own_count;
     const int64_t prefix_step = p.kv_heads * rows, prefix_first = kv_head * rows + row, own_step = (int64_t)p.kv_heads * p.group;
-    const int64_t own_first = ((int64_t)own.first * p.kv_heads + kv_head) * p.group + in_group;
+    const int64_t own_first = ((int64_t)own_before * p.kv_heads + kv_head) * p.group + in_group;
     float top = -INFINITY, sum = 0.f, out[kColumns];
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) out[c] = 0.f;
@@ -99,31 +99,39 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 // ---- host side -------------------------------------------------------------------------------------------
 
 struct AttendPlan {
-    int64_t prefix_step;          // keys of a stretch of the prefix
-    int prefix_splits;
-    int prefix_parts;             // of a row
-    int wide_tiles;               // CTAs for a stretch and a key head
-    int64_t own_items;            // at most
-    int64_t floats(int64_t rows, int64_t kv_heads, int64_t group, int64_t dim) const {      // of the scratch
+    int wide_tiles;               // CTAs for a stretch of the prefix and a key head
+    int most_splits;              // stretches of the prefix, at most
+    int prefix_parts;             // of a row, at most
+    int own_ctas;                 // -1: the GPU settles it
+    int64_t ctas;
+    int64_t own_items;            // stretches of own keys, at most
+    int64_t floats(int64_t rows, int64_t kv_heads, int64_t group, int64_t dim) const {      // of the scratch, behind its first part
         return (prefix_parts * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
     }
 };
+static int64_t plan_words(int64_t batch) { return (batch + 2 + 3) / 4 * 4; }
 static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
     AttendPlan plan = {};
     const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group, row_tiles = (rows + kPrefixRows - 1) / kPrefixRows;
+    const int64_t most = a.table_columns * a.page_size, heads = a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
     plan.wide_tiles = (int)((row_tiles + 1) / 2);
+    plan.own_ctas = -1;
+    plan.ctas = sms;
     if (a.prefix_length > 0) {
-        // a CTA an SM, as long as there are tiles of keys
-        const int64_t wanted = std::max<int64_t>(1, sms / ((int64_t)plan.wide_tiles * a.kv_heads)), tiles = (a.prefix_length + kPrefixKeys - 1) / kPrefixKeys;
-        plan.prefix_step = (tiles + wanted - 1) / wanted * kPrefixKeys;
-        plan.prefix_splits = (int)((a.prefix_length + plan.prefix_step - 1) / plan.prefix_step);
-        plan.prefix_parts = plan.prefix_splits * (row_tiles % 2 ? 2 : 1);
+        // a CTA an SM, one of them at least for the sequences, as long as there are tiles of keys
+        const int64_t units = plan.wide_tiles * (int64_t)a.kv_heads, tiles = (a.prefix_length + kPrefixKeys - 1) / kPrefixKeys;
+        if (units + (most > 0) > sms) {
+            // more than there are SMs for already: the sequences get an SM of four
+            plan.most_splits = 1;
+            plan.own_ctas = most > 0 ? (sms + 3) / 4 : 0;
+            plan.ctas = units + plan.own_ctas;
+        } else {
+            plan.most_splits = (int)std::min<int64_t>(tiles, (sms - (most > 0)) / units);
+        }
+        plan.prefix_parts = plan.most_splits * (row_tiles % 2 ? 2 : 1);
     }
-    const int64_t most = a.table_columns * a.page_size;
     if (most > 0) {
-        // eight stretches for each of the warps that have them, where the tables hold so many
-        const int64_t tiles = a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
-        const int64_t extra = std::min<int64_t>((8 * kFewWarps * sms + tiles - 1) / tiles, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
+        const int64_t extra = std::min<int64_t>((4 * kOwnWarps * (int64_t)sms + heads - 1) / heads, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
         plan.own_items = a.batch + extra;
     }
     return plan;
@@ -176,12 +184,10 @@ static int attend(const AttendArgs& p, const mps_prefix_attend& a, unsigned int 
         MPS_CUDA_TRY(cudaFuncSetAttribute(attend_kernel<DIM, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixShape<DIM>::kSmem));
         ready.fetch_or(uint64_t(1) << (d.ordinal & 63), std::memory_order_release);
     }
-    if (ctas) {
-        PrefixMaps maps = {};
-        if (p.prefix_units) rc = page_maps(maps, a);
-        if (!rc) rc = launch_overlapping_smem("attend_kernel", attend_kernel<DIM, BF16>, ctas, dim3(kPrefixThreads), PrefixShape<DIM>::kSmem, st, p, maps);
-        if (rc) return rc;
-    }
+    PrefixMaps maps = {};
+    if (p.prefix) rc = page_maps(maps, a);
+    if (!rc) rc = launch_overlapping_smem("attend_kernel", attend_kernel<DIM, BF16>, ctas, dim3(kAttendThreads), PrefixShape<DIM>::kSmem, st, p, maps);
+    if (rc) return rc;
     const int64_t q_heads = (int64_t)p.kv_heads * p.group;
     if (a.batch * q_heads <= kJoinFewHeads)
         return launch_overlapping("attend_join_kernel", attend_join_kernel<DIM, BF16, kJoinWarps>, (unsigned int)(a.batch * q_heads), dim3(kJoinWarps * 32), st, p);
@@ -197,7 +203,7 @@ extern "C" int64_t mps_prefix_attend_scratch_bytes(const mps_prefix_attend* args
     Device d;
     if (current_device(d)) return -1;
     const int64_t group = args->q_heads / args->kv_heads;
-    return attend_plan(*args, d.sms).floats(args->batch * group, args->kv_heads, group, args->dim) * 4 + 64;
+    return attend_plan(*args, d.sms).floats(args->batch * group, args->kv_heads, group, args->dim) * 4 + plan_words(args->batch) * 4;
 }
 
 extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scratch, int64_t scratch_bytes, void* workspace, int64_t workspace_bytes,
@@ -232,7 +238,7 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     AttendArgs p = {};
     const int64_t group = a.q_heads / a.kv_heads, rows = a.batch * group;
     const AttendPlan plan = attend_plan(a, d.sms);
-    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15u) || scratch_bytes < plan.floats(rows, a.kv_heads, group, a.dim) * 4) {
+    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15u) || scratch_bytes < plan.floats(rows, a.kv_heads, group, a.dim) * 4 + plan_words(a.batch) * 4) {
         set_error("mps_prefix_attend_tokens: scratch missing, unaligned or too small");
         return MPS_ERR_WORKSPACE;
     }
@@ -254,10 +260,11 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     p.v_page = a.v_page_stride; p.v_slot = a.v_slot_stride; p.v_head = a.v_head_stride;
     p.table_columns = a.table_columns;
     p.most_own = a.table_columns * a.page_size;
-    p.prefix = a.prefix_length;
-    p.prefix_step = plan.prefix_step;
-    p.prefix_splits = plan.prefix_splits;
-    p.own_items = plan.own_items;
+    p.prefix = (int32_t)a.prefix_length;
+    p.wide_tiles = plan.wide_tiles;
+    p.most_splits = plan.most_splits;
+    p.own_items = (int32_t)plan.own_items;
+    p.own_ctas = plan.own_ctas;
     p.pages = (int32_t)a.pages;
     p.page_shift = __builtin_ctzll((unsigned long long)a.page_size);
     p.page_mask = a.page_size - 1;
@@ -268,14 +275,16 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     p.q_factor = a.scale > 0.f ? 1 : a.scale < 0.f ? -1 : a.scale == 0.f ? 0 : 1;
     p.scale_log2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
     const int64_t prefix_parts = plan.prefix_parts * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
-    p.prefix_o = static_cast<float*>(scratch);
+    p.plan = static_cast<int32_t*>(scratch);
+    p.prefix_o = static_cast<float*>(scratch) + plan_words(a.batch);
     p.own_o = p.prefix_o + prefix_parts * a.dim;
     p.prefix_ml = reinterpret_cast<float2*>(p.own_o + own_parts * a.dim);
     p.own_ml = p.prefix_ml + prefix_parts;
-    const int64_t units = (int64_t)plan.prefix_splits * a.kv_heads * plan.wide_tiles, own_units = plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns);
-    if (units > 0x7FFFFFFF || own_units > 0x7FFFFFFF) { set_error("mps_prefix_attend_tokens: too much work for one launch"); return MPS_ERR_INVALID; }
-    p.prefix_units = (int32_t)units;
-    const unsigned int ctas = (unsigned int)std::max(units, std::min<int64_t>(d.sms, (own_units + kFewWarps - 1) / kFewWarps));
+    if (plan.ctas > 0x7FFFFFFF || plan.own_items * a.kv_heads * ((group + kFewColumns - 1) / kFewColumns) > 0x7FFFFFFF) {
+        set_error("mps_prefix_attend_tokens: too much work for one launch");
+        return MPS_ERR_INVALID;
+    }
+    const unsigned int ctas = (unsigned int)plan.ctas;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a.dim == 64) return a.dtype == MPS_BF16 ? attend<64, true>(p, a, ctas, st) : attend<64, false>(p, a, ctas, st);
     return a.dtype == MPS_BF16 ? attend<128, true>(p, a, ctas, st) : attend<128, false>(p, a, ctas, st);
