@@ -31,7 +31,7 @@ struct PrefixShape {
     static constexpr int kRing = 2 * kStage;                                  // behind two tiles of queries
     static constexpr int kBars = kRing + kStages * kStage;
     static_assert(FewShape<DIM>::kSmem <= kBars, "the sequences' own keys take the same place in the CTAs that have them");
-    static constexpr int kSmem = kBars + (2 * kStages + 7) * 8 + 32;
+    static constexpr int kSmem = kBars + (2 * kStages + 9) * 8 + 32;
     static constexpr int kColumns = 512;                                      // S, S, O, O
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -42,6 +42,12 @@ __device__ __forceinline__ void page_box(uint32_t dst, const CUtensorMap* map, i
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(column), "r"(slot), "r"(head), "r"(page), "r"(bar) : "memory");
 }
+// The largest of three; NaN where there is one.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // 2^x, off by 2^-22 of itself: far below what P is rounded by.  (Results below 2^-126 become 0.)
 __device__ __forceinline__ float fast_exp2(float x) {
     float r;
@@ -49,11 +55,20 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return r;
 }
 
-// The largest of three; NaN where there is one.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
+// The same by multiplications and additions, for a part of the exponentials, so that the unit that makes them is not alone with them: x is a whole number and a
+// rest of half at most, whose power is the polynomial that has 2^x's values at the zeros of Chebyshev's polynomial of degree six on [-1/2, 1/2] (off by
+// 2^-22); the whole number is added to the exponent.  Below 2^-126 it stays there.
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+    const auto both = [](float c) { return make_float2(c, c); };
+    x = make_float2(max3(x.x, -126.f, -126.f), max3(x.y, -126.f, -126.f));
+    const float2 one = both(1.f), shifted = fma2(x, one, both(12582912.f)), whole = fma2(shifted, one, both(-12582912.f));      // 1.5 2^23: rounds to whole numbers
+    const float2 f = fma2(whole, both(-1.f), x);
+    float2 r = fma2(f, both(0.0013390863314270973f), both(0.009676031768321991f));
+    r = fma2(f, r, both(0.055503569543361664f));
+    r = fma2(f, r, both(0.2402210682630539f));
+    r = fma2(f, r, both(0.6931471824645996f));
+    r = fma2(f, r, both(1.0000001192092896f));
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(shifted.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(shifted.y) << 23)));
 }
 // Logits of 32 keys from `key` on: minus infinity for keys behind the stretch's last, and for those of pages outside the cache.
 __device__ __forceinline__ void leave_gaps(const AttendArgs& p, int key, int key_end, uint32_t (&v)[32]) {
@@ -82,11 +97,12 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
     const auto s_full = [&](int g) { return bar0 + 8u * (2 * S::kStages + g); };
     const auto p_ready = [&](int g, int half) { return bar0 + 8u * (2 * S::kStages + 2 + 2 * g + half); };      // of 64 keys
-    const uint32_t done = bar0 + 8u * (2 * S::kStages + 6);
+    const auto half_done = [&](int g) { return bar0 + 8u * (2 * S::kStages + 6 + g); };              // with the first 64 of them
+    const uint32_t done = bar0 + 8u * (2 * S::kStages + 8);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g, 0), 4); mbar_init(p_ready(g, 1), 4); }
+        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g, 0), 4); mbar_init(p_ready(g, 1), 4); mbar_init(half_done(g), 1); }
         mbar_init(done, 1);
         failed = 0u;
         absent = 0u;
@@ -195,6 +211,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
 #pragma unroll
                     for (int i = half * 4; i < half * 4 + 4; ++i)      // 16 keys on: two groups of eight rows
                         half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i || turn ? 1u : 0u);
+                    if (half == 0) tensor_commit(lead, half_done(g));
                 }
             };
             // values behind the prefix's last are what the page holds, which may be NaN: rows of zeros instead
@@ -290,70 +307,72 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
             if (!ok) break;
             tensor_fence_after();
             if (some) {
-                // The logits are read twice, 32 columns at a time and the next ones on their way: for the largest, and to be replaced by the weights.
-                const int j = paired ? turn : 2 * turn + g;
-                const int left = key_end - key0 - j * kPrefixKeys;
-                const bool gaps = left < kPrefixKeys || absent;
+                // 64 keys at a time: the tensor cores multiply the first half's weights while the second's are made.
+                const int j = paired ? turn : 2 * turn + g, key = key0 + j * kPrefixKeys;
+                const bool gaps = key_end - key < kPrefixKeys || absent;
                 uint32_t s[2][32];
                 tmem_ask32(s_mine, s[0]);
-                float top[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t(&v)[32] = s[c & 1];
-                    tmem_arrived(v);
-                    tmem_ask32(s_mine + (c + 1) % 4 * 32, s[(c + 1) & 1]);
-                    if (gaps) leave_gaps(p, key0 + j * kPrefixKeys + c * 32, key_end, v);
-                    if (c == 0) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) top[i] = __uint_as_float(v[i]);
-                    }
-#pragma unroll
-                    for (int i = c ? 0 : 4; i < 32; i += 8) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (i + k + 4 < 32) top[k] = max3(top[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + k + 4]));
-                            else top[k] = max3(top[k], __uint_as_float(v[i + k]), __uint_as_float(v[i + k]));
-                    }
-                }
-                const float high = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
-                if (turn == 0) {
-                    m = high;
-                } else if (__any_sync(0xFFFFFFFFu, !(high <= m + kRescale))) {
-                    const float next = max3(m, high, high), up = fast_exp2(m - (next == -INFINITY ? 0.f : next));
-                    m = next;
-                    sum.x *= up;
-                    sum.y *= up;
-                    tmem_arrived(s[0]);
-#pragma unroll 1
-                    for (int c = 0; c < DIM / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ask32(o_mine + c * 32, o);
-                        tmem_arrived(o);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
-                        tmem_store32(o_mine + c * 32, o);
-                    }
-                }
-                const float from = m == -INFINITY ? 0.f : m;
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), from2 = make_float2(-from, -from), one2 = make_float2(1.f, 1.f);
+                tmem_ask32(s_mine + 32, s[1]);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
+                    tmem_arrived(s[0]);
+                    tmem_arrived(s[1]);
+                    if (gaps) {
+                        leave_gaps(p, key + half * 64, key_end, s[0]);
+                        leave_gaps(p, key + half * 64 + 32, key_end, s[1]);
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        top[k] = max3(__uint_as_float(s[0][k]), __uint_as_float(s[1][k]), __uint_as_float(s[0][k + 4]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 4]), __uint_as_float(s[0][k + 8]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 8]), __uint_as_float(s[0][k + 12]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 12]), __uint_as_float(s[0][k + 16]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 16]), __uint_as_float(s[0][k + 20]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 20]), __uint_as_float(s[0][k + 24]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 24]), __uint_as_float(s[0][k + 28]));
+                        top[k] = max3(top[k], __uint_as_float(s[1][k + 28]), __uint_as_float(s[1][k + 28]));
+                    }
+                    const float high = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
+                    if (turn == 0 && half == 0) {
+                        m = high;
+                    } else if (const bool grown = !(high <= m + kRescale); __any_sync(0xFFFFFFFFu, grown)) {
+                        // of the result so far, the weights of this tile's first half may still be on their way into it
+                        if (half == 1 && !warp_wait(half_done(g), (uint32_t)turn & 1u, &failed)) break;
+                        tensor_fence_after();
+                        // rows that have not keep their scale: what a row gets does not go by its neighbours
+                        const float next = grown ? max3(m, high, high) : m, up = grown ? fast_exp2(m - (next == -INFINITY ? 0.f : next)) : 1.f;
+                        m = next;
+                        sum.x *= up;
+                        sum.y *= up;
+#pragma unroll 1
+                        for (int c = 0; c < DIM / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ask32(o_mine + c * 32, o);
+                            tmem_arrived(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
+                            tmem_store32(o_mine + c * 32, o);
+                        }
+                    }
+                    const float from = m == -INFINITY ? 0.f : m;
+                    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), from2 = make_float2(-from, -from), one2 = make_float2(1.f, 1.f);
                     uint32_t w[32];
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        const int c = half * 2 + part;
-                        uint32_t(&v)[32] = s[c & 1];
-                        tmem_arrived(v);
-                        if (c < 3) tmem_ask32(s_mine + (c + 1) * 32, s[(c + 1) & 1]);
-                        if (gaps) leave_gaps(p, key0 + j * kPrefixKeys + c * 32, key_end, v);
+                    for (int c = 0; c < 2; ++c) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float2 e = fma2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), scale2, from2);
-                            e.x = fast_exp2(e.x);
-                            e.y = fast_exp2(e.y);
+                            float2 e = fma2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, from2);
+                            if (i % 3 == 2) {
+                                e = poly_exp2(e);
+                            } else {
+                                e.x = fast_exp2(e.x);
+                                e.y = fast_exp2(e.y);
+                            }
                             sum = fma2(e, one2, sum);
-                            w[part * 16 + i] = pack_pair<BF16>(e.x, e.y);
+                            w[c * 16 + i] = pack_pair<BF16>(e.x, e.y);
                         }
+                        if (half == 0) tmem_ask32(s_mine + 64 + c * 32, s[c]);
                     }
                     tmem_store32(s_mine + half * 32, w);
                     tmem_stored();
