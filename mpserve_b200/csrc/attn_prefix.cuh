@@ -2,13 +2,11 @@
 //
 // A query of the batch is a row: row b * group + g of key head h is query head h * group + g of sequence b.  A CTA has one stretch of the prefix for up to 256 rows, in
 // two groups of four warps; keys and values come 128 at a time into a ring in shared memory, page by page as tiled copies.
-//   S = Q K^T   128 x 64 in tensor memory, operands from shared memory;
+//   S = Q K^T   128 x 128 in tensor memory, operands from shared memory;
 //   P = 2^(S - m) in the cache's type, which takes S's place: a thread has a row, so that maxima and sums need no other thread;
 //   O += P V    128 x dim in tensor memory, P from there.
-// A group has two places for S, for the halves of a tile of 128 keys: the next S is there when a P is done, and nobody waits for the tensor cores, which work for
-// the other half and the other group meanwhile.  (With one place of 128 keys a group's steps are a chain, softmax, P V, Q K^T, of 4100 cycles.)  With more than 128 rows each
-// group has 128 of them and both use the same keys; with no more (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of
-// keys in turn, and their results are two parts.
+// While one group makes its P, the tensor cores work for the other.  With more than 128 rows each group has 128 of them and both use the same keys; with no more
+// (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of keys in turn, and their results are two parts.
 //
 // O is scaled anew only where a row's largest logit has grown by more than 2^8 since it last was: P is then at most 2^8, which is far from the end of
 // either type's range, and what m a part refers to does not matter when parts are joined.  P is rounded to 16 bits, as the tensor cores take it: a relative
@@ -33,7 +31,7 @@ struct PrefixShape {
     static constexpr int kRing = 2 * kStage;                                  // behind two tiles of queries
     static constexpr int kBars = kRing + kStages * kStage;
     static_assert(FewShape<DIM>::kSmem <= kBars, "the sequences' own keys take the same place in the CTAs that have them");
-    static constexpr int kSmem = kBars + (2 * kStages + 11) * 8 + 32;
+    static constexpr int kSmem = kBars + (2 * kStages + 7) * 8 + 32;
     static constexpr int kColumns = 512;                                      // S, S, O, O
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -44,10 +42,10 @@ __device__ __forceinline__ void page_box(uint32_t dst, const CUtensorMap* map, i
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(map), "r"(column), "r"(slot), "r"(head), "r"(page), "r"(bar) : "memory");
 }
-// The largest of three; NaN where there is one.
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// The larger; NaN where there is one.
+__device__ __forceinline__ float max2(float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 // 2^x, off by 2^-22 of itself: far below what P is rounded by.  (Results below 2^-126 become 0.)
@@ -57,21 +55,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return r;
 }
 
-// The same by multiplications and additions, for a part of the exponentials, so that the unit that makes them is not alone with them: x is a whole number and a
-// rest of half at most, whose power is the polynomial that has 2^x's values at the zeros of Chebyshev's polynomial of degree six on [-1/2, 1/2] (off by
-// 2^-22); the whole number is added to the exponent.  Below 2^-126 it stays there.
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-    const auto both = [](float c) { return make_float2(c, c); };
-    x = make_float2(max3(x.x, -126.f, -126.f), max3(x.y, -126.f, -126.f));
-    const float2 one = both(1.f), shifted = fma2(x, one, both(12582912.f)), whole = fma2(shifted, one, both(-12582912.f));      // 1.5 2^23: rounds to whole numbers
-    const float2 f = fma2(whole, both(-1.f), x);
-    float2 r = fma2(f, both(0.0013390863314270973f), both(0.009676031768321991f));
-    r = fma2(f, r, both(0.055503569543361664f));
-    r = fma2(f, r, both(0.2402210682630539f));
-    r = fma2(f, r, both(0.6931471824645996f));
-    r = fma2(f, r, both(1.0000001192092896f));
-    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(shifted.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(shifted.y) << 23)));
-}
 // Logits of 32 keys from `key` on: minus infinity for keys behind the stretch's last, and for those of pages outside the cache.
 __device__ __forceinline__ void leave_gaps(const AttendArgs& p, int key, int key_end, uint32_t (&v)[32]) {
 #pragma unroll
@@ -97,17 +80,13 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
     volatile uint32_t& absent = *reinterpret_cast<volatile uint32_t*>(smem + S::kSmem - 8);      // pages of this stretch lie outside the cache
     const auto full = [&](int s) { return bar0 + 8u * s; };
     const auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
-    const auto s_full = [&](int g, int h) { return bar0 + 8u * (2 * S::kStages + 2 * g + h); };                // of 64 keys
-    const auto p_ready = [&](int g, int h) { return bar0 + 8u * (2 * S::kStages + 4 + 2 * g + h); };
-    const auto added = [&](int g) { return bar0 + 8u * (2 * S::kStages + 8 + g); };                            // P V to the result
-    const uint32_t done = bar0 + 8u * (2 * S::kStages + 10);
+    const auto s_full = [&](int g) { return bar0 + 8u * (2 * S::kStages + g); };
+    const auto p_ready = [&](int g, int half) { return bar0 + 8u * (2 * S::kStages + 2 + 2 * g + half); };      // of 64 keys
+    const uint32_t done = bar0 + 8u * (2 * S::kStages + 6);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int g = 0; g < 2; ++g) {
-            for (int h = 0; h < 2; ++h) { mbar_init(s_full(g, h), 1); mbar_init(p_ready(g, h), 4); }
-            mbar_init(added(g), 1);
-        }
+        for (int g = 0; g < 2; ++g) { mbar_init(s_full(g), 1); mbar_init(p_ready(g, 0), 4); mbar_init(p_ready(g, 1), 4); }
         mbar_init(done, 1);
         failed = 0u;
         absent = 0u;
@@ -193,28 +172,30 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
             prepared();
             tensor_fence_after();
             const uint32_t lead = elect_one();
-            const uint32_t qk = half_instruction(BF16, kPrefixKeys / 2, false), pv = half_instruction(BF16, DIM, true);
+            const uint32_t qk = half_instruction(BF16, kPrefixKeys, false), pv = half_instruction(BF16, DIM, true);
             bool ok = true;
             const auto arrived = [&](int n) { ok = ok && warp_wait(full(n % S::kStages), (uint32_t)(n / S::kStages) & 1u, &failed); };
-            // of half a tile's keys
-            const auto logits = [&](int g, int j, int h) {
-                const uint32_t q = base + (paired ? g : 0) * S::kStage, k = ring + key_number(j) % S::kStages * S::kStage + h * (S::kHalf / 2);
+            const auto logits = [&](int g, int j) {
+                const uint32_t q = base + (paired ? g : 0) * S::kStage, k = ring + key_number(j) % S::kStages * S::kStage;
 #pragma unroll
-                for (int c = 0; c < S::kHalves; ++c)
+                for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)      // 32 bytes on: two in the descriptors' unit
-                        half_multiply(lead, s_at + g * 128 + h * 64, operand_desc(q + c * S::kHalf) + 2 * i, operand_desc(k + c * S::kHalf) + 2 * i, qk, c + i ? 1u : 0u);
-                tensor_commit(lead, s_full(g, h));
+                        half_multiply(lead, s_at + g * 128, operand_desc(q + h * S::kHalf) + 2 * i, operand_desc(k + h * S::kHalf) + 2 * i, qk, h + i ? 1u : 0u);
+                tensor_commit(lead, s_full(g));
             };
-            const auto results = [&](int g, int j, int h, int turn) {
-                ok = ok && warp_wait(p_ready(g, h), (uint32_t)turn & 1u, &failed);
-                if (!ok) return;
-                tensor_fence_after();
-                const uint32_t v = ring + value_number(j) % S::kStages * S::kStage + h * (S::kHalf / 2);
+            // half by half, as the weights come
+            const auto results = [&](int g, int j, int turn) {
+                const uint32_t v = ring + value_number(j) % S::kStages * S::kStage;
 #pragma unroll
-                for (int i = 0; i < kPrefixKeys / 32; ++i)      // 16 keys on: two groups of eight rows
-                    half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + h * 64 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i + h || turn ? 1u : 0u);
-                tensor_commit(lead, added(g));
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && warp_wait(p_ready(g, half), (uint32_t)turn & 1u, &failed);
+                    if (!ok) return;
+                    tensor_fence_after();
+#pragma unroll
+                    for (int i = half * 4; i < half * 4 + 4; ++i)      // 16 keys on: two groups of eight rows
+                        half_multiply_kept(lead, o_at + g * 128, s_at + g * 128 + i * 8, wide_operand_desc(v, S::kHalf) + i * (2048 >> 4), pv, i || turn ? 1u : 0u);
+                }
             };
             // values behind the prefix's last are what the page holds, which may be NaN: rows of zeros instead
             const auto values = [&](int j) {
@@ -231,33 +212,41 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
             };
             arrived(0);
             if (ok) {
-                for (int h = 0; h < 2; ++h) {
-                    logits(0, 0, h);
-                    if (paired) logits(1, 0, h);
-                }
+                logits(0, 0);
+                if (paired) logits(1, 0);
                 tensor_commit(lead, empty(0));
             }
             if (!paired && tiles > 1) {
                 arrived(key_number(1));
                 if (ok) {
-                    for (int h = 0; h < 2; ++h) logits(1, 1, h);
+                    logits(1, 1);
                     tensor_commit(lead, empty(key_number(1) % S::kStages));
                 }
             }
-            // what takes the place of a P that has been multiplied comes right after it
             for (int j = 0; j < tiles && ok; ++j) {
-                const int next = paired ? j + 1 : j + 2, first = paired ? 0 : j & 1, last = paired ? 1 : j & 1;
                 values(j);
-                if (next < tiles) arrived(key_number(next));
-                for (int h = 0; h < 2 && ok; ++h) {
-                    for (int g = first; g <= last && ok; ++g) {
-                        results(g, j, h, paired ? j : j >> 1);
-                        if (ok && next < tiles) logits(g, next, h);
+                if (paired) {
+                    if (j + 1 < tiles) arrived(key_number(j + 1));
+                    for (int g = 0; g < 2 && ok; ++g) {
+                        results(g, j, j);
+                        if (!ok) break;
+                        if (g) tensor_commit(lead, empty(value_number(j) % S::kStages));
+                        if (j + 1 < tiles) {
+                            logits(g, j + 1);
+                            if (g) tensor_commit(lead, empty(key_number(j + 1) % S::kStages));
+                        }
+                    }
+                } else {
+                    results(j & 1, j, j >> 1);
+                    if (!ok) break;
+                    tensor_commit(lead, empty(value_number(j) % S::kStages));
+                    if (j + 2 < tiles) {
+                        arrived(key_number(j + 2));
+                        if (!ok) break;
+                        logits(j & 1, j + 2);
+                        tensor_commit(lead, empty(key_number(j + 2) % S::kStages));
                     }
                 }
-                if (!ok) break;
-                tensor_commit(lead, empty(value_number(j) % S::kStages));
-                if (next < tiles) tensor_commit(lead, empty(key_number(next) % S::kStages));
             }
             tensor_commit(lead, done);
             warp_wait(done, 0, &failed);
@@ -294,97 +283,74 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
         const uint32_t mine = (uint32_t)(warp & 3) << 21, s_mine = s_at + g * 128 + mine, o_mine = o_at + g * 128 + mine;
         const int turns = paired ? tiles : (tiles - g + 1) / 2;
         float m = -INFINITY;
-        float2 sum = make_float2(0.f, 0.f);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
         bool ok = true;
-        uint32_t s[2][32];
-        bool asked_for = false;      // this half's logits, while the last one's weights were made
-#pragma unroll 1
-        for (int step = 0; step < 2 * turns; ++step) {
-            const int h = step & 1, turn = step >> 1;
-            if (!some) {
-                ok = warp_wait(s_full(g, h), (uint32_t)turn & 1u, &failed);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive(p_ready(g, h));
-                continue;
-            }
-            if (!asked_for) {
-                ok = warp_wait(s_full(g, h), (uint32_t)turn & 1u, &failed);
-                if (!ok) break;
-                tensor_fence_after();
-                tmem_ask32(s_mine + h * 64, s[0]);
-                tmem_ask32(s_mine + h * 64 + 32, s[1]);
-            }
-            const int key = key0 + (paired ? turn : 2 * turn + g) * kPrefixKeys + h * 64;
-            tmem_arrived(s[0]);
-            tmem_arrived(s[1]);
-            if (key_end - key < 64 || absent) {
-                leave_gaps(p, key, key_end, s[0]);
-                leave_gaps(p, key + 32, key_end, s[1]);
-            }
-            float top[4];
+        for (int turn = 0; turn < turns; ++turn) {
+            ok = warp_wait(s_full(g), (uint32_t)turn & 1u, &failed);
+            if (!ok) break;
+            tensor_fence_after();
+            if (some) {
+                const int j = paired ? turn : 2 * turn + g, key = key0 + j * kPrefixKeys;
+                uint32_t s[4][32];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                top[k] = max3(__uint_as_float(s[0][k]), __uint_as_float(s[1][k]), __uint_as_float(s[0][k + 4]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 4]), __uint_as_float(s[0][k + 8]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 8]), __uint_as_float(s[0][k + 12]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 12]), __uint_as_float(s[0][k + 16]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 16]), __uint_as_float(s[0][k + 20]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 20]), __uint_as_float(s[0][k + 24]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 24]), __uint_as_float(s[0][k + 28]));
-                top[k] = max3(top[k], __uint_as_float(s[1][k + 28]), __uint_as_float(s[1][k + 28]));
-            }
-            const float high = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * p.scale_log2;
-            if (step == 0) {
-                m = high;
-            } else if (const bool grown = !(high <= m + kRescale); __any_sync(0xFFFFFFFFu, grown)) {
-                // the last half's weights may still be on their way into the result
-                ok = warp_wait(added(g), (uint32_t)(step - 1) & 1u, &failed);
-                if (!ok) break;
-                tensor_fence_after();
-                // rows that have not keep their scale: what a row gets does not go by its neighbours
-                const float next = grown ? max3(m, high, high) : m, up = grown ? fast_exp2(m - (next == -INFINITY ? 0.f : next)) : 1.f;
-                m = next;
-                sum.x *= up;
-                sum.y *= up;
-#pragma unroll 1
-                for (int c = 0; c < DIM / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ask32(o_mine + c * 32, o);
-                    tmem_arrived(o);
+                for (int c = 0; c < 4; ++c) tmem_ask32(s_mine + c * 32, s[c]);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
-                    tmem_store32(o_mine + c * 32, o);
+                for (int c = 0; c < 4; ++c) tmem_arrived(s[c]);
+                if (key_end - key < kPrefixKeys || absent) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) leave_gaps(p, key + c * 32, key_end, s[c]);
                 }
-            }
-            const float from = m == -INFINITY ? 0.f : m;
-            const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), from2 = make_float2(-from, -from), one2 = make_float2(1.f, 1.f);
-            uint32_t w[32];
-            const int next = step + 1;
+                float top[8];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+                for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(s[0][i]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float2 e = fma2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, from2);
-                    if (i % 3 == 2) {
-                        e = poly_exp2(e);
-                    } else {
-                        e.x = fast_exp2(e.x);
-                        e.y = fast_exp2(e.y);
+                for (int i = 8; i < kPrefixKeys; ++i) top[i & 7] = max2(top[i & 7], __uint_as_float(s[i >> 5][i & 31]));
+                const float high = max2(max2(max2(top[0], top[1]), max2(top[2], top[3])), max2(max2(top[4], top[5]), max2(top[6], top[7]))) * p.scale_log2;
+                if (turn == 0) {
+                    m = high;
+                } else if (const bool grown = !(high <= m + kRescale); __any_sync(0xFFFFFFFFu, grown)) {
+                    // rows that have not keep their scale: what a row gets does not go by its neighbours
+                    const float next = grown ? max2(m, high) : m, up = grown ? fast_exp2(m - (next == -INFINITY ? 0.f : next)) : 1.f;
+                    m = next;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[i] *= up;
+#pragma unroll 1
+                    for (int c = 0; c < DIM / 16; ++c) {
+                        float o[16];
+                        tmem_load16(o_mine + c * 16, o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] *= up;
+                        tmem_store16(o_mine + c * 16, o);
                     }
-                    sum = fma2(e, one2, sum);
-                    w[c * 16 + i] = pack_pair<BF16>(e.x, e.y);
                 }
-                if (c == 0) {
-                    asked_for = next < 2 * turns && __all_sync(0xFFFFFFFFu, mbar_try_wait(s_full(g, next & 1), (uint32_t)(next >> 1) & 1u));
-                    tensor_fence_after();
+                const float from = m == -INFINITY ? 0.f : m;
+                // the tensor cores multiply the first half's weights while the second's are made
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        // nothing waits for what was begun right before it: two warps a scheduler do not hide that
+                        float e[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) e[i] = fmaf(__uint_as_float(s[half * 2 + c][i]), p.scale_log2, -from);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) e[i] = fast_exp2(e[i]);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[i & 3] += e[i];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[c * 16 + i] = pack_pair<BF16>(e[2 * i], e[2 * i + 1]);
+                    }
+                    tmem_store32(s_mine + half * 32, w);
+                    tmem_stored();
+                    tensor_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready(g, half));
                 }
-                if (asked_for) tmem_ask32(s_mine + (next & 1) * 64 + c * 32, s[c]);
+            } else if (lane == 0) {
+                mbar_arrive(p_ready(g, 0));
+                mbar_arrive(p_ready(g, 1));
             }
-            tmem_store32(s_mine + h * 64, w);
-            tmem_stored();
-            tensor_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready(g, h));
         }
         ok = ok && warp_wait(done, 0, &failed);
         tensor_fence_after();
@@ -413,7 +379,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
                     if (row - lane + r < rows) *reinterpret_cast<uint4*>(p.prefix_o + (first_part + r) * DIM + c * 32 + piece * 4) = v;
                 }
             }
-            if (row < rows) p.prefix_ml[part] = make_float2(m, sum.x + sum.y);
+            if (row < rows) p.prefix_ml[part] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
     }
     __syncwarp();
