@@ -127,13 +127,18 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
     const auto key_number = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
     const auto value_number = [&](int j) { return j + 1 < tiles ? 2 * j + 2 : 2 * tiles - 1; };
 
-    // What the softmax warps and the multiplying one wait for: the queries in shared memory, and whether pages are absent.
-    const auto prepared = [&]() { asm volatile("bar.sync 1, 288;" ::: "memory"); };
+    // What the softmax warps and the multiplying one wait for: the queries in shared memory, and (from warps 10 and 11) whether pages are absent.
+    const auto prepared = [&]() { asm volatile("bar.sync 1, 352;" ::: "memory"); };
 
     // a row's 128 logits want more registers than a 512th of them: the other warps give up theirs (256 x 192 + 128 x 64 + 128 x 64 = 512 x 128)
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 9) {
+        if (warp == 10 || warp == 11) {
+            const int first = key0 >> p.page_shift, last = (key_end - 1) >> p.page_shift;
+            for (int i = first + threadIdx.x - 320; i <= last; i += 64)
+                if ((uint32_t)p.prefix_table[i] >= (uint32_t)p.pages) absent = 1u;
+            prepared();
+        } else if (warp == 9) {
             const int box = (int)min(p.page_mask + 1, (int64_t)kPrefixKeys), boxes = kPrefixKeys / box;
             // this lane's box of a tile: its page (the one behind the last, which gives zeros, for one outside), or -1
             const auto page_of = [&](int j) {
@@ -254,27 +259,26 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // the queries, as the tensor cores read them: 16-byte pieces XORed with the row; eight at a time under way
-        constexpr int kAhead = DIM / 16;      // pieces of a row by 256 threads
+        constexpr int kAhead = DIM / 16, kRowStep = 256 / (DIM / 8);      // pieces of a tile by 256 threads, and how many rows on the next one is
         for (int tile = 0; tile < (paired ? 2 : 1); ++tile) {
             uint4 v[kAhead];
+            const int r0 = threadIdx.x / (DIM / 8), piece = threadIdx.x % (DIM / 8), row0 = (x * 2 + tile) * kPrefixRows + r0;
+            int sequence = row0 / p.group, in_group = row0 % p.group;
+            const int sequences = kRowStep / p.group, others = kRowStep % p.group;
+            const uint16_t* q = p.q + (int64_t)kv_head * p.group * p.q_head + piece * 8;
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int r = (i * 256 + threadIdx.x) / (DIM / 8), piece = threadIdx.x % (DIM / 8), row = (x * 2 + tile) * kPrefixRows + r;
                 v[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (row < rows) v[i] = *reinterpret_cast<const uint4*>(p.q + (int64_t)(row / p.group) * p.q_token + (int64_t)(kv_head * p.group + row % p.group) * p.q_head + piece * 8);
+                if (sequence < p.batch) v[i] = *reinterpret_cast<const uint4*>(q + sequence * p.q_token + in_group * p.q_head);
+                sequence += sequences;
+                in_group += others;
+                if (in_group >= p.group) { in_group -= p.group; ++sequence; }
             }
+            uint8_t* to = smem + tile * S::kStage + piece / 8 * S::kHalf + r0 * 128 + (((piece & 7) ^ (r0 & 7)) << 4);      // the rows' steps are multiples of eight
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const int r = (i * 256 + threadIdx.x) / (DIM / 8), piece = threadIdx.x % (DIM / 8);
-                *reinterpret_cast<uint4*>(smem + tile * S::kStage + piece / 8 * S::kHalf + r * 128 + (((piece & 7) ^ (r & 7)) << 4)) =
-                    make_uint4(query_pair<BF16>(v[i].x, p.q_factor), query_pair<BF16>(v[i].y, p.q_factor), query_pair<BF16>(v[i].z, p.q_factor),
-                               query_pair<BF16>(v[i].w, p.q_factor));
-            }
-        }
-        {
-            const int first = key0 >> p.page_shift, last = (key_end - 1) >> p.page_shift;
-            for (int i = first + threadIdx.x; i <= last; i += 256)
-                if ((uint32_t)p.prefix_table[i] >= (uint32_t)p.pages) absent = 1u;
+            for (int i = 0; i < kAhead; ++i)
+                *reinterpret_cast<uint4*>(to + i * kRowStep * 128) = make_uint4(query_pair<BF16>(v[i].x, p.q_factor), query_pair<BF16>(v[i].y, p.q_factor),
+                                                                               query_pair<BF16>(v[i].z, p.q_factor), query_pair<BF16>(v[i].w, p.q_factor));
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the tensor core reads what was written here
         prepared();
@@ -359,10 +363,12 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
             // by way of the ring, whose tiles have been multiplied: straight from the registers every store would touch 32 rows
             const uint32_t rows_at = ring + warp * (32 * 128);      // 32 rows of 32 columns, pieces XORed with the row
             const int64_t first_part = part - lane;
+            uint32_t all[DIM / 32][32];
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) tmem_ask32(o_mine + c * 32, all[c]);
 #pragma unroll
             for (int c = 0; c < DIM / 32; ++c) {
-                uint32_t o[32];
-                tmem_ask32(o_mine + c * 32, o);
+                uint32_t(&o)[32] = all[c];
                 tmem_arrived(o);
                 __syncwarp();
 #pragma unroll

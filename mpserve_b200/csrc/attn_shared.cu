@@ -12,9 +12,9 @@ namespace mps {
 
 // ---- the parts of a query joined -----------------------------------------------------------------------
 //
-// A warp has a head of a sequence, its lanes the columns, eight parts at a time under way; with many parts of few heads four warps share them.  (One after the
+// A warp has a head of a sequence, its lanes the columns, eight parts at a time under way; with few heads eight warps share one's parts.  (One after the
 // other, a warp to a head, the parts of four sequences behind 1024 took 43 us.)
-constexpr int kJoinWarps = 4, kJoinAhead = 8;
+constexpr int kJoinWarps = 8, kJoinAhead = 8;
 constexpr int64_t kJoinFewHeads = 1024;
 template <int DIM, bool BF16, int SHARE>
 __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
