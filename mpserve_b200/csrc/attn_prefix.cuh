@@ -358,23 +358,23 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
         }
         ok = ok && warp_wait(done, 0, &failed);
         tensor_fence_after();
+        const float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!paired) {
+            float2* turn_ml = reinterpret_cast<float2*>(smem + S::kRing + 65536);      // of both groups; behind what the rows pass through below
+            turn_ml[threadIdx.x] = make_float2(m, total);
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+        }
         if (ok && some) {
-            const int64_t part = ((int64_t)(paired ? stretch : 2 * stretch + g) * p.kv_heads + kv_head) * rows + row;
-            // by way of the ring, whose tiles have been multiplied: straight from the registers every store would touch 32 rows
-            const uint32_t rows_at = ring + warp * (32 * 128);      // 32 rows of 32 columns, pieces XORed with the row
-            const int64_t first_part = part - lane;
-            uint32_t all[DIM / 32][32];
-#pragma unroll
-            for (int c = 0; c < DIM / 32; ++c) tmem_ask32(o_mine + c * 32, all[c]);
-#pragma unroll
-            for (int c = 0; c < DIM / 32; ++c) {
-                uint32_t(&o)[32] = all[c];
-                tmem_arrived(o);
+            // By way of the ring, whose tiles have been multiplied: straight from the registers every store would touch 32 rows.  There: 32 rows of 32 columns,
+            // pieces XORed with the row.
+            const uint32_t rows_at = ring + warp * (32 * 128);
+            const int64_t part = ((int64_t)stretch * p.kv_heads + kv_head) * rows + row, first_part = part - lane;
+            const auto store = [&](int column, const auto& o) {
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rows_at + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(turns ? o[4 * i] : 0u),
-                                 "r"(turns ? o[4 * i + 1] : 0u), "r"(turns ? o[4 * i + 2] : 0u), "r"(turns ? o[4 * i + 3] : 0u) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(rows_at + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(o[4 * i]), "r"(o[4 * i + 1]),
+                                 "r"(o[4 * i + 2]), "r"(o[4 * i + 3]) : "memory");
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -382,10 +382,43 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
                     uint4 v;
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                  : "r"(rows_at + r * 128 + ((piece ^ (r & 7)) << 4)) : "memory");
-                    if (row - lane + r < rows) *reinterpret_cast<uint4*>(p.prefix_o + (first_part + r) * DIM + c * 32 + piece * 4) = v;
+                    if (row - lane + r < rows) *reinterpret_cast<uint4*>(p.prefix_o + (first_part + r) * DIM + column + piece * 4) = v;
                 }
+            };
+            if (paired) {
+                uint32_t o[DIM / 32][32];
+#pragma unroll
+                for (int c = 0; c < DIM / 32; ++c) tmem_ask32(o_mine + c * 32, o[c]);
+#pragma unroll
+                for (int c = 0; c < DIM / 32; ++c) {
+                    tmem_arrived(o[c]);
+                    store(c * 32, o[c]);
+                }
+                if (row < rows) p.prefix_ml[part] = make_float2(m, total);
+            } else {
+                // both groups' sums of the same rows become one, each group half of the columns: half as many parts to write and to join (with two, 32 sequences
+                // behind 8192 wrote 11.5 MB of them)
+                const float2* turn_ml = reinterpret_cast<const float2*>(smem + S::kRing + 65536);
+                const float2 first = turn_ml[threadIdx.x & 127], second = turn_ml[128 + (threadIdx.x & 127)];
+                const float high = max2(first.x, second.x), from = high == -INFINITY ? 0.f : high, f0 = fast_exp2(first.x - from), f1 = fast_exp2(second.x - from);
+                const uint32_t o_half = o_at + mine + g * (DIM / 2);
+                uint32_t o0[DIM / 64][32], o1[DIM / 64][32];
+#pragma unroll
+                for (int c = 0; c < DIM / 64; ++c) {
+                    tmem_ask32(o_half + c * 32, o0[c]);
+                    tmem_ask32(o_half + 128 + c * 32, o1[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < DIM / 64; ++c) {
+                    tmem_arrived(o0[c]);
+                    tmem_arrived(o1[c]);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)      // of one tile the second group has had none, and nothing is in its sums
+                        o0[c][i] = __float_as_uint(fmaf(__uint_as_float(o0[c][i]), f0, tiles > 1 ? __uint_as_float(o1[c][i]) * f1 : 0.f));
+                    store(g * (DIM / 2) + c * 32, o0[c]);
+                }
+                if (g == 0 && row < rows) p.prefix_ml[part] = make_float2(high, fmaf(first.y, f0, second.y * f1));
             }
-            if (row < rows) p.prefix_ml[part] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
     }
     __syncwarp();

@@ -24,12 +24,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     griddep_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q_heads = p.kv_heads * p.group, tiles = (q_heads + kHeads - 1) / kHeads;
     const int sequence = blockIdx.x / tiles, head = blockIdx.x % tiles * kHeads + warp / SHARE, share = warp % SHARE;
-    const int stretches = p.plan[0], own_before = p.plan[1 + sequence], own_count = p.plan[2 + sequence] - own_before;
+    const int splits = p.plan[0], own_before = p.plan[1 + sequence], own_count = p.plan[2 + sequence] - own_before;
     if (SHARE == 1 && head >= q_heads) return;
     const int kv_head = head / p.group, in_group = head % p.group;
-    const int64_t rows = (int64_t)p.batch * p.group, twice = (rows + kPrefixRows - 1) / kPrefixRows / 2 * 2 * kPrefixRows, row = (int64_t)sequence * p.group + in_group;
-    // rows from `twice` on have two parts of each stretch of the prefix
-    const int splits = row < twice ? stretches : 2 * stretches, count = splits + own_count;
+    const int64_t rows = (int64_t)p.batch * p.group, row = (int64_t)sequence * p.group + in_group;
+    const int count = splits + own_count;
     const int64_t prefix_step = p.kv_heads * rows, prefix_first = kv_head * rows + row, own_step = (int64_t)p.kv_heads * p.group;
     const int64_t own_first = ((int64_t)own_before * p.kv_heads + kv_head) * p.group + in_group;
     float top = -INFINITY, sum = 0.f, out[kColumns];
@@ -101,12 +100,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 struct AttendPlan {
     int wide_tiles;               // CTAs for a stretch of the prefix and a key head
     int most_splits;              // stretches of the prefix, at most
-    int prefix_parts;             // of a row, at most
     int own_ctas;                 // -1: the GPU settles it
     int64_t ctas;
     int64_t own_items;            // stretches of own keys, at most
     int64_t floats(int64_t rows, int64_t kv_heads, int64_t group, int64_t dim) const {      // of the scratch, behind its first part
-        return (prefix_parts * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
+        return (most_splits * kv_heads * rows + own_items * kv_heads * group) * (dim + 2);
     }
 };
 static int64_t plan_words(int64_t batch) { return (batch + 2 + 3) / 4 * 4; }
@@ -128,7 +126,6 @@ static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
         } else {
             plan.most_splits = (int)std::min<int64_t>(tiles, (sms - (most > 0)) / units);
         }
-        plan.prefix_parts = plan.most_splits * (row_tiles % 2 ? 2 : 1);
     }
     if (most > 0) {
         const int64_t extra = std::min<int64_t>((4 * kOwnWarps * (int64_t)sms + heads - 1) / heads, a.batch * ((most + kOwnLeast - 1) / kOwnLeast));
@@ -274,7 +271,7 @@ extern "C" int mps_prefix_attend_tokens(const mps_prefix_attend* args, void* scr
     // a negative scale is the queries' sign, one of 0 makes them zeros: what multiplies the logits is positive, and the largest stays the largest
     p.q_factor = a.scale > 0.f ? 1 : a.scale < 0.f ? -1 : a.scale == 0.f ? 0 : 1;
     p.scale_log2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.4426950408889634f;
-    const int64_t prefix_parts = plan.prefix_parts * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
+    const int64_t prefix_parts = plan.most_splits * a.kv_heads * rows, own_parts = plan.own_items * a.kv_heads * group;
     p.plan = static_cast<int32_t*>(scratch);
     p.prefix_o = static_cast<float*>(scratch) + plan_words(a.batch);
     p.own_o = p.prefix_o + prefix_parts * a.dim;
