@@ -6,12 +6,14 @@
 //   P = 2^(S - m) in the cache's type, which takes S's place: a thread has a row, so that maxima and sums need no other thread;
 //   O += P V    128 x dim in tensor memory, P from there.
 // While one group makes its P, the tensor cores work for the other.  With more than 128 rows each group has 128 of them and both use the same keys; with no more
-// (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of keys in turn, and their results are two parts.
+// (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of keys in turn, and add their results up at the end.
 //
 // O is scaled anew only where a row's largest logit has grown by more than 2^8 since it last was: P is then at most 2^8, which is far from the end of
 // either type's range, and what m a part refers to does not matter when parts are joined.  P is rounded to 16 bits, as the tensor cores take it: a relative
 // 2^-8 (BF16) of every weight by itself, below what the result is rounded by.  Sums are of P as it was before.
-// Bounds: for many rows the tensor cores and the exponentials alike (128 x 128 logits are 1024 cycles of each per group at the nominal rates), for few the memory.
+// Bounds: for many rows the softmax.  A period of 128 keys by 256 rows takes 3750 cycles: 2560 of a row's softmax (500 to fetch it, 290 for its maximum, the rest for
+// exponentials, sums and packing; 128 x 128 exponentials are 1024 of a scheduler's at the nominal rate) and 690 of two hand-overs, where the products are 2048 for both groups.
+// 128 sequences behind 32768 keys with none of their own take 84 to 88 us (32 query heads, 8 key heads of 128).  For few rows the memory.
 #pragma once
 
 #include <cuda.h>
@@ -22,7 +24,7 @@
 namespace mps {
 
 constexpr int kAttendThreads = 512;
-constexpr float kRescale = 8.f;      // in powers of two
+constexpr float kRescale = 8.f;      // in powers of two; with 0, scaling with every larger maximum, 128 sequences behind 32768 keys took 88.7 us instead of 83.4
 
 template <int DIM>
 struct PrefixShape {

@@ -127,7 +127,9 @@ constexpr int kInt4Workers = 8, kInt4Adders = 4, kInt4Threads = (2 + kInt4Worker
 constexpr int kInt4StageTiles = 2;
 constexpr int kInt4Buffers = 4, kInt4Sums = 4, kInt4MostParts = 8;
 constexpr int kInt4Smem = 227 << 10;
-constexpr int kInt4FewTokens = 32;
+// Up to 16 tokens codes stay in registers (1, 8 and 16 tokens through 14336 x 4096: 10.6, 10.7 and 13.3 us); more tokens there want as many registers again and took 30 us
+// for 17 to 32, where the other kernel takes 16 for 33 and 17 for 64.
+constexpr int kInt4FewTokens = 16;
 
 struct Int4Args {
     const uint8_t* w;
@@ -240,7 +242,7 @@ __device__ __forceinline__ void token_boxes(uint32_t dst, const CUtensorMap* map
     }
 }
 
-// ---- up to 32 tokens: codes stay in registers -----------------------------------------------------------
+// ---- up to 16 tokens: codes stay in registers -----------------------------------------------------------
 //
 // Sixteen warps, four sets of four that take tiles in turn, a warp 32 rows: a code word becomes the left operand of an m16n8k16 where it is, and a group's products
 // are multiplied by its scale in registers.  Bound: memory; taking codes apart (11 instructions for eight codes, seven of them on a pipe that takes two a
@@ -324,13 +326,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
             const uint8_t* tile = smem + s * S::kStage + S::kX + set % kInt4StageTiles * S::kTile;
             const uint4* codes = reinterpret_cast<const uint4*>(tile + quarter * 2048) + lane;
             const uint32_t* words = reinterpret_cast<const uint32_t*>(tile + kInt4CodeBytes) + quarter * (S::kGroups * 32) + g;
-            uint2 b[TOKENS <= 16 ? kTiles : 1][8];
-            if (TOKENS <= 16) {
+            uint2 b[kTiles][8];
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
+            for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) b[TOKENS <= 16 ? n : 0][k] = *reinterpret_cast<const uint2*>(x + x_at[k & 3] + (k >> 2) * (TOKENS * 128) + n * 1024);
-            }
+                for (int k = 0; k < 8; ++k) b[n][k] = *reinterpret_cast<const uint2*>(x + x_at[k & 3] + (k >> 2) * (TOKENS * 128) + n * 1024);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint4 w[2] = {codes[h * 64], codes[h * 64 + 32]};
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
                     const uint32_t a[4] = {masks.pair(v, 0, zlo), masks.pair(v, 1, zhi), masks.pair(v, 2, zlo), masks.pair(v, 3, zhi)};
 #pragma unroll
                     for (int n = 0; n < kTiles; ++n) {
-                        const uint2 y = TOKENS <= 16 ? b[TOKENS <= 16 ? n : 0][k] : *reinterpret_cast<const uint2*>(x + x_at[k & 3] + (k >> 2) * (TOKENS * 128) + n * 1024);
+                        const uint2 y = b[n][k];
                         if (k * kParts % 8 == 0) multiply_first<BF16>(sums[n][c], a, y.x, y.y);
                         else multiply<BF16>(sums[n][c], a, y.x, y.y);
                     }
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) int4_few_kernel(const Int4Args
 //   0 copies;  1 multiplies: features (left operand, tensor memory) by tokens (right operand, shared memory), a group of columns into an accumulator of its own;
 //   2 to 9 take codes apart and store them in tensor memory, four warps a tile, 32 rows each: two tiles at a time, since what one takes is mostly waits in a row;
 //   10 to 13 add the groups' accumulators up, times their scales: a thread has a feature, its tokens are in registers.
-// Bound: the left operand: its 32 KB of a tile cost the tensor core some 700 cycles, however few tokens there are.
+// Bound: handing over.  16 columns by 64 tokens take the tensor core 33 cycles, a tile 260; each of the tile's groups waits some 150 for codes, products or sums of the other side.
 template <int TOKENS, int GROUP, bool BF16>
 __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4Args p, const __grid_constant__ CUtensorMap x_map) {
     using S = Int4Tensor<TOKENS, GROUP>;
@@ -557,13 +557,12 @@ __global__ void __launch_bounds__(kInt4Threads, 1) int4_tensor_kernel(const Int4
                 if (g) ok = ok && warp_wait(summed(d), (uint32_t)(n / kInt4Sums) & 1u, &failed);
                 if (!ok) break;
                 tensor_fence_after();
-                constexpr int kStep = TOKENS < 32 ? TOKENS : 32;
+                constexpr int kStep = 32;
 #pragma unroll
                 for (int c = 0; c < TOKENS; c += kStep) {
                     if (c < tokens) {
                         float v[kStep];
-                        if constexpr (kStep == 16) tmem_load16(from + d * TOKENS + c, v);
-                        else tmem_load32(from + d * TOKENS + c, v);
+                        tmem_load32(from + d * TOKENS + c, v);
                         const float2 s2 = make_float2(scale[g], scale[g]);
 #pragma unroll
                         for (int t = 0; t < kStep; t += 2) {
@@ -660,8 +659,8 @@ static int launch_tokens(const Int4Args& p, const Int4Tokens& x, int group, cons
 }
 template <bool BF16>
 static int launch_product(const Int4Args& p, const Int4Tokens& x, int group, const Device& d, cudaStream_t st) {
-    return p.tokens <= 8 ? launch_tokens<8, BF16>(p, x, group, d, st) : p.tokens <= 16 ? launch_tokens<16, BF16>(p, x, group, d, st)
-         : p.tokens <= 32 ? launch_tokens<32, BF16>(p, x, group, d, st) : launch_tokens<64, BF16>(p, x, group, d, st);
+    return p.tokens <= 8 ? launch_tokens<8, BF16>(p, x, group, d, st) : p.tokens <= kInt4FewTokens ? launch_tokens<16, BF16>(p, x, group, d, st)
+                                                                           : launch_tokens<64, BF16>(p, x, group, d, st);
 }
 
 // Tokens whose rows do not begin at multiples of 16 bytes, as tiled copies want them, or lie over one another: copied into rows that do.
