@@ -103,6 +103,8 @@ class KvCache:
                     raise ValueError(f"{name} has places that share memory")
                 if n > 1:
                     reach = s * (n - 1) + reach
+        if torch.cuda.is_available():
+            _workspace(k_pages.get_device())      # there before the first call, which may be captured: a graph's own memory goes with it
         self._k_pages, self._v_pages = k_pages, v_pages
 
     k_pages = property(lambda self: self._k_pages)

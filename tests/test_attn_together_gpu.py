@@ -146,3 +146,12 @@ def test_gradients_do_not_pass():
     layer = _Layer(11, 2)
     layer.x.requires_grad_()
     assert not any(t.requires_grad for t in layer.step())
+
+
+def test_a_cache_brings_the_workspace(monkeypatch):
+    """A first call that is captured must not allocate it: it would be the graph's."""
+    monkeypatch.setattr(mx4, "_workspaces", {})
+    pages = torch.zeros((2, PAGE, KV_HEADS, DIM), dtype=torch.bfloat16, device="cuda")
+    attention.KvCache(pages, pages.clone())
+    kept = mx4._workspaces[pages.get_device()]
+    assert not kept.any()
