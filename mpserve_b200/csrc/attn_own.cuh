@@ -10,6 +10,10 @@
 
 namespace mps {
 
+// Weights are 2^(logit - m), rounded to the cache's type before they multiply the values.  In F16 m is so many powers of two below the largest logit: weights are at most
+// 2^15, and the small ones keep their digits down to 2^-29 of the largest.
+constexpr float kOwnLift = 15.f;
+
 template <int DIM>
 struct FewShape {
     static constexpr int kRow = DIM * 2, kBlock = 16 * kRow, kStage = 2 * kBlock;      // 16 keys, then their values
@@ -128,6 +132,7 @@ __device__ __forceinline__ void attend_own(const AttendArgs& p, int own_step, ui
             float top = fmaxf(s[i], s[i + 2]);
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+            if (!BF16) top -= kOwnLift;
             top = fmaxf(top, m[i]);
             const float base = top == -INFINITY ? 0.f : top;
             up[i] = exp2f(m[i] - base);

@@ -8,9 +8,11 @@
 // While one group makes its P, the tensor cores work for the other.  With more than 128 rows each group has 128 of them and both use the same keys; with no more
 // (or for the last 128 of an odd number of such tiles) the groups take the stretch's tiles of keys in turn, and add their results up at the end.
 //
-// O is scaled anew only where a row's largest logit has grown by more than 2^8 since it last was: P is then at most 2^8, which is far from the end of
-// either type's range, and what m a part refers to does not matter when parts are joined.  P is rounded to 16 bits, as the tensor cores take it: a relative
-// 2^-8 (BF16) of every weight by itself, below what the result is rounded by.  Sums are of P as it was before.
+// O is scaled anew only where a row's largest logit has grown by more than 2^kRescale since it last was; what m a part refers to does not matter when parts are
+// joined.  P is rounded to 16 bits, as the tensor cores take it: a relative 2^-8 (BF16) or 2^-11 (F16) of every weight by itself, no more than what the result is rounded by.
+// Sums are of P as it was before.  BF16 has FP32's range, and m is the largest logit: P is at most 2^8.  F16 has numbers down to 2^-14, and below that steps of 2^-24: there m is
+// 2^12 below the largest logit, P at most 2^15, a weight keeps its 2^-11 down to 2^-26 of the stretch's largest and is off by 2^-37 of that beyond.  (With m the largest
+// logit itself, 99 keys behind one that weighed e^17 as much and had no value lost 44 % of their result.)
 // Bounds: for many rows the softmax.  A period of 128 keys by 256 rows takes 3750 cycles: 2560 of a row's softmax (500 to fetch it, 290 for its maximum, the rest for
 // exponentials, sums and packing; 128 x 128 exponentials are 1024 of a scheduler's at the nominal rate) and 690 of two hand-overs, where the products are 2048 for both groups.
 // 128 sequences behind 32768 keys with none of their own take 84 to 88 us (32 query heads, 8 key heads of 128).  For few rows the memory.
@@ -24,7 +26,10 @@
 namespace mps {
 
 constexpr int kAttendThreads = 512;
-constexpr float kRescale = 8.f;      // in powers of two; with 0, scaling with every larger maximum, 128 sequences behind 32768 keys took 88.7 us instead of 83.4
+// In powers of two.  Of BF16 with a kRescale of 0, scaling with every larger maximum, 128 sequences behind 32768 keys took 88.7 us instead of 83.4; F16 takes 85.3, and
+// without a lift and with a kRescale of 8 took 84.2.
+template <bool BF16> constexpr float kLift = BF16 ? 0.f : 12.f;
+template <bool BF16> constexpr float kRescale = BF16 ? 8.f : 3.f;
 
 template <int DIM>
 struct PrefixShape {
@@ -311,10 +316,11 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
                 for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(s[0][i]);
 #pragma unroll
                 for (int i = 8; i < kPrefixKeys; ++i) top[i & 7] = max2(top[i & 7], __uint_as_float(s[i >> 5][i & 31]));
-                const float high = max2(max2(max2(top[0], top[1]), max2(top[2], top[3])), max2(max2(top[4], top[5]), max2(top[6], top[7]))) * p.scale_log2;
+                float high = max2(max2(max2(top[0], top[1]), max2(top[2], top[3])), max2(max2(top[4], top[5]), max2(top[6], top[7]))) * p.scale_log2;
+                if (!BF16) high -= kLift<BF16>;
                 if (turn == 0) {
                     m = high;
-                } else if (const bool grown = !(high <= m + kRescale); __any_sync(0xFFFFFFFFu, grown)) {
+                } else if (const bool grown = !(high <= m + kRescale<BF16>); __any_sync(0xFFFFFFFFu, grown)) {
                     // rows that have not keep their scale: what a row gets does not go by its neighbours
                     const float next = grown ? max2(m, high) : m, up = grown ? fast_exp2(m - (next == -INFINITY ? 0.f : next)) : 1.f;
                     m = next;

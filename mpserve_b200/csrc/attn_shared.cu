@@ -2,7 +2,7 @@
 //
 //   out = sum_k softmax_k(scale q . key_k) value_k      over the prefix's keys and those of the sequence's own table
 //
-// Both lie in one paged cache.  A part of the keys gives, for a query, the largest logit m, l = sum_k 2^(logit_k - m) and o = sum_k 2^(logit_k - m) value_k (logits
+// Both lie in one paged cache.  A part of the keys gives, for a query, a number m near the largest logit, l = sum_k 2^(logit_k - m) and o = sum_k 2^(logit_k - m) value_k (logits
 // in units of log 2); parts join as
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
 // whatever the keys were split into, so that the prefix is read once for many queries and every sequence's own keys once, each in as many parts as fill the GPU.
