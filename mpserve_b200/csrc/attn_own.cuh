@@ -132,7 +132,7 @@ __device__ __forceinline__ void attend_own(const AttendArgs& p, int own_step, ui
             float top = fmaxf(s[i], s[i + 2]);
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-            if (!BF16) top -= kOwnLift;
+            if (!BF16) top = __fadd_ru(top, -kOwnLift);      // not below, however far FP32's numbers lie apart
             top = fmaxf(top, m[i]);
             const float base = top == -INFINITY ? 0.f : top;
             up[i] = exp2f(m[i] - base);

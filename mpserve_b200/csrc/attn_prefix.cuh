@@ -26,10 +26,14 @@
 namespace mps {
 
 constexpr int kAttendThreads = 512;
-// In powers of two.  Of BF16 with a kRescale of 0, scaling with every larger maximum, 128 sequences behind 32768 keys took 88.7 us instead of 83.4; F16 takes 85.3, and
-// without a lift and with a kRescale of 8 took 84.2.
+// In powers of two.  Of BF16 with a kRescale of 0, scaling with every larger maximum, 128 sequences behind 32768 keys took 88.7 us instead of 83.4; F16 takes 86.4, and
+// with a kRescale of 8 and nothing to keep small weights' digits took 84.2.
 template <bool BF16> constexpr float kLift = BF16 ? 0.f : 12.f;
 template <bool BF16> constexpr float kRescale = BF16 ? 8.f : 3.f;
+// Logits are scaled and have m taken off in one rounding, m being a rounded number: it may lie so far from the largest logit as FP32's rounding goes, and beyond 2^28 (F16) or
+// 2^31 (BF16) that is past the type's range, either way.  Rows whose largest is beyond this are scaled, rounded, first, as m was.  (To look for them costs 128 sequences behind
+// 32768 with up to 1024 own keys each 2 of 118 us.)
+constexpr float kWide = 1048576.f;
 
 template <int DIM>
 struct PrefixShape {
@@ -316,11 +320,19 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
                 for (int i = 0; i < 8; ++i) top[i] = __uint_as_float(s[0][i]);
 #pragma unroll
                 for (int i = 8; i < kPrefixKeys; ++i) top[i & 7] = max2(top[i & 7], __uint_as_float(s[i >> 5][i & 31]));
-                float high = max2(max2(max2(top[0], top[1]), max2(top[2], top[3])), max2(max2(top[4], top[5]), max2(top[6], top[7]))) * p.scale_log2;
-                if (!BF16) high -= kLift<BF16>;
+                float factor = p.scale_log2, high = max2(max2(max2(top[0], top[1]), max2(top[2], top[3])), max2(max2(top[4], top[5]), max2(top[6], top[7]))) * factor;
+                if (const bool wide = fabsf(high) > kWide; __any_sync(0xFFFFFFFFu, wide)) {
+                    const float now = wide ? factor : 1.f;      // a row's arithmetic does not go by its neighbours
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[c][i] = __float_as_uint(__uint_as_float(s[c][i]) * now);
+                    factor = wide ? 1.f : factor;
+                }
+                if (!BF16) high = __fadd_ru(high, -kLift<BF16>);      // not below the logit less the lift, and the sum not above, however far FP32's numbers lie apart
                 if (turn == 0) {
                     m = high;
-                } else if (const bool grown = !(high <= m + kRescale<BF16>); __any_sync(0xFFFFFFFFu, grown)) {
+                } else if (const bool grown = !(high <= __fadd_rd(m, kRescale<BF16>)); __any_sync(0xFFFFFFFFu, grown)) {
                     // rows that have not keep their scale: what a row gets does not go by its neighbours
                     const float next = grown ? max2(m, high) : m, up = grown ? fast_exp2(m - (next == -INFINITY ? 0.f : next)) : 1.f;
                     m = next;
@@ -345,7 +357,7 @@ __global__ void __launch_bounds__(kAttendThreads, 1) attend_kernel(const AttendA
                         // nothing waits for what was begun right before it: two warps a scheduler do not hide that
                         float e[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) e[i] = fmaf(__uint_as_float(s[half * 2 + c][i]), p.scale_log2, -from);
+                        for (int i = 0; i < 32; ++i) e[i] = fmaf(__uint_as_float(s[half * 2 + c][i]), factor, -from);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) e[i] = fast_exp2(e[i]);
 #pragma unroll

@@ -45,3 +45,27 @@ def test_one_key_that_dominates_and_has_no_value(dtype, where, keys, nats, place
         off = off + 2.0 ** -37 * mass
     ref.within(out, want, off)
     assert ((lse.double() - want_lse).abs() <= lse_off + ref.STEP * want_lse.abs()).all()
+
+
+@pytest.mark.parametrize("dtype,size", [("f16", 2.0 ** 15), ("bf16", 2.0 ** 15), ("bf16", 2.0 ** 40)])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_logits_with_no_digits_behind_the_point(dtype, size, where, sign):
+    """Logits whose FP32 steps are far apart: one key has all the weight, and its value is the result."""
+    g, kind, heads, page, keys = ref.generator(5), ref.TYPES[dtype], 8, 16, 300
+    shape = (-(-keys // page), page, heads, 64)
+    k, v = torch.zeros(shape, dtype=kind, device="cuda"), ref.randn(g, *shape, dtype=kind)
+    others = -1 if sign == 1 else -1.5      # times the best one's, or below it
+    k[..., 0] = others * size
+    k[150 // page, 150 % page, :, 0] = sign * size
+    q = torch.zeros((40, heads, 64), dtype=kind, device="cuda")
+    q[..., 0] = ((torch.rand((40, heads), generator=g, device="cuda") + 0.9) * size).to(kind)
+    q[7] = 0      # between such rows one whose keys have equal weights
+    (out, lse), rest = _call(q, k, v, where, keys)
+    best = v[150 // page, 150 % page]
+    keep = [b for b in range(40) if b != 7]
+    assert torch.equal(out[keep], best.expand(40, heads, 64)[keep])
+    want = q[..., 0].double() * size * sign
+    assert ((lse.double() - want).abs() <= 8 * ref.STEP * want.abs())[keep].all()
+    want, want_lse, off, _ = ref.attend(q[7:8], k, v, rest[0][7:8], rest[1][7:8], rest[2], rest[3], 1.0)
+    ref.within(out[7:8], want, off)
