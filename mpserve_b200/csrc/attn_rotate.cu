@@ -327,7 +327,12 @@ __global__ void __launch_bounds__(kRotateAnyWarps * 32) rotate_any_kernel(const 
 template <int LANES>
 static int launch_rotate(const RotateArgs& p, cudaStream_t st) {
     const int heads = p.a.q_heads + (p.a.v ? 2 : 1) * p.a.kv_heads;
-    if (p.a.tokens > kRotateFewTokens) {
+    const auto threads = [&](int steps) { return ((heads + steps - 1) / steps * LANES + 31) / 32 * 32; };
+    // Every head at once, where a CTA has the threads; in three or four steps, where 512 threads have that many (two steps of those would be 1024 threads' one).  64 query and
+    // 8 key heads of 128 in three steps take 3.5 us for a token, 7.0 for 400 and 11.3 for 888; in two of 1024 threads 3.2, 8.2 and 15.5; with warps a token 3.2, 8.4 and 11.2.
+    int steps = 1;
+    if (threads(1) > 1024) steps = threads(3) <= 512 ? 3 : threads(4) <= 512 ? 4 : 0;
+    if (p.a.tokens > kRotateFewTokens || !steps) {
         // as many warps for a token as there are places for on the GPU, and passes for
         const int passes = (heads * LANES + 31) / 32;
         int share = 1;
@@ -337,21 +342,11 @@ static int launch_rotate(const RotateArgs& p, cudaStream_t st) {
         return p.a.dtype == MPS_F32 ? launch_overlapping("rotate_many_kernel", rotate_many_kernel<LANES, true>, (unsigned int)ctas, dim3(kRotateWarps * 32), st, p, share)
                                     : launch_overlapping("rotate_many_kernel", rotate_many_kernel<LANES, false>, (unsigned int)ctas, dim3(kRotateWarps * 32), st, p, share);
     }
-    // every head at once, where a CTA has the threads
-    const int all = (heads * LANES + 31) / 32 * 32;
-    int steps = 1;
-    while (steps < 4 && (all + steps - 1) / steps > 1024) ++steps;
-    const int threads = ((heads + steps - 1) / steps * LANES + 31) / 32 * 32;
-    if (threads > (steps == 1 ? 1024 : 512)) return launch_overlapping("rotate_any_kernel", rotate_any_kernel, (unsigned int)p.a.tokens, dim3(kRotateAnyWarps * 32), st, p);
     const unsigned int ctas = (unsigned int)p.a.tokens;
-    if (p.a.dtype == MPS_F32) {
-        static void (*const kernels[4])(RotateArgs) = {rotate_kernel<LANES, 1, true>, rotate_kernel<LANES, 2, true>, rotate_kernel<LANES, 3, true>,
-                                                       rotate_kernel<LANES, 4, true>};
-        return launch_overlapping("rotate_kernel", kernels[steps - 1], ctas, dim3(threads), st, p);
-    }
-    static void (*const kernels[4])(RotateArgs) = {rotate_kernel<LANES, 1, false>, rotate_kernel<LANES, 2, false>, rotate_kernel<LANES, 3, false>,
-                                                   rotate_kernel<LANES, 4, false>};
-    return launch_overlapping("rotate_kernel", kernels[steps - 1], ctas, dim3(threads), st, p);
+    const dim3 block((unsigned int)threads(steps));
+    if (p.a.dtype == MPS_F32)
+        return launch_overlapping("rotate_kernel", steps == 1 ? rotate_kernel<LANES, 1, true> : steps == 3 ? rotate_kernel<LANES, 3, true> : rotate_kernel<LANES, 4, true>, ctas, block, st, p);
+    return launch_overlapping("rotate_kernel", steps == 1 ? rotate_kernel<LANES, 1, false> : steps == 3 ? rotate_kernel<LANES, 3, false> : rotate_kernel<LANES, 4, false>, ctas, block, st, p);
 }
 
 }  // namespace mps
