@@ -61,6 +61,9 @@ constexpr int kFewColumns = 8;             // query heads of a key head that go 
 
 struct AttendSplit { int splits, step, own_ctas, own_step; };      // of the prefix: stretches, and tiles of one; of own keys: CTAs, and keys of a stretch
 
+// Of a CTA that has so many tiles of the prefix's keys (up to 2^23).
+__host__ __device__ constexpr int64_t prefix_cycles(int tiles, int tile_cycles) { return kPrefixStart + (int64_t)tiles * tile_cycles; }
+
 // Lengths are at most 2^30.
 __device__ __forceinline__ int own_length(const AttendArgs& p, int b) { return min(max(p.lengths[b], 0), (int)p.most_own); }
 
@@ -85,17 +88,19 @@ __device__ __forceinline__ AttendSplit split_work(const AttendArgs& p, int ctas)
     } else if (tiles) {
         const int tile_cycles = (p.batch * p.group + kPrefixRows - 1) / kPrefixRows > 1 ? kPrefixPaired : kPrefixSingle;
         const float own_cycles = (float)keys * (float)heads * (float)(DIM * 4 / kOwnBytesPerCycle);
-        int best = 0x7FFFFFFF, best_splits = 1;
+        int64_t best = INT64_MAX;
+        int best_splits = 1;
         for (int s = lane + 1; s <= p.most_splits; s += 32) {
             const int left = ctas - units * s;
             if (keys && left < 1) break;
-            const float cost = fmaxf((float)(kPrefixStart + (tiles + s - 1) / s * tile_cycles), keys ? kOwnStart + own_cycles / (float)left : 0.f);
-            const int rounded = (int)fminf(cost, 2e9f);
-            if (rounded < best) { best = rounded; best_splits = s; }
+            const float own = keys ? kOwnStart + own_cycles / (float)left : 0.f;
+            const int64_t cost = max(prefix_cycles((tiles + s - 1) / s, tile_cycles), (int64_t)fminf(own, 1e18f));
+            if (cost < best) { best = cost; best_splits = s; }
         }
 #pragma unroll
         for (int x = 16; x; x >>= 1) {
-            const int cost = __shfl_xor_sync(0xFFFFFFFFu, best, x), s = __shfl_xor_sync(0xFFFFFFFFu, best_splits, x);
+            const int64_t cost = __shfl_xor_sync(0xFFFFFFFFu, best, x);
+            const int s = __shfl_xor_sync(0xFFFFFFFFu, best_splits, x);
             if (cost < best || (cost == best && s < best_splits)) { best = cost; best_splits = s; }
         }
         r.step = (tiles + best_splits - 1) / best_splits;
