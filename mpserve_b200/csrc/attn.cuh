@@ -64,6 +64,12 @@ struct AttendSplit { int splits, step, own_ctas, own_step; };      // of the pre
 // Of a CTA that has so many tiles of the prefix's keys (up to 2^23).
 __host__ __device__ constexpr int64_t prefix_cycles(int tiles, int tile_cycles) { return kPrefixStart + (int64_t)tiles * tile_cycles; }
 
+// Keys of a stretch, a multiple of 64: so many own keys in all in so many places.  No sequence is longer than 2^30, however many there are of them.
+__host__ __device__ constexpr int own_stretch(int64_t keys, int64_t places) {
+    const int64_t step = ((keys + places - 1) / places + 63) / 64 * 64;
+    return step < kOwnLeast ? kOwnLeast : step > MPS_MOST_KEYS ? (int)MPS_MOST_KEYS : (int)step;
+}
+
 // Lengths are at most 2^30.
 __device__ __forceinline__ int own_length(const AttendArgs& p, int b) { return min(max(p.lengths[b], 0), (int)p.most_own); }
 
@@ -110,7 +116,7 @@ __device__ __forceinline__ AttendSplit split_work(const AttendArgs& p, int ctas)
     if (p.own_items) {
         // four stretches for each of the warps that have them
         const int64_t places = min((int64_t)(p.own_items - p.batch), max((int64_t)1, ((int64_t)r.own_ctas * (4 * kOwnWarps) + heads - 1) / heads));
-        r.own_step = (int)max((int64_t)kOwnLeast, ((keys + places - 1) / places + 63) / 64 * 64);
+        r.own_step = own_stretch(keys, places);
     }
     return r;
 }
