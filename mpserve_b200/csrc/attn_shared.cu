@@ -146,7 +146,7 @@ static int check_attend(const mps_prefix_attend& a) {
         set_error("mps_prefix_attend_tokens: the size of a page must be a power of two from 16 to 2^20, pages below 2^31");
         return MPS_ERR_INVALID;
     }
-    if (a.table_columns < 0 || a.table_columns * a.page_size > MPS_MOST_KEYS || a.prefix_length < 0 || a.prefix_length > MPS_MOST_KEYS) {
+    if (a.table_columns < 0 || a.table_columns > MPS_MOST_KEYS / a.page_size || a.prefix_length < 0 || a.prefix_length > MPS_MOST_KEYS) {
         set_error("mps_prefix_attend_tokens: a table and the prefix may have at most %lld keys", (long long)MPS_MOST_KEYS);
         return MPS_ERR_INVALID;
     }
