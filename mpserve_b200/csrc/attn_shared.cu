@@ -120,9 +120,11 @@ static AttendPlan attend_plan(const mps_prefix_attend& a, int sms) {
         // a CTA an SM, one of them at least for the sequences, as long as there are tiles of keys
         const int64_t units = plan.wide_tiles * (int64_t)a.kv_heads, tiles = (a.prefix_length + kPrefixKeys - 1) / kPrefixKeys;
         if (units + (most > 0) > sms) {
-            // more than there are SMs for already: the sequences get an SM of four
+            // More than there are SMs for already: the sequences get a CTA an SM behind them.  1200 sequences (32 query, 8 key heads of 128) behind 300 keys with up to 100 of
+            // their own take 128 us, with a CTA for every second SM 149, for every fourth 224, with two an SM 141; behind 2048 with up to 512 319, 421, 687 and 323; 4096 behind
+            // 8192 with up to 100 865, 855, 1096 and 874.
             plan.most_splits = 1;
-            plan.own_ctas = most > 0 ? (sms + 3) / 4 : 0;
+            plan.own_ctas = most > 0 ? sms : 0;
             plan.ctas = units + plan.own_ctas;
         } else {
             plan.most_splits = (int)std::min<int64_t>(tiles, (sms - (most > 0)) / units);
