@@ -222,7 +222,7 @@ def build_awq_bucket(bf16_params, int4_values_u8, scales_u16, max_len, threads_p
     if int4_values_u8.dtype != torch.uint8:
         raise ValueError("int4_values_u8 must be torch.uint8")
     if scales_u16.dtype != torch.uint16:
-        raise ValueError("scales_u16 must be torch.uint16 (bf16 raw bits)")
+        raise ValueError("scales_u16 must be torch.uint16 (raw bits)")
     if max_len <= 0 or max_len > 15:
         raise ValueError("max_len must be in (0,15]")
     if threads_per_block <= 0 or threads_per_block > 1024:
@@ -273,7 +273,7 @@ def build_awq_by_scale(bf16_values, int4_values, scales_u16, max_len, threads, g
     if int4_values.dtype != torch.uint8:
         raise ValueError("int4_values_u8 must be torch.uint8")
     if scales_u16.dtype != torch.uint16:
-        raise ValueError("scales_u16 must be torch.uint16 (bf16 raw bits)")
+        raise ValueError("scales_u16 must be torch.uint16 (raw bits)")
     if max_len <= 0 or max_len > 15:
         raise ValueError("max_len must be in (0,15]")
     if threads <= 0 or threads > 1024:
@@ -351,7 +351,7 @@ def build_awq_shared(bf16_params, int4_values_u8, scales_u16, max_len):
     if int4_values_u8.dtype != torch.uint8:
         raise ValueError("int4_values_u8 must be torch.uint8")
     if scales_u16.dtype != torch.uint16:
-        raise ValueError("scales_u16 must be torch.uint16 (bf16 raw bits)")
+        raise ValueError("scales_u16 must be torch.uint16 (raw bits)")
     if max_len <= 0 or max_len > 20:
         raise ValueError("max_len must be in (0,20]")
     if max_len > 15:

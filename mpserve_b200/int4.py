@@ -62,8 +62,10 @@ def _check(w, name: str) -> int:
 
 def from_parts(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *, group: int = 128) -> Int4Tensor:
     """A weight from its parts: ``codes`` ``uint8 [rows, cols]``, one of 0 to 15 a byte, ``scales`` ``[rows, ceil(cols / group)]`` (float16, bfloat16, or
-    uint16 with float16's bits, as the AWQ entries of this library take them) and ``zeros`` ``uint8`` of the same shape, 0 to 15, or None: 8 everywhere.
-    ``group`` is 32, 64 or 128."""
+    uint16, which is read as float16's bits) and ``zeros`` ``uint8`` of the same shape, 0 to 15, or None: 8 everywhere.
+    ``group`` is 32, 64 or 128.
+
+    The AWQ entries of this library take scales as uint16, too, and compare their bits only: bfloat16's would do there, and come here as ``scales.view(torch.bfloat16)``."""
     if group not in GROUPS:
         raise ValueError(f"group must be one of {GROUPS}")
     if not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[1] == 0:
