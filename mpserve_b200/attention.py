@@ -219,7 +219,8 @@ def norm_rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotar
     given) and rotated by its token's position; new, contiguous tensors of the same dtype.
 
     ``q`` and ``k`` may be views of one projection's result (unit stride along ``dim``).  ``positions``: int32 or int64, ``[tokens]`` or ``[axes, tokens]``.  Angles are
-    exact to FP32 however far the position; all else is FP32, rounded once."""
+    products in 64 bits taken modulo a turn: off by 2^-51 of the whole angle, ``position * frequency``, which FP32 does not show up to 2^27, and beyond that by FP32's rounding of
+    what is left of it.  All else is FP32, rounded once."""
     return _rotate(q, k, None, positions, rotary, None, None, q_weight, k_weight, eps)
 
 

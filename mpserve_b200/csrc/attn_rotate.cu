@@ -5,7 +5,7 @@
 //
 // A pair is (j, j + rotated / 2), or neighbours (2 j, 2 j + 1).  An angle of a far position has more revolutions than FP32 has digits: position times
 // frequency, in revolutions, is an FP64 product, whose whole part is dropped in FP64; what is left is below half a revolution and its sine and cosine
-// are FP32's.  All other arithmetic is FP32, rounded once to the output's type.
+// are FP32's.  (The frequency in revolutions and the product are off by 2^-51 of the whole angle together.)  All other arithmetic is FP32, rounded once to the output's type.
 //
 // Eight values of a head are a lane's, four and the four that they are paired with, so that four to 32 lanes have a head and a pair never changes lanes.  With few
 // tokens a CTA has one, all heads at once, and its first threads make the token's cosines and sines while the heads are on their way; with many a warp has
