@@ -112,6 +112,8 @@ def linear(x: torch.Tensor, w: Int4Tensor, *, dtype: torch.dtype | None = None) 
     """``x @ w.T``: ``x`` ``[..., cols]`` in bfloat16 or float16, ``w`` ``[rows, cols]``; sums are FP32, rounded once to ``dtype``, bfloat16 or
     float16, by default ``x``'s.
 
+    A group's products are summed before its scale multiplies them: a bfloat16 token beyond 2^116 may pass FP32's range there, though its result would not.
+
     Made for the tokens of a decoding step.  Any number of them is served, 64 at a time."""
     index = _check(w, "w")
     rows, cols, stride = _matrix(x, "x")
