@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t query_pair(uint32_t pair, int factor) {
 // of stretches of the prefix that leave a CTA for the sequences, the one with which the slower side is soonest done.  What a side takes, in cycles, from
 // measurements at 1.9 GHz: a CTA that has a part of the prefix, its start and end and 128 keys for 256 rows or for 128; one that has sequences, its start and a
 // byte.  What counts is how one side stands to the other: side by side both are slower (3750 cycles, 27 bytes a cycle), in the same ratio.  With 3750 and 50, 128 sequences behind
-// 32768 with up to 1024 own keys each took 161 us, with these and with 3750 and 40 118 to 121.
+// 32768 with up to 1024 own keys each took 161 us, with these and with 3750 and 40 118 to 121.  Heads of 64 and F16 share them (a key's cycles are rounded down to a whole number).
 constexpr int kPrefixKeys = 128, kPrefixRows = 128;
 constexpr int kPrefixStart = 9000, kPrefixPaired = 3000, kPrefixSingle = 1800, kOwnStart = 6000, kOwnBytesPerCycle = 50;
 constexpr int kOwnWarps = 14;              // that have own keys, of a CTA

@@ -8,7 +8,7 @@
 // are FP32's.  (The frequency in revolutions and the product are off by 2^-51 of the whole angle together.)  All other arithmetic is FP32, rounded once to the output's type.
 //
 // Eight values of a head are a lane's, four and the four that they are paired with, so that four to 32 lanes have a head and a pair never changes lanes.  With few
-// tokens a CTA has one, all heads at once, and its first threads make the token's cosines and sines while the heads are on their way; with many a warp has
+// tokens a CTA has one, all heads at once or, of 1024 to 2048 lanes, in three or four steps, and its first threads make the token's cosines and sines while the heads are on their way; with many a warp has
 // one, makes them for itself and goes through the heads with four of them on their way, without a barrier.  Bounds: memory, for a few tokens the launch.
 #include <initializer_list>
 
@@ -17,8 +17,8 @@
 namespace mps {
 
 constexpr int kHeadMostDim = 256;
-// Up to six a SM a token has a CTA: 32 query and 8 key heads of 128 take 2.5 us for 148 tokens and 4.6 for 400, with a warp a token 5.5 and 7.4; 2048 tokens take 16.0 that
-// way and 11.9 with a warp each.
+// Up to six a SM a token has a CTA: 32 query and 8 key heads of 128 take 2.5 us for 148 tokens and 4.6 for 400, with a warp a token 5.5 and 7.4; 2048 tokens take 16.5 that
+// way and 13.3 with a warp each.
 constexpr int64_t kRotateFewTokens = 888;
 
 struct RotateArgs {

@@ -38,7 +38,7 @@ def test_heads_on_both_sides_of_the_number_of_sms(heads, prefix, own):
 @pytest.mark.parametrize("own", [0, 90])
 @pytest.mark.parametrize("batch,dim,dtype", [(1152, 128, "bf16"), (1200, 64, "f16"), (1217, 128, "bf16")])
 def test_many_sequences(prefix, own, batch, dim, dtype):
-    # 8 key heads and tiles of 64 sequences in pairs: 72, 76 and 77 pairs' halves; the last is an odd tile
+    # a pair of tiles has 64 sequences: 18, 19 and 20 pairs for each of 8 key heads, the last of 1217 sequences with one tile
     _check(batch, 32, 8, prefix, own, dim, dtype=dtype, look_at=[*range(0, batch, 41), *range(batch - 3, batch)])
 
 
