@@ -12,7 +12,7 @@
 // joined.  P is rounded to 16 bits, as the tensor cores take it: a relative 2^-8 (BF16) or 2^-11 (F16) of every weight by itself, no more than what the result is rounded by.
 // Sums are of P as it was before.  BF16 has FP32's range, and m is the largest logit: P is at most 2^8.  F16 has numbers down to 2^-14, and below that steps of 2^-24: there m is
 // 2^12 below the largest logit, P at most 2^15, a weight keeps its 2^-11 down to 2^-26 of the stretch's largest and is off by 2^-37 of that beyond.  (With m the largest
-// logit itself, 99 keys behind one that weighed e^17 as much and had no value lost 44 % of their result.)
+// logit itself, keys behind one that weighed e^17 as much and had no value gave a result 44 % off: 2^-24.5 became 2^-24.)
 // Bounds: for many rows the softmax.  A period of 128 keys by 256 rows takes 3750 cycles: 2560 of a row's softmax (500 to fetch it, 290 for its maximum, the rest for
 // exponentials, sums and packing; 128 x 128 exponentials are 1024 of a scheduler's at the nominal rate) and 690 of two hand-overs, where the products are 2048 for both groups.
 // 128 sequences behind 32768 keys with none of their own take 84 to 88 us (32 query heads, 8 key heads of 128).  For few rows the memory.

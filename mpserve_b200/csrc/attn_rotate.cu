@@ -8,8 +8,8 @@
 // are FP32's.  (The frequency in revolutions and the product are off by 2^-51 of the whole angle together.)  All other arithmetic is FP32, rounded once to the output's type.
 //
 // Eight values of a head are a lane's, four and the four that they are paired with, so that four to 32 lanes have a head and a pair never changes lanes.  With few
-// tokens a CTA has one, all heads at once or, of 1024 to 2048 lanes, in three or four steps, and its first threads make the token's cosines and sines while the heads are on their way; with many a warp has
-// one, makes them for itself and goes through the heads with four of them on their way, without a barrier.  Bounds: memory, for a few tokens the launch.
+// tokens a CTA has one, all heads at once or, of 1024 to 2048 lanes, in three or four steps, and its first threads make the token's cosines and sines while the heads are
+// on their way; with many a warp has one, makes them for itself and goes through the heads with four of them on their way, without a barrier.  Bounds: memory, for a few tokens the launch.
 #include <initializer_list>
 
 #include "mx4.cuh"
